@@ -34,14 +34,21 @@ extern "C" {
 #endif
 
 /* Element types, numbered as ggml numbers them (GGML_TYPE_F32 = 0,
- * GGML_TYPE_F16 = 1); the only two the reference's operations take
- * (mul_mat.cc:181-194, conv2d.cc:320-331, attention.cc:828-845). */
-enum { SDHIP_TYPE_F32 = 0, SDHIP_TYPE_F16 = 1 };
+ * GGML_TYPE_F16 = 1, GGML_TYPE_Q4_0 = 2, GGML_TYPE_Q4_1 = 3).  The first two
+ * are those the reference's operations take (mul_mat.cc:181-194,
+ * conv2d.cc:320-331, attention.cc:828-845).  The last two are weights of
+ * MUL_MAT in blocks of 32 along ne[0]: Q4_0, 18 bytes, a half-precision scale
+ * d and 16 bytes, w = d (q - 8); Q4_1, 20 bytes, d, a half-precision least
+ * value m and 16 bytes, w = d q + m; byte j holds q of the block's number j in
+ * its low four bits and of number 16 + j in its high ones.  A tensor of them
+ * has nb[0] the bytes of a block, as ggml_tensor has. */
+enum { SDHIP_TYPE_F32 = 0, SDHIP_TYPE_F16 = 1, SDHIP_TYPE_Q4_0 = 2, SDHIP_TYPE_Q4_1 = 3 };
 
 typedef enum { SDHIP_OK = 0, SDHIP_UNSUPPORTED = 1, SDHIP_ERROR = 2 } sdhip_status;
 
 /* A tensor as ggml_tensor describes its memory: ne[] extents, nb[] strides in
- * bytes (nb[0] the element size for the layouts taken), data on the device. */
+ * bytes (nb[0] the element size -- of Q4_0 and Q4_1 the block size -- for the
+ * layouts taken), data on the device. */
 typedef struct sdhip_tensor {
     int32_t type;
     int64_t ne[4];
@@ -168,6 +175,13 @@ int sdhip_profile_entry(int i, const char **name, double *total_ms, int64_t *lau
  * single-precision weights their planes; otherwise, for a product of few
  * output blocks and long K (split along K), the splits' partial sums; 0
  * else.  A buffer short of sdhip_mul_mat_work_size is SDHIP_ERROR.
+ *
+ * Weights of 4 bits (Q4_0, Q4_1; no counterpart in the reference, which leaves
+ * them to ggml): ne[0] a multiple of 32, rows nb[1] apart, any even number of
+ * bytes that holds a row, at an even address; from one row of x up, where the
+ * others begin at 16.  The products are those of the exact weights with x in
+ * 22 bits or more of each row's greatest number, whatever bits asks for; the
+ * output shares no byte with w or x.
  * Replaces mul_mat_supported / mul_mat_work_size / mul_mat_compute
  * (sources/ops.h:40-44; mul_mat.cc:181-194, 205-215, 1175-1196). */
 int sdhip_mul_mat_supported(const sdhip_tensor *w, const sdhip_tensor *x, const sdhip_tensor *y);
@@ -283,6 +297,49 @@ sdhip_status sdhip_group_norm_static(const sdhip_tensor *x, const sdhip_tensor *
 int sdhip_norm_supported(const sdhip_tensor *x, const sdhip_tensor *y);
 sdhip_status sdhip_norm(const sdhip_tensor *x, const sdhip_tensor *y, float eps, const sdhip_epilogue *chain,
                         void *stream);
+
+/* The norms after and before a block of a transformer, with the gate and the
+ * residual between them, in one pass over the rows (ne[0]): the reference has
+ * no such node; its graphs hold NORM, MUL, ADD nodes one by one.
+ *
+ *   z = post(y)                                             after the block
+ *   s = residual_scale residual + branch_scale (gate z)     -> sum
+ *   n = pre(s)                                              before the next -> out
+ *
+ * where a norm of a row v is, by its kind,
+ *   NONE   v
+ *   LAYER  (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps)
+ *   RMS    v / sqrt(mean(v^2) + eps)
+ * times (weight + weight_offset) where weight is not NULL, plus bias where
+ * that is not NULL (weight_offset 1 takes a scale given as its difference
+ * from 1, as a modulation by the timestep gives it).
+ *
+ * y, residual, sum and out are F32 of one shape, nb[0] = 4, other strides any
+ * multiple of 4 bytes; weight, bias and gate F32, nb[0] = 4, broadcast along each dimension
+ * whose extent is 1.  NULL post: z = y.  NULL gate: 1.  NULL y (then post and
+ * gate are NULL too): s = residual_scale residual, the norm before a first
+ * block.  NULL sum: s is not written.  NULL pre and out: no norm after.  sum
+ * and out each may be y's or residual's own memory in the same layout; else
+ * what a call writes shares no byte range with what it reads, and sum and out
+ * share none, nor do two rows of one of them: SDHIP_UNSUPPORTED.  Sums over a
+ * row are taken in double.  No work buffer. */
+enum { SDHIP_ROW_NORM_NONE = 0, SDHIP_ROW_NORM_LAYER = 1, SDHIP_ROW_NORM_RMS = 2 };
+
+typedef struct sdhip_row_norm {
+    int32_t kind;
+    float eps;
+    float weight_offset;
+    const sdhip_tensor *weight;
+    const sdhip_tensor *bias;
+} sdhip_row_norm;
+
+int sdhip_norm_residual_supported(const sdhip_tensor *y, const sdhip_row_norm *post, const sdhip_tensor *gate,
+                                  const sdhip_tensor *residual, const sdhip_tensor *sum, const sdhip_row_norm *pre,
+                                  const sdhip_tensor *out);
+sdhip_status sdhip_norm_residual(const sdhip_tensor *y, const sdhip_row_norm *post, const sdhip_tensor *gate,
+                                 float branch_scale, const sdhip_tensor *residual, float residual_scale,
+                                 const sdhip_tensor *sum, const sdhip_row_norm *pre, const sdhip_tensor *out,
+                                 void *stream);
 
 /* ---------------------------------------------------------------- the graph */
 

@@ -174,6 +174,11 @@ bool in_range(Range r, long v, const char *&takes) {
 bool holds_f32(const sdhip_tensor *t) { return t != nullptr && t->type == SDHIP_TYPE_F32 && t->nb[0] == 4; }
 bool holds_f16(const sdhip_tensor *t) { return t != nullptr && t->type == SDHIP_TYPE_F16 && t->nb[0] == 2; }
 
+bool holds_q4(const sdhip_tensor *t) {
+    return t != nullptr && q4_type(t->type) && t->nb[0] == q4_block_bytes(t->type) && t->ne[0] >= kBlock &&
+           t->ne[0] % kBlock == 0;
+}
+
 bool contiguous(const sdhip_tensor *t) {
     const int64_t size = t->type == SDHIP_TYPE_F16 ? 2 : 4;
     return t->nb[0] == size && t->nb[1] == t->nb[0] * t->ne[0] && t->nb[2] == t->nb[1] * t->ne[1] &&
@@ -198,11 +203,13 @@ bool same_layout(const sdhip_tensor *a, const sdhip_tensor *b) {
 int64_t nelements(const sdhip_tensor *t) { return t->ne[0] * t->ne[1] * t->ne[2] * t->ne[3]; }
 
 size_t tensor_span(const sdhip_tensor *t) {
-    size_t n = t->type == SDHIP_TYPE_F16 ? 2 : 4;
+    const bool q4 = q4_type(t->type);
+    size_t n = q4 ? static_cast<size_t>(q4_block_bytes(t->type)) : t->type == SDHIP_TYPE_F16 ? 2 : 4;
     for (int k = 0; k < 4; ++k) {
         if (t->ne[k] <= 0) return 0;
         if (t->nb[k] < 0) return SIZE_MAX;
-        const uint64_t reach = static_cast<uint64_t>(t->ne[k] - 1) * static_cast<uint64_t>(t->nb[k]);
+        const int64_t count = q4 && k == 0 ? ceil_div(t->ne[0], kBlock) : t->ne[k];
+        const uint64_t reach = static_cast<uint64_t>(count - 1) * static_cast<uint64_t>(t->nb[k]);
         if (reach > SIZE_MAX - n) return SIZE_MAX;
         n += static_cast<size_t>(reach);
     }

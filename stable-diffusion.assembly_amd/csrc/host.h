@@ -108,12 +108,18 @@ sdhip_status launched(hipError_t e, const char *what);
 
 bool holds_f32(const sdhip_tensor *t);
 bool holds_f16(const sdhip_tensor *t);
+// Weights of 4 bits in ggml's blocks of 32 (Q4_0, Q4_1), whole blocks along
+// ne[0]; and the bytes of a block of such a type.
+bool holds_q4(const sdhip_tensor *t);
+constexpr int64_t kBlock = 32;
+inline bool q4_type(int32_t type) { return type == SDHIP_TYPE_Q4_0 || type == SDHIP_TYPE_Q4_1; }
+inline int64_t q4_block_bytes(int32_t type) { return type == SDHIP_TYPE_Q4_0 ? 18 : 20; }
 bool contiguous(const sdhip_tensor *t);
 bool same_shape(const sdhip_tensor *a, const sdhip_tensor *b);
 bool same_layout(const sdhip_tensor *a, const sdhip_tensor *b);
 int64_t nelements(const sdhip_tensor *t);
-// The bytes from a tensor's first element to one past its last (ggml_nbytes
-// of one-element blocks); 0 for an empty tensor, SIZE_MAX where a stride is
+// The bytes from a tensor's first element (or block) to one past its last
+// (ggml_nbytes); 0 for an empty tensor, SIZE_MAX where a stride is
 // negative (its reach is not bounded here, so it is taken to reach anything).
 size_t tensor_span(const sdhip_tensor *t);
 // Whether the bytes [a, a + an) and [b, b + bn) share any: the addresses

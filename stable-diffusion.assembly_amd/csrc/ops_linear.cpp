@@ -1,12 +1,14 @@
 // MUL_MAT and MUL_MAT with the gated GELU after it (mul_mat.cc), on the
 // device: the predicates of mul_mat_supported (mul_mat.cc:181-194) and
 // mul_mat_gated_supported (mul_mat.cc:1128-1151), then the split-FP16 MFMA
-// product (gemm.hip) or, with bits, the quantized one (quant.hip).
+// product (gemm.hip) or, with bits, the quantized one (quant.hip); weights of
+// 4 bits, which the reference leaves to ggml, by their own product (q4.hip).
 
 #include <hip/hip_runtime.h>
 
 #include "host.h"
 #include "kernels.h"
+#include "q4.h"
 #include "quant.h"
 
 namespace sdhip {
@@ -43,6 +45,57 @@ MulMatArgs args_of(const sdhip_tensor *w, const sdhip_tensor *x, const sdhip_ten
     return a;
 }
 
+Q4Args q4_args_of(const sdhip_tensor *w, const sdhip_tensor *x, const sdhip_tensor *y) {
+    Q4Args a{};
+    a.x = static_cast<const float *>(x->data);
+    a.ldx = x->nb[1] / 4;
+    a.w = static_cast<const uint8_t *>(w->data);
+    a.row_bytes = w->nb[1];
+    a.least = w->type == SDHIP_TYPE_Q4_1;
+    a.K = w->ne[0];
+    a.N = w->ne[1];
+    a.M = x->ne[1] * x->ne[2] * x->ne[3];
+    a.ne1 = y->ne[1];
+    a.ne2 = y->ne[2];
+    a.ldy = y->nb[1] / 4;
+    return a;
+}
+
+// Weights of 4 bits: one matrix of whole blocks of 32 along K, its rows any
+// even number of bytes apart that holds one, from one row of x up; extents
+// counted in 32 bits.
+bool q4_supported(const sdhip_tensor *w, const sdhip_tensor *x, const sdhip_tensor *y) {
+    const int64_t bytes = q4_block_bytes(w->type);
+    if (w->ne[0] > INT32_MAX || w->ne[1] < 1 || w->ne[1] > INT32_MAX || w->ne[2] != 1 || w->ne[3] != 1 ||
+        w->nb[1] % 2 != 0 || w->nb[1] < bytes * (w->ne[0] / kBlock) || reinterpret_cast<uintptr_t>(w->data) % 2 != 0) {
+        return false;
+    }
+    int64_t rows = 1;
+    for (int k = 1; k < 4; ++k) {
+        if (x->ne[k] < 1 || x->ne[k] > INT32_MAX || y->ne[k] != x->ne[k]) return false;
+        rows *= x->ne[k];
+        if (rows > INT32_MAX) return false;
+    }
+    return x->ne[0] == w->ne[0] && y->ne[0] == w->ne[1] && holds_f32(x) && contiguous(x) && holds_f32(y) &&
+           contiguous(y);
+}
+
+// The product of 4-bit weights into a.y, which what it reads shares no byte with.
+sdhip_status q4_mul_mat(const Q4Args &a, const sdhip_tensor *w, const sdhip_tensor *x, int64_t columns,
+                        hipStream_t stream, const char *what) {
+    if (w->data == nullptr || x->data == nullptr || a.y == nullptr) {
+        return fail(SDHIP_ERROR, "%s: a tensor without data", what);
+    }
+    if ((reinterpret_cast<uintptr_t>(x->data) | reinterpret_cast<uintptr_t>(a.y)) % 4 != 0) {
+        return fail(SDHIP_ERROR, "%s: single precision at an address that is no multiple of 4", what);
+    }
+    const size_t on = static_cast<size_t>((a.M - 1) * a.ldy + columns) * 4;
+    if (overlaps(a.y, on, w->data, nbytes(w)) || overlaps(a.y, on, x->data, nbytes(x))) {
+        return fail(SDHIP_ERROR, "%s: the output lies over an operand", what);
+    }
+    return launched(launch_q4_mul_mat(a, stream), what);
+}
+
 }  // namespace
 
 // Whether the product is quantized (mul_mat.cc:95-105): bits asks for the
@@ -61,6 +114,7 @@ extern "C" {
 
 int sdhip_mul_mat_supported(const sdhip_tensor *w, const sdhip_tensor *x, const sdhip_tensor *y) {
     if (w == nullptr || x == nullptr || y == nullptr) return 0;
+    if (holds_q4(w)) return q4_supported(w, x, y);
     // The weights are one matrix of FP16 or single precision, the other
     // operand and the result contiguous single precision, the products large
     // enough to pay for the launch (mul_mat.cc:181-194).
@@ -74,6 +128,7 @@ int sdhip_mul_mat_supported(const sdhip_tensor *w, const sdhip_tensor *x, const 
 
 size_t sdhip_mul_mat_work_size(const sdhip_tensor *w, const sdhip_tensor *x, const sdhip_tensor *y) {
     if (!sdhip_mul_mat_supported(w, x, y)) return 0;
+    if (q4_type(w->type)) return 0;
     if (mul_mat_quantized(x)) {
         return quantized_linear_work_size(w->ne[0], w->ne[1], x->ne[1] * x->ne[2] * x->ne[3]);
     }
@@ -106,14 +161,22 @@ sdhip_status sdhip_mul_mat(const sdhip_tensor *w, const sdhip_tensor *x, const s
     if (!sdhip_mul_mat_supported(w, x, y)) {
         return fail(SDHIP_UNSUPPORTED, "mul_mat: operands not taken");
     }
-    MulMatArgs a = args_of(w, x, y);
     ChainRun run;
     sdhip_status s = chain_plan(y, chain, run);
     if (s != SDHIP_OK) return s;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (q4_type(w->type)) {
+        Q4Args q = q4_args_of(w, x, y);
+        q.chain = run.fused;
+        q.y = run.out;
+        q.from_redirect = run.from_redirect;
+        s = q4_mul_mat(q, w, x, q.N, st, "mul_mat");
+        return s == SDHIP_OK ? chain_after(run, st) : s;
+    }
+    MulMatArgs a = args_of(w, x, y);
     a.chain = run.fused;
     a.y = run.out;
     a.from_redirect = run.from_redirect;
-    const hipStream_t st = static_cast<hipStream_t>(stream);
     if (mul_mat_quantized(x)) {
         const size_t need = quantized_linear_work_size(a.K, a.N, a.M);
         if (const sdhip_status ws = check_work("mul_mat", work, work_size, need); ws != SDHIP_OK) return ws;
@@ -138,7 +201,7 @@ int sdhip_mul_mat_gated_supported(const sdhip_tensor *w, const sdhip_tensor *x, 
     if (!sdhip_mul_mat_supported(w, x, y) || out == nullptr || y->ne[0] % 2 != 0) return 0;
     const int64_t half = y->ne[0] / 2;
     // Quantized, each half's columns begin a panel (mul_mat.cc:1129-1132).
-    if (mul_mat_quantized(x) && half % 16 != 0) return 0;
+    if (!q4_type(w->type) && mul_mat_quantized(x) && half % 16 != 0) return 0;
     // What the result is written to is not what the product reads
     // (mul_mat.cc:1133-1149).
     const size_t on = nbytes(out);
@@ -168,8 +231,8 @@ sdhip_status sdhip_mul_mat_gated(const sdhip_tensor *w, const sdhip_tensor *x, c
                            x->ne[1] * x->ne[2] * x->ne[3], y->ne[0] / 2, y->nb[1] / 4, out->nb[1] / 4,
                            static_cast<hipStream_t>(stream));
     }
-    MulMatArgs a = args_of(w, x, y);
-    sdhip_status s = device_chain(chain, y->ne, a.chain);
+    DevChain steps;
+    sdhip_status s = device_chain(chain, y->ne, steps);
     if (s != SDHIP_OK) return s;
     const size_t on = nbytes(out);
     for (int i = 0; chain != nullptr && i < chain->count; ++i) {
@@ -178,10 +241,20 @@ sdhip_status sdhip_mul_mat_gated(const sdhip_tensor *w, const sdhip_tensor *x, c
             return fail(SDHIP_UNSUPPORTED, "mul_mat_gated: the output overlaps a chain operand");
         }
     }
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (q4_type(w->type)) {
+        Q4Args q = q4_args_of(w, x, y);
+        q.chain = steps;
+        q.y = static_cast<float *>(out->data);
+        q.ldy = out->nb[1] / 4;
+        q.half = y->ne[0] / 2;
+        return q4_mul_mat(q, w, x, q.half, st, "mul_mat_gated");
+    }
+    MulMatArgs a = args_of(w, x, y);
+    a.chain = steps;
     a.y = static_cast<float *>(out->data);
     a.ldy = out->nb[1] / 4;
     a.half = y->ne[0] / 2;
-    const hipStream_t st = static_cast<hipStream_t>(stream);
     if (mul_mat_quantized(x)) {
         const size_t need = quantized_linear_work_size(a.K, a.N, a.M);
         if (const sdhip_status ws = check_work("mul_mat_gated", work, work_size, need); ws != SDHIP_OK) return ws;

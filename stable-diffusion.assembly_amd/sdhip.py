@@ -16,9 +16,14 @@ LIB_PATH = os.path.join(HERE, "libsdhip.so")
 
 TYPE_F32 = 0
 TYPE_F16 = 1
+TYPE_Q4_0 = 2
+TYPE_Q4_1 = 3
+BLOCK = 32  # weights of a block of Q4_0 or Q4_1 ...
+BLOCK_BYTES = {TYPE_Q4_0: 18, TYPE_Q4_1: 20}  # ... and its bytes
 OK, UNSUPPORTED, ERROR = 0, 1, 2
 STEP_ADD, STEP_MUL, STEP_SILU = 0, 1, 2
 MAX_STEPS = 6
+ROW_NORM_NONE, ROW_NORM_LAYER, ROW_NORM_RMS = 0, 1, 2
 
 
 class Tensor(ctypes.Structure):
@@ -40,6 +45,18 @@ class Epilogue(ctypes.Structure):
         ("steps", Step * MAX_STEPS),
         ("redirect", ctypes.POINTER(Tensor)),
         ("from_redirect", ctypes.c_int32),
+    ]
+
+
+class RowNorm(ctypes.Structure):
+    """sdhip_row_norm: a norm of rows and what it is multiplied by and added."""
+
+    _fields_ = [
+        ("kind", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("weight_offset", ctypes.c_float),
+        ("weight", ctypes.POINTER(Tensor)),
+        ("bias", ctypes.POINTER(Tensor)),
     ]
 
 
@@ -73,6 +90,7 @@ class NodePlan(ctypes.Structure):
 
 _T = ctypes.POINTER(Tensor)
 _E = ctypes.POINTER(Epilogue)
+_R = ctypes.POINTER(RowNorm)
 _P = ctypes.c_void_p
 _SZ = ctypes.c_size_t
 _I6 = ctypes.c_int32 * 6
@@ -110,6 +128,9 @@ SIGNATURES = [
     ("sdhip_group_norm_static", ctypes.c_int, [_T, _T, ctypes.c_int, ctypes.c_float, _E, _P]),
     ("sdhip_norm_supported", ctypes.c_int, [_T, _T]),
     ("sdhip_norm", ctypes.c_int, [_T, _T, ctypes.c_float, _E, _P]),
+    ("sdhip_norm_residual_supported", ctypes.c_int, [_T, _R, _T, _T, _T, _R, _T]),
+    ("sdhip_norm_residual", ctypes.c_int,
+     [_T, _R, _T, ctypes.c_float, _T, ctypes.c_float, _T, _R, _T, _P]),
     ("sdhip_plan_nodes", ctypes.c_int,
      [ctypes.POINTER(ctypes.POINTER(Node)), ctypes.c_int, ctypes.c_int, ctypes.POINTER(NodePlan)]),
     ("sdhip_compute_nodes", ctypes.c_int,
@@ -147,8 +168,25 @@ def check(status, what):
         raise SdhipError(status, what)
 
 
+def _block_desc(t):
+    """The descriptor of 4-bit weights: bytes [N, K / 32, 18] (Q4_0) or
+    [N, K / 32, 20] (Q4_1), each row's blocks side by side."""
+    types = {size: code for code, size in BLOCK_BYTES.items()}
+    if t.dim() != 3 or t.shape[2] not in types:
+        raise ValueError(f"4-bit weights are bytes [N, K / {BLOCK}, 18 or 20], not {list(t.shape)}")
+    n, blocks, size = t.shape
+    if t.stride(2) != 1 or t.stride(1) != size:
+        raise ValueError("the blocks of a row of 4-bit weights are not side by side")
+    row = t.stride(0)
+    return view_desc(t.data_ptr(), types[size], [BLOCK * blocks, n, 1, 1], [size, row, row * n, row * n])
+
+
 def desc(t):
-    """The ggml descriptor of a torch tensor of at most 4 dimensions."""
+    """The ggml descriptor of a torch tensor of at most 4 dimensions; of bytes
+    [N, K / 32, 18] or [N, K / 32, 20], that of the N x K weights of 4 bits
+    (Q4_0, Q4_1) that they hold."""
+    if t.dtype == torch.uint8:
+        return _block_desc(t)
     if t.dim() > 4:
         raise ValueError("at most 4 dimensions")
     d = Tensor()
@@ -217,7 +255,8 @@ def _work(nbytes, device):
 
 
 def mul_mat(w, x, y, chain=None, work=None):
-    """y (ne = [N, M...]) = x W^T with the chain; w: [N, K] f16, x: [..., K] f32."""
+    """y (ne = [N, M...]) = x W^T with the chain; w: [N, K] f16 or f32, or 4-bit
+    weights as bytes (desc); x: [..., K] f32."""
     lib = load()
     dw, dx, dy = desc(w), desc(x), desc(y)
     size = lib.sdhip_mul_mat_work_size(dw, dx, dy)
@@ -298,6 +337,30 @@ def group_norm_static(x, y, groups, eps, chain=None):
 def norm(x, y, eps, chain=None):
     check(load().sdhip_norm(desc(x), desc(y), eps, ctypes.byref(chain) if chain else None, stream_handle()),
           "norm")
+
+
+def row_norm(kind="none", eps=0.0, weight=None, bias=None, weight_offset=0.0):
+    """A norm for norm_residual: 'none', 'layer' or 'rms', times (weight +
+    weight_offset), plus bias (torch tensors that broadcast over the rows)."""
+    r = RowNorm()
+    r.kind = {"none": ROW_NORM_NONE, "layer": ROW_NORM_LAYER, "rms": ROW_NORM_RMS}[kind]
+    r.eps = eps
+    r.weight_offset = weight_offset
+    descs = [desc(t) if t is not None else None for t in (weight, bias)]
+    r._held = (descs, weight, bias)  # kept alive with the norm
+    for name, d in zip(("weight", "bias"), descs):
+        if d is not None:
+            setattr(r, name, ctypes.pointer(d))
+    return r
+
+
+def norm_residual(y, residual, sum=None, out=None, post=None, pre=None, gate=None, branch_scale=1.0,
+                  residual_scale=1.0):
+    """sum = residual_scale residual + branch_scale (gate post(y)), out = pre(sum);
+    post and pre from row_norm, y, sum and out tensors or None."""
+    dy, ds, do, dg = (desc(t) if t is not None else None for t in (y, sum, out, gate))
+    check(load().sdhip_norm_residual(dy, post, dg, branch_scale, desc(residual), residual_scale, ds, pre, do,
+                                     stream_handle()), "norm_residual")
 
 
 def profile_enable(on=True):
