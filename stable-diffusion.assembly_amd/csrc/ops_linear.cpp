@@ -81,8 +81,8 @@ bool q4_supported(const sdhip_tensor *w, const sdhip_tensor *x, const sdhip_tens
 }
 
 // The product of 4-bit weights into a.y, which what it reads shares no byte with.
-sdhip_status q4_mul_mat(const Q4Args &a, const sdhip_tensor *w, const sdhip_tensor *x, int64_t columns,
-                        hipStream_t stream, const char *what) {
+sdhip_status q4_mul_mat(const Q4Args &a, const sdhip_tensor *w, const sdhip_tensor *x, int64_t columns, void *work,
+                        size_t work_size, hipStream_t stream, const char *what) {
     if (w->data == nullptr || x->data == nullptr || a.y == nullptr) {
         return fail(SDHIP_ERROR, "%s: a tensor without data", what);
     }
@@ -93,7 +93,9 @@ sdhip_status q4_mul_mat(const Q4Args &a, const sdhip_tensor *w, const sdhip_tens
     if (overlaps(a.y, on, w->data, nbytes(w)) || overlaps(a.y, on, x->data, nbytes(x))) {
         return fail(SDHIP_ERROR, "%s: the output lies over an operand", what);
     }
-    return launched(launch_q4_mul_mat(a, stream), what);
+    const size_t need = q4_work_size(a.M, a.N, a.K, a.least != 0);
+    if (const sdhip_status ws = check_work(what, work, work_size, need); ws != SDHIP_OK) return ws;
+    return launched(launch_q4_mul_mat(a, work, stream), what);
 }
 
 }  // namespace
@@ -128,7 +130,9 @@ int sdhip_mul_mat_supported(const sdhip_tensor *w, const sdhip_tensor *x, const 
 
 size_t sdhip_mul_mat_work_size(const sdhip_tensor *w, const sdhip_tensor *x, const sdhip_tensor *y) {
     if (!sdhip_mul_mat_supported(w, x, y)) return 0;
-    if (q4_type(w->type)) return 0;
+    if (q4_type(w->type)) {
+        return q4_work_size(x->ne[1] * x->ne[2] * x->ne[3], w->ne[1], w->ne[0], w->type == SDHIP_TYPE_Q4_1);
+    }
     if (mul_mat_quantized(x)) {
         return quantized_linear_work_size(w->ne[0], w->ne[1], x->ne[1] * x->ne[2] * x->ne[3]);
     }
@@ -170,7 +174,7 @@ sdhip_status sdhip_mul_mat(const sdhip_tensor *w, const sdhip_tensor *x, const s
         q.chain = run.fused;
         q.y = run.out;
         q.from_redirect = run.from_redirect;
-        s = q4_mul_mat(q, w, x, q.N, st, "mul_mat");
+        s = q4_mul_mat(q, w, x, q.N, work, work_size, st, "mul_mat");
         return s == SDHIP_OK ? chain_after(run, st) : s;
     }
     MulMatArgs a = args_of(w, x, y);
@@ -248,7 +252,7 @@ sdhip_status sdhip_mul_mat_gated(const sdhip_tensor *w, const sdhip_tensor *x, c
         q.y = static_cast<float *>(out->data);
         q.ldy = out->nb[1] / 4;
         q.half = y->ne[0] / 2;
-        return q4_mul_mat(q, w, x, q.half, st, "mul_mat_gated");
+        return q4_mul_mat(q, w, x, q.half, work, work_size, st, "mul_mat_gated");
     }
     MulMatArgs a = args_of(w, x, y);
     a.chain = steps;

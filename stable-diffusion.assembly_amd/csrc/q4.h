@@ -28,6 +28,9 @@ struct Q4Args {
     DevChain chain;
 };
 
-hipError_t launch_q4_mul_mat(const Q4Args &a, hipStream_t stream);
+// The work buffer of a product (gated or not) of M rows: its operands as the
+// kernels read them; 0 for few rows.
+size_t q4_work_size(int64_t M, int64_t N, int64_t K, bool least);
+hipError_t launch_q4_mul_mat(const Q4Args &a, void *work, hipStream_t stream);
 
 }  // namespace sdhip

@@ -96,6 +96,35 @@ __device__ __forceinline__ void split8(const float4v &low, const float4v &high, 
     }
 }
 
+__device__ __forceinline__ float4v load4(const float *p) {
+    float4v v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+
+// The greatest magnitude of four numbers, as bits.
+__device__ __forceinline__ uint32_t magnitude(const float4v &v) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t p = __builtin_bit_cast(uint32_t, static_cast<float>(v[k])) & 0x7fffffffu;
+        m = m > p ? m : p;
+    }
+    return m;
+}
+
+// The chain over 8 rows m[e] (those past M as the last) of column n.
+__device__ __forceinline__ void apply_chain_rows(const Q4Args &a, float (&v)[8], const int (&m)[8], int64_t n) {
+    apply_chain_block(a.chain, v, [&](int s, int e) {
+        const DevStep &st = a.chain.steps[s];
+        const int64_t row = m[e] < a.M ? m[e] : a.M - 1;
+        if (st.flat123) return n * st.nb[0] + row * st.nb[1];
+        uint32_t i1, i2, i3;
+        split_index(static_cast<uint32_t>(row), static_cast<uint32_t>(a.ne1), static_cast<uint32_t>(a.ne2), i1, i2, i3);
+        return n * st.nb[0] + i1 * st.nb[1] + i2 * st.nb[2] + i3 * st.nb[3];
+    });
+}
+
 // ------------------------------------------------------------------ copies
 
 // A copy of 16 bytes a lane (1 KB) or 4 into LDS at `to` and on, lane after
@@ -221,15 +250,8 @@ __global__ __launch_bounds__(kFewThreads, 4) void q4_few_kernel(FewArgs f) {
             char *place = lds + kPartBytes * u + 128 * (lane >> 2) + 16 * (lane & 3);
             const float4v low = *reinterpret_cast<const float4v *>(place);
             const float4v high = *reinterpret_cast<const float4v *>(place + 64);
-            uint32_t v = 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint32_t p = __builtin_bit_cast(uint32_t, static_cast<float>(low[k])) & 0x7fffffffu;
-                const uint32_t q = __builtin_bit_cast(uint32_t, static_cast<float>(high[k])) & 0x7fffffffu;
-                v = v > p ? v : p;
-                v = v > q ? v : q;
-            }
-            const uint32_t e = scale_exponent(wave_greatest(v));
+            const uint32_t p = magnitude(low), q = magnitude(high);
+            const uint32_t e = scale_exponent(wave_greatest(p > q ? p : q));
             half8 hi, lo;
             split8(low, high, power(e), hi, lo);
             *reinterpret_cast<half8 *>(place) = hi;
@@ -450,12 +472,461 @@ hipError_t few_rows(const Q4Args &a, hipStream_t stream) {
     return launch_few<LEAST, GATED, 16>(a, stream);
 }
 
+// ------------------------------------------------------------------ many rows
+
+// More rows of x: both operands are first laid out in the work buffer as the
+// products' lanes read them (q4_operands_kernel), then multiplied by tiles
+// (q4_tiles_kernel).
+//
+// x: for every block and 32 rows 4 KB, [16 numbers' half of the block][hi, lo]
+// [lane][8], lane 32 h + row holding the block's word 2 half + h of its row, the
+// 8 numbers in widen's order; a row has one scale, from its greatest number.
+// The weights: for every block and 32 rows of them 640 bytes, the two words
+// of lane 32 h + row side by side, then the 32 rows' d in single precision.  For
+// the gated product 32 rows of each half of the weights take turns.
+//
+// Q4_1's offsets c times the blocks' sums of x are a product of their own, 32
+// blocks its step, of three bfloat16 parts each (24 bits of any magnitude): six
+// MFMAs for what would be 32 multiplications and additions an output.  Both
+// lie as the MFMA reads them, 6 KB a 32 rows and 32 blocks: [16 blocks][part]
+// [lane 32 h + row][8 blocks].
+constexpr int kRowsTile = 32;
+constexpr int64_t kNumbersBytes = 4096, kWordsBytes = 640, kOffsetsBytes = 6144;
+
+struct TileArgs {
+    Q4Args a;
+    char *numbers, *words;  // x's parts; the weights' words and scales
+    float *back;            // a row of x's scale out of its sums
+    char *sums, *offsets;   // Q4_1: the blocks' sums of x; c
+    int32_t blocks, groups;  // of 32 numbers; of 32 blocks
+    int32_t row_tiles, column_tiles;  // 32 rows each, whole workgroups' of them
+    int32_t x_groups;       // workgroups that lay x out
+    int32_t m_blocks, n_blocks;
+};
+
+// v in three bfloat16 parts, each what the ones before leave.
+__device__ __forceinline__ void split_bf16(float v, __bf16 (&p)[3]) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        p[i] = static_cast<__bf16>(v);
+        // An infinity is all in the first.
+        v = __builtin_isinf(v) ? 0.0f : v - static_cast<float>(p[i]);
+    }
+}
+
+constexpr int kOperandThreads = 256;
+
+// Workgroups of two kinds: 4 rows of x, a wave each, or 32 rows of the weights by 16 blocks.
+template <bool LEAST, bool GATED>
+__global__ __launch_bounds__(kOperandThreads) void q4_operands_kernel(TileArgs t) {
+    const Q4Args &a = t.a;
+    constexpr int kSize = LEAST ? 20 : 18;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (static_cast<int>(blockIdx.x) < t.x_groups) {
+        const int64_t m = static_cast<int64_t>(blockIdx.x) * 4 + wave;
+        if (m >= a.M) return;
+        const float *x = a.x + m * a.ldx + 4 * (lane & 3);
+        uint32_t v = 0;
+        for (int b = lane >> 2; b < t.blocks; b += 16) {
+            const float4v low = load4(x + b * kBlock), high = load4(x + b * kBlock + 16);
+            const uint32_t p = magnitude(low), q = magnitude(high);
+            v = v > p ? v : p;
+            v = v > q ? v : q;
+        }
+        const uint32_t e = scale_exponent(wave_greatest(v));
+        const float scale = power(e);
+        if (lane == 0) t.back[m] = power(254 - e);
+        const int64_t tile = m / kRowsTile;
+        const int row = static_cast<int>(m % kRowsTile), word = lane & 3;
+        const int end = LEAST ? t.groups * 32 : t.blocks;
+        for (int b = lane >> 2; b < end; b += 16) {
+            float sum = 0.0f;
+            if (b < t.blocks) {
+                const float4v low = load4(x + b * kBlock), high = load4(x + b * kBlock + 16);
+                half8 hi, lo;
+                split8(low, high, scale, hi, lo);
+                char *to = t.numbers + (b * static_cast<int64_t>(t.row_tiles) + tile) * kNumbersBytes + (word >> 1) * 2048 +
+                           ((word & 1) * 32 + row) * 16;
+                *reinterpret_cast<half8 *>(to) = hi;
+                *reinterpret_cast<half8 *>(to + 1024) = lo;
+                if constexpr (LEAST) {
+                    sum = ((low[0] + low[1]) + (low[2] + low[3])) + ((high[0] + high[1]) + (high[2] + high[3]));
+                    sum *= scale;
+                }
+            }
+            if constexpr (LEAST) {
+                sum += __shfl_xor(sum, 1, 64);
+                sum += __shfl_xor(sum, 2, 64);
+                if (word == 0) {
+                    __bf16 p[3];
+                    split_bf16(sum, p);
+                    char *to = t.sums + ((b >> 5) * static_cast<int64_t>(t.row_tiles) + tile) * kOffsetsBytes +
+                               ((b >> 4) & 1) * 3072 + (((b >> 3) & 1) * 32 + row) * 16 + 2 * (b & 7);
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) *reinterpret_cast<__bf16 *>(to + 1024 * i) = p[i];
+                }
+            }
+        }
+        return;
+    }
+    // Rows of pieces that hold 16 blocks wherever they begin, an odd number of
+    // them to spread the rows over the banks.
+    constexpr int kRow = LEAST ? 21 : 19;
+    constexpr int kRounds = (kRowsTile * kRow + kOperandThreads - 1) / kOperandThreads;
+    __shared__ __attribute__((aligned(16))) char lds[kRounds * kOperandThreads * 16];
+    const int strips = LEAST ? 2 * t.groups : (t.blocks + 15) / 16;
+    const int item = static_cast<int>(blockIdx.x) - t.x_groups;
+    const int tile = item / strips, b0 = item % strips * 16;
+    const int count = t.blocks - b0 < 16 ? t.blocks - b0 : 16;  // 0 and less: zeros of offsets only
+    const auto weights = [&](int r) {
+        const int64_t columns = GATED ? a.half : a.N;
+        const int64_t n = (GATED ? tile >> 1 : tile) * kRowsTile + r;
+        return a.w + ((n < columns ? n : columns - 1) + (GATED && (tile & 1) ? a.half : 0)) * a.row_bytes + b0 * kSize;
+    };
+    if (count > 0) {
+#pragma unroll
+        for (int i = 0; i < kRounds; ++i) {
+            const int slot = kOperandThreads * i + tid;
+            const int row = slot / kRow < kRowsTile ? slot / kRow : kRowsTile - 1;
+            const uint8_t *at = weights(row);
+            const int skip = static_cast<int>(reinterpret_cast<uintptr_t>(at) & 15);
+            const int piece = 16 * (slot - kRow * row), last = (skip + kSize * count - 1) & ~15;
+            fetch16(at - skip + (piece < last ? piece : last), lds_address(lds) + kOperandThreads * 16 * i + 1024 * wave);
+        }
+        fetched<0>();
+    }
+    lds_barrier();
+    const int col = lane & 31, h = lane >> 5;
+    const char *mine = lds + 16 * kRow * col + static_cast<int>(reinterpret_cast<uintptr_t>(weights(col)) & 15);
+    for (int i = wave; i < count; i += kOperandThreads / 64) {
+        const char *block = mine + kSize * i;
+        uint32_t w[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) __builtin_memcpy(&w[s], block + kSize - 16 + 8 * s + 4 * h, 4);
+        _Float16 d;
+        __builtin_memcpy(&d, block, 2);
+        char *to = t.words + ((b0 + i) * static_cast<int64_t>(t.column_tiles) + tile) * kWordsBytes;
+        *reinterpret_cast<uint2 *>(to + 8 * lane) = make_uint2(w[0], w[1]);
+        if (h == 0) *reinterpret_cast<float *>(to + 512 + 4 * col) = static_cast<float>(d);
+    }
+    if constexpr (LEAST) {
+        if (wave == 0) {
+            // Lane 32 h + row: the offsets of the strip's blocks 8 h .. 8 h + 7.
+            typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+            bf16x8 p[3];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int i = 8 * h + j;
+                float c = 0.0f;
+                if (i < count) {
+                    _Float16 d, least;
+                    __builtin_memcpy(&d, mine + kSize * i, 2);
+                    __builtin_memcpy(&least, mine + kSize * i + 2, 2);
+                    c = __builtin_fmaf(8.0f, static_cast<float>(d), static_cast<float>(least));
+                }
+                __bf16 q[3];
+                split_bf16(c, q);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) p[k][j] = q[k];
+            }
+            char *to = t.offsets + ((b0 >> 5) * static_cast<int64_t>(t.column_tiles) + tile) * kOffsetsBytes +
+                       ((b0 >> 4) & 1) * 3072 + 16 * lane;
+#pragma unroll
+            for (int k = 0; k < 3; ++k) *reinterpret_cast<bf16x8 *>(to + 1024 * k) = p[k];
+        }
+    }
+}
+
+// Tiles of 64 WM rows of x by 64 WN of the weights, a wave 64 x 64 of them and
+// one block of every WK: 16 v_mfma_f32_32x32x16_f16 a block.  The operands of
+// WK blocks come into LDS in runs, three stages of them in turn, asked for two
+// stages ahead.  A block's sums of products are scaled by d, 64 operations
+// beside the 36 that widen the words: 464 of the vector units' cycles a block
+// to 512 of the MFMA's.
+template <int WM, int WN, int WK>
+struct Tiles {
+    static constexpr int kWaves = WM * WN * WK;
+    static constexpr int kThreads = 64 * kWaves;
+    static constexpr int kNumbers = WM * 2 * 4;                   // KB a block
+    static constexpr int kWords = (WN * 2 * kWordsBytes + 1023) / 1024;  // KB a block, rounded up
+    static constexpr int kPerBlock = kNumbers + kWords;
+    static constexpr int kStage = WK * kPerBlock * 1024;
+    static constexpr int kCopies = (WK * kPerBlock + kWaves - 1) / kWaves;  // a wave's, a stage
+    static constexpr int kStages = 3;
+    static constexpr int kLds = kStages * kStage > (WK > 1 ? kWaves * 16384 : 0) ? kStages * kStage : kWaves * 16384;
+};
+
+template <bool LEAST, bool GATED, int WM, int WN, int WK>
+__global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs t) {
+    using L = Tiles<WM, WN, WK>;
+    const Q4Args &a = t.a;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wk = wave % WK, wn = wave / WK % WN, wm = wave / (WK * WN);
+    const uint32_t at = xcd_swizzle(blockIdx.x, gridDim.x);
+    const int mb = at / t.n_blocks, nb = at - mb * t.n_blocks;
+    const int stages = (t.blocks + WK - 1) / WK;
+    const int64_t numbers_step = t.row_tiles * kNumbersBytes, words_step = t.column_tiles * kWordsBytes;
+    const char *numbers = t.numbers + mb * (WM * 2) * kNumbersBytes + 16 * lane;
+    const char *words = t.words + nb * (WN * 2) * kWordsBytes + 16 * lane;
+    const uint32_t base = lds_address(lds);
+    const auto copy_stage = [&](int s, int buffer) {
+#pragma unroll
+        for (int c = 0; c < L::kCopies; ++c) {
+            int q = wave * L::kCopies + c;
+            q = q < WK * L::kPerBlock ? q : WK * L::kPerBlock - 1;
+            const int k = q / L::kPerBlock, r = q - k * L::kPerBlock;
+            const int64_t b = s * WK + k < t.blocks ? s * WK + k : t.blocks - 1;
+            fetch16(r < L::kNumbers ? numbers + b * numbers_step + 1024 * r
+                                    : words + b * words_step + 1024 * (r - L::kNumbers),
+                    base + buffer * L::kStage + 1024 * q);
+        }
+    };
+    float16v acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = float16v{};
+    copy_stage(0, 0);
+    if (stages > 1) copy_stage(1, 1);
+    const uint32_t magic = opaque(kMagic);
+    const char *x = lds + wk * (L::kPerBlock * 1024) + wm * 8192 + 16 * lane;
+    const char *w = lds + wk * (L::kPerBlock * 1024) + L::kNumbers * 1024 + wn * 2 * static_cast<int>(kWordsBytes);
+    int buffer = 0;
+    for (int s = 0; s < stages; ++s) {
+        if (s + 1 < stages) {
+            fetched<L::kCopies>();
+        } else {
+            fetched<0>();
+        }
+        lds_barrier();  // every wave's copies of this stage are in, and the stage before is read
+        if (s + 2 < stages) copy_stage(s + 2, buffer == 0 ? 2 : buffer - 1);
+        if (s * WK + wk < t.blocks) {
+            const char *xs = x + buffer * L::kStage, *ws = w + buffer * L::kStage;
+            half8 n[2][2][2];  // [32 rows][half of the block][hi, lo]
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int p = 0; p < 4; ++p) n[i][p >> 1][p & 1] = *reinterpret_cast<const half8 *>(xs + 4096 * i + 1024 * p);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint2 pair = *reinterpret_cast<const uint2 *>(ws + kWordsBytes * j + 8 * lane);
+                const float d = *reinterpret_cast<const float *>(ws + kWordsBytes * j + 512 + 4 * (lane & 31));
+                const half8 v[2] = {widen(pair.x, magic), widen(pair.y, magic)};
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float16v p = __builtin_amdgcn_mfma_f32_32x32x16_f16(n[i][0][1], v[0], float16v{}, 0, 0, 0);
+                    p = __builtin_amdgcn_mfma_f32_32x32x16_f16(n[i][1][1], v[1], p, 0, 0, 0);
+                    p = __builtin_amdgcn_mfma_f32_32x32x16_f16(n[i][0][0], v[0], p, 0, 0, 0);
+                    p = __builtin_amdgcn_mfma_f32_32x32x16_f16(n[i][1][0], v[1], p, 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_fmaf(d, p[e], acc[i][j][e]);
+                }
+            }
+        }
+        buffer = buffer == 2 ? 0 : buffer + 1;
+    }
+    if constexpr (LEAST) {
+        typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+        for (int g = wk; g < t.groups; g += WK) {
+            const char *sums = t.sums + (g * static_cast<int64_t>(t.row_tiles) + mb * (WM * 2) + wm * 2) * kOffsetsBytes + 16 * lane;
+            const char *offs = t.offsets + (g * static_cast<int64_t>(t.column_tiles) + nb * (WN * 2) + wn * 2) * kOffsetsBytes + 16 * lane;
+#pragma unroll 1
+            for (int s = 0; s < 2; ++s) {
+                bf16x8 u[2][3], v[2][3];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) {
+                        u[i][p] = *reinterpret_cast<const bf16x8 *>(sums + i * kOffsetsBytes + 3072 * s + 1024 * p);
+                        v[i][p] = *reinterpret_cast<const bf16x8 *>(offs + i * kOffsetsBytes + 3072 * s + 1024 * p);
+                    }
+                // The parts' products down to 2^-16 of the whole, the least first.
+#pragma unroll
+                for (int total = 2; total >= 0; --total)
+#pragma unroll
+                    for (int p = 0; p <= total; ++p)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)
+                                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[i][p], v[j][total - p], acc[i][j], 0, 0, 0);
+            }
+        }
+    }
+    // The outputs, 8 rows of both columns of 32 a time: quarter q of a wave's,
+    // rows 16 (q % 2) + .. of its 32 q / 2; the waves of WK blocks take a part
+    // of the quarters each, and add up what the others have of them.
+    const int m0 = mb * (64 * WM) + wm * 64, n0 = GATED ? nb * (32 * WN) + wn * 32 : nb * (64 * WN) + wn * 64;
+    const int64_t columns = GATED ? a.half : a.N;
+    const int col = lane & 31, h = lane >> 5;
+    const auto write = [&](int i, int half, float (&v)[2][8]) {
+        int m[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            m[e] = m0 + 32 * i + tile_row(8 * half + e) + 4 * h;
+            const float back = t.back[m[e]];
+            v[0][e] *= back;
+            v[1][e] *= back;
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            int64_t n = GATED ? n0 + col : n0 + 32 * j + col;
+            const bool real = n < columns;
+            n = (real ? n : columns - 1) + (GATED && j ? a.half : 0);
+            if (!GATED && a.from_redirect) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (real && m[e] < a.M) v[j][e] = a.y[m[e] * a.ldy + n] + v[j][e];
+            }
+            apply_chain_rows(a, v[j], m, n);
+            if (!GATED) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (real && m[e] < a.M) a.y[m[e] * a.ldy + n] = v[j][e];
+            }
+        }
+        if (GATED && n0 + col < columns) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (m[e] < a.M) a.y[m[e] * a.ldy + n0 + col] = v[0][e] * gelu(v[1][e]);
+        }
+    };
+    if constexpr (WK == 1) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float v[2][8];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[j][e] = acc[q >> 1][j][8 * (q & 1) + e];
+            write(q >> 1, q & 1, v);
+        }
+    } else {
+        lds_barrier();  // the last stage is read
+        float *sums = reinterpret_cast<float *>(lds) + wave * 4096 + lane;  // [quarter][j][e][lane]
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sums[((q * 2 + j) * 8 + e) * 64] = acc[q >> 1][j][8 * (q & 1) + e];
+        lds_barrier();
+        const float *all = reinterpret_cast<const float *>(lds) + (wave - wk) * 4096 + lane;
+#pragma unroll 1
+        for (int q = wk; q < 4; q += WK) {
+            float v[2][8];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float s = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < WK; ++k) s += all[k * 4096 + ((q * 2 + j) * 8 + e) * 64];
+                    v[j][e] = s;
+                }
+            write(q >> 1, q & 1, v);
+        }
+    }
+}
+
+template <bool LEAST, bool GATED, int WM, int WN, int WK>
+hipError_t launch_tiles(TileArgs t, hipStream_t stream) {
+    using L = Tiles<WM, WN, WK>;
+    static const hipError_t attr =
+        hipFuncSetAttribute(reinterpret_cast<const void *>(&q4_tiles_kernel<LEAST, GATED, WM, WN, WK>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, L::kLds);
+    if (attr != hipSuccess) return attr;
+    t.m_blocks = static_cast<int32_t>(ceil_div(t.a.M, 64 * WM));
+    t.n_blocks = static_cast<int32_t>(GATED ? ceil_div(t.a.half, 32 * WN) : ceil_div(t.a.N, 64 * WN));
+    SDHIP_LAUNCH((q4_tiles_kernel<LEAST, GATED, WM, WN, WK>), dim3(static_cast<uint32_t>(t.m_blocks * t.n_blocks)),
+                 dim3(L::kThreads), L::kLds, stream, t);
+    return hipGetLastError();
+}
+
+// The work buffer's parts.
+struct TilesWork {
+    size_t numbers, words, back, sums, offsets, bytes;
+    int64_t row_tiles, column_tiles, blocks, groups;
+};
+
+TilesWork tiles_work(int64_t M, int64_t N, int64_t half, int64_t K, bool least) {
+    TilesWork w{};
+    // Whole workgroups' tiles, whichever shape is taken: up to 128 rows by 256.
+    w.row_tiles = round_up(ceil_div(M, kRowsTile), 4);
+    w.column_tiles = round_up(half ? 2 * ceil_div(half, kRowsTile) : ceil_div(N, kRowsTile), 8);
+    w.blocks = K / kBlock;
+    w.groups = least ? ceil_div(w.blocks, 32) : 0;
+    size_t at = 0;
+    const auto take = [&](int64_t bytes) {
+        const size_t from = at;
+        at += static_cast<size_t>(round_up(bytes, 256));
+        return from;
+    };
+    w.numbers = take(w.blocks * w.row_tiles * kNumbersBytes);
+    w.words = take(w.blocks * w.column_tiles * kWordsBytes + 1024);  // the last run's copies end past it
+    w.back = take(w.row_tiles * kRowsTile * 4);
+    w.sums = take(w.groups * w.row_tiles * kOffsetsBytes);
+    w.offsets = take(w.groups * w.column_tiles * kOffsetsBytes);
+    w.bytes = at;
+    return w;
+}
+
+template <bool LEAST, bool GATED>
+hipError_t many_rows(const Q4Args &a, void *work, hipStream_t stream) {
+    const TilesWork w = tiles_work(a.M, a.N, a.half, a.K, LEAST);
+    TileArgs t{};
+    t.a = a;
+    char *p = static_cast<char *>(work);
+    t.numbers = p + w.numbers;
+    t.words = p + w.words;
+    t.back = reinterpret_cast<float *>(p + w.back);
+    t.sums = p + w.sums;
+    t.offsets = p + w.offsets;
+    t.blocks = static_cast<int32_t>(w.blocks);
+    t.groups = static_cast<int32_t>(w.groups);
+    t.row_tiles = static_cast<int32_t>(w.row_tiles);
+    t.column_tiles = static_cast<int32_t>(w.column_tiles);
+    t.x_groups = static_cast<int32_t>(ceil_div(a.M, 4));
+    const int64_t tiles = GATED ? 2 * ceil_div(a.half, kRowsTile) : ceil_div(a.N, kRowsTile);
+    const int64_t strips = LEAST ? 2 * w.groups : ceil_div(w.blocks, 16);
+    SDHIP_LAUNCH((q4_operands_kernel<LEAST, GATED>), dim3(static_cast<uint32_t>(t.x_groups + tiles * strips)),
+                 dim3(kOperandThreads), 0, stream, t);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    // The shape whose workgroups take the fewest stages one after another on
+    // a CU, the larger where that is alike; sums split over waves cost about 4
+    // stages more to add up.
+    const int64_t cus = compute_units(), columns = 2 * (GATED ? a.half : a.N / 2 + a.N % 2);
+    const auto cost = [&](int rows, int cols, int split) {
+        return ceil_div(ceil_div(a.M, rows) * ceil_div(columns, cols), cus) * (ceil_div(w.blocks, split) + 4) + (split > 1 ? 4 : 0);
+    };
+    const int64_t c0 = cost(128, 256, 1), c1 = cost(128, 128, 2), c2 = cost(64, 128, 4);
+    if (c0 <= c1 && c0 <= c2) return launch_tiles<LEAST, GATED, 2, 4, 1>(t, stream);
+    if (c1 <= c2) return launch_tiles<LEAST, GATED, 2, 2, 2>(t, stream);
+    return launch_tiles<LEAST, GATED, 1, 2, 4>(t, stream);
+}
+
+// Up to 16 rows go through q4_few_kernel, which needs no work buffer.
+bool few(int64_t rows) { return rows <= 16; }
+
 }  // namespace
 
-hipError_t launch_q4_mul_mat(const Q4Args &a, hipStream_t stream) {
+size_t q4_work_size(int64_t M, int64_t N, int64_t K, bool least) {
+    if (few(M)) return 0;
+    // The plain and the gated product of one size take one size of buffer.
+    const size_t plain = tiles_work(M, N, 0, K, least).bytes;
+    const size_t gated = N % 2 == 0 ? tiles_work(M, N, N / 2, K, least).bytes : 0;
+    return plain > gated ? plain : gated;
+}
+
+hipError_t launch_q4_mul_mat(const Q4Args &a, void *work, hipStream_t stream) {
     KernelScope scope(a.half ? "q4.gated" : "q4", stream);
-    if (a.half) return a.least ? few_rows<true, true>(a, stream) : few_rows<false, true>(a, stream);
-    return a.least ? few_rows<true, false>(a, stream) : few_rows<false, false>(a, stream);
+    if (few(a.M)) {
+        if (a.half) return a.least ? few_rows<true, true>(a, stream) : few_rows<false, true>(a, stream);
+        return a.least ? few_rows<true, false>(a, stream) : few_rows<false, false>(a, stream);
+    }
+    if (a.half) return a.least ? many_rows<true, true>(a, work, stream) : many_rows<false, true>(a, work, stream);
+    return a.least ? many_rows<true, false>(a, work, stream) : many_rows<false, false>(a, work, stream);
 }
 
 }  // namespace sdhip

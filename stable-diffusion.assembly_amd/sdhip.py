@@ -223,6 +223,7 @@ def epilogue(steps=(), redirect=None, from_redirect=False):
     """steps: ('add'|'mul', tensor) or ('silu', None); redirect: a torch tensor."""
     e = Epilogue()
     e.count = len(steps)
+    e._held = [operand for _, operand in steps] + [redirect]  # kept alive with the epilogue
     kinds = {"add": STEP_ADD, "mul": STEP_MUL, "silu": STEP_SILU}
     for i, (kind, operand) in enumerate(steps):
         e.steps[i].kind = kinds[kind]
