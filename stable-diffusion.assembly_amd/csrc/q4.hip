@@ -113,18 +113,6 @@ __device__ __forceinline__ uint32_t magnitude(const float4v &v) {
     return m;
 }
 
-// The chain over 8 rows m[e] (those past M as the last) of column n.
-__device__ __forceinline__ void apply_chain_rows(const Q4Args &a, float (&v)[8], const int (&m)[8], int64_t n) {
-    apply_chain_block(a.chain, v, [&](int s, int e) {
-        const DevStep &st = a.chain.steps[s];
-        const int64_t row = m[e] < a.M ? m[e] : a.M - 1;
-        if (st.flat123) return n * st.nb[0] + row * st.nb[1];
-        uint32_t i1, i2, i3;
-        split_index(static_cast<uint32_t>(row), static_cast<uint32_t>(a.ne1), static_cast<uint32_t>(a.ne2), i1, i2, i3);
-        return n * st.nb[0] + i1 * st.nb[1] + i2 * st.nb[2] + i3 * st.nb[3];
-    });
-}
-
 // ------------------------------------------------------------------ copies
 
 // A copy of 16 bytes a lane (1 KB) or 4 into LDS at `to` and on, lane after
@@ -139,6 +127,12 @@ __device__ __forceinline__ void fetch16(const void *from, uint32_t to) {
 __device__ __forceinline__ void fetch4(const void *from, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(to)),
                  "v"(from)
+                 : "memory");
+}
+
+// fetch16 from an address the wave's lanes share and an offset of each.
+__device__ __forceinline__ void fetch16(const char *from, uint32_t offset, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(from)
                  : "memory");
 }
 
@@ -650,8 +644,8 @@ struct Tiles {
     static constexpr int kNumbers = WM * 2 * 4;                   // KB a block
     static constexpr int kWords = (WN * 2 * kWordsBytes + 1023) / 1024;  // KB a block, rounded up
     static constexpr int kPerBlock = kNumbers + kWords;
-    static constexpr int kStage = WK * kPerBlock * 1024;
     static constexpr int kCopies = (WK * kPerBlock + kWaves - 1) / kWaves;  // a wave's, a stage
+    static constexpr int kStage = kCopies * kWaves * 1024;
     static constexpr int kStages = 3;
     static constexpr int kLds = kStages * kStage > (WK > 1 ? kWaves * 16384 : 0) ? kStages * kStage : kWaves * 16384;
 };
@@ -666,144 +660,172 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs
     const uint32_t at = xcd_swizzle(blockIdx.x, gridDim.x);
     const int mb = at / t.n_blocks, nb = at - mb * t.n_blocks;
     const int stages = (t.blocks + WK - 1) / WK;
-    const int64_t numbers_step = t.row_tiles * kNumbersBytes, words_step = t.column_tiles * kWordsBytes;
-    const char *numbers = t.numbers + mb * (WM * 2) * kNumbersBytes + 16 * lane;
-    const char *words = t.words + nb * (WN * 2) * kWordsBytes + 16 * lane;
-    const uint32_t base = lds_address(lds);
-    const auto copy_stage = [&](int s, int buffer) {
+    // A wave's copies of a stage: kCopies KB of its WK kPerBlock, the last ones
+    // perhaps again.  A block past the last is the last.
+    const char *from[L::kCopies];
+    int64_t step[L::kCopies];
+    int block[L::kCopies];
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(lds) + 1024 * wave * L::kCopies);
 #pragma unroll
-        for (int c = 0; c < L::kCopies; ++c) {
-            int q = wave * L::kCopies + c;
-            q = q < WK * L::kPerBlock ? q : WK * L::kPerBlock - 1;
-            const int k = q / L::kPerBlock, r = q - k * L::kPerBlock;
-            const int64_t b = s * WK + k < t.blocks ? s * WK + k : t.blocks - 1;
-            fetch16(r < L::kNumbers ? numbers + b * numbers_step + 1024 * r
-                                    : words + b * words_step + 1024 * (r - L::kNumbers),
-                    base + buffer * L::kStage + 1024 * q);
-        }
+    for (int c = 0; c < L::kCopies; ++c) {
+        int q = wave * L::kCopies + c;
+        q = q < WK * L::kPerBlock ? q : WK * L::kPerBlock - 1;
+        const int r = q % L::kPerBlock;
+        block[c] = q / L::kPerBlock;
+        from[c] = r < L::kNumbers ? t.numbers + mb * (WM * 2) * kNumbersBytes + 1024 * r
+                                  : t.words + nb * (WN * 2) * kWordsBytes + 1024 * (r - L::kNumbers);
+        step[c] = r < L::kNumbers ? t.row_tiles * kNumbersBytes : t.column_tiles * kWordsBytes;
+    }
+    const auto copy = [&](int s, int buffer, int c) {
+        const int b = s * WK + block[c] < t.blocks ? s * WK + block[c] : t.blocks - 1;
+        fetch16(from[c] + b * step[c], 16 * lane, to + buffer * L::kStage + 1024 * c);
     };
+#pragma unroll
+    for (int s = 0; s < 3; ++s)
+#pragma unroll
+        for (int c = 0; c < L::kCopies; ++c) copy(s, s, c);
     float16v acc[2][2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc[i][j] = float16v{};
-    copy_stage(0, 0);
-    if (stages > 1) copy_stage(1, 1);
     const uint32_t magic = opaque(kMagic);
     const char *x = lds + wk * (L::kPerBlock * 1024) + wm * 8192 + 16 * lane;
     const char *w = lds + wk * (L::kPerBlock * 1024) + L::kNumbers * 1024 + wn * 2 * static_cast<int>(kWordsBytes);
-    int buffer = 0;
-    for (int s = 0; s < stages; ++s) {
-        if (s + 1 < stages) {
-            fetched<L::kCopies>();
-        } else {
-            fetched<0>();
+    struct Operands {
+        half8 n[2][2][2];  // [32 rows][half of the block][hi, lo]
+        half8 v[2][2];     // [32 rows of the weights][half of the block]
+        float d[2];
+    };
+    const auto read = [&](Operands &o, int buffer) {
+        const char *xs = x + buffer * L::kStage, *ws = w + buffer * L::kStage;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int p = 0; p < 4; ++p) o.n[i][p >> 1][p & 1] = *reinterpret_cast<const half8 *>(xs + 4096 * i + 1024 * p);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint2 pair = *reinterpret_cast<const uint2 *>(ws + kWordsBytes * j + 8 * lane);
+            o.d[j] = *reinterpret_cast<const float *>(ws + kWordsBytes * j + 512 + 4 * (lane & 31));
+            o.v[j][0] = widen(pair.x, magic);
+            o.v[j][1] = widen(pair.y, magic);
         }
-        lds_barrier();  // every wave's copies of this stage are in, and the stage before is read
-        if (s + 2 < stages) copy_stage(s + 2, buffer == 0 ? 2 : buffer - 1);
-        if (s * WK + wk < t.blocks) {
-            const char *xs = x + buffer * L::kStage, *ws = w + buffer * L::kStage;
-            half8 n[2][2][2];  // [32 rows][half of the block][hi, lo]
+    };
+    const auto product = [&](const Operands &o, int i, int j) {
+        float16v p = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.n[i][0][1], o.v[j][0], float16v{}, 0, 0, 0);
+        p = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.n[i][1][1], o.v[j][1], p, 0, 0, 0);
+        p = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.n[i][0][0], o.v[j][0], p, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(o.n[i][1][0], o.v[j][1], p, 0, 0, 0);
+    };
+    const auto add = [&](int i, int j, float d, const float16v &p) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_fmaf(d, p[e], acc[i][j][e]);
+    };
+    // A block's four products; a product's sums are added up while the MFMA
+    // makes the next one's, the last's in the next block.
+    float16v kept = float16v{};
+    float kept_d = 0.0f;
+    const auto multiply = [&](const Operands &o, auto between) {
+        const float16v p00 = product(o, 0, 0);
+        between(0);
+        add(1, 1, kept_d, kept);
+        const float16v p10 = product(o, 1, 0);
+        between(1);
+        add(0, 0, o.d[0], p00);
+        const float16v p01 = product(o, 0, 1);
+        between(2);
+        add(1, 0, o.d[0], p10);
+        kept = product(o, 1, 1);
+        between(3);
+        add(0, 1, o.d[1], p01);
+        kept_d = o.d[1];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
+        }
+    };
+    fetched<2 * L::kCopies>();
+    lds_barrier();
+    Operands even, odd;
+    read(even, 0);
+    int buffer = 0;
+    // Stage s is multiplied from registers while stage s + 1 is read into
+    // others; s + 2 is under way and s + 3 takes the buffer that s was read
+    // from -- for the last stages, the last one again.
+    const auto stage = [&](int s, const Operands &now, Operands &next) {
+        fetched<L::kCopies>();
+        lds_barrier();  // every wave's copies of stage s + 1 are in, and stage s is read
+        const int free = buffer;
+        buffer = buffer == 2 ? 0 : buffer + 1;
+        multiply(now, [&](int k) {
+            if (k == 0) read(next, buffer);
+#pragma unroll
+            for (int c = 0; c < L::kCopies; ++c)
+                if (c * 4 / L::kCopies == k) copy(s + 3, free, c);
+        });
+    };
+    int s = 0;
+#pragma unroll 1
+    for (; s + 2 < stages; s += 2) {
+        stage(s, even, odd);
+        stage(s + 1, odd, even);
+    }
+    if (s + 1 < stages) {
+        stage(s, even, odd);
+        even = odd;
+        ++s;
+    }
+    if (s * WK + wk < t.blocks) multiply(even, [](int) {});
+    add(1, 1, kept_d, kept);
+    fetched<0>();
+    if constexpr (LEAST) {
+        typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+        struct Parts {
+            bf16x8 u[2][3], v[2][3];
+        };
+        // Step k: 16 blocks, half k % 2 of the wave's group k / 2.
+        const int steps = wk < t.groups ? 2 * ((t.groups - wk + WK - 1) / WK) : 0;
+        const auto load = [&](int k, Parts &o) {
+            const int64_t g = wk + (k >> 1) * WK;
+            const char *sums = t.sums + (g * t.row_tiles + mb * (WM * 2) + wm * 2) * kOffsetsBytes + 3072 * (k & 1) + 16 * lane;
+            const char *offs = t.offsets + (g * t.column_tiles + nb * (WN * 2) + wn * 2) * kOffsetsBytes + 3072 * (k & 1) + 16 * lane;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int p = 0; p < 4; ++p) n[i][p >> 1][p & 1] = *reinterpret_cast<const half8 *>(xs + 4096 * i + 1024 * p);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint2 pair = *reinterpret_cast<const uint2 *>(ws + kWordsBytes * j + 8 * lane);
-                const float d = *reinterpret_cast<const float *>(ws + kWordsBytes * j + 512 + 4 * (lane & 31));
-                const half8 v[2] = {widen(pair.x, magic), widen(pair.y, magic)};
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float16v p = __builtin_amdgcn_mfma_f32_32x32x16_f16(n[i][0][1], v[0], float16v{}, 0, 0, 0);
-                    p = __builtin_amdgcn_mfma_f32_32x32x16_f16(n[i][1][1], v[1], p, 0, 0, 0);
-                    p = __builtin_amdgcn_mfma_f32_32x32x16_f16(n[i][0][0], v[0], p, 0, 0, 0);
-                    p = __builtin_amdgcn_mfma_f32_32x32x16_f16(n[i][1][0], v[1], p, 0, 0, 0);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_fmaf(d, p[e], acc[i][j][e]);
+                for (int p = 0; p < 3; ++p) {
+                    o.u[i][p] = *reinterpret_cast<const bf16x8 *>(sums + i * kOffsetsBytes + 1024 * p);
+                    o.v[i][p] = *reinterpret_cast<const bf16x8 *>(offs + i * kOffsetsBytes + 1024 * p);
                 }
-            }
-        }
-        buffer = buffer == 2 ? 0 : buffer + 1;
-    }
-    if constexpr (LEAST) {
-        typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-        for (int g = wk; g < t.groups; g += WK) {
-            const char *sums = t.sums + (g * static_cast<int64_t>(t.row_tiles) + mb * (WM * 2) + wm * 2) * kOffsetsBytes + 16 * lane;
-            const char *offs = t.offsets + (g * static_cast<int64_t>(t.column_tiles) + nb * (WN * 2) + wn * 2) * kOffsetsBytes + 16 * lane;
+        };
+        // The parts' products down to 2^-16 of the whole, the least first.
+        const auto multiply_parts = [&](const Parts &o) {
+#pragma unroll
+            for (int total = 2; total >= 0; --total)
+#pragma unroll
+                for (int p = 0; p <= total; ++p)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(o.u[i][p], o.v[j][total - p], acc[i][j], 0, 0, 0);
+        };
+        Parts a0, a1;
+        if (steps > 0) load(0, a0);
 #pragma unroll 1
-            for (int s = 0; s < 2; ++s) {
-                bf16x8 u[2][3], v[2][3];
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int p = 0; p < 3; ++p) {
-                        u[i][p] = *reinterpret_cast<const bf16x8 *>(sums + i * kOffsetsBytes + 3072 * s + 1024 * p);
-                        v[i][p] = *reinterpret_cast<const bf16x8 *>(offs + i * kOffsetsBytes + 3072 * s + 1024 * p);
-                    }
-                // The parts' products down to 2^-16 of the whole, the least first.
-#pragma unroll
-                for (int total = 2; total >= 0; --total)
-#pragma unroll
-                    for (int p = 0; p <= total; ++p)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-#pragma unroll
-                            for (int j = 0; j < 2; ++j)
-                                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[i][p], v[j][total - p], acc[i][j], 0, 0, 0);
-            }
+        for (int k = 0; k < steps; k += 2) {
+            load(k + 1, a1);
+            multiply_parts(a0);
+            if (k + 2 < steps) load(k + 2, a0);
+            multiply_parts(a1);
         }
     }
-    // The outputs, 8 rows of both columns of 32 a time: quarter q of a wave's,
-    // rows 16 (q % 2) + .. of its 32 q / 2; the waves of WK blocks take a part
-    // of the quarters each, and add up what the others have of them.
-    const int m0 = mb * (64 * WM) + wm * 64, n0 = GATED ? nb * (32 * WN) + wn * 32 : nb * (64 * WN) + wn * 64;
-    const int64_t columns = GATED ? a.half : a.N;
-    const int col = lane & 31, h = lane >> 5;
-    const auto write = [&](int i, int half, float (&v)[2][8]) {
-        int m[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            m[e] = m0 + 32 * i + tile_row(8 * half + e) + 4 * h;
-            const float back = t.back[m[e]];
-            v[0][e] *= back;
-            v[1][e] *= back;
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            int64_t n = GATED ? n0 + col : n0 + 32 * j + col;
-            const bool real = n < columns;
-            n = (real ? n : columns - 1) + (GATED && j ? a.half : 0);
-            if (!GATED && a.from_redirect) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (real && m[e] < a.M) v[j][e] = a.y[m[e] * a.ldy + n] + v[j][e];
-            }
-            apply_chain_rows(a, v[j], m, n);
-            if (!GATED) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (real && m[e] < a.M) a.y[m[e] * a.ldy + n] = v[j][e];
-            }
-        }
-        if (GATED && n0 + col < columns) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (m[e] < a.M) a.y[m[e] * a.ldy + n0 + col] = v[0][e] * gelu(v[1][e]);
-        }
-    };
-    if constexpr (WK == 1) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            float v[2][8];
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[j][e] = acc[q >> 1][j][8 * (q & 1) + e];
-            write(q >> 1, q & 1, v);
-        }
-    } else {
-        lds_barrier();  // the last stage is read
+    // The outputs by quarters of the wave's, 8 rows a lane of both its columns:
+    // rows 16 (q % 2) .. of its 32 q / 2.  The waves of WK blocks add up a part
+    // of the quarters each; a wave alone takes one or two at a time.
+    constexpr int kQuarters = WK == 4 || (WK == 1 && GATED) ? 1 : 2;
+    if constexpr (WK > 1) {
+        lds_barrier();  // the last stage is read, and no copy is under way
         float *sums = reinterpret_cast<float *>(lds) + wave * 4096 + lane;  // [quarter][j][e][lane]
 #pragma unroll
         for (int q = 0; q < 4; ++q)
@@ -812,21 +834,117 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs
 #pragma unroll
                 for (int e = 0; e < 8; ++e) sums[((q * 2 + j) * 8 + e) * 64] = acc[q >> 1][j][8 * (q & 1) + e];
         lds_barrier();
-        const float *all = reinterpret_cast<const float *>(lds) + (wave - wk) * 4096 + lane;
-#pragma unroll 1
-        for (int q = wk; q < 4; q += WK) {
-            float v[2][8];
+    }
+    const float *all = reinterpret_cast<const float *>(lds) + (wave - wk) * 4096 + lane;
+    const int64_t columns = GATED ? a.half : a.N;
+    const int m0 = mb * (64 * WM) + wm * 64 + 4 * (lane >> 5), n0 = nb * (GATED ? 32 * WN : 64 * WN) + wn * (GATED ? 32 : 64) + (lane & 31);
+#pragma unroll
+    for (int round = 0; round < 4 / WK / kQuarters; ++round) {
+        const int q0 = WK == 1 ? kQuarters * round : wk * kQuarters;
+        float v[kQuarters][2][8];
+#pragma unroll
+        for (int q = 0; q < kQuarters; ++q)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    float s = 0.0f;
+                    if constexpr (WK == 1) {
+                        v[q][j][e] = acc[(kQuarters * round + q) >> 1][j][8 * ((kQuarters * round + q) & 1) + e];
+                    } else {
+                        v[q][j][e] = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < WK; ++k) s += all[k * 4096 + ((q * 2 + j) * 8 + e) * 64];
-                    v[j][e] = s;
+                        for (int k = 0; k < WK; ++k) v[q][j][e] += all[k * 4096 + (((q0 + q) * 2 + j) * 8 + e) * 64];
+                    }
                 }
-            write(q >> 1, q & 1, v);
+        const auto row_of = [&](int q, int e) { return m0 + 16 * (q0 + q) + tile_row(e); };
+        const auto column_of = [&](int j) -> int64_t {  // j's column, or the last there is
+            const int64_t n = GATED ? n0 : n0 + 32 * j;
+            return (n < columns ? n : columns - 1) + (GATED && j ? a.half : 0);
+        };
+        const int64_t last = a.M - 1;
+#pragma unroll
+        for (int q = 0; q < kQuarters; ++q)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float back = t.back[row_of(q, e)];
+                v[q][0][e] *= back;
+                v[q][1][e] *= back;
+            }
+        if (!GATED && a.from_redirect) {
+#pragma unroll
+            for (int q = 0; q < kQuarters; ++q)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int64_t m = row_of(q, e) < last ? row_of(q, e) : last;
+                        v[q][j][e] = a.y[m * a.ldy + column_of(j)] + v[q][j][e];
+                    }
         }
+        // The chain, a step's operands all asked for before one is used.
+#pragma unroll 1
+        for (int c = 0; c < a.chain.count; ++c) {
+            const DevStep &st = a.chain.steps[c];
+            if (st.kind == kSilu) {
+#pragma unroll
+                for (int q = 0; q < kQuarters; ++q)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[q][j][e] = silu(v[q][j][e]);
+                continue;
+            }
+            float o[kQuarters][2][8];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float *at = st.operand + column_of(j) * st.nb[0];
+                if (st.flat123 && st.nb[1] == 0) {
+                    const float one = *at;
+#pragma unroll
+                    for (int q = 0; q < kQuarters; ++q)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) o[q][j][e] = one;
+                } else if (st.flat123) {
+#pragma unroll
+                    for (int q = 0; q < kQuarters; ++q)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            o[q][j][e] = at[(row_of(q, e) < last ? row_of(q, e) : last) * st.nb[1]];
+                } else {
+#pragma unroll
+                    for (int q = 0; q < kQuarters; ++q)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int64_t m = row_of(q, e) < last ? row_of(q, e) : last;
+                            uint32_t i1, i2, i3;
+                            split_index(static_cast<uint32_t>(m), static_cast<uint32_t>(a.ne1), static_cast<uint32_t>(a.ne2),
+                                        i1, i2, i3);
+                            o[q][j][e] = at[i1 * st.nb[1] + i2 * st.nb[2] + i3 * st.nb[3]];
+                        }
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < kQuarters; ++q)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        v[q][j][e] = st.kind == kAdd ? __fadd_rn(v[q][j][e], o[q][j][e]) : __fmul_rn(v[q][j][e], o[q][j][e]);
+        }
+#pragma unroll
+        for (int q = 0; q < kQuarters; ++q)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int64_t m = row_of(q, e);
+                if (m > last) continue;
+                float *y = a.y + m * a.ldy;
+                if (GATED) {
+                    if (n0 < columns) y[n0] = v[q][0][e] * gelu(v[q][1][e]);
+                } else {
+                    if (n0 < columns) y[n0] = v[q][0][e];
+                    if (n0 + 32 < columns) y[n0 + 32] = v[q][1][e];
+                }
+            }
     }
 }
 
