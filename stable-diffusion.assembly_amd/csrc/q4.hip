@@ -650,6 +650,18 @@ struct Tiles {
     static constexpr int kLds = kStages * kStage > (WK > 1 ? kWaves * 16384 : 0) ? kStages * kStage : kWaves * 16384;
 };
 
+// The order of what was written since the last sched_barrier: four MFMAs, N
+// vector operations after each.
+template <int N>
+__device__ __forceinline__ void mixed() {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, N, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 template <bool LEAST, bool GATED, int WM, int WN, int WK>
 __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs t) {
     using L = Tiles<WM, WN, WK>;
@@ -695,6 +707,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs
     struct Operands {
         half8 n[2][2][2];  // [32 rows][half of the block][hi, lo]
         half8 v[2][2];     // [32 rows of the weights][half of the block]
+        uint2 words[2];    // v before it is widened
         float d[2];
     };
     const auto read = [&](Operands &o, int buffer) {
@@ -705,11 +718,13 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs
             for (int p = 0; p < 4; ++p) o.n[i][p >> 1][p & 1] = *reinterpret_cast<const half8 *>(xs + 4096 * i + 1024 * p);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const uint2 pair = *reinterpret_cast<const uint2 *>(ws + kWordsBytes * j + 8 * lane);
+            o.words[j] = *reinterpret_cast<const uint2 *>(ws + kWordsBytes * j + 8 * lane);
             o.d[j] = *reinterpret_cast<const float *>(ws + kWordsBytes * j + 512 + 4 * (lane & 31));
-            o.v[j][0] = widen(pair.x, magic);
-            o.v[j][1] = widen(pair.y, magic);
         }
+    };
+    const auto widen_words = [&](Operands &o, int j) {
+        o.v[j][0] = widen(o.words[j].x, magic);
+        o.v[j][1] = widen(o.words[j].y, magic);
     };
     const auto product = [&](const Operands &o, int i, int j) {
         float16v p = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.n[i][0][1], o.v[j][0], float16v{}, 0, 0, 0);
@@ -726,29 +741,31 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs
     float16v kept = float16v{};
     float kept_d = 0.0f;
     const auto multiply = [&](const Operands &o, auto between) {
+        __builtin_amdgcn_sched_barrier(0);
         const float16v p00 = product(o, 0, 0);
         between(0);
         add(1, 1, kept_d, kept);
+        mixed<4>();
         const float16v p10 = product(o, 1, 0);
         between(1);
         add(0, 0, o.d[0], p00);
+        mixed<4>();
         const float16v p01 = product(o, 0, 1);
         between(2);
         add(1, 0, o.d[0], p10);
+        mixed<9>();
         kept = product(o, 1, 1);
         between(3);
         add(0, 1, o.d[1], p01);
         kept_d = o.d[1];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
-        }
+        mixed<9>();
     };
     fetched<2 * L::kCopies>();
     lds_barrier();
     Operands even, odd;
     read(even, 0);
+    widen_words(even, 0);
+    widen_words(even, 1);
     int buffer = 0;
     // Stage s is multiplied from registers while stage s + 1 is read into
     // others; s + 2 is under way and s + 3 takes the buffer that s was read
@@ -760,6 +777,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs
         buffer = buffer == 2 ? 0 : buffer + 1;
         multiply(now, [&](int k) {
             if (k == 0) read(next, buffer);
+            if (k >= 2) widen_words(next, k - 2);
 #pragma unroll
             for (int c = 0; c < L::kCopies; ++c)
                 if (c * 4 / L::kCopies == k) copy(s + 3, free, c);
@@ -970,9 +988,9 @@ struct TilesWork {
 
 TilesWork tiles_work(int64_t M, int64_t N, int64_t half, int64_t K, bool least) {
     TilesWork w{};
-    // Whole workgroups' tiles, whichever shape is taken: up to 128 rows by 256.
+    // Whole workgroups' tiles, whichever shape is taken: up to 128 rows by 128.
     w.row_tiles = round_up(ceil_div(M, kRowsTile), 4);
-    w.column_tiles = round_up(half ? 2 * ceil_div(half, kRowsTile) : ceil_div(N, kRowsTile), 8);
+    w.column_tiles = round_up(half ? 2 * ceil_div(half, kRowsTile) : ceil_div(N, kRowsTile), 4);
     w.blocks = K / kBlock;
     w.groups = least ? ceil_div(w.blocks, 32) : 0;
     size_t at = 0;
@@ -1011,16 +1029,17 @@ hipError_t many_rows(const Q4Args &a, void *work, hipStream_t stream) {
     SDHIP_LAUNCH((q4_operands_kernel<LEAST, GATED>), dim3(static_cast<uint32_t>(t.x_groups + tiles * strips)),
                  dim3(kOperandThreads), 0, stream, t);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-    // The shape whose workgroups take the fewest stages one after another on
-    // a CU, the larger where that is alike; sums split over waves cost about 4
-    // stages more to add up.
+    // Tiles of 128 x 128 for two workgroups a CU or more go by four waves, each
+    // all of K: the two do not wait at one barrier (1976 rows of 1280 -> 2 x 5120
+    // gated 127 us, by eight waves 142).  Fewer are split along K inside a
+    // workgroup, by the shape of less stages one after another on a CU (1976
+    // rows of 1280 -> 1280: 128 x 128 by two 35.0 us, 64 x 128 by four 41.7; 33
+    // rows of 2080 -> 1111 43.2 and 29.6).
     const int64_t cus = compute_units(), columns = 2 * (GATED ? a.half : a.N / 2 + a.N % 2);
-    const auto cost = [&](int rows, int cols, int split) {
-        return ceil_div(ceil_div(a.M, rows) * ceil_div(columns, cols), cus) * (ceil_div(w.blocks, split) + 4) + (split > 1 ? 4 : 0);
-    };
-    const int64_t c0 = cost(128, 256, 1), c1 = cost(128, 128, 2), c2 = cost(64, 128, 4);
-    if (c0 <= c1 && c0 <= c2) return launch_tiles<LEAST, GATED, 2, 4, 1>(t, stream);
-    if (c1 <= c2) return launch_tiles<LEAST, GATED, 2, 2, 2>(t, stream);
+    const auto tiles_of = [&](int rows, int cols) { return ceil_div(a.M, rows) * ceil_div(columns, cols); };
+    const auto cost = [&](int rows, int split) { return ceil_div(tiles_of(rows, 128), cus) * (ceil_div(w.blocks, split) + 8); };
+    if (tiles_of(128, 128) >= 2 * cus) return launch_tiles<LEAST, GATED, 2, 2, 1>(t, stream);
+    if (cost(128, 2) <= cost(64, 4)) return launch_tiles<LEAST, GATED, 2, 2, 2>(t, stream);
     return launch_tiles<LEAST, GATED, 1, 2, 4>(t, stream);
 }
 
