@@ -3,6 +3,11 @@
 // a row's norm by its mean and the mean of its squares about it (LAYER), or
 // about 0 (RMS), both summed in double: no square of a single-precision
 // number passes it, and the mean is held in two single-precision parts.
+//
+// Bound by memory: each number of y and residual is read once and each of sum
+// and out written once, the row in registers between its sums, T threads a
+// row, up to 4 Q numbers each (norm_residual_rows_kernel); longer rows are
+// read again for every sum (norm_residual_long_kernel).
 
 #include "host.h"
 #include "profile.h"
@@ -15,7 +20,7 @@ namespace {
 constexpr int kThreads = 256;
 
 struct Place {
-    int64_t i1, i2, i3;
+    uint32_t i1, i2, i3;
 };
 
 __device__ __forceinline__ int64_t row_at(const int64_t (&nb)[4], const Place &p) {
@@ -54,7 +59,8 @@ __device__ __forceinline__ double block_sum(double v, double *lds) {
 __global__ __launch_bounds__(kThreads) void norm_residual_long_kernel(ResidualArgs a) {
     __shared__ double lds[kThreads / 64];
     const int64_t row = blockIdx.x;
-    const Place p{row % a.ne1, (row / a.ne1) % a.ne2, row / (a.ne1 * a.ne2)};
+    Place p;
+    split_index(static_cast<uint32_t>(row), static_cast<uint32_t>(a.ne1), static_cast<uint32_t>(a.ne2), p.i1, p.i2, p.i3);
     const float *y = a.y != nullptr ? a.y + row_at(a.ynb, p) : nullptr;
     const float *r = a.residual + row_at(a.rnb, p);
     float *sum = a.sum != nullptr ? a.sum + row_at(a.snb, p) : nullptr;
@@ -107,11 +113,195 @@ __global__ __launch_bounds__(kThreads) void norm_residual_long_kernel(ResidualAr
     }
 }
 
+// T threads a row (T = 64: four rows a workgroup), each holding 4 Q numbers
+// of it: Q quads T apart where rows lie at multiples of 16 bytes (QUADS), else
+// 4 Q numbers T apart.
+template <int T, int Q, bool QUADS>
+__global__ __launch_bounds__(T == 64 ? 256 : T) void norm_residual_rows_kernel(ResidualArgs a) {
+    __shared__ double lds[4][T / 64];  // a sum each: no sum waits for the one before to be read
+    const int tid = T == 64 ? threadIdx.x & 63 : threadIdx.x;
+    const uint32_t row = T == 64 ? blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
+    if (row >= static_cast<uint32_t>(a.rows)) return;  // T = 64 only: its waves meet at no barrier
+    Place p;
+    split_index(row, static_cast<uint32_t>(a.ne1), static_cast<uint32_t>(a.ne2), p.i1, p.i2, p.i3);
+    const int n = static_cast<int>(a.ne0);
+    const auto at = [&](int u, int k) { return QUADS ? 4 * (tid + T * u) + k : tid + T * (4 * u + k); };
+    const auto load = [&](const float *from, float (&v)[Q][4]) {
+#pragma unroll
+        for (int u = 0; u < Q; ++u) {
+            if constexpr (QUADS) {
+                float4v q = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (at(u, 0) < n) q = *reinterpret_cast<const float4v *>(from + at(u, 0));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[u][k] = q[k];
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[u][k] = at(u, k) < n ? from[at(u, k)] : 0.0f;
+            }
+        }
+    };
+    const auto store = [&](float *to, const float (&v)[Q][4]) {
+#pragma unroll
+        for (int u = 0; u < Q; ++u) {
+            if constexpr (QUADS) {
+                if (at(u, 0) < n) *reinterpret_cast<float4v *>(to + at(u, 0)) = float4v{v[u][0], v[u][1], v[u][2], v[u][3]};
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (at(u, k) < n) to[at(u, k)] = v[u][k];
+            }
+        }
+    };
+    // An operand's numbers for the row: read as the rows are where it lies so,
+    // else one number for all or each where it is.
+    const auto operand = [&](const RowOperand &o, float (&v)[Q][4]) {
+        const float *from = o.data + row_at(o.nb, p);
+        if (o.nb[0] == 1 && (!QUADS || reinterpret_cast<uintptr_t>(from) % 16 == 0)) {
+            load(from, v);
+            return;
+        }
+#pragma unroll
+        for (int u = 0; u < Q; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[u][k] = at(u, k) < n ? from[at(u, k) * o.nb[0]] : 0.0f;
+    };
+    int sums = 0;
+    const auto total = [&](double v) {
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+        if constexpr (T > 64) {
+            if ((tid & 63) == 0) lds[sums][tid >> 6] = v;
+            __syncthreads();
+            v = 0.0;
+#pragma unroll
+            for (int w = 0; w < T / 64; ++w) v += lds[sums][w];
+            ++sums;
+        }
+        return v;
+    };
+    const auto stats = [&](int32_t kind, float eps, const float (&v)[Q][4]) {
+        double mean = 0.0, squares = 0.0;
+        if (kind == SDHIP_ROW_NORM_LAYER) {
+            double s = 0.0;
+#pragma unroll
+            for (int u = 0; u < Q; ++u)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s += static_cast<double>(v[u][k]);
+            mean = total(s) / static_cast<double>(n);
+        }
+#pragma unroll
+        for (int u = 0; u < Q; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const double d = at(u, k) < n ? static_cast<double>(v[u][k]) - mean : 0.0;
+                squares = __builtin_fma(d, d, squares);
+            }
+        return moments(kind, mean, total(squares), static_cast<double>(n), eps);
+    };
+    const auto affine = [&](const RowNorm &w, float (&v)[Q][4]) {
+        if (w.weight.data != nullptr) {
+            float o[Q][4];
+            operand(w.weight, o);
+#pragma unroll
+            for (int u = 0; u < Q; ++u)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[u][k] = __fmul_rn(v[u][k], __fadd_rn(o[u][k], w.offset));
+        }
+        if (w.bias.data != nullptr) {
+            float o[Q][4];
+            operand(w.bias, o);
+#pragma unroll
+            for (int u = 0; u < Q; ++u)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[u][k] = __fadd_rn(v[u][k], o[u][k]);
+        }
+    };
+    float s[Q][4];
+    if (a.y != nullptr) {
+        float z[Q][4];
+        load(a.y + row_at(a.ynb, p), z);
+        load(a.residual + row_at(a.rnb, p), s);
+        if (a.post.kind != SDHIP_ROW_NORM_NONE) {
+            const Moments m = stats(a.post.kind, a.post.eps, z);
+#pragma unroll
+            for (int u = 0; u < Q; ++u)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) z[u][k] = normed(z[u][k], m);
+        }
+        affine(a.post, z);
+        if (a.gate.data != nullptr) {
+            float o[Q][4];
+            operand(a.gate, o);
+#pragma unroll
+            for (int u = 0; u < Q; ++u)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) z[u][k] = __fmul_rn(z[u][k], o[u][k]);
+        }
+#pragma unroll
+        for (int u = 0; u < Q; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                s[u][k] = __fadd_rn(__fmul_rn(a.residual_scale, s[u][k]), __fmul_rn(a.branch_scale, z[u][k]));
+    } else {
+        load(a.residual + row_at(a.rnb, p), s);
+#pragma unroll
+        for (int u = 0; u < Q; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[u][k] = __fmul_rn(a.residual_scale, s[u][k]);
+    }
+    if (a.sum != nullptr) store(a.sum + row_at(a.snb, p), s);
+    if (a.out == nullptr) return;
+    if (a.pre.kind != SDHIP_ROW_NORM_NONE) {
+        const Moments m = stats(a.pre.kind, a.pre.eps, s);
+#pragma unroll
+        for (int u = 0; u < Q; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[u][k] = normed(s[u][k], m);
+    }
+    affine(a.pre, s);
+    store(a.out + row_at(a.onb, p), s);
+}
+
+template <int T, int Q>
+void launch_rows(const ResidualArgs &a, bool quads, hipStream_t stream) {
+    const dim3 grid(static_cast<uint32_t>(T == 64 ? ceil_div(a.rows, 4) : a.rows)), block(T == 64 ? 256 : T);
+    if (quads) {
+        SDHIP_LAUNCH((norm_residual_rows_kernel<T, Q, true>), grid, block, 0, stream, a);
+    } else {
+        SDHIP_LAUNCH((norm_residual_rows_kernel<T, Q, false>), grid, block, 0, stream, a);
+    }
+}
+
 }  // namespace
 
 hipError_t launch_norm_residual(const ResidualArgs &a, hipStream_t stream) {
     KernelScope scope("norm_residual", stream);
-    SDHIP_LAUNCH(norm_residual_long_kernel, dim3(static_cast<uint32_t>(a.rows)), dim3(kThreads), 0, stream, a);
+    const auto quads = [&](const float *p, const int64_t (&nb)[4]) {
+        return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && nb[1] % 4 == 0 && nb[2] % 4 == 0 && nb[3] % 4 == 0);
+    };
+    const bool q = a.ne0 % 4 == 0 && quads(a.y, a.ynb) && quads(a.residual, a.rnb) && quads(a.sum, a.snb) && quads(a.out, a.onb);
+    const bool many = a.rows >= 4 * static_cast<int64_t>(compute_units());
+    if (a.ne0 <= 256) {
+        launch_rows<64, 1>(a, q, stream);
+    } else if (a.ne0 <= 512) {
+        launch_rows<64, 2>(a, q, stream);
+    } else if (many && a.ne0 <= 1280) {
+        launch_rows<64, 5>(a, q, stream);
+    } else if (a.ne0 <= 1024) {
+        launch_rows<256, 1>(a, q, stream);
+    } else if (a.ne0 <= 2048) {
+        launch_rows<256, 2>(a, q, stream);
+    } else if (many && a.ne0 <= 5120) {
+        launch_rows<256, 5>(a, q, stream);
+    } else if (a.ne0 <= 4096) {
+        launch_rows<1024, 1>(a, q, stream);
+    } else if (a.ne0 <= 8192) {
+        launch_rows<1024, 2>(a, q, stream);
+    } else if (a.ne0 <= 16384) {
+        launch_rows<1024, 4>(a, q, stream);
+    } else {
+        SDHIP_LAUNCH(norm_residual_long_kernel, dim3(static_cast<uint32_t>(a.rows)), dim3(kThreads), 0, stream, a);
+    }
     return hipGetLastError();
 }
 
