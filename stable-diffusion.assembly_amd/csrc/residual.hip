@@ -280,6 +280,10 @@ hipError_t launch_norm_residual(const ResidualArgs &a, hipStream_t stream) {
         return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && nb[1] % 4 == 0 && nb[2] % 4 == 0 && nb[3] % 4 == 0);
     };
     const bool q = a.ne0 % 4 == 0 && quads(a.y, a.ynb) && quads(a.residual, a.rnb) && quads(a.sum, a.snb) && quads(a.out, a.onb);
+    // As few threads a row as hold it in 16 or 20 numbers each, and of up to
+    // 1280 numbers a wave alone where there are rows for every wave (2 x 988
+    // rows of 1280: 11.0 us, by four waves 13.5; 400 rows 5.8 and 5.5; one row of
+    // 4096 by four waves 5.1 us, by sixteen 6.2; 2 x 4096 rows of 5120 122 and 210).
     const bool many = a.rows >= 4 * static_cast<int64_t>(compute_units());
     if (a.ne0 <= 256) {
         launch_rows<64, 1>(a, q, stream);
@@ -291,12 +295,12 @@ hipError_t launch_norm_residual(const ResidualArgs &a, hipStream_t stream) {
         launch_rows<256, 1>(a, q, stream);
     } else if (a.ne0 <= 2048) {
         launch_rows<256, 2>(a, q, stream);
-    } else if (many && a.ne0 <= 5120) {
-        launch_rows<256, 5>(a, q, stream);
     } else if (a.ne0 <= 4096) {
-        launch_rows<1024, 1>(a, q, stream);
+        launch_rows<256, 4>(a, q, stream);
+    } else if (a.ne0 <= 5120) {
+        launch_rows<256, 5>(a, q, stream);
     } else if (a.ne0 <= 8192) {
-        launch_rows<1024, 2>(a, q, stream);
+        launch_rows<512, 4>(a, q, stream);
     } else if (a.ne0 <= 16384) {
         launch_rows<1024, 4>(a, q, stream);
     } else {
