@@ -113,6 +113,61 @@ __device__ __forceinline__ uint32_t magnitude(const float4v &v) {
     return m;
 }
 
+constexpr int kFewThreads = 512;
+
+// The outputs of a workgroup of kFewThreads from its splits' sums in LDS, `step`
+// apart, `count` outputs, with GATED the second half's behind them: their sums
+// in the splits' order, times what `place` gives with an output's row (M or
+// more: none) and column; the redirect's number first, the chain, the gated
+// GELU.  E of a thread's at a time, so that their loads go out together.
+template <bool GATED, int E, class Place>
+__device__ __forceinline__ void write_outputs(const Q4Args &a, const float *sums, int splits, int step, int count, int tid,
+                                              int columns, Place place) {
+    constexpr int kHalves = GATED ? 2 : 1;
+#pragma unroll 1
+    for (int first = tid; first < count; first += E * kFewThreads) {
+        int64_t m[E];
+        int n[E];
+        bool real[E];
+        float v[kHalves * E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int at = first + kFewThreads * e < count ? first + kFewThreads * e : first;
+            const float back = place(at, m[e], n[e]);
+            real[e] = first + kFewThreads * e < count && m[e] < a.M && n[e] < columns;
+            m[e] = m[e] < a.M ? m[e] : a.M - 1;
+            n[e] = n[e] < columns ? n[e] : columns - 1;
+#pragma unroll
+            for (int p = 0; p < kHalves; ++p) {
+                float s[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) s[k] = sums[(k < splits ? k : 0) * step + p * count + at];
+                float total = s[0];
+#pragma unroll
+                for (int k = 1; k < 8; ++k) total = k < splits ? total + s[k] : total;
+                v[kHalves * e + p] = total * back;
+            }
+        }
+        if (!GATED && a.from_redirect) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[kHalves * e] = a.y[m[e] * a.ldy + n[e]] + v[kHalves * e];
+        }
+        apply_chain_block(a.chain, v, [&](int s, int i) {
+            const DevStep &st = a.chain.steps[s];
+            const int64_t at = (n[i / kHalves] + (i % kHalves) * static_cast<int64_t>(columns)) * st.nb[0];
+            const int64_t row = m[i / kHalves];
+            if (st.flat123) return at + row * st.nb[1];
+            uint32_t i1, i2, i3;
+            split_index(static_cast<uint32_t>(row), static_cast<uint32_t>(a.ne1), static_cast<uint32_t>(a.ne2), i1, i2, i3);
+            return at + i1 * st.nb[1] + i2 * st.nb[2] + i3 * st.nb[3];
+        });
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (real[e]) a.y[m[e] * a.ldy + n[e]] = GATED ? v[kHalves * e] * gelu(v[kHalves * e + kHalves - 1]) : v[kHalves * e];
+        }
+    }
+}
+
 // ------------------------------------------------------------------ copies
 
 // A copy of 16 bytes a lane (1 KB) or 4 into LDS at `to` and on, lane after
@@ -169,7 +224,7 @@ __device__ __forceinline__ void fetched() {
 // its hi in the first register and its lo in the second, up to 8 two a group,
 // so that one MFMA takes both parts; from 9 on two do.
 constexpr int kFewWaves = 8;
-constexpr int kFewThreads = 64 * kFewWaves;
+static_assert(kFewThreads == 64 * kFewWaves);
 constexpr int kUnit = 8;        // blocks
 // A part of x: 16 blocks of a row, their parts 128 bytes a block (hi, then lo,
 // of the four groups), and 16 bytes that spread the rows over the banks.
@@ -402,32 +457,27 @@ __global__ __launch_bounds__(kFewThreads, 4) void q4_few_kernel(FewArgs f) {
 #pragma unroll
     for (int e = 0; e < R; ++e) sums[((split * P + tile) * R + e) * 64 + lane] = sum[e];
     lds_barrier();
-#pragma unroll 1
-    for (int at = tid; at < outs * R * 64; at += kFewThreads) {
+    const auto place = [&](int at, int64_t &m, int &out) {
         const int row = R * ((at & 63) >> 4) + (at >> 6) % R;
-        const int out = n0 + 16 * (at / (64 * R)) + (at & 15);
-        if (row >= rows || out >= columns) continue;
-        const int64_t m = m0 + row;
-        float *y = a.y + m * a.ldy + out;
-        float v[GATED ? 2 : 1];
-#pragma unroll
-        for (int p = 0; p < (GATED ? 2 : 1); ++p) {
-            v[p] = 0.0f;
-#pragma unroll 1
-            for (int u = 0; u < S; ++u) v[p] += sums[(u * P + p * outs) * R * 64 + at];
-        }
-        if (a.from_redirect) v[0] = *y + v[0];
-        if (a.chain.count > 0) {
-            uint32_t i1, i2, i3;
-            split_index(static_cast<uint32_t>(m), static_cast<uint32_t>(a.ne1), static_cast<uint32_t>(a.ne2), i1, i2, i3);
-            apply_chain_block(a.chain, v, [&](int s, int p) {
-                const DevStep &st = a.chain.steps[s];
-                return (out + p * static_cast<int64_t>(columns)) * st.nb[0] + i1 * st.nb[1] + i2 * st.nb[2] +
-                       i3 * st.nb[3];
-            });
-        }
-        *y = GATED ? v[0] * gelu(v[GATED ? 1 : 0]) : v[0];
+        m = row < rows ? m0 + row : a.M;
+        out = n0 + 16 * (at / (64 * R)) + (at & 15);
+        return 1.0f;
+    };
+    if (outs * R * 64 <= kFewThreads) {
+        write_outputs<GATED, 1>(a, sums, S, P * R * 64, outs * R * 64, tid, columns, place);
+    } else {
+        write_outputs<GATED, R>(a, sums, S, P * R * 64, outs * R * 64, tid, columns, place);
     }
+}
+
+// The splits of K: until the device's waves all have one, two workgroups a CU,
+// within the units of a chunk.
+int few_splits(int64_t N, int64_t K, int rows, bool gated) {
+    const int64_t tiles = ceil_div(N, 16), units = ceil_div(K / kBlock, kUnit), chunk = kFewParts / rows * kPart / kUnit;
+    const int64_t waves = static_cast<int64_t>(compute_units()) * 2 * kFewWaves;
+    int splits = 1;
+    while (splits < (gated ? 4 : 8) && tiles * splits * 2 <= waves && splits < units && splits < chunk) splits *= 2;
+    return splits;
 }
 
 template <bool LEAST, bool GATED, int ROWS>
@@ -440,13 +490,8 @@ hipError_t launch_few(const Q4Args &a, hipStream_t stream) {
     f.a = a;
     f.splits = 1;
     const int64_t columns = GATED ? a.half : a.N;
-    const int64_t tiles = ceil_div(a.N, 16), units = ceil_div(a.K / kBlock, kUnit);
     const int64_t parts = ceil_div(a.K / kBlock, kPart) * ROWS;
-    const int64_t chunk = kFewParts / ROWS * kPart / kUnit;
-    // Splits until the device's waves all have one, two workgroups a CU.
-    const int64_t waves = static_cast<int64_t>(compute_units()) * 2 * kFewWaves;
-    const int most = GATED ? 4 : 8;
-    while (f.splits < most && tiles * f.splits * 2 <= waves && f.splits < units && f.splits < chunk) f.splits *= 2;
+    f.splits = few_splits(a.N, a.K, ROWS, GATED);
     f.tiles = kFewWaves / f.splits;
     const dim3 grid(static_cast<uint32_t>(ceil_div(columns, 16 * (GATED ? f.tiles / 2 : f.tiles))),
                     static_cast<uint32_t>(ceil_div(a.M, ROWS)));
@@ -508,50 +553,75 @@ __device__ __forceinline__ void split_bf16(float v, __bf16 (&p)[3]) {
     }
 }
 
-constexpr int kOperandThreads = 256;
+constexpr int kOperandThreads = 512;
+constexpr int kOperandRows = 8;  // of x a workgroup
 
-// Workgroups of two kinds: 4 rows of x, a wave each, or 32 rows of the weights by 16 blocks.
+// Workgroups of two kinds: 8 rows of x, or 32 rows of the weights by 32 blocks.
+// A wave takes 2 blocks of the 8 rows at a time, 8 lanes a row, so that what it
+// reads of a row lies together and what it writes of them does too; the first
+// kKept such times are kept in registers while the rows' greatest are found
+// (1976 rows of 5120: 30 us with a row a wave, written 16 bytes here and there).
 template <bool LEAST, bool GATED>
 __global__ __launch_bounds__(kOperandThreads) void q4_operands_kernel(TileArgs t) {
     const Q4Args &a = t.a;
     constexpr int kSize = LEAST ? 20 : 18;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if (static_cast<int>(blockIdx.x) < t.x_groups) {
-        const int64_t m = static_cast<int64_t>(blockIdx.x) * 4 + wave;
-        if (m >= a.M) return;
-        const float *x = a.x + m * a.ldx + 4 * (lane & 3);
-        uint32_t v = 0;
-        for (int b = lane >> 2; b < t.blocks; b += 16) {
-            const float4v low = load4(x + b * kBlock), high = load4(x + b * kBlock + 16);
-            const uint32_t p = magnitude(low), q = magnitude(high);
-            v = v > p ? v : p;
-            v = v > q ? v : q;
-        }
-        const uint32_t e = scale_exponent(wave_greatest(v));
-        const float scale = power(e);
-        if (lane == 0) t.back[m] = power(254 - e);
-        const int64_t tile = m / kRowsTile;
-        const int row = static_cast<int>(m % kRowsTile), word = lane & 3;
-        const int end = LEAST ? t.groups * 32 : t.blocks;
-        for (int b = lane >> 2; b < end; b += 16) {
-            float sum = 0.0f;
+        constexpr int kWaves = kOperandThreads / 64, kKept = 6;
+        __shared__ uint32_t greatest[kWaves][kOperandRows];
+        const int64_t m = static_cast<int64_t>(blockIdx.x) * kOperandRows + (lane >> 3);
+        const int word = lane & 3, first = 2 * wave + ((lane >> 2) & 1);
+        const float *x = a.x + (m < a.M ? m : a.M - 1) * a.ldx + 4 * word;
+        const auto load = [&](int b, float4v &low, float4v &high) {
+            low = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+            high = low;
             if (b < t.blocks) {
-                const float4v low = load4(x + b * kBlock), high = load4(x + b * kBlock + 16);
+                low = load4(x + b * static_cast<int64_t>(kBlock));
+                high = load4(x + b * static_cast<int64_t>(kBlock) + 16);
+            }
+        };
+        const auto greater = [](uint32_t p, uint32_t q) { return p > q ? p : q; };
+        float4v low[kKept], high[kKept];
+#pragma unroll
+        for (int i = 0; i < kKept; ++i) load(first + 2 * kWaves * i, low[i], high[i]);
+        uint32_t v = 0;
+#pragma unroll
+        for (int i = 0; i < kKept; ++i) v = greater(v, greater(magnitude(low[i]), magnitude(high[i])));
+        for (int b = first + 2 * kWaves * kKept; b < t.blocks; b += 2 * kWaves) {
+            float4v l, h;
+            load(b, l, h);
+            v = greater(v, greater(magnitude(l), magnitude(h)));
+        }
+        v = greater(v, __builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, true));   // lanes i ^ 1
+        v = greater(v, __builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, true));   // i ^ 2
+        v = greater(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true));  // 8 lanes mirrored
+        if ((lane & 7) == 0) greatest[wave][lane >> 3] = v;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) v = greater(v, greatest[w][lane >> 3]);
+        const uint32_t e = scale_exponent(v);
+        const float scale = power(e);
+        if (m < a.M && wave == 0 && (lane & 7) == 0) t.back[m] = power(254 - e);
+        const int64_t tile = m / kRowsTile;
+        const int row = static_cast<int>(m % kRowsTile);
+        const auto write = [&](int b, const float4v &l, const float4v &h) {
+            float sum = 0.0f;
+            if (b < t.blocks && m < a.M) {
                 half8 hi, lo;
-                split8(low, high, scale, hi, lo);
+                split8(l, h, scale, hi, lo);
                 char *to = t.numbers + (b * static_cast<int64_t>(t.row_tiles) + tile) * kNumbersBytes + (word >> 1) * 2048 +
                            ((word & 1) * 32 + row) * 16;
                 *reinterpret_cast<half8 *>(to) = hi;
                 *reinterpret_cast<half8 *>(to + 1024) = lo;
                 if constexpr (LEAST) {
-                    sum = ((low[0] + low[1]) + (low[2] + low[3])) + ((high[0] + high[1]) + (high[2] + high[3]));
+                    sum = ((l[0] + l[1]) + (l[2] + l[3])) + ((h[0] + h[1]) + (h[2] + h[3]));
                     sum *= scale;
                 }
             }
             if constexpr (LEAST) {
                 sum += __shfl_xor(sum, 1, 64);
                 sum += __shfl_xor(sum, 2, 64);
-                if (word == 0) {
+                if (word == 0 && m < a.M && b < t.groups * 32) {
                     __bf16 p[3];
                     split_bf16(sum, p);
                     char *to = t.sums + ((b >> 5) * static_cast<int64_t>(t.row_tiles) + tile) * kOffsetsBytes +
@@ -560,17 +630,28 @@ __global__ __launch_bounds__(kOperandThreads) void q4_operands_kernel(TileArgs t
                     for (int i = 0; i < 3; ++i) *reinterpret_cast<__bf16 *>(to + 1024 * i) = p[i];
                 }
             }
+        };
+#pragma unroll
+        for (int i = 0; i < kKept; ++i) write(first + 2 * kWaves * i, low[i], high[i]);
+        // Q4_1: the sums of the blocks that fill the last 32 are 0.
+        for (int b = first + 2 * kWaves * kKept; b < (LEAST ? t.groups * 32 : t.blocks); b += 2 * kWaves) {
+            float4v l, h;
+            load(b, l, h);
+            write(b, l, h);
         }
         return;
     }
-    // Rows of pieces that hold 16 blocks wherever they begin, an odd number of
-    // them to spread the rows over the banks.
+    // Strips of 16 blocks, one for each half of the workgroup.  Rows of pieces
+    // that hold 16 blocks wherever they begin, an odd number of them to spread
+    // the rows over the banks.
     constexpr int kRow = LEAST ? 21 : 19;
-    constexpr int kRounds = (kRowsTile * kRow + kOperandThreads - 1) / kOperandThreads;
-    __shared__ __attribute__((aligned(16))) char lds[kRounds * kOperandThreads * 16];
-    const int strips = LEAST ? 2 * t.groups : (t.blocks + 15) / 16;
+    constexpr int kHalf = kOperandThreads / 2;
+    constexpr int kRounds = (kRowsTile * kRow + kHalf - 1) / kHalf;
+    __shared__ __attribute__((aligned(16))) char lds[2][kRounds * kHalf * 16];
+    const int pairs = LEAST ? t.groups : (t.blocks + 31) / 32;
     const int item = static_cast<int>(blockIdx.x) - t.x_groups;
-    const int tile = item / strips, b0 = item % strips * 16;
+    const int half = wave / (kHalf / 64), place = tid & (kHalf - 1);
+    const int tile = item / pairs, b0 = (item % pairs * 2 + half) * 16;
     const int count = t.blocks - b0 < 16 ? t.blocks - b0 : 16;  // 0 and less: zeros of offsets only
     const auto weights = [&](int r) {
         const int64_t columns = GATED ? a.half : a.N;
@@ -580,19 +661,20 @@ __global__ __launch_bounds__(kOperandThreads) void q4_operands_kernel(TileArgs t
     if (count > 0) {
 #pragma unroll
         for (int i = 0; i < kRounds; ++i) {
-            const int slot = kOperandThreads * i + tid;
+            const int slot = kHalf * i + place;
             const int row = slot / kRow < kRowsTile ? slot / kRow : kRowsTile - 1;
             const uint8_t *at = weights(row);
             const int skip = static_cast<int>(reinterpret_cast<uintptr_t>(at) & 15);
             const int piece = 16 * (slot - kRow * row), last = (skip + kSize * count - 1) & ~15;
-            fetch16(at - skip + (piece < last ? piece : last), lds_address(lds) + kOperandThreads * 16 * i + 1024 * wave);
+            fetch16(at - skip + (piece < last ? piece : last),
+                    lds_address(lds[half]) + kHalf * 16 * i + 1024 * (wave & (kHalf / 64 - 1)));
         }
         fetched<0>();
     }
     lds_barrier();
     const int col = lane & 31, h = lane >> 5;
-    const char *mine = lds + 16 * kRow * col + static_cast<int>(reinterpret_cast<uintptr_t>(weights(col)) & 15);
-    for (int i = wave; i < count; i += kOperandThreads / 64) {
+    const char *mine = lds[half] + 16 * kRow * col + static_cast<int>(reinterpret_cast<uintptr_t>(weights(col)) & 15);
+    for (int i = wave & (kHalf / 64 - 1); i < count; i += kHalf / 64) {
         const char *block = mine + kSize * i;
         uint32_t w[2];
 #pragma unroll
@@ -604,7 +686,7 @@ __global__ __launch_bounds__(kOperandThreads) void q4_operands_kernel(TileArgs t
         if (h == 0) *reinterpret_cast<float *>(to + 512 + 4 * col) = static_cast<float>(d);
     }
     if constexpr (LEAST) {
-        if (wave == 0) {
+        if ((wave & (kHalf / 64 - 1)) == 0) {
             // Lane 32 h + row: the offsets of the strip's blocks 8 h .. 8 h + 7.
             typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
             bf16x8 p[3];
@@ -980,17 +1062,219 @@ hipError_t launch_tiles(TileArgs t, hipStream_t stream) {
     return hipGetLastError();
 }
 
+// ------------------------------------------------------------------ rows between
+
+// Rows of x too many to split in every workgroup and too few for tiles: x is
+// laid out as for the tiles, the weights are read as they are.  A workgroup
+// takes P tiles of 32 rows of the weights by S splits of K, a wave each, and
+// 32 MT rows of x; a wave's weights come into LDS of its own by units of 8
+// blocks, two of them in flight, as few rows' do, and x from L2 as the MFMA's
+// lanes want it, a block ahead.  Q4_1's offsets go by bfloat16 parts as the
+// tiles' do, a unit's 8 blocks one step of v_mfma_f32_32x32x8_bf16.
+constexpr int kMidCopies = 6;
+constexpr int kMidUnitBytes = kMidCopies * 1024;
+
+struct MidArgs {
+    TileArgs t;
+    int32_t splits, tiles;  // S, P
+};
+
+template <bool LEAST, bool GATED, int MT>
+__global__ __launch_bounds__(kFewThreads, 2) void q4_mid_kernel(MidArgs f) {
+    const TileArgs &t = f.t;
+    const Q4Args &a = t.a;
+    constexpr int kSize = LEAST ? 20 : 18;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, h = lane >> 5;
+    const int S = f.splits, P = f.tiles;
+    const int split = wave & (S - 1), tile = wave / S;
+    const int blocks = t.blocks;
+    const int units = (blocks + kUnit - 1) / kUnit;
+    const int outs = GATED ? P / 2 : P;  // tiles of the output
+    const int columns = static_cast<int>(GATED ? a.half : a.N);
+    const int n0 = static_cast<int>(blockIdx.x) * (32 * outs);
+    const auto weights = [&](int c) {  // row c of the wave's tile, or the last there is
+        const bool second = GATED && tile >= outs;
+        const int n = n0 + 32 * (second ? tile - outs : tile) + c;
+        return a.w + ((n < columns ? n : columns - 1) + (second ? columns : 0)) * a.row_bytes;
+    };
+    const uint8_t *source[kMidCopies];
+    int skip[kMidCopies], piece[kMidCopies];
+#pragma unroll
+    for (int c = 0; c < kMidCopies; ++c) {
+        const int slot = 64 * c + lane, row = slot / kPieces < 32 ? slot / kPieces : 31;
+        const uint8_t *at = weights(row);
+        skip[c] = static_cast<int>(reinterpret_cast<uintptr_t>(at) & 15);
+        source[c] = at - skip[c];
+        piece[c] = 16 * (slot - kPieces * row);
+    }
+    char *ring = lds + wave * (2 * kMidUnitBytes);
+    const auto copy_unit = [&](int u, int buffer) {
+        const int count = blocks - kUnit * u < kUnit ? blocks - kUnit * u : kUnit;
+#pragma unroll
+        for (int c = 0; c < kMidCopies; ++c) {
+            const int last = (skip[c] + kSize * count - 1) & ~15;
+            fetch16(source[c] + u * (kUnit * kSize) + (piece[c] < last ? piece[c] : last),
+                    lds_address(ring) + buffer * kMidUnitBytes + 1024 * c);
+        }
+    };
+    if (split < units) copy_unit(split, 0);
+    if (split + S < units) copy_unit(split + S, 1);
+    // Words h and 2 + h of this lane's row, of the first block and the second.
+    const char *mine = ring + 16 * kPieces * col + static_cast<int>(reinterpret_cast<uintptr_t>(weights(col)) & 15);
+    const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(mine + kSize - 16) & 2);
+    const char *words[2] = {mine + kSize - 16 + 4 * h - odd, mine + 2 * kSize - 16 + 4 * h - (LEAST ? odd : 2 - odd)};
+    const uint32_t shift[2] = {8u * odd, LEAST ? 8u * odd : 16u - 8u * odd};
+    const uint32_t magic = opaque(kMagic);
+    const char *numbers = t.numbers + static_cast<int64_t>(blockIdx.y) * MT * kNumbersBytes + 16 * lane;
+    const int64_t numbers_step = t.row_tiles * kNumbersBytes;
+    struct Numbers {
+        half8 n[MT][2][2];  // [32 rows][half of the block][hi, lo]
+    };
+    const auto load_numbers = [&](int b, Numbers &o) {
+        const char *from = numbers + (b < blocks ? b : blocks - 1) * numbers_step;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int p = 0; p < 4; ++p) o.n[i][p >> 1][p & 1] = *reinterpret_cast<const half8 *>(from + 4096 * i + 1024 * p);
+    };
+    float16v acc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i] = float16v{};
+    // x of the next kAheadX blocks: those past a unit's are the wave's next
+    // unit's, asked for before that one's successor is copied, behind which
+    // they would wait.
+    constexpr int kAheadX = 4;
+    Numbers x[kAheadX];
+#pragma unroll
+    for (int i = 0; i < kAheadX; ++i) load_numbers(kUnit * split + i, x[i]);
+    int buffer = 0;
+#pragma unroll 1
+    for (int u = split; u < units; u += S) {
+        if (u + S < units) {
+            fetched<kMidCopies>();
+        } else {
+            fetched<0>();
+        }
+        const int count = blocks - kUnit * u < kUnit ? blocks - kUnit * u : kUnit;
+        const char *row = mine + buffer * kMidUnitBytes;
+        const auto add_block = [&](int i, const Numbers &x) {
+            const uint32_t *at = reinterpret_cast<const uint32_t *>(words[i & 1] + buffer * kMidUnitBytes + kSize * (i & ~1));
+            _Float16 d;
+            __builtin_memcpy(&d, row + kSize * i, 2);
+            half8 v[2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+                v[s] = widen(__builtin_amdgcn_alignbit(at[2 * s + 1], at[2 * s], shift[i & 1]), magic);
+            const float scale = static_cast<float>(d);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                float16v p = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.n[m][0][1], v[0], float16v{}, 0, 0, 0);
+                p = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.n[m][1][1], v[1], p, 0, 0, 0);
+                p = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.n[m][0][0], v[0], p, 0, 0, 0);
+                p = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.n[m][1][0], v[1], p, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[m][e] = __builtin_fmaf(scale, p[e], acc[m][e]);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i) {
+            if (i < count) add_block(i, x[i % kAheadX]);
+            load_numbers(i < kAheadX ? kUnit * u + i + kAheadX : kUnit * (u + S) + i - kAheadX, x[i % kAheadX]);
+        }
+        if constexpr (LEAST) {
+            // Lane 32 h + row: the offsets of blocks 4 h .. 4 h + 3.
+            typedef short short4v __attribute__((ext_vector_type(4)));
+            short4v q[3];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int k = 4 * h + j;
+                float c = 0.0f;
+                if (k < count) {
+                    _Float16 d, least;
+                    __builtin_memcpy(&d, row + kSize * k, 2);
+                    __builtin_memcpy(&least, row + kSize * k + 2, 2);
+                    c = __builtin_fmaf(8.0f, static_cast<float>(d), static_cast<float>(least));
+                }
+                __bf16 parts[3];
+                split_bf16(c, parts);
+#pragma unroll
+                for (int p = 0; p < 3; ++p) q[p][j] = __builtin_bit_cast(short, parts[p]);
+            }
+            const char *sums = t.sums + ((u >> 2) * static_cast<int64_t>(t.row_tiles) + blockIdx.y * MT) * kOffsetsBytes +
+                               ((u >> 1) & 1) * 3072 + ((u & 1) * 32 + col) * 16 + 8 * h;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                short4v s[3];
+#pragma unroll
+                for (int p = 0; p < 3; ++p) s[p] = *reinterpret_cast<const short4v *>(sums + m * kOffsetsBytes + 1024 * p);
+#pragma unroll
+                for (int total = 2; total >= 0; --total)
+#pragma unroll
+                    for (int p = 0; p <= total; ++p)
+                        acc[m] = __builtin_amdgcn_mfma_f32_32x32x8bf16_1k(s[p], q[total - p], acc[m], 0, 0, 0);
+            }
+        }
+        if (u + 2 * S < units) {
+            // The unit is read: the one two on takes its place.
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+            copy_unit(u + 2 * S, buffer);
+        }
+        buffer ^= 1;
+    }
+    lds_barrier();
+    float *sums = reinterpret_cast<float *>(lds);  // [split][tile][32 rows][register][lane]
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sums[(((split * P + tile) * MT + m) * 16 + e) * 64 + lane] = acc[m][e];
+    lds_barrier();
+    constexpr int kTile = MT * 1024;
+    const int64_t m0 = static_cast<int64_t>(blockIdx.y) * (32 * MT);
+    const auto place = [&](int at, int64_t &m, int &out) {
+        m = m0 + 32 * ((at >> 10) % MT) + tile_row((at >> 6) & 15) + 4 * ((at >> 5) & 1);
+        out = n0 + 32 * (at / kTile) + (at & 31);
+        return t.back[m < a.M ? m : a.M - 1];
+    };
+    if (outs == 1) {
+        write_outputs<GATED, kTile / kFewThreads>(a, sums, S, P * kTile, kTile, tid, columns, place);
+    } else {
+        write_outputs<GATED, 8>(a, sums, S, P * kTile, outs * kTile, tid, columns, place);
+    }
+}
+
+template <bool LEAST, bool GATED, int MT>
+hipError_t launch_mid(const TileArgs &t, hipStream_t stream) {
+    constexpr int kLds = kFewWaves * 2 * kMidUnitBytes;
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&q4_mid_kernel<LEAST, GATED, MT>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    if (attr != hipSuccess) return attr;
+    MidArgs f{t, 1, kFewWaves};
+    const int64_t columns = GATED ? t.a.half : t.a.N, tiles = ceil_div(t.a.N, 32), rows = ceil_div(t.a.M, 32 * MT);
+    // Splits until every wave of the device has one.
+    const int64_t waves = static_cast<int64_t>(compute_units()) * kFewWaves, units = ceil_div(t.blocks, kUnit);
+    const int most = GATED ? 4 : 8;
+    while (f.splits < most && tiles * rows * f.splits * 2 <= waves && f.splits < units) f.splits *= 2;
+    f.tiles = kFewWaves / f.splits;
+    const dim3 grid(static_cast<uint32_t>(ceil_div(columns, 32 * (GATED ? f.tiles / 2 : f.tiles))), static_cast<uint32_t>(rows));
+    SDHIP_LAUNCH((q4_mid_kernel<LEAST, GATED, MT>), grid, dim3(kFewThreads), kLds, stream, f);
+    return hipGetLastError();
+}
+
 // The work buffer's parts.
 struct TilesWork {
     size_t numbers, words, back, sums, offsets, bytes;
     int64_t row_tiles, column_tiles, blocks, groups;
 };
 
-TilesWork tiles_work(int64_t M, int64_t N, int64_t half, int64_t K, bool least) {
+// With `weights` those too are laid out, for the tiles.
+TilesWork tiles_work(int64_t M, int64_t N, int64_t half, int64_t K, bool least, bool weights) {
     TilesWork w{};
     // Whole workgroups' tiles, whichever shape is taken: up to 128 rows by 128.
     w.row_tiles = round_up(ceil_div(M, kRowsTile), 4);
-    w.column_tiles = round_up(half ? 2 * ceil_div(half, kRowsTile) : ceil_div(N, kRowsTile), 4);
+    w.column_tiles = !weights ? 0 : round_up(half ? 2 * ceil_div(half, kRowsTile) : ceil_div(N, kRowsTile), 4);
     w.blocks = K / kBlock;
     w.groups = least ? ceil_div(w.blocks, 32) : 0;
     size_t at = 0;
@@ -1008,10 +1292,11 @@ TilesWork tiles_work(int64_t M, int64_t N, int64_t half, int64_t K, bool least) 
     return w;
 }
 
+// The operands laid out in the work buffer.
 template <bool LEAST, bool GATED>
-hipError_t many_rows(const Q4Args &a, void *work, hipStream_t stream) {
-    const TilesWork w = tiles_work(a.M, a.N, a.half, a.K, LEAST);
-    TileArgs t{};
+hipError_t lay_out(const Q4Args &a, void *work, bool weights, TileArgs &t, hipStream_t stream) {
+    const TilesWork w = tiles_work(a.M, a.N, a.half, a.K, LEAST, weights);
+    t = TileArgs{};
     t.a = a;
     char *p = static_cast<char *>(work);
     t.numbers = p + w.numbers;
@@ -1023,12 +1308,25 @@ hipError_t many_rows(const Q4Args &a, void *work, hipStream_t stream) {
     t.groups = static_cast<int32_t>(w.groups);
     t.row_tiles = static_cast<int32_t>(w.row_tiles);
     t.column_tiles = static_cast<int32_t>(w.column_tiles);
-    t.x_groups = static_cast<int32_t>(ceil_div(a.M, 4));
-    const int64_t tiles = GATED ? 2 * ceil_div(a.half, kRowsTile) : ceil_div(a.N, kRowsTile);
-    const int64_t strips = LEAST ? 2 * w.groups : ceil_div(w.blocks, 16);
-    SDHIP_LAUNCH((q4_operands_kernel<LEAST, GATED>), dim3(static_cast<uint32_t>(t.x_groups + tiles * strips)),
+    t.x_groups = static_cast<int32_t>(ceil_div(a.M, kOperandRows));
+    const int64_t tiles = !weights ? 0 : GATED ? 2 * ceil_div(a.half, kRowsTile) : ceil_div(a.N, kRowsTile);
+    const int64_t pairs = ceil_div(w.blocks, 32);
+    SDHIP_LAUNCH((q4_operands_kernel<LEAST, GATED>), dim3(static_cast<uint32_t>(t.x_groups + tiles * pairs)),
                  dim3(kOperandThreads), 0, stream, t);
-    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    return hipGetLastError();
+}
+
+template <bool LEAST, bool GATED>
+hipError_t between_rows(const Q4Args &a, void *work, hipStream_t stream) {
+    TileArgs t;
+    if (const hipError_t e = lay_out<LEAST, GATED>(a, work, false, t, stream); e != hipSuccess) return e;
+    return a.M <= 32 ? launch_mid<LEAST, GATED, 1>(t, stream) : launch_mid<LEAST, GATED, 2>(t, stream);
+}
+
+template <bool LEAST, bool GATED>
+hipError_t many_rows(const Q4Args &a, void *work, hipStream_t stream) {
+    TileArgs t;
+    if (const hipError_t e = lay_out<LEAST, GATED>(a, work, true, t, stream); e != hipSuccess) return e;
     // Tiles of 128 x 128 for two workgroups a CU or more go by four waves, each
     // all of K: the two do not wait at one barrier (1976 rows of 1280 -> 2 x 5120
     // gated 127 us, by eight waves 142).  Fewer are split along K inside a
@@ -1037,33 +1335,57 @@ hipError_t many_rows(const Q4Args &a, void *work, hipStream_t stream) {
     // rows of 2080 -> 1111 43.2 and 29.6).
     const int64_t cus = compute_units(), columns = 2 * (GATED ? a.half : a.N / 2 + a.N % 2);
     const auto tiles_of = [&](int rows, int cols) { return ceil_div(a.M, rows) * ceil_div(columns, cols); };
-    const auto cost = [&](int rows, int split) { return ceil_div(tiles_of(rows, 128), cus) * (ceil_div(w.blocks, split) + 8); };
+    const auto cost = [&](int rows, int split) { return ceil_div(tiles_of(rows, 128), cus) * (ceil_div(t.blocks, split) + 8); };
     if (tiles_of(128, 128) >= 2 * cus) return launch_tiles<LEAST, GATED, 2, 2, 1>(t, stream);
     if (cost(128, 2) <= cost(64, 4)) return launch_tiles<LEAST, GATED, 2, 2, 2>(t, stream);
     return launch_tiles<LEAST, GATED, 1, 2, 4>(t, stream);
 }
 
-// Up to 16 rows go through q4_few_kernel, which needs no work buffer.
-bool few(int64_t rows) { return rows <= 16; }
+// Which kernels a product of these extents takes, gated or not.
+enum class Form { few, between, many };
+
+// The form with no work buffer up to 16 rows, and as long as its workgroups of
+// 16 rows are on the device at once, or twice where K is short (64 rows of 1280
+// -> 1280: 9.4 us, laid out 13.4, by tiles 19.1; 128 rows 16.9, 13.7 and 19.6; 128
+// of 768 -> 1280 12.1, 15.1 and 15.4).  Then x laid out, up to as many rows and
+// columns as its L2 reads are fewer than the tiles' (256 rows of 4096 -> 4096
+// 40.9 us, by tiles 44.8; 64 of 1280 -> 10240 21.1 and 23.3, 96 29.4 and 24.1).
+Form form_of(int64_t M, int64_t N, int64_t K) {
+    if (M <= 16) return Form::few;
+    const int64_t at_once = static_cast<int64_t>(compute_units()) * 2;
+    const int64_t groups = ceil_div(M, 16) * ceil_div(ceil_div(N, 16) * few_splits(N, K, 16, false), kFewWaves);
+    if (groups <= at_once || (groups <= 2 * at_once && K <= 1024)) return Form::few;
+    return M <= 384 && ceil_div(M, 64) * N <= 16384 ? Form::between : Form::many;
+}
 
 }  // namespace
 
 size_t q4_work_size(int64_t M, int64_t N, int64_t K, bool least) {
-    if (few(M)) return 0;
+    const Form form = form_of(M, N, K);
+    if (form == Form::few) return 0;
     // The plain and the gated product of one size take one size of buffer.
-    const size_t plain = tiles_work(M, N, 0, K, least).bytes;
-    const size_t gated = N % 2 == 0 ? tiles_work(M, N, N / 2, K, least).bytes : 0;
+    const bool weights = form == Form::many;
+    const size_t plain = tiles_work(M, N, 0, K, least, weights).bytes;
+    const size_t gated = N % 2 == 0 ? tiles_work(M, N, N / 2, K, least, weights).bytes : 0;
     return plain > gated ? plain : gated;
+}
+
+template <bool LEAST, bool GATED>
+static hipError_t launch_form(const Q4Args &a, void *work, hipStream_t stream) {
+    switch (form_of(a.M, a.N, a.K)) {
+    case Form::few:
+        return few_rows<LEAST, GATED>(a, stream);
+    case Form::between:
+        return between_rows<LEAST, GATED>(a, work, stream);
+    default:
+        return many_rows<LEAST, GATED>(a, work, stream);
+    }
 }
 
 hipError_t launch_q4_mul_mat(const Q4Args &a, void *work, hipStream_t stream) {
     KernelScope scope(a.half ? "q4.gated" : "q4", stream);
-    if (few(a.M)) {
-        if (a.half) return a.least ? few_rows<true, true>(a, stream) : few_rows<false, true>(a, stream);
-        return a.least ? few_rows<true, false>(a, stream) : few_rows<false, false>(a, stream);
-    }
-    if (a.half) return a.least ? many_rows<true, true>(a, work, stream) : many_rows<false, true>(a, work, stream);
-    return a.least ? many_rows<true, false>(a, work, stream) : many_rows<false, false>(a, work, stream);
+    if (a.half) return a.least ? launch_form<true, true>(a, work, stream) : launch_form<false, true>(a, work, stream);
+    return a.least ? launch_form<true, false>(a, work, stream) : launch_form<false, false>(a, work, stream);
 }
 
 }  // namespace sdhip
