@@ -121,7 +121,10 @@ const char *sdhip_last_error(void);
  * instead of the panel kernels; 2: panels of 64 x 160 only, not 64 x 64),
  * conv_panels (0:
  * 1x1 convolutions by the 64 x 64 core), conv3x3_direct (0: F(4x4,3x3) where its
- * nine taps would be taken directly),
+ * nine taps would be taken directly), q4_form (1 .. 5: the products of 4-bit
+ * weights by one of their forms -- each workgroup's rows of x split in it, x laid
+ * out first, or both operands, tiles of 128 x 128 by four waves, by eight, or of
+ * 64 x 128 -- whatever the size),
  * attention_generic, attention_fp32 (forms to compare, same results within
  * the bounds -- qgemm_core's bit for bit), each taking only its documented
  * values.  Returns SDHIP_ERROR
@@ -181,7 +184,10 @@ int sdhip_profile_entry(int i, const char **name, double *total_ms, int64_t *lau
  * bytes that holds a row, at an even address; from one row of x up, where the
  * others begin at 16.  The products are those of the exact weights with x in
  * 22 bits or more of each row's greatest number, whatever bits asks for; the
- * output shares no byte with w or x.
+ * output shares no byte with w or x.  The work buffer: for more rows than a
+ * workgroup's, x in FP16 parts, and for many rows the weights' words and scales
+ * in the order the products read them.  An infinity in x reaches its own row only,
+ * with Q4_1, whose products are two sums, as infinities or NaN.
  * Replaces mul_mat_supported / mul_mat_work_size / mul_mat_compute
  * (sources/ops.h:40-44; mul_mat.cc:181-194, 205-215, 1175-1196). */
 int sdhip_mul_mat_supported(const sdhip_tensor *w, const sdhip_tensor *x, const sdhip_tensor *y);

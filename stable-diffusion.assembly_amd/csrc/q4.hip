@@ -1292,6 +1292,10 @@ TilesWork tiles_work(int64_t M, int64_t N, int64_t half, int64_t K, bool least, 
     return w;
 }
 
+// Which kernels a product of these extents takes, gated or not, numbered as
+// the q4_form tuning asks for them.
+enum class Form { few = 1, between, tiles4, tiles8, tiles64 };
+
 // The operands laid out in the work buffer.
 template <bool LEAST, bool GATED>
 hipError_t lay_out(const Q4Args &a, void *work, bool weights, TileArgs &t, hipStream_t stream) {
@@ -1324,38 +1328,44 @@ hipError_t between_rows(const Q4Args &a, void *work, hipStream_t stream) {
 }
 
 template <bool LEAST, bool GATED>
-hipError_t many_rows(const Q4Args &a, void *work, hipStream_t stream) {
+hipError_t many_rows(const Q4Args &a, Form form, void *work, hipStream_t stream) {
     TileArgs t;
     if (const hipError_t e = lay_out<LEAST, GATED>(a, work, true, t, stream); e != hipSuccess) return e;
+    switch (form) {
+    case Form::tiles4:
+        return launch_tiles<LEAST, GATED, 2, 2, 1>(t, stream);
+    case Form::tiles8:
+        return launch_tiles<LEAST, GATED, 2, 2, 2>(t, stream);
+    default:
+        return launch_tiles<LEAST, GATED, 1, 2, 4>(t, stream);
+    }
+}
+
+Form form_of(int64_t M, int64_t N, int64_t K) {
+    const int64_t cus = compute_units();
+    const int64_t groups = ceil_div(M, 16) * ceil_div(ceil_div(N, 16) * few_splits(N, K, 16, false), kFewWaves);
+    const int asked = tuning().q4_form;
+    // A launch holds 65535 groups of rows at most.
+    if (asked > 0 && !(asked == 1 && M > 16 * 65535) && !(asked == 2 && M > 32 * 65535)) return static_cast<Form>(asked);
+    // With no work buffer up to 16 rows, and as long as the workgroups of 16
+    // rows are on the device at once, or twice where K is short (64 rows of 1280
+    // -> 1280: 9.4 us, laid out 13.4, by tiles 19.1; 128 rows 16.9, 13.7 and 19.6;
+    // 128 of 768 -> 1280 12.1, 15.1 and 15.4).
+    if (M <= 16 || groups <= 2 * cus || (groups <= 4 * cus && K <= 1024)) return Form::few;
+    // Then x laid out, up to as many rows and columns as its L2 reads are
+    // fewer than the tiles' (256 rows of 4096 -> 4096 40.9 us, by tiles 44.8; 64
+    // of 1280 -> 10240 21.1 and 23.3, 96 29.4 and 24.1).
+    if (M <= 384 && ceil_div(M, 64) * N <= 16384) return Form::between;
     // Tiles of 128 x 128 for two workgroups a CU or more go by four waves, each
     // all of K: the two do not wait at one barrier (1976 rows of 1280 -> 2 x 5120
-    // gated 127 us, by eight waves 142).  Fewer are split along K inside a
+    // gated 126 us, by eight waves 142).  Fewer are split along K inside a
     // workgroup, by the shape of less stages one after another on a CU (1976
     // rows of 1280 -> 1280: 128 x 128 by two 35.0 us, 64 x 128 by four 41.7; 33
     // rows of 2080 -> 1111 43.2 and 29.6).
-    const int64_t cus = compute_units(), columns = 2 * (GATED ? a.half : a.N / 2 + a.N % 2);
-    const auto tiles_of = [&](int rows, int cols) { return ceil_div(a.M, rows) * ceil_div(columns, cols); };
-    const auto cost = [&](int rows, int split) { return ceil_div(tiles_of(rows, 128), cus) * (ceil_div(t.blocks, split) + 8); };
-    if (tiles_of(128, 128) >= 2 * cus) return launch_tiles<LEAST, GATED, 2, 2, 1>(t, stream);
-    if (cost(128, 2) <= cost(64, 4)) return launch_tiles<LEAST, GATED, 2, 2, 2>(t, stream);
-    return launch_tiles<LEAST, GATED, 1, 2, 4>(t, stream);
-}
-
-// Which kernels a product of these extents takes, gated or not.
-enum class Form { few, between, many };
-
-// The form with no work buffer up to 16 rows, and as long as its workgroups of
-// 16 rows are on the device at once, or twice where K is short (64 rows of 1280
-// -> 1280: 9.4 us, laid out 13.4, by tiles 19.1; 128 rows 16.9, 13.7 and 19.6; 128
-// of 768 -> 1280 12.1, 15.1 and 15.4).  Then x laid out, up to as many rows and
-// columns as its L2 reads are fewer than the tiles' (256 rows of 4096 -> 4096
-// 40.9 us, by tiles 44.8; 64 of 1280 -> 10240 21.1 and 23.3, 96 29.4 and 24.1).
-Form form_of(int64_t M, int64_t N, int64_t K) {
-    if (M <= 16) return Form::few;
-    const int64_t at_once = static_cast<int64_t>(compute_units()) * 2;
-    const int64_t groups = ceil_div(M, 16) * ceil_div(ceil_div(N, 16) * few_splits(N, K, 16, false), kFewWaves);
-    if (groups <= at_once || (groups <= 2 * at_once && K <= 1024)) return Form::few;
-    return M <= 384 && ceil_div(M, 64) * N <= 16384 ? Form::between : Form::many;
+    const auto tiles_of = [&](int rows) { return ceil_div(M, rows) * ceil_div(N, 128); };
+    const auto cost = [&](int rows, int split) { return ceil_div(tiles_of(rows), cus) * (ceil_div(K / kBlock, split) + 8); };
+    if (tiles_of(128) >= 2 * cus) return Form::tiles4;
+    return cost(128, 2) <= cost(64, 4) ? Form::tiles8 : Form::tiles64;
 }
 
 }  // namespace
@@ -1364,7 +1374,7 @@ size_t q4_work_size(int64_t M, int64_t N, int64_t K, bool least) {
     const Form form = form_of(M, N, K);
     if (form == Form::few) return 0;
     // The plain and the gated product of one size take one size of buffer.
-    const bool weights = form == Form::many;
+    const bool weights = form != Form::between;
     const size_t plain = tiles_work(M, N, 0, K, least, weights).bytes;
     const size_t gated = N % 2 == 0 ? tiles_work(M, N, N / 2, K, least, weights).bytes : 0;
     return plain > gated ? plain : gated;
@@ -1372,14 +1382,10 @@ size_t q4_work_size(int64_t M, int64_t N, int64_t K, bool least) {
 
 template <bool LEAST, bool GATED>
 static hipError_t launch_form(const Q4Args &a, void *work, hipStream_t stream) {
-    switch (form_of(a.M, a.N, a.K)) {
-    case Form::few:
-        return few_rows<LEAST, GATED>(a, stream);
-    case Form::between:
-        return between_rows<LEAST, GATED>(a, work, stream);
-    default:
-        return many_rows<LEAST, GATED>(a, work, stream);
-    }
+    const Form form = form_of(a.M, a.N, a.K);
+    if (form == Form::few) return few_rows<LEAST, GATED>(a, stream);
+    if (form == Form::between) return between_rows<LEAST, GATED>(a, work, stream);
+    return many_rows<LEAST, GATED>(a, form, work, stream);
 }
 
 hipError_t launch_q4_mul_mat(const Q4Args &a, void *work, hipStream_t stream) {

@@ -372,3 +372,190 @@ def test_refusals_leave_the_output(gpu):
     assert lib.sdhip_mul_mat(dw, dx, none, *args) == sdhip.ERROR
     torch.cuda.synchronize()
     assert torch.isnan(y).all()
+
+
+FORMS = [1, 2, 3, 4, 5]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("rows", [1, 16, 17, 31, 33, 64, 65, 127, 128, 130, 200, 257])
+def test_forms(gpu, kind, form, rows):
+    """Every form at rows and columns at both sides of its tiles' limits, few
+    blocks of K and many, and counts of them that end inside a stage."""
+    sdhip.set_tuning(f"q4_form={form}")
+    try:
+        for k, n in [(32, 1), (64, 31), (96, 33), (128, 64), (160, 65), (224, 127), (1056, 129), (1568, 257), (2080, 300)]:
+            y, exact, mag = run(gpu, kind, rows, k, n, seed=rows * 10 + k + n)
+            err = orc.metric(y.cpu().numpy(), exact, mag)
+            print(f"{kind} form {form} {rows} x {k} -> {n}: {err:.3g} of {q4_lib.bound(k):.3g}")
+            assert err <= q4_lib.bound(k)
+    finally:
+        sdhip.set_tuning("")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("rows,k,n", [(1, 64, 2), (33, 320, 62), (70, 352, 258), (150, 1120, 130), (300, 96, 514)])
+def test_forms_gated(gpu, kind, form, rows, k, n):
+    sdhip.set_tuning(f"q4_form={form}")
+    try:
+        r = rng(rows + n)
+        blocks = q4_lib.random_blocks(r, kind, n, k)
+        x, bias, scale = uniform(r, (rows, k), 1.0), uniform(r, (n,), 1.0), uniform(r, (rows, 1), 1.0)
+        steps = [("add", dev(bias, gpu)), ("mul", dev(scale, gpu))]
+        y, out = unwritten((rows, n), gpu), unwritten((rows, n // 2), gpu)
+        sdhip.mul_mat_gated(dev(blocks, gpu), dev(x, gpu), y, out, sdhip.epilogue(steps))
+    finally:
+        sdhip.set_tuning("")
+    exact, mag = q4_lib.exact(blocks, x)
+    p, size = (exact + bias) * scale, (mag + np.abs(bias)) * np.abs(scale)
+    a, g = p[:, :n // 2], p[:, n // 2:]
+    err = q4_lib.bound(k, 2)
+    allowed = np.abs(gelu64(g)) * err * size[:, :n // 2] + 1.13 * np.abs(a) * err * size[:, n // 2:]
+    allowed = allowed * (1 + 1e-3) + 2.0 ** -20 * np.abs(a) * np.abs(g) + err * err * size[:, :n // 2] * size[:, n // 2:]
+    diff = np.abs(out.cpu().numpy() - a * gelu64(g))
+    assert torch.isnan(y).all() and np.isfinite(diff).all() and (diff <= allowed + 1e-30).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("end", ["own", "redirect", "from_redirect"])
+def test_forms_chain(gpu, form, end):
+    """A bias, a number for each row, a number for each matrix of rows, then
+    the residual; x of [3, rows, k]."""
+    rows, k, n = 50, 352, 130
+    r = rng(form)
+    blocks = q4_lib.random_blocks(r, "q4_1", n, k)
+    x = uniform(r, (3, rows, k), 1.0)
+    bias, scale, shift = uniform(r, (n,), 1.0), uniform(r, (3, rows, 1), 1.0), uniform(r, (3, 1, n), 1.0)
+    res = uniform(r, (3, rows, n), 1.0)
+    steps = [("add", dev(bias, gpu)), ("mul", dev(scale, gpu)), ("add", dev(shift, gpu))]
+    res_d = dev(res, gpu)
+    out = None
+    if end == "redirect":
+        out = unwritten((3, rows, n), gpu)
+    elif end == "from_redirect":
+        out = res_d.clone()
+    if end != "from_redirect":
+        steps.append(("add", res_d))
+    y = unwritten((3, rows, n), gpu)
+    sdhip.set_tuning(f"q4_form={form}")
+    try:
+        sdhip.mul_mat(dev(blocks, gpu), dev(x, gpu), y,
+                      sdhip.epilogue(steps, redirect=out, from_redirect=end == "from_redirect"))
+    finally:
+        sdhip.set_tuning("")
+    exact, mag = (t.reshape(y.shape) for t in q4_lib.exact(blocks, x.reshape(-1, k)))
+    first = res if end == "from_redirect" else 0.0 * res
+    last = res - first
+    want = (first + exact + bias) * scale + shift + last
+    size = (np.abs(first) + mag + np.abs(bias)) * np.abs(scale) + np.abs(shift) + np.abs(last)
+    got = (y if out is None else out).cpu().numpy()
+    assert orc.metric(got, want, size) <= q4_lib.bound(k, 5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("gap,offset", [(2, 0), (14, 6)])
+def test_forms_rows_apart(gpu, kind, form, gap, offset):
+    rows, k, n = 70, 544, 100
+    row = k // 32 * q4_lib.BYTES[kind] + gap
+    sdhip.set_tuning(f"q4_form={form}")
+    try:
+        y, exact, mag = run(gpu, kind, rows, k, n, seed=gap + offset, layout=(row, offset))
+        assert orc.metric(y.cpu().numpy(), exact, mag) <= q4_lib.bound(k)
+    finally:
+        sdhip.set_tuning("")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("form", FORMS)
+def test_forms_ranges(gpu, kind, form):
+    """Rows of magnitudes far apart, rows of zeros, and with Q4_0 an infinity
+    and a NaN, which stay in their rows."""
+    rows, k, n = 70, 640, 70
+    r = rng(form)
+    blocks = q4_lib.random_blocks(r, kind, n, k)
+    size = q4_lib.BYTES[kind]
+    blocks[:, 1, size - 16 + 3] = (blocks[:, 1, size - 16 + 3] & 0xf0) | 11  # number 35 of each row: q - 8 = 3
+    x = (uniform(r, (rows, k), 1.0) * 2.0 ** r.integers(-60, 60, (rows, 1))).astype(np.float32)
+    x[2::3] = 0
+    x[4, 35], x[7, 7] = np.inf, np.nan
+    y = unwritten((rows, n), gpu)
+    sdhip.set_tuning(f"q4_form={form}")
+    try:
+        sdhip.mul_mat(dev(blocks, gpu), dev(x, gpu), y)
+    finally:
+        sdhip.set_tuning("")
+    got = y.cpu().numpy()
+    assert (got[2::3] == 0).all() and np.isnan(got[7]).all() and not np.isfinite(got[4]).any()
+    if kind == "q4_0":
+        w, _ = q4_lib.widen(blocks)
+        assert (got[4] == np.where(w[:, 35] > 0, np.inf, -np.inf)).all()
+    keep = [i for i in range(rows) if i % 3 != 2 and i not in (4, 7)]
+    exact, mag = q4_lib.exact(blocks, x[keep])
+    assert orc.metric(got[keep], exact, mag) <= q4_lib.bound(k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMS)
+def test_forms_captured(gpu, form):
+    r = rng(form)
+    rows, k, n = 70, 640, 320
+    w, x = dev(q4_lib.random_blocks(r, "q4_1", n, k), gpu), dev(uniform(r, (rows, k), 1.0), gpu)
+    y, unused, out = (unwritten(s, gpu) for s in ((rows, n), (rows, n), (rows, n // 2)))
+    sdhip.set_tuning(f"q4_form={form}")
+    try:
+        size = sdhip.load().sdhip_mul_mat_work_size(sdhip.desc(w), sdhip.desc(x), sdhip.desc(y))
+        work = torch.empty(max(size, 16), dtype=torch.uint8, device=gpu)
+
+        def calls():  # one after the other, by one work buffer
+            sdhip.mul_mat(w, x, y, work=work)
+            sdhip.mul_mat_gated(w, x, unused, out, work=work)
+
+        calls()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            with torch.cuda.graph(graph, stream=side):
+                calls()
+        torch.cuda.current_stream().wait_stream(side)
+        for i in range(3):
+            x.copy_(dev(uniform(rng(50 + i), (rows, k), 1.0), gpu))
+            calls()
+            want = y.clone(), out.clone()
+            y.fill_(float("nan"))
+            out.fill_(float("nan"))
+            work.fill_(255)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want[0]) and torch.equal(out, want[1])
+    finally:
+        sdhip.set_tuning("")
+
+
+@pytest.mark.gpu
+def test_work_buffer_is_all_that_is_written(gpu):
+    """Every form with a work buffer of exactly its size, between guards."""
+    r = rng(1)
+    for form in FORMS[1:]:
+        for kind, rows, k, n in (("q4_0", 70, 352, 100), ("q4_1", 129, 1056, 130), ("q4_1", 1, 32, 2)):
+            w, x = dev(q4_lib.random_blocks(r, kind, n, k), gpu), dev(uniform(r, (rows, k), 1.0), gpu)
+            y, out = unwritten((rows, n), gpu), unwritten((rows, n // 2), gpu)
+            sdhip.set_tuning(f"q4_form={form}")
+            try:
+                size = sdhip.load().sdhip_mul_mat_work_size(sdhip.desc(w), sdhip.desc(x), sdhip.desc(y))
+                buf = torch.full((size + 8192,), 77, dtype=torch.uint8, device=gpu)
+                sdhip.mul_mat(w, x, y, work=buf[4096:4096 + size])
+                sdhip.mul_mat_gated(w, x, y, out, work=buf[4096:4096 + size])
+            finally:
+                sdhip.set_tuning("")
+            assert (buf[:4096] == 77).all() and (buf[4096 + size:] == 77).all(), (form, kind)

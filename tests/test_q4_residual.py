@@ -196,3 +196,25 @@ def test_norms_refused():
     none = rows(2, 9, 64, data=None)
     assert lib.sdhip_norm_residual(A, norm(), None, 1.0, none, 1.0, C, norm(), D, None) == sdhip.ERROR
     assert lib.sdhip_norm_residual(A, norm(), None, 1.0, None, 1.0, C, norm(), D, None) == sdhip.UNSUPPORTED
+
+
+def test_forms_tuning():
+    lib = sdhip.load()
+    w, x, y = blocks(Q4_0, 320, 320), rows(40, 320), rows(40, 320)
+    try:
+        for bad in ("q4_form=6", "q4_form=-1"):
+            with pytest.raises(sdhip.SdhipError):
+                sdhip.set_tuning(bad)
+        sizes = []
+        for form in range(1, 6):
+            sdhip.set_tuning(f"q4_form={form}")
+            assert sdhip.get_tuning("q4_form") == form
+            sizes.append(lib.sdhip_mul_mat_work_size(w, x, y))
+        assert sizes[0] == 0 < sizes[1] < sizes[2] and sizes[2] == sizes[3] == sizes[4]
+    finally:
+        sdhip.set_tuning("")
+    assert sdhip.get_tuning("q4_form") == 0
+    assert lib.sdhip_mul_mat_work_size(w, rows(1, 320), rows(1, 320)) == 0
+    big = rows(4000, 320), rows(4000, 320)
+    assert lib.sdhip_mul_mat(w, *big[:1], rows(4000, 320, data=99 * FAKE), None, None, 0, None) == sdhip.ERROR
+    assert b"work" in lib.sdhip_last_error()
