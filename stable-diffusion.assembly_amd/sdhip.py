@@ -237,7 +237,10 @@ def epilogue(steps=(), redirect=None, from_redirect=False):
 
 
 def stream_handle():
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    """torch's current stream on the current device, as the library takes it:
+    by torch's own accessor of the handle, since making a torch.cuda.Stream of it
+    took 2.9 us of a call's 6.8, this 0.3."""
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def set_tuning(text=""):
