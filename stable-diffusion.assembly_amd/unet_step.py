@@ -4,7 +4,8 @@ This measures the "UNet step ms" half of the metric: one forward pass of
 SD1.5's UNet at 512x512 (latent 64x64, batch 2 for classifier-free guidance,
 a 77-token context of 768), random-initialised weights of that architecture
 (FP16 conv and linear weights ~N(0, 0.02), as the reference's tests fill
-them), with every node the reference takes over from ggml -- CONV_2D,
+them; the linear layers' in ggml's 4-bit blocks where the model is made with
+weights="q4_0" or "q4_1"), with every node the reference takes over from ggml -- CONV_2D,
 MUL_MAT, the gated GEGLU product, FLASH_ATTN_EXT, GROUP_NORM, NORM and the
 chains after them -- run by libsdhip.  The nodes the reference does not take
 (ggml computes them: nearest upsampling, concatenation, the permutes between
@@ -33,6 +34,51 @@ import torch.nn.functional as F
 import sdhip
 
 GELU_K = 1.5957691216057308  # 2 sqrt(2 / pi), the reference's gelu (scalar_math.h:55-63)
+
+
+# ---------------------------------------------------------------- 4-bit weights
+
+
+def quantize(w, kind):
+    """Weights [n, k], k a multiple of 32, as the bytes of ggml's 4-bit blocks,
+    [n, k / 32, 18] (kind "q4_0": a scale of the sign that gives a block's
+    furthest number -8 of it) or [n, k / 32, 20] ("q4_1": from a block's least
+    number to its greatest in 15 steps)."""
+    n, k = w.shape
+    size = sdhip.BLOCK_BYTES[{"q4_0": sdhip.TYPE_Q4_0, "q4_1": sdhip.TYPE_Q4_1}[kind]]
+    if w.device.type == "meta":
+        return torch.empty((n, k // sdhip.BLOCK, size), dtype=torch.uint8, device="meta")
+    w = w.float().reshape(n, k // sdhip.BLOCK, sdhip.BLOCK)
+    if kind == "q4_0":
+        heads = [torch.gather(w, -1, w.abs().argmax(dim=-1, keepdim=True)) / -8.0]
+        zero = -8.0 * heads[0].half().float()
+    else:
+        least = w.amin(dim=-1, keepdim=True)
+        heads = [(w.amax(dim=-1, keepdim=True) - least) / 15.0, least]
+        zero = least.half().float()
+    d = heads[0].half().float()
+    q = torch.where(d == 0, torch.zeros_like(w), ((w - zero) / d).round()).clamp(0, 15).to(torch.uint8)
+    nibbles = q[..., :16] | (q[..., 16:] << 4)
+    return torch.cat([h.half().contiguous().view(torch.uint8) for h in heads] + [nibbles], dim=-1).contiguous()
+
+
+def extents(w):
+    """(n, k) of a linear layer's weights, FP16 [n, k] or 4-bit blocks."""
+    return (w.shape[0], w.shape[1] * sdhip.BLOCK) if w.dtype == torch.uint8 else tuple(w.shape)
+
+
+def widen(w, dtype):
+    """A linear layer's weights [n, k] as numbers of `dtype`."""
+    if w.dtype != torch.uint8:
+        return w.to(dtype)
+    n, k = extents(w)
+    size = w.shape[2]
+    nibbles = w[..., size - 16:]
+    q = torch.cat([nibbles & 15, nibbles >> 4], dim=-1).to(dtype)
+    d = w[..., 0:2].contiguous().view(torch.float16).to(dtype)
+    if size == sdhip.BLOCK_BYTES[sdhip.TYPE_Q4_0]:
+        return (d * (q - 8)).reshape(n, k)
+    return (d * q + w[..., 2:4].contiguous().view(torch.float16).to(dtype)).reshape(n, k)
 
 
 class Config:
@@ -80,7 +126,7 @@ class Ops:
         self.count(f"conv{kh}x{kw}", 2.0 * n * oc * oh * ow * ic * kh * kw)
 
     def count_linear(self, x, w):
-        n, k = w.shape
+        n, k = extents(w)
         self.count("linear", 2.0 * (x.numel() // k) * n * k)
 
     def count_attention(self, q, k, heads):
@@ -150,10 +196,10 @@ class HipOps(Ops):
         return y
 
     def linear(self, x, w, bias=None, add=()):
-        n, k = w.shape
+        n, k = extents(w)
         m = x.numel() // k
         self.count_linear(x, w)
-        if m < 16:
+        if m < 16 and w.dtype != torch.uint8:
             # Not taken by the reference (mul_mat.cc:181-194): ggml's node,
             # with the weights widened once and kept, as ggml's CPU backend
             # reads them without converting the tensor each time.
@@ -177,7 +223,7 @@ class HipOps(Ops):
         return y
 
     def geglu(self, x, w, bias):
-        n, k = w.shape
+        n, k = extents(w)
         m = x.numel() // k
         self.count_linear(x, w)
         y = torch.empty((*x.shape[:-1], n), device=x.device)  # described, never written
@@ -235,7 +281,7 @@ class TorchOps(Ops):
 
     def linear(self, x, w, bias=None, add=()):
         self.count_linear(x, w)
-        y = x @ w.to(self.dtype).t()
+        y = x @ widen(w, self.dtype).t()
         if bias is not None:
             y = y + bias.to(self.dtype)
         for a in add:
@@ -271,11 +317,14 @@ def timestep_embedding(t, dim, dtype):
 
 class Model:
     """SD1.5's UNet with random weights: FP16 weight tensors ~N(0, 0.02),
-    biases ~N(0, 0.01), norm scales ~N(1, 0.1) and shifts ~N(0, 0.1)."""
+    biases ~N(0, 0.01), norm scales ~N(1, 0.1) and shifts ~N(0, 0.1).  With
+    weights "q4_0" or "q4_1" the linear layers' are those numbers in 4-bit
+    blocks, where a row is of whole blocks."""
 
-    def __init__(self, cfg, device, seed=0):
+    def __init__(self, cfg, device, seed=0, weights="f16"):
         self.cfg = cfg
         self.device = device
+        self.weights = weights
         gdev = device if torch.device(device).type == "cuda" else "cpu"
         self.gen = torch.Generator(device=gdev).manual_seed(seed)
         self.gdev = gdev
@@ -324,8 +373,12 @@ class Model:
     def _w(self, *shape):
         return self._randn(*shape, std=0.02).to(torch.float16)
 
+    def _linear_w(self, n, k):
+        w = self._w(n, k)
+        return w if self.weights == "f16" or k % sdhip.BLOCK else quantize(w, self.weights)
+
     def _lin(self, n, k, bias=True):
-        return (self._w(n, k), self._randn(n, std=0.01) if bias else None)
+        return (self._linear_w(n, k), self._randn(n, std=0.01) if bias else None)
 
     def _conv(self, oc, ic, k):
         return (self._w(oc, ic, k, k), self._randn(oc, std=0.01))
@@ -511,19 +564,21 @@ class SdxlBlock:
     projections (no bias), self-attention over `heads` heads, the output
     projection with its bias and the residual, LayerNorm, the GEGLU FF
     (C -> 2 x 4C with bias, gated) and its projection back with bias and the
-    residual; FP16 weights ~N(0, 0.02), biases ~N(0, 0.01), norms ~N(1, 0.1) /
-    ~N(0, 0.1).  `forward(ops, x)` for tokens x [b, L, C]."""
+    residual; FP16 weights ~N(0, 0.02), or those in 4-bit blocks (weights "q4_0"
+    or "q4_1"), biases ~N(0, 0.01), norms ~N(1, 0.1) / ~N(0, 0.1).
+    `forward(ops, x)` for tokens x [b, L, C]."""
 
-    def __init__(self, device, channels=1280, heads=20, seed=0):
+    def __init__(self, device, channels=1280, heads=20, seed=0, weights="f16"):
         m = object.__new__(Model)
         m.device = device
+        m.weights = weights
         gdev = device if torch.device(device).type == "cuda" else "cpu"
         m.gen = torch.Generator(device=gdev).manual_seed(seed)
         m.gdev = gdev
         c = channels
         self.heads = heads
         self.ln1, self.ln2 = m._norm(c), m._norm(c)
-        self.wq, self.wk, self.wv = (m._w(c, c) for _ in range(3))
+        self.wq, self.wk, self.wv = (m._linear_w(c, c) for _ in range(3))
         self.wo = m._lin(c, c)
         self.ff1 = m._lin(8 * c, c)
         self.ff2 = m._lin(c, 4 * c)
