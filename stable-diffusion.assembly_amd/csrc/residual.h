@@ -29,6 +29,7 @@ struct ResidualArgs {
     float *out;  // or null
     int64_t ynb[4], rnb[4], snb[4], onb[4];
     int64_t ne0, ne1, ne2, rows;
+    int64_t first;  // the launch's first row
     float branch_scale, residual_scale;
     RowNorm post, pre;
     RowOperand gate;

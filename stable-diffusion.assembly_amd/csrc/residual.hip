@@ -58,9 +58,9 @@ __device__ __forceinline__ double block_sum(double v, double *lds) {
 // A row a workgroup, read again for each of its sums: rows of any length.
 __global__ __launch_bounds__(kThreads) void norm_residual_long_kernel(ResidualArgs a) {
     __shared__ double lds[kThreads / 64];
-    const int64_t row = blockIdx.x;
+    const uint32_t row = static_cast<uint32_t>(a.first) + blockIdx.x;
     Place p;
-    split_index(static_cast<uint32_t>(row), static_cast<uint32_t>(a.ne1), static_cast<uint32_t>(a.ne2), p.i1, p.i2, p.i3);
+    split_index(row, static_cast<uint32_t>(a.ne1), static_cast<uint32_t>(a.ne2), p.i1, p.i2, p.i3);
     const float *y = a.y != nullptr ? a.y + row_at(a.ynb, p) : nullptr;
     const float *r = a.residual + row_at(a.rnb, p);
     float *sum = a.sum != nullptr ? a.sum + row_at(a.snb, p) : nullptr;
@@ -120,7 +120,8 @@ template <int T, int Q, bool QUADS>
 __global__ __launch_bounds__(T == 64 ? 256 : T) void norm_residual_rows_kernel(ResidualArgs a) {
     __shared__ double lds[4][T / 64];  // a sum each: no sum waits for the one before to be read
     const int tid = T == 64 ? threadIdx.x & 63 : threadIdx.x;
-    const uint32_t row = T == 64 ? blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
+    const uint32_t row = static_cast<uint32_t>(a.first) +
+                         (T == 64 ? blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x);
     if (row >= static_cast<uint32_t>(a.rows)) return;  // T = 64 only: its waves meet at no barrier
     Place p;
     split_index(row, static_cast<uint32_t>(a.ne1), static_cast<uint32_t>(a.ne2), p.i1, p.i2, p.i3);
@@ -262,14 +263,27 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void norm_residual_rows_kernel(R
     store(a.out + row_at(a.onb, p), s);
 }
 
-template <int T, int Q>
-void launch_rows(const ResidualArgs &a, bool quads, hipStream_t stream) {
-    const dim3 grid(static_cast<uint32_t>(T == 64 ? ceil_div(a.rows, 4) : a.rows)), block(T == 64 ? 256 : T);
-    if (quads) {
-        SDHIP_LAUNCH((norm_residual_rows_kernel<T, Q, true>), grid, block, 0, stream, a);
-    } else {
-        SDHIP_LAUNCH((norm_residual_rows_kernel<T, Q, false>), grid, block, 0, stream, a);
+// A launch holds 2^32 - 1 threads at most: 2^31 of them at a time, `threads` a row.
+template <class Launch>
+hipError_t by_rows(ResidualArgs a, int threads, Launch launch) {
+    const int64_t most = (int64_t{1} << 31) / threads;
+    for (; a.first < a.rows; a.first += most) {
+        launch(a, a.rows - a.first < most ? a.rows - a.first : most);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
+    return hipSuccess;
+}
+
+template <int T, int Q>
+hipError_t launch_rows(const ResidualArgs &args, bool quads, hipStream_t stream) {
+    return by_rows(args, T, [&](const ResidualArgs &a, int64_t rows) {
+        const dim3 grid(static_cast<uint32_t>(T == 64 ? ceil_div(rows, 4) : rows)), block(T == 64 ? 256 : T);
+        if (quads) {
+            SDHIP_LAUNCH((norm_residual_rows_kernel<T, Q, true>), grid, block, 0, stream, a);
+        } else {
+            SDHIP_LAUNCH((norm_residual_rows_kernel<T, Q, false>), grid, block, 0, stream, a);
+        }
+    });
 }
 
 }  // namespace
@@ -285,28 +299,18 @@ hipError_t launch_norm_residual(const ResidualArgs &a, hipStream_t stream) {
     // rows of 1280: 11.0 us, by four waves 13.5; 400 rows 5.8 and 5.5; one row of
     // 4096 by four waves 5.1 us, by sixteen 6.2; 2 x 4096 rows of 5120 122 and 210).
     const bool many = a.rows >= 4 * static_cast<int64_t>(compute_units());
-    if (a.ne0 <= 256) {
-        launch_rows<64, 1>(a, q, stream);
-    } else if (a.ne0 <= 512) {
-        launch_rows<64, 2>(a, q, stream);
-    } else if (many && a.ne0 <= 1280) {
-        launch_rows<64, 5>(a, q, stream);
-    } else if (a.ne0 <= 1024) {
-        launch_rows<256, 1>(a, q, stream);
-    } else if (a.ne0 <= 2048) {
-        launch_rows<256, 2>(a, q, stream);
-    } else if (a.ne0 <= 4096) {
-        launch_rows<256, 4>(a, q, stream);
-    } else if (a.ne0 <= 5120) {
-        launch_rows<256, 5>(a, q, stream);
-    } else if (a.ne0 <= 8192) {
-        launch_rows<512, 4>(a, q, stream);
-    } else if (a.ne0 <= 16384) {
-        launch_rows<1024, 4>(a, q, stream);
-    } else {
-        SDHIP_LAUNCH(norm_residual_long_kernel, dim3(static_cast<uint32_t>(a.rows)), dim3(kThreads), 0, stream, a);
-    }
-    return hipGetLastError();
+    if (a.ne0 <= 256) return launch_rows<64, 1>(a, q, stream);
+    if (a.ne0 <= 512) return launch_rows<64, 2>(a, q, stream);
+    if (many && a.ne0 <= 1280) return launch_rows<64, 5>(a, q, stream);
+    if (a.ne0 <= 1024) return launch_rows<256, 1>(a, q, stream);
+    if (a.ne0 <= 2048) return launch_rows<256, 2>(a, q, stream);
+    if (a.ne0 <= 4096) return launch_rows<256, 4>(a, q, stream);
+    if (a.ne0 <= 5120) return launch_rows<256, 5>(a, q, stream);
+    if (a.ne0 <= 8192) return launch_rows<512, 4>(a, q, stream);
+    if (a.ne0 <= 16384) return launch_rows<1024, 4>(a, q, stream);
+    return by_rows(a, kThreads, [&](const ResidualArgs &part, int64_t rows) {
+        SDHIP_LAUNCH(norm_residual_long_kernel, dim3(static_cast<uint32_t>(rows)), dim3(kThreads), 0, stream, part);
+    });
 }
 
 }  // namespace sdhip

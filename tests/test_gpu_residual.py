@@ -260,3 +260,19 @@ def test_captured_and_replayed(gpu, dim):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(s, want[0]) and torch.equal(o, want[1])
+
+
+@pytest.mark.gpu
+def test_more_rows_than_a_launch_takes(gpu):
+    """2^25 + 5 rows: a launch of 64 threads a row takes 2^25 of them."""
+    rows, dim = 2 ** 25 + 5, 4
+    y = torch.randn((rows, dim), device=gpu, generator=torch.Generator(gpu).manual_seed(5))
+    res = torch.randn((rows, dim), device=gpu, generator=torch.Generator(gpu).manual_seed(6))
+    out = torch.full_like(y, float("nan"))
+    sdhip.norm_residual(y, res, None, out, sdhip.row_norm("rms", 1e-6), sdhip.row_norm("none", 0.0))
+    torch.cuda.synchronize()
+    for part in (slice(0, 9), slice(rows // 2, rows // 2 + 9), slice(rows - 9, rows)):
+        v, r = y[part].double(), res[part].double()
+        z = v * (v.square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+        assert ((out[part].double() - (r + z)).abs() <= 10 * U * (z.abs() + r.abs())).all()
+    assert not out.isnan().any()
