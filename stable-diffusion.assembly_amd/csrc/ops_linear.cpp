@@ -62,20 +62,24 @@ Q4Args q4_args_of(const sdhip_tensor *w, const sdhip_tensor *x, const sdhip_tens
 }
 
 // Weights of 4 bits: one matrix of whole blocks of 32 along K, its rows any
-// even number of bytes apart that holds one, from one row of x up; extents
-// counted in 32 bits.
+// even number of bytes apart that holds one, from one row of x up.  Extents to
+// what a launch counts, 2^32 threads: by 512 of them, 8 rows of x a workgroup
+// or 32 rows by 1024 numbers of the weights; 64 x 128 outputs.
 bool q4_supported(const sdhip_tensor *w, const sdhip_tensor *x, const sdhip_tensor *y) {
+    constexpr int64_t kMost = int64_t{1} << 25, kWeights = int64_t{1} << 36, kOutputs = int64_t{1} << 35;
     const int64_t bytes = q4_block_bytes(w->type);
-    if (w->ne[0] > INT32_MAX || w->ne[1] < 1 || w->ne[1] > INT32_MAX || w->ne[2] != 1 || w->ne[3] != 1 ||
-        w->nb[1] % 2 != 0 || w->nb[1] < bytes * (w->ne[0] / kBlock) || reinterpret_cast<uintptr_t>(w->data) % 2 != 0) {
+    if (w->ne[0] > INT32_MAX || w->ne[1] < 1 || w->ne[1] > kMost || w->ne[1] > kWeights / w->ne[0] || w->ne[2] != 1 ||
+        w->ne[3] != 1 || w->nb[1] % 2 != 0 || w->nb[1] < bytes * (w->ne[0] / kBlock) ||
+        reinterpret_cast<uintptr_t>(w->data) % 2 != 0) {
         return false;
     }
     int64_t rows = 1;
     for (int k = 1; k < 4; ++k) {
-        if (x->ne[k] < 1 || x->ne[k] > INT32_MAX || y->ne[k] != x->ne[k]) return false;
+        if (x->ne[k] < 1 || x->ne[k] > kMost || y->ne[k] != x->ne[k]) return false;
         rows *= x->ne[k];
-        if (rows > INT32_MAX) return false;
+        if (rows > kMost) return false;
     }
+    if (w->ne[1] > kOutputs / rows) return false;
     return x->ne[0] == w->ne[0] && y->ne[0] == w->ne[1] && holds_f32(x) && contiguous(x) && holds_f32(y) &&
            contiguous(y);
 }

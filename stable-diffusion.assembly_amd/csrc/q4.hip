@@ -215,14 +215,22 @@ __device__ __forceinline__ void fetched() {
 // own as the 16-byte pieces of memory that hold them, wherever in those a
 // row begins (loads of each block by a lane of its own, at even addresses 18
 // bytes apart, moved 16384 rows of 4096 at 2.7 TB/s, aligned pieces at 5.3).
+// Each piece copied holds a byte of the row's, so none is of a page that the
+// weights are not in.
 // x is copied into LDS before them and split there, a wave taking 512 numbers
 // of a row at a time, each such part with a scale of its own and in its own
 // place; where x's rows take more than 64 KB, in chunks of K of as many parts
 // as fit.  Short calls spend their time on what runs once -- instructions
-// fetched, addresses, a barrier -- so little does.  The 16 rows of an MFMA are 4 on each group of lanes, of
-// which a result's 4 registers are the sums: up to 4 rows of x are one a group,
-// its hi in the first register and its lo in the second, up to 8 two a group,
-// so that one MFMA takes both parts; from 9 on two do.
+// fetched, addresses, a barrier -- so little does.
+//
+// The 16 rows of an MFMA are 4 on each group of lanes, of which a result's 4
+// registers are the sums: up to 4 rows of x are one a group, its hi in the
+// first register and its lo in the second, up to 8 two a group, so that one
+// MFMA takes both parts; from 9 on two do.
+//
+// 1 row of 1280 -> 1280: 3.9 us (an empty launch 1.7); of 4096 -> 16384, Q4_1,
+// 11.2 us, 3.7 TB/s of weights; 2 rows of 1280 -> 20160 9.0; 33 rows of 2080 ->
+// 1111 12.8; 154 of 768 -> 1280 10.8.
 constexpr int kFewWaves = 8;
 static_assert(kFewThreads == 64 * kFewWaves);
 constexpr int kUnit = 8;        // blocks
@@ -717,8 +725,11 @@ __global__ __launch_bounds__(kOperandThreads) void q4_operands_kernel(TileArgs t
 // one block of every WK: 16 v_mfma_f32_32x32x16_f16 a block.  The operands of
 // WK blocks come into LDS in runs, three stages of them in turn, asked for two
 // stages ahead.  A block's sums of products are scaled by d, 64 operations
-// beside the 36 that widen the words: 464 of the vector units' cycles a block
-// to 512 of the MFMA's.
+// beside the 36 that widen the words, 400 of the vector units' cycles a block
+// to 512 of the MFMA's.  Large products run at the clock that their power
+// leaves (1976 rows of 1280 -> 2 x 5120 gated 126 us; without any one of the
+// copies, the scaling, the widening or the barriers 116 .. 127, without the reads
+// of LDS 98).
 template <int WM, int WN, int WK>
 struct Tiles {
     static constexpr int kWaves = WM * WN * WK;

@@ -559,3 +559,22 @@ def test_work_buffer_is_all_that_is_written(gpu):
             finally:
                 sdhip.set_tuning("")
             assert (buf[:4096] == 77).all() and (buf[4096 + size:] == 77).all(), (form, kind)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", [0] + FORMS)
+def test_more_groups_of_rows_than_a_grid_s_second_dimension(gpu, form):
+    """16 65535 + 3 rows and more: whatever form is asked for, one that takes them."""
+    rows, k, n = 16 * 65535 + 3, 32, 5
+    r = rng(form)
+    blocks = q4_lib.random_blocks(r, "q4_0", n, k)
+    x = uniform(r, (rows, k), 1.0)
+    y = unwritten((rows, n), gpu)
+    sdhip.set_tuning(f"q4_form={form}")
+    try:
+        sdhip.mul_mat(dev(blocks, gpu), dev(x, gpu), y, sdhip.epilogue([]))
+        torch.cuda.synchronize()
+    finally:
+        sdhip.set_tuning("")
+    exact, mag = q4_lib.exact(blocks, x)
+    assert orc.metric(y.cpu().numpy(), exact, mag) <= q4_lib.bound(k)

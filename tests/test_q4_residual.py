@@ -69,6 +69,23 @@ def test_products_refused(kind):
     assert not lib.sdhip_mul_mat_gated_supported(good, x, rows(4, 70, data=99 * FAKE), rows(4, 35))
 
 
+def test_extents_that_a_launch_counts():
+    """Up to 2^25 rows of x and of the weights, 2^36 weights, 2^35 outputs."""
+    lib = sdhip.load()
+
+    def taken(m, n, k):
+        y = 1 << 50
+        return bool(lib.sdhip_mul_mat_supported(blocks(Q4_0, n, k), rows(m, k, data=1 << 45), rows(m, n, data=y)))
+
+    most = 1 << 25
+    assert taken(most, 1, 32) and not taken(most + 1, 1, 32)
+    assert taken(1, most, 32) and not taken(1, most + 1, 32)
+    assert taken(1, most, 2048) and not taken(1, most, 2080)
+    assert taken(1024, most, 32) and not taken(1025, most, 32)
+    assert not taken(1, 1, 1 << 31)
+    assert not lib.sdhip_mul_mat_supported(blocks(Q4_0, 1, 32), rows(2, 2, most // 2, 32), rows(2, 2, most // 2, 1))
+
+
 def test_product_over_an_operand_is_an_error():
     lib = sdhip.load()
     w, x = blocks(Q4_0, 320, 320), rows(4, 320)
