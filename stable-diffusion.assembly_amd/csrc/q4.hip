@@ -14,6 +14,8 @@
 // both parts), whose sums in single precision are then scaled by d and added
 // up; so no weight is rounded.
 
+#include <cmath>
+
 #include "host.h"
 #include "profile.h"
 #include "q4.h"
@@ -205,7 +207,7 @@ __device__ __forceinline__ void fetched() {
 
 // ------------------------------------------------------------------ few rows
 
-// Up to 16 rows of x.  A workgroup takes P tiles of 16 rows of the weights
+// Up to 16 rows of x a workgroup.  It takes P tiles of 16 rows of the weights
 // (with GATED, P / 2 of each half) by S splits of K, a wave each, P S = 8; a
 // split is every S-th unit of 8 blocks, and the splits' sums are added at the
 // end in their order.
@@ -230,7 +232,7 @@ __device__ __forceinline__ void fetched() {
 //
 // 1 row of 1280 -> 1280: 3.9 us (an empty launch 1.7); of 4096 -> 16384, Q4_1,
 // 11.2 us, 3.7 TB/s of weights; 2 rows of 1280 -> 20160 9.0; 33 rows of 2080 ->
-// 1111 12.8; 154 of 768 -> 1280 10.8.
+// 1111 8.8; 154 of 768 -> 1280 7.1.
 constexpr int kFewWaves = 8;
 static_assert(kFewThreads == 64 * kFewWaves);
 constexpr int kUnit = 8;        // blocks
@@ -478,28 +480,55 @@ __global__ __launch_bounds__(kFewThreads, 4) void q4_few_kernel(FewArgs f) {
     }
 }
 
-// The splits of K: until the device's waves all have one, two workgroups a CU,
-// within the units of a chunk.
-int few_splits(int64_t N, int64_t K, int rows, bool gated) {
-    const int64_t tiles = ceil_div(N, 16), units = ceil_div(K / kBlock, kUnit), chunk = kFewParts / rows * kPart / kUnit;
-    const int64_t waves = static_cast<int64_t>(compute_units()) * 2 * kFewWaves;
-    int splits = 1;
-    while (splits < (gated ? 4 : 8) && tiles * splits * 2 <= waves && splits < units && splits < chunk) splits *= 2;
-    return splits;
+// Rows a workgroup and splits of K: those of the least time, in us.  Beyond
+// 2.5 us that a call takes anyhow workgroups that share a CU add up: a part of x
+// 0.08, a unit of a wave's weights 0.8 (1.28 where its MFMAs are two), and a
+// start of 1.04 for every two that fit its LDS at once, or one (within 7 % of
+// what 630 calls of 1 .. 154 rows took, 320 -> 320 to 4096 -> 16384; the choices
+// by it 0.2 % slower than the fastest of all).  With 16 rows throughout, 33 rows
+// of 2080 -> 1111 took 12.8 us, now 8.8; 16 of 1280 -> 10240 16.6, now 9.9; 24 of
+// 768 -> 1280 6.8, now 5.0.  With 8 at most, 256 of 1280 -> 1280 18.7, now 14.6.
+struct FewShape {
+    int rows, splits;
+    float time;
+};
+
+FewShape few_shape(int64_t M, int64_t N, int64_t K, bool gated) {
+    constexpr int64_t kLdsBytes = 160 * 1024;
+    const auto shifted = [](int64_t v, int by) { return (v + (int64_t{1} << by) - 1) >> by; };  // v / 2^by, rounded up
+    const int64_t cus = compute_units(), tiles = ceil_div(N, 16), units = ceil_div(K / kBlock, kUnit);
+    FewShape best{0, 0, 0.0f};
+    int64_t least = 0;
+    for (int r = 0; r <= 4; ++r) {
+        const int64_t groups = shifted(M, r), parts = ceil_div(K / kBlock, kPart) << r;
+        const int64_t chunk = (kFewParts >> r) * (kPart / kUnit);
+        const bool two = 2 * ((parts < kFewParts ? parts : kFewParts) * kPartBytes + kFewWaves * kRing) <= kLdsBytes;
+        for (int s = 0; groups <= 65535 && s <= (gated ? 2 : 3); ++s) {
+            if (s > 0 && ((1 << (s - 1)) >= units || (1 << s) > chunk)) break;
+            const int64_t each = ceil_div(groups * ceil_div(tiles << s, kFewWaves), cus);  // a CU's workgroups
+            // In 0.08 us.
+            const int64_t cost = each * (shifted(units, s) * (r < 4 ? 10 : 16) + parts) + (two ? shifted(each, 1) : each) * 13;
+            if (best.rows == 0 || cost < least) {
+                best = {1 << r, 1 << s, 2.5f + 0.08f * static_cast<float>(cost)};
+                least = cost;
+            }
+        }
+        if ((1 << r) >= M) break;
+    }
+    return best;
 }
 
 template <bool LEAST, bool GATED, int ROWS>
-hipError_t launch_few(const Q4Args &a, hipStream_t stream) {
+hipError_t launch_few(const Q4Args &a, int splits, hipStream_t stream) {
     static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&q4_few_kernel<LEAST, GATED, ROWS>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize,
                                                        kFewParts * kPartBytes + kFewWaves * kRing);
     if (attr != hipSuccess) return attr;
     FewArgs f{};
     f.a = a;
-    f.splits = 1;
+    f.splits = splits;
     const int64_t columns = GATED ? a.half : a.N;
     const int64_t parts = ceil_div(a.K / kBlock, kPart) * ROWS;
-    f.splits = few_splits(a.N, a.K, ROWS, GATED);
     f.tiles = kFewWaves / f.splits;
     const dim3 grid(static_cast<uint32_t>(ceil_div(columns, 16 * (GATED ? f.tiles / 2 : f.tiles))),
                     static_cast<uint32_t>(ceil_div(a.M, ROWS)));
@@ -512,11 +541,19 @@ hipError_t launch_few(const Q4Args &a, hipStream_t stream) {
 
 template <bool LEAST, bool GATED>
 hipError_t few_rows(const Q4Args &a, hipStream_t stream) {
-    if (a.M == 1) return launch_few<LEAST, GATED, 1>(a, stream);
-    if (a.M == 2) return launch_few<LEAST, GATED, 2>(a, stream);
-    if (a.M <= 4) return launch_few<LEAST, GATED, 4>(a, stream);
-    if (a.M <= 8) return launch_few<LEAST, GATED, 8>(a, stream);
-    return launch_few<LEAST, GATED, 16>(a, stream);
+    const FewShape shape = few_shape(a.M, a.N, a.K, GATED);
+    switch (shape.rows) {
+    case 1:
+        return launch_few<LEAST, GATED, 1>(a, shape.splits, stream);
+    case 2:
+        return launch_few<LEAST, GATED, 2>(a, shape.splits, stream);
+    case 4:
+        return launch_few<LEAST, GATED, 4>(a, shape.splits, stream);
+    case 8:
+        return launch_few<LEAST, GATED, 8>(a, shape.splits, stream);
+    default:
+        return launch_few<LEAST, GATED, 16>(a, shape.splits, stream);
+    }
 }
 
 // ------------------------------------------------------------------ many rows
@@ -1256,19 +1293,24 @@ __global__ __launch_bounds__(kFewThreads, 2) void q4_mid_kernel(MidArgs f) {
     }
 }
 
+// Splits of K until every wave of the device has one.
+int mid_splits(int64_t M, int64_t N, int64_t K, bool gated) {
+    const int64_t waves = static_cast<int64_t>(compute_units()) * kFewWaves, units = ceil_div(K / kBlock, kUnit);
+    const int64_t tiles = ceil_div(N, 32) * ceil_div(M, M <= 32 ? 32 : 64);
+    int splits = 1;
+    while (splits < (gated ? 4 : 8) && tiles * splits * 2 <= waves && splits < units) splits *= 2;
+    return splits;
+}
+
 template <bool LEAST, bool GATED, int MT>
 hipError_t launch_mid(const TileArgs &t, hipStream_t stream) {
     constexpr int kLds = kFewWaves * 2 * kMidUnitBytes;
     static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&q4_mid_kernel<LEAST, GATED, MT>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (attr != hipSuccess) return attr;
-    MidArgs f{t, 1, kFewWaves};
-    const int64_t columns = GATED ? t.a.half : t.a.N, tiles = ceil_div(t.a.N, 32), rows = ceil_div(t.a.M, 32 * MT);
-    // Splits until every wave of the device has one.
-    const int64_t waves = static_cast<int64_t>(compute_units()) * kFewWaves, units = ceil_div(t.blocks, kUnit);
-    const int most = GATED ? 4 : 8;
-    while (f.splits < most && tiles * rows * f.splits * 2 <= waves && f.splits < units) f.splits *= 2;
-    f.tiles = kFewWaves / f.splits;
+    const int64_t columns = GATED ? t.a.half : t.a.N, rows = ceil_div(t.a.M, 32 * MT);
+    const int splits = mid_splits(t.a.M, t.a.N, t.a.K, GATED);
+    const MidArgs f{t, splits, kFewWaves / splits};
     const dim3 grid(static_cast<uint32_t>(ceil_div(columns, 32 * (GATED ? f.tiles / 2 : f.tiles))), static_cast<uint32_t>(rows));
     SDHIP_LAUNCH((q4_mid_kernel<LEAST, GATED, MT>), grid, dim3(kFewThreads), kLds, stream, f);
     return hipGetLastError();
@@ -1352,31 +1394,45 @@ hipError_t many_rows(const Q4Args &a, Form form, void *work, hipStream_t stream)
     }
 }
 
+// Up to 16 rows need no work buffer; more go by the form of the least time, in
+// us: a few percent to 14 off for 158 calls of 6 .. 400 rows, 320 -> 320 to 4096
+// -> 16384, and the choices by it 0.7 % slower than the fastest of all.
 Form form_of(int64_t M, int64_t N, int64_t K) {
-    const int64_t cus = compute_units();
-    const int64_t groups = ceil_div(M, 16) * ceil_div(ceil_div(N, 16) * few_splits(N, K, 16, false), kFewWaves);
     const int asked = tuning().q4_form;
     // A launch holds 65535 groups of rows at most.
     if (asked > 0 && !(asked == 1 && M > 16 * 65535) && !(asked == 2 && M > 32 * 65535)) return static_cast<Form>(asked);
-    // With no work buffer up to 16 rows, and as long as the workgroups of 16
-    // rows are on the device at once, or twice where K is short (64 rows of 1280
-    // -> 1280: 9.4 us, laid out 13.4, by tiles 19.1; 128 rows 16.9, 13.7 and 19.6;
-    // 128 of 768 -> 1280 12.1, 15.1 and 15.4).
-    if (M <= 16 || groups <= 2 * cus || (groups <= 4 * cus && K <= 1024)) return Form::few;
-    // Then x laid out, up to as many rows and columns as its L2 reads are
-    // fewer than the tiles' (256 rows of 4096 -> 4096 40.9 us, by tiles 44.8; 64
-    // of 1280 -> 10240 21.1 and 23.3, 96 29.4 and 24.1).
-    if (M <= 384 && ceil_div(M, 64) * N <= 16384) return Form::between;
-    // Tiles of 128 x 128 for two workgroups a CU or more go by four waves, each
-    // all of K: the two do not wait at one barrier (1976 rows of 1280 -> 2 x 5120
-    // gated 126 us, by eight waves 142).  Fewer are split along K inside a
-    // workgroup, by the shape of less stages one after another on a CU (1976
-    // rows of 1280 -> 1280: 128 x 128 by two 35.0 us, 64 x 128 by four 41.7; 33
-    // rows of 2080 -> 1111 43.2 and 29.6).
-    const auto tiles_of = [&](int rows) { return ceil_div(M, rows) * ceil_div(N, 128); };
-    const auto cost = [&](int rows, int split) { return ceil_div(tiles_of(rows), cus) * (ceil_div(K / kBlock, split) + 8); };
-    if (tiles_of(128) >= 2 * cus) return Form::tiles4;
-    return cost(128, 2) <= cost(64, 4) ? Form::tiles8 : Form::tiles64;
+    if (M <= 16) return Form::few;
+    const float cus = static_cast<float>(compute_units()), blocks = static_cast<float>(K / kBlock);
+    const float x = static_cast<float>(M) * static_cast<float>(K) * 1e-6f, w = static_cast<float>(N) * static_cast<float>(K) * 1e-6f;
+    Form best = Form::few;
+    float least = 0.0f;
+    const auto take = [&](Form form, float time) {
+        if (least == 0.0f || time < least) {
+            best = form;
+            least = time;
+        }
+    };
+    // A CU's workgroups, one after another, of `count`.
+    const auto rounds = [&](int64_t count) { return std::ceil(static_cast<float>(count) / cus); };
+    if (M <= 16 * 65535) take(Form::few, few_shape(M, N, K, false).time);
+    if (M <= 32 * 65535) {
+        // x is laid out; then by units of a wave's, of 32 rows of x or 64.
+        const int64_t splits = mid_splits(M, N, K, false);
+        const float units = static_cast<float>(ceil_div(ceil_div(K / kBlock, kUnit), splits));
+        const int64_t groups = ceil_div(M, M <= 32 ? 32 : 64) * ceil_div(ceil_div(N, 32) * splits, kFewWaves);
+        take(Form::between, 2.0f * x + rounds(groups) * (M <= 32 ? 6.5f + 5.0f * units : 9.0f + 7.0f * units));
+    }
+    // Both are laid out.  Tiles of 128 x 128 by four waves are two a CU, each all
+    // of K, and the two do not wait at one barrier (1976 rows of 1280 -> 2 x 5120
+    // gated 126 us, by eight waves 142); by eight waves, or of 64 x 128, they are
+    // split along K inside a workgroup (1976 rows of 1280 -> 1280: 128 x 128 by
+    // two 35.0 us, 64 x 128 by four 41.7).
+    const float both = 3.5f * x + 0.3f * w;
+    const float of128 = rounds(ceil_div(M, 128) * ceil_div(N, 128)), of64 = rounds(ceil_div(M, 64) * ceil_div(N, 128));
+    take(Form::tiles4, 6.5f + both + 4.5f * std::ceil(of128 / 2.0f) + 0.48f * blocks * of128);
+    take(Form::tiles8, 2.0f + both + of128 * (9.0f + 0.8f * std::ceil(blocks / 2.0f)));
+    take(Form::tiles64, 2.0f + both + of64 * (6.5f + 0.93f * std::ceil(blocks / 4.0f)));
+    return best;
 }
 
 }  // namespace

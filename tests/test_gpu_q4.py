@@ -578,3 +578,34 @@ def test_more_groups_of_rows_than_a_grid_s_second_dimension(gpu, form):
         sdhip.set_tuning("")
     exact, mag = q4_lib.exact(blocks, x)
     assert orc.metric(y.cpu().numpy(), exact, mag) <= q4_lib.bound(k)
+
+
+# Sizes by which the first form takes 1, 2, 4 and 8 rows a workgroup and K in 1,
+# 2, 4 and 8 splits, x in one chunk and in several.
+SHAPES = [(2, 96, 33), (1, 2080, 40001), (2, 544, 33), (2, 2080, 33), (100, 96, 257), (5, 544, 5001), (5, 2080, 5001),
+          (31, 544, 257), (16, 2080, 257), (15, 96, 5001), (33, 2080, 1000), (64, 544, 257), (31, 8224, 257),
+          (7, 96, 20000), (15, 544, 5001), (33, 544, 1000), (15, 8224, 1000), (257, 544, 1000), (16, 4128, 5000),
+          (16, 96, 20000), (256, 1280, 1280)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,k,n", SHAPES)
+def test_shapes_of_few_rows(gpu, kind, rows, k, n):
+    sdhip.set_tuning("q4_form=1")
+    try:
+        y, exact, mag = run(gpu, kind, rows, k, n, seed=rows + k + n)
+    finally:
+        sdhip.set_tuning("")
+    err = orc.metric(y.cpu().numpy(), exact, mag)
+    print(f"{kind} {rows} x {k} -> {n}: {err:.3g} of {q4_lib.bound(k):.3g}")
+    assert err <= q4_lib.bound(k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,k,n", [(2, 96, 1000), (2, 544, 1000), (33, 96, 1000), (9, 544, 1000), (31, 96, 2500),
+                                      (33, 2080, 1000), (7, 544, 2500), (7, 96, 20000), (31, 544, 2500), (33, 544, 1000),
+                                      (257, 544, 1000), (256, 1280, 1280)])
+def test_shapes_of_few_rows_gated(gpu, kind, rows, k, n):
+    test_forms_gated(gpu, kind, 1, rows, k, n)
