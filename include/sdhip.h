@@ -121,10 +121,10 @@ const char *sdhip_last_error(void);
  * instead of the panel kernels; 2: panels of 64 x 160 only, not 64 x 64),
  * conv_panels (0:
  * 1x1 convolutions by the 64 x 64 core), conv3x3_direct (0: F(4x4,3x3) where its
- * nine taps would be taken directly), q4_form (1 .. 5: the products of 4-bit
+ * nine taps would be taken directly), q4_form (1 .. 6: the products of 4-bit
  * weights by one of their forms -- each workgroup's rows of x split in it, x laid
- * out first, or both operands, tiles of 128 x 128 by four waves, by eight, or of
- * 64 x 128 -- whatever the size),
+ * out first, or both operands, tiles of 128 x 128 by four waves, by eight, of
+ * 64 x 128, or, not the gated ones, of 64 x 192 -- whatever the size),
  * attention_generic, attention_fp32 (forms to compare, same results within
  * the bounds -- qgemm_core's bit for bit), each taking only its documented
  * values.  Returns SDHIP_ERROR

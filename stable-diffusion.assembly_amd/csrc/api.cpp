@@ -159,8 +159,8 @@ bool in_range(Range r, long v, const char *&takes) {
         takes = "0, 1 or 2";
         return v >= 0 && v <= 2;
     case kForm:
-        takes = "0 to 5";
-        return v >= 0 && v <= 5;
+        takes = "0 to 6";
+        return v >= 0 && v <= 6;
     case kNonNegative:
         takes = "0 or more";
         return v >= 0 && v <= INT32_MAX;

@@ -71,9 +71,9 @@ struct Tuning {
     int conv3x3_direct = 1;
     // This library's own: the products of 4-bit weights by one form, or 0 to
     // choose by the size, for comparison; results agree within the same bound.
-    // 1 a workgroup's rows of x split in it; 2 x laid out first; 3 .. 5 both
-    // operands laid out first, tiles of 128 x 128 by four waves, by eight, or of
-    // 64 x 128.
+    // 1 a workgroup's rows of x split in it; 2 x laid out first; 3 .. 6 both
+    // operands laid out first, tiles of 128 x 128 by four waves, by eight, of
+    // 64 x 128, or of 64 x 192 (gated: chosen by the size).
     int q4_form = 0;
     // This library's own: attention by its generic form (1) even where the
     // fast one takes the operands (0), for comparison; results agree within

@@ -758,26 +758,28 @@ __global__ __launch_bounds__(kOperandThreads) void q4_operands_kernel(TileArgs t
     }
 }
 
-// Tiles of 64 WM rows of x by 64 WN of the weights, a wave 64 x 64 of them and
-// one block of every WK: 16 v_mfma_f32_32x32x16_f16 a block.  The operands of
+// Tiles of 64 WM rows of x by 32 TN WN of the weights, a wave 64 x 32 TN of them
+// and one block of every WK: 8 TN v_mfma_f32_32x32x16_f16 a block.  The operands of
 // WK blocks come into LDS in runs, three stages of them in turn, asked for two
-// stages ahead.  A block's sums of products are scaled by d, 64 operations
-// beside the 36 that widen the words, 400 of the vector units' cycles a block
-// to 512 of the MFMA's.  Large products run at the clock that their power
+// stages ahead.  With TN 2 a block's sums of products are scaled by d, 64
+// operations beside the 36 that widen the words, 400 of the vector units' cycles
+// a block to 512 of the MFMA's.  Large products run at the clock that their power
 // leaves (1976 rows of 1280 -> 2 x 5120 gated 126 us; without any one of the
 // copies, the scaling, the widening or the barriers 116 .. 127, without the reads
 // of LDS 98).
-template <int WM, int WN, int WK>
+template <int WM, int WN, int WK, int TN>
 struct Tiles {
     static constexpr int kWaves = WM * WN * WK;
     static constexpr int kThreads = 64 * kWaves;
     static constexpr int kNumbers = WM * 2 * 4;                   // KB a block
-    static constexpr int kWords = (WN * 2 * kWordsBytes + 1023) / 1024;  // KB a block, rounded up
+    static constexpr int kWords = (WN * TN * kWordsBytes + 1023) / 1024;  // KB a block, rounded up
     static constexpr int kPerBlock = kNumbers + kWords;
     static constexpr int kCopies = (WK * kPerBlock + kWaves - 1) / kWaves;  // a wave's, a stage
     static constexpr int kStage = kCopies * kWaves * 1024;
     static constexpr int kStages = 3;
-    static constexpr int kLds = kStages * kStage > (WK > 1 ? kWaves * 16384 : 0) ? kStages * kStage : kWaves * 16384;
+    static constexpr int kJoined = TN % 2 == 0 ? 2 : 1;  // of the TN whose sums the waves of WK blocks add up at a time
+    static constexpr int kSums = WK > 1 ? kWaves * kJoined * 8192 : 0;
+    static constexpr int kLds = kStages * kStage > kSums ? kStages * kStage : kSums;
 };
 
 // The order of what was written since the last sched_barrier: four MFMAs, N
@@ -792,9 +794,9 @@ __device__ __forceinline__ void mixed() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-template <bool LEAST, bool GATED, int WM, int WN, int WK>
+template <bool LEAST, bool GATED, int WM, int WN, int WK, int TN>
 __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs t) {
-    using L = Tiles<WM, WN, WK>;
+    using L = Tiles<WM, WN, WK, TN>;
     const Q4Args &a = t.a;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -815,7 +817,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs
         const int r = q % L::kPerBlock;
         block[c] = q / L::kPerBlock;
         from[c] = r < L::kNumbers ? t.numbers + mb * (WM * 2) * kNumbersBytes + 1024 * r
-                                  : t.words + nb * (WN * 2) * kWordsBytes + 1024 * (r - L::kNumbers);
+                                  : t.words + nb * (WN * TN) * kWordsBytes + 1024 * (r - L::kNumbers);
         step[c] = r < L::kNumbers ? t.row_tiles * kNumbersBytes : t.column_tiles * kWordsBytes;
     }
     const auto copy = [&](int s, int buffer, int c) {
@@ -826,19 +828,19 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs
     for (int s = 0; s < 3; ++s)
 #pragma unroll
         for (int c = 0; c < L::kCopies; ++c) copy(s, s, c);
-    float16v acc[2][2];
+    float16v acc[2][TN];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = float16v{};
+        for (int j = 0; j < TN; ++j) acc[i][j] = float16v{};
     const uint32_t magic = opaque(kMagic);
     const char *x = lds + wk * (L::kPerBlock * 1024) + wm * 8192 + 16 * lane;
-    const char *w = lds + wk * (L::kPerBlock * 1024) + L::kNumbers * 1024 + wn * 2 * static_cast<int>(kWordsBytes);
+    const char *w = lds + wk * (L::kPerBlock * 1024) + L::kNumbers * 1024 + wn * TN * static_cast<int>(kWordsBytes);
     struct Operands {
         half8 n[2][2][2];  // [32 rows][half of the block][hi, lo]
-        half8 v[2][2];     // [32 rows of the weights][half of the block]
-        uint2 words[2];    // v before it is widened
-        float d[2];
+        half8 v[TN][2];    // [32 rows of the weights][half of the block]
+        uint2 words[TN];   // v before it is widened
+        float d[TN];
     };
     const auto read = [&](Operands &o, int buffer) {
         const char *xs = x + buffer * L::kStage, *ws = w + buffer * L::kStage;
@@ -847,7 +849,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs
 #pragma unroll
             for (int p = 0; p < 4; ++p) o.n[i][p >> 1][p & 1] = *reinterpret_cast<const half8 *>(xs + 4096 * i + 1024 * p);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < TN; ++j) {
             o.words[j] = *reinterpret_cast<const uint2 *>(ws + kWordsBytes * j + 8 * lane);
             o.d[j] = *reinterpret_cast<const float *>(ws + kWordsBytes * j + 512 + 4 * (lane & 31));
         }
@@ -866,36 +868,39 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_fmaf(d, p[e], acc[i][j][e]);
     };
-    // A block's four products; a product's sums are added up while the MFMA
-    // makes the next one's, the last's in the next block.
+    // A block's products; a product's sums are added up while the MFMA makes the
+    // next one's, the last's in the next block.
     float16v kept = float16v{};
     float kept_d = 0.0f;
     const auto multiply = [&](const Operands &o, auto between) {
         __builtin_amdgcn_sched_barrier(0);
-        const float16v p00 = product(o, 0, 0);
-        between(0);
-        add(1, 1, kept_d, kept);
-        mixed<4>();
-        const float16v p10 = product(o, 1, 0);
-        between(1);
-        add(0, 0, o.d[0], p00);
-        mixed<4>();
-        const float16v p01 = product(o, 0, 1);
-        between(2);
-        add(1, 0, o.d[0], p10);
-        mixed<9>();
-        kept = product(o, 1, 1);
-        between(3);
-        add(0, 1, o.d[1], p01);
-        kept_d = o.d[1];
-        mixed<9>();
+        float16v p = kept;
+        float d = kept_d;
+        int i = 1, j = TN - 1;
+#pragma unroll
+        for (int k = 0; k < 2 * TN; ++k) {
+            const float16v next = product(o, k & 1, k >> 1);
+            between(k);
+            add(i, j, d, p);
+            p = next;
+            i = k & 1;
+            j = k >> 1;
+            d = o.d[j];
+            if (k < TN) {
+                mixed<4>();
+            } else {
+                mixed<9>();
+            }
+        }
+        kept = p;
+        kept_d = d;
     };
     fetched<2 * L::kCopies>();
     lds_barrier();
     Operands even, odd;
     read(even, 0);
-    widen_words(even, 0);
-    widen_words(even, 1);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) widen_words(even, j);
     int buffer = 0;
     // Stage s is multiplied from registers while stage s + 1 is read into
     // others; s + 2 is under way and s + 3 takes the buffer that s was read
@@ -907,10 +912,10 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs
         buffer = buffer == 2 ? 0 : buffer + 1;
         multiply(now, [&](int k) {
             if (k == 0) read(next, buffer);
-            if (k >= 2) widen_words(next, k - 2);
+            if (k >= TN) widen_words(next, k - TN);
 #pragma unroll
             for (int c = 0; c < L::kCopies; ++c)
-                if (c * 4 / L::kCopies == k) copy(s + 3, free, c);
+                if (c * 2 * TN / L::kCopies == k) copy(s + 3, free, c);
         });
     };
     int s = 0;
@@ -925,26 +930,26 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs
         ++s;
     }
     if (s * WK + wk < t.blocks) multiply(even, [](int) {});
-    add(1, 1, kept_d, kept);
+    add(1, TN - 1, kept_d, kept);
     fetched<0>();
     if constexpr (LEAST) {
         typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
         struct Parts {
-            bf16x8 u[2][3], v[2][3];
+            bf16x8 u[2][3], v[TN][3];
         };
         // Step k: 16 blocks, half k % 2 of the wave's group k / 2.
         const int steps = wk < t.groups ? 2 * ((t.groups - wk + WK - 1) / WK) : 0;
         const auto load = [&](int k, Parts &o) {
             const int64_t g = wk + (k >> 1) * WK;
             const char *sums = t.sums + (g * t.row_tiles + mb * (WM * 2) + wm * 2) * kOffsetsBytes + 3072 * (k & 1) + 16 * lane;
-            const char *offs = t.offsets + (g * t.column_tiles + nb * (WN * 2) + wn * 2) * kOffsetsBytes + 3072 * (k & 1) + 16 * lane;
+            const char *offs = t.offsets + (g * t.column_tiles + nb * (WN * TN) + wn * TN) * kOffsetsBytes + 3072 * (k & 1) + 16 * lane;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int p = 0; p < 3; ++p) {
 #pragma unroll
-                for (int p = 0; p < 3; ++p) {
-                    o.u[i][p] = *reinterpret_cast<const bf16x8 *>(sums + i * kOffsetsBytes + 1024 * p);
-                    o.v[i][p] = *reinterpret_cast<const bf16x8 *>(offs + i * kOffsetsBytes + 1024 * p);
-                }
+                for (int i = 0; i < 2; ++i) o.u[i][p] = *reinterpret_cast<const bf16x8 *>(sums + i * kOffsetsBytes + 1024 * p);
+#pragma unroll
+                for (int j = 0; j < TN; ++j) o.v[j][p] = *reinterpret_cast<const bf16x8 *>(offs + j * kOffsetsBytes + 1024 * p);
+            }
         };
         // The parts' products down to 2^-16 of the whole, the least first.
         const auto multiply_parts = [&](const Parts &o) {
@@ -955,7 +960,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j)
+                        for (int j = 0; j < TN; ++j)
                             acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(o.u[i][p], o.v[j][total - p], acc[i][j], 0, 0, 0);
         };
         Parts a0, a1;
@@ -968,32 +973,37 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs
             multiply_parts(a1);
         }
     }
-    // The outputs by quarters of the wave's, 8 rows a lane of both its columns:
-    // rows 16 (q % 2) .. of its 32 q / 2.  The waves of WK blocks add up a part
-    // of the quarters each; a wave alone takes one or two at a time.
+    // The outputs by quarters of the wave's, 8 rows a lane of kJoined of its
+    // columns: rows 16 (q % 2) .. of its 32 q / 2.  The waves of WK blocks add up
+    // a part of the quarters each; a wave alone takes one or two at a time.
+    constexpr int J = L::kJoined;
     constexpr int kQuarters = WK == 4 || (WK == 1 && GATED) ? 1 : 2;
-    if constexpr (WK > 1) {
-        lds_barrier();  // the last stage is read, and no copy is under way
-        float *sums = reinterpret_cast<float *>(lds) + wave * 4096 + lane;  // [quarter][j][e][lane]
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sums[((q * 2 + j) * 8 + e) * 64] = acc[q >> 1][j][8 * (q & 1) + e];
-        lds_barrier();
-    }
-    const float *all = reinterpret_cast<const float *>(lds) + (wave - wk) * 4096 + lane;
+    constexpr int kWaveSums = J * 2048;  // floats
+    static_assert(!GATED || TN == 2);
+    const float *all = reinterpret_cast<const float *>(lds) + (wave - wk) * kWaveSums + lane;
     const int64_t columns = GATED ? a.half : a.N;
-    const int m0 = mb * (64 * WM) + wm * 64 + 4 * (lane >> 5), n0 = nb * (GATED ? 32 * WN : 64 * WN) + wn * (GATED ? 32 : 64) + (lane & 31);
+    const int m0 = mb * (64 * WM) + wm * 64 + 4 * (lane >> 5);
+    const int first = (nb * WN + wn) * (GATED ? 32 : 32 * TN) + (lane & 31);
 #pragma unroll
-    for (int round = 0; round < 4 / WK / kQuarters; ++round) {
+    for (int round = 0; round < TN / J * (4 / WK / kQuarters); ++round) {
+        const int j0 = WK == 1 ? 0 : J * round, n0 = first + 32 * j0;
+        if constexpr (WK > 1) {
+            lds_barrier();  // the last stage is read, and no copy is under way; the sums before are
+            float *sums = reinterpret_cast<float *>(lds) + wave * kWaveSums + lane;  // [quarter][j][e][lane]
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sums[((q * J + j) * 8 + e) * 64] = acc[q >> 1][j0 + j][8 * (q & 1) + e];
+            lds_barrier();
+        }
         const int q0 = WK == 1 ? kQuarters * round : wk * kQuarters;
-        float v[kQuarters][2][8];
+        float v[kQuarters][J][8];
 #pragma unroll
         for (int q = 0; q < kQuarters; ++q)
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < J; ++j)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     if constexpr (WK == 1) {
@@ -1001,7 +1011,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs
                     } else {
                         v[q][j][e] = 0.0f;
 #pragma unroll
-                        for (int k = 0; k < WK; ++k) v[q][j][e] += all[k * 4096 + (((q0 + q) * 2 + j) * 8 + e) * 64];
+                        for (int k = 0; k < WK; ++k) v[q][j][e] += all[k * kWaveSums + (((q0 + q) * J + j) * 8 + e) * 64];
                     }
                 }
         const auto row_of = [&](int q, int e) { return m0 + 16 * (q0 + q) + tile_row(e); };
@@ -1015,14 +1025,14 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float back = t.back[row_of(q, e)];
-                v[q][0][e] *= back;
-                v[q][1][e] *= back;
+#pragma unroll
+                for (int j = 0; j < J; ++j) v[q][j][e] *= back;
             }
         if (!GATED && a.from_redirect) {
 #pragma unroll
             for (int q = 0; q < kQuarters; ++q)
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+                for (int j = 0; j < J; ++j)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const int64_t m = row_of(q, e) < last ? row_of(q, e) : last;
@@ -1037,14 +1047,14 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs
 #pragma unroll
                 for (int q = 0; q < kQuarters; ++q)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
+                    for (int j = 0; j < J; ++j)
 #pragma unroll
                         for (int e = 0; e < 8; ++e) v[q][j][e] = silu(v[q][j][e]);
                 continue;
             }
-            float o[kQuarters][2][8];
+            float o[kQuarters][J][8];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < J; ++j) {
                 const float *at = st.operand + column_of(j) * st.nb[0];
                 if (st.flat123 && st.nb[1] == 0) {
                     const float one = *at;
@@ -1074,7 +1084,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs
 #pragma unroll
             for (int q = 0; q < kQuarters; ++q)
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+                for (int j = 0; j < J; ++j)
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
                         v[q][j][e] = st.kind == kAdd ? __fadd_rn(v[q][j][e], o[q][j][e]) : __fmul_rn(v[q][j][e], o[q][j][e]);
@@ -1086,26 +1096,27 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void q4_tiles_kernel(TileArgs
                 const int64_t m = row_of(q, e);
                 if (m > last) continue;
                 float *y = a.y + m * a.ldy;
-                if (GATED) {
+                if constexpr (GATED) {
                     if (n0 < columns) y[n0] = v[q][0][e] * gelu(v[q][1][e]);
                 } else {
-                    if (n0 < columns) y[n0] = v[q][0][e];
-                    if (n0 + 32 < columns) y[n0 + 32] = v[q][1][e];
+#pragma unroll
+                    for (int j = 0; j < J; ++j)
+                        if (n0 + 32 * j < columns) y[n0 + 32 * j] = v[q][j][e];
                 }
             }
     }
 }
 
-template <bool LEAST, bool GATED, int WM, int WN, int WK>
+template <bool LEAST, bool GATED, int WM, int WN, int WK, int TN>
 hipError_t launch_tiles(TileArgs t, hipStream_t stream) {
-    using L = Tiles<WM, WN, WK>;
+    using L = Tiles<WM, WN, WK, TN>;
     static const hipError_t attr =
-        hipFuncSetAttribute(reinterpret_cast<const void *>(&q4_tiles_kernel<LEAST, GATED, WM, WN, WK>),
+        hipFuncSetAttribute(reinterpret_cast<const void *>(&q4_tiles_kernel<LEAST, GATED, WM, WN, WK, TN>),
                             hipFuncAttributeMaxDynamicSharedMemorySize, L::kLds);
     if (attr != hipSuccess) return attr;
     t.m_blocks = static_cast<int32_t>(ceil_div(t.a.M, 64 * WM));
-    t.n_blocks = static_cast<int32_t>(GATED ? ceil_div(t.a.half, 32 * WN) : ceil_div(t.a.N, 64 * WN));
-    SDHIP_LAUNCH((q4_tiles_kernel<LEAST, GATED, WM, WN, WK>), dim3(static_cast<uint32_t>(t.m_blocks * t.n_blocks)),
+    t.n_blocks = static_cast<int32_t>(GATED ? ceil_div(t.a.half, 32 * WN) : ceil_div(t.a.N, 32 * TN * WN));
+    SDHIP_LAUNCH((q4_tiles_kernel<LEAST, GATED, WM, WN, WK, TN>), dim3(static_cast<uint32_t>(t.m_blocks * t.n_blocks)),
                  dim3(L::kThreads), L::kLds, stream, t);
     return hipGetLastError();
 }
@@ -1325,9 +1336,10 @@ struct TilesWork {
 // With `weights` those too are laid out, for the tiles.
 TilesWork tiles_work(int64_t M, int64_t N, int64_t half, int64_t K, bool least, bool weights) {
     TilesWork w{};
-    // Whole workgroups' tiles, whichever shape is taken: up to 128 rows by 128.
+    // Whole workgroups' tiles, whichever shape is taken: 64 or 128 rows by 128
+    // or 192.
     w.row_tiles = round_up(ceil_div(M, kRowsTile), 4);
-    w.column_tiles = !weights ? 0 : round_up(half ? 2 * ceil_div(half, kRowsTile) : ceil_div(N, kRowsTile), 4);
+    w.column_tiles = !weights ? 0 : round_up(half ? 2 * ceil_div(half, kRowsTile) : ceil_div(N, kRowsTile), 12);
     w.blocks = K / kBlock;
     w.groups = least ? ceil_div(w.blocks, 32) : 0;
     size_t at = 0;
@@ -1347,7 +1359,7 @@ TilesWork tiles_work(int64_t M, int64_t N, int64_t half, int64_t K, bool least, 
 
 // Which kernels a product of these extents takes, gated or not, numbered as
 // the q4_form tuning asks for them.
-enum class Form { few = 1, between, tiles4, tiles8, tiles64 };
+enum class Form { few = 1, between, tiles4, tiles8, tiles64, tiles192 };
 
 // The operands laid out in the work buffer.
 template <bool LEAST, bool GATED>
@@ -1386,21 +1398,27 @@ hipError_t many_rows(const Q4Args &a, Form form, void *work, hipStream_t stream)
     if (const hipError_t e = lay_out<LEAST, GATED>(a, work, true, t, stream); e != hipSuccess) return e;
     switch (form) {
     case Form::tiles4:
-        return launch_tiles<LEAST, GATED, 2, 2, 1>(t, stream);
+        return launch_tiles<LEAST, GATED, 2, 2, 1, 2>(t, stream);
     case Form::tiles8:
-        return launch_tiles<LEAST, GATED, 2, 2, 2>(t, stream);
+        return launch_tiles<LEAST, GATED, 2, 2, 2, 2>(t, stream);
+    case Form::tiles192:
+        if constexpr (!GATED) return launch_tiles<LEAST, GATED, 1, 2, 4, 3>(t, stream);
+        [[fallthrough]];
     default:
-        return launch_tiles<LEAST, GATED, 1, 2, 4>(t, stream);
+        return launch_tiles<LEAST, GATED, 1, 2, 4, 2>(t, stream);
     }
 }
 
 // Up to 16 rows need no work buffer; more go by the form of the least time, in
-// us: a few percent to 14 off for 158 calls of 6 .. 400 rows, 320 -> 320 to 4096
-// -> 16384, and the choices by it 0.7 % slower than the fastest of all.
-Form form_of(int64_t M, int64_t N, int64_t K) {
+// us: within 6 to 14 % of what 300 calls of 17 .. 8192 rows took, 320 -> 320 to 4096
+// -> 16384, and the choices by it 1 % slower than the fastest of all.  Tiles of
+// 192 are not paired for the gated product.
+Form form_of(int64_t M, int64_t N, int64_t K, bool gated) {
     const int asked = tuning().q4_form;
     // A launch holds 65535 groups of rows at most.
-    if (asked > 0 && !(asked == 1 && M > 16 * 65535) && !(asked == 2 && M > 32 * 65535)) return static_cast<Form>(asked);
+    if (asked > 0 && !(asked == 1 && M > 16 * 65535) && !(asked == 2 && M > 32 * 65535) && !(asked == 6 && gated)) {
+        return static_cast<Form>(asked);
+    }
     if (M <= 16) return Form::few;
     const float cus = static_cast<float>(compute_units()), blocks = static_cast<float>(K / kBlock);
     const float x = static_cast<float>(M) * static_cast<float>(K) * 1e-6f, w = static_cast<float>(N) * static_cast<float>(K) * 1e-6f;
@@ -1414,42 +1432,45 @@ Form form_of(int64_t M, int64_t N, int64_t K) {
     };
     // A CU's workgroups, one after another, of `count`.
     const auto rounds = [&](int64_t count) { return std::ceil(static_cast<float>(count) / cus); };
-    if (M <= 16 * 65535) take(Form::few, few_shape(M, N, K, false).time);
+    if (M <= 16 * 65535) take(Form::few, few_shape(M, N, K, gated).time);
     if (M <= 32 * 65535) {
         // x is laid out; then by units of a wave's, of 32 rows of x or 64.
-        const int64_t splits = mid_splits(M, N, K, false);
+        const int64_t splits = mid_splits(M, N, K, gated);
         const float units = static_cast<float>(ceil_div(ceil_div(K / kBlock, kUnit), splits));
         const int64_t groups = ceil_div(M, M <= 32 ? 32 : 64) * ceil_div(ceil_div(N, 32) * splits, kFewWaves);
         take(Form::between, 2.0f * x + rounds(groups) * (M <= 32 ? 6.5f + 5.0f * units : 9.0f + 7.0f * units));
     }
     // Both are laid out.  Tiles of 128 x 128 by four waves are two a CU, each all
     // of K, and the two do not wait at one barrier (1976 rows of 1280 -> 2 x 5120
-    // gated 126 us, by eight waves 142); by eight waves, or of 64 x 128, they are
-    // split along K inside a workgroup (1976 rows of 1280 -> 1280: 128 x 128 by
-    // two 35.0 us, 64 x 128 by four 41.7).
-    const float both = 3.5f * x + 0.3f * w;
+    // gated 126 us, by eight waves 142); by eight waves, or of 64 rows, they are
+    // split along K inside a workgroup (1976 rows of 5120 -> 1280, tiles that
+    // leave some CUs without one: 128 x 128 by four waves 99.6 us, by eight 87.8, 64
+    // x 128 99.1, 64 x 192 78.4; 988 rows of 1280 -> 1280 35.4, 31.2, 23.9, 29.1).
+    const float both = 1.9f * x + 0.3f * w;
     const float of128 = rounds(ceil_div(M, 128) * ceil_div(N, 128)), of64 = rounds(ceil_div(M, 64) * ceil_div(N, 128));
-    take(Form::tiles4, 6.5f + both + 4.5f * std::ceil(of128 / 2.0f) + 0.48f * blocks * of128);
-    take(Form::tiles8, 2.0f + both + of128 * (9.0f + 0.8f * std::ceil(blocks / 2.0f)));
-    take(Form::tiles64, 2.0f + both + of64 * (6.5f + 0.93f * std::ceil(blocks / 4.0f)));
+    const float of192 = rounds(ceil_div(M, 64) * ceil_div(N, 192));
+    take(Form::tiles4, 4.2f + both + 8.5f * std::ceil(of128 / 2.0f) + 0.46f * blocks * of128);
+    take(Form::tiles8, 3.0f + both + of128 * (8.7f + 0.8f * std::ceil(blocks / 2.0f)));
+    take(Form::tiles64, 4.5f + both + of64 * (6.0f + 0.92f * std::ceil(blocks / 4.0f)));
+    if (!gated) take(Form::tiles192, 4.7f + both + of192 * (10.2f + 1.12f * std::ceil(blocks / 4.0f)));
     return best;
 }
 
 }  // namespace
 
 size_t q4_work_size(int64_t M, int64_t N, int64_t K, bool least) {
-    const Form form = form_of(M, N, K);
-    if (form == Form::few) return 0;
+    const auto bytes = [&](bool gated) -> size_t {
+        const Form form = form_of(M, N, K, gated);
+        return form == Form::few ? 0 : tiles_work(M, N, gated ? N / 2 : 0, K, least, form != Form::between).bytes;
+    };
     // The plain and the gated product of one size take one size of buffer.
-    const bool weights = form != Form::between;
-    const size_t plain = tiles_work(M, N, 0, K, least, weights).bytes;
-    const size_t gated = N % 2 == 0 ? tiles_work(M, N, N / 2, K, least, weights).bytes : 0;
+    const size_t plain = bytes(false), gated = N % 2 == 0 ? bytes(true) : 0;
     return plain > gated ? plain : gated;
 }
 
 template <bool LEAST, bool GATED>
 static hipError_t launch_form(const Q4Args &a, void *work, hipStream_t stream) {
-    const Form form = form_of(a.M, a.N, a.K);
+    const Form form = form_of(a.M, a.N, a.K, GATED);
     if (form == Form::few) return few_rows<LEAST, GATED>(a, stream);
     if (form == Form::between) return between_rows<LEAST, GATED>(a, work, stream);
     return many_rows<LEAST, GATED>(a, form, work, stream);

@@ -374,7 +374,7 @@ def test_refusals_leave_the_output(gpu):
     assert torch.isnan(y).all()
 
 
-FORMS = [1, 2, 3, 4, 5]
+FORMS = [1, 2, 3, 4, 5, 6]
 
 
 @pytest.mark.gpu

@@ -219,15 +219,15 @@ def test_forms_tuning():
     lib = sdhip.load()
     w, x, y = blocks(Q4_0, 320, 320), rows(40, 320), rows(40, 320)
     try:
-        for bad in ("q4_form=6", "q4_form=-1"):
+        for bad in ("q4_form=7", "q4_form=-1"):
             with pytest.raises(sdhip.SdhipError):
                 sdhip.set_tuning(bad)
         sizes = []
-        for form in range(1, 6):
+        for form in range(1, 7):
             sdhip.set_tuning(f"q4_form={form}")
             assert sdhip.get_tuning("q4_form") == form
             sizes.append(lib.sdhip_mul_mat_work_size(w, x, y))
-        assert sizes[0] == 0 < sizes[1] < sizes[2] and sizes[2] == sizes[3] == sizes[4]
+        assert sizes[0] == 0 < sizes[1] < sizes[2] and sizes[2] == sizes[3] == sizes[4] == sizes[5]
     finally:
         sdhip.set_tuning("")
     assert sdhip.get_tuning("q4_form") == 0
