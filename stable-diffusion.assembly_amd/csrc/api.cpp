@@ -185,8 +185,12 @@ bool holds_q4(const sdhip_tensor *t) {
 
 bool contiguous(const sdhip_tensor *t) {
     const int64_t size = t->type == SDHIP_TYPE_F16 ? 2 : 4;
-    return t->nb[0] == size && t->nb[1] == t->nb[0] * t->ne[0] && t->nb[2] == t->nb[1] * t->ne[1] &&
-           t->nb[3] == t->nb[2] * t->ne[2];
+    if (t->nb[0] != size) return false;
+    for (int k = 1; k < 4; ++k) {
+        int64_t next;
+        if (__builtin_mul_overflow(t->nb[k - 1], t->ne[k - 1], &next) || t->nb[k] != next) return false;
+    }
+    return true;
 }
 
 bool same_shape(const sdhip_tensor *a, const sdhip_tensor *b) {
@@ -212,10 +216,12 @@ size_t tensor_span(const sdhip_tensor *t) {
     for (int k = 0; k < 4; ++k) {
         if (t->ne[k] <= 0) return 0;
         if (t->nb[k] < 0) return SIZE_MAX;
-        const int64_t count = q4 && k == 0 ? ceil_div(t->ne[0], kBlock) : t->ne[k];
-        const uint64_t reach = static_cast<uint64_t>(count - 1) * static_cast<uint64_t>(t->nb[k]);
-        if (reach > SIZE_MAX - n) return SIZE_MAX;
-        n += static_cast<size_t>(reach);
+        const int64_t count = q4 && k == 0 ? (t->ne[0] - 1) / kBlock + 1 : t->ne[k];
+        size_t reach;
+        if (__builtin_mul_overflow(static_cast<size_t>(count - 1), static_cast<size_t>(t->nb[k]), &reach) || reach > SIZE_MAX - n) {
+            return SIZE_MAX;
+        }
+        n += reach;
     }
     return n;
 }
