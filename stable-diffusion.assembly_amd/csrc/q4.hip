@@ -231,7 +231,7 @@ __device__ __forceinline__ void fetched() {
 // MFMA takes both parts; from 9 on two do.
 //
 // 1 row of 1280 -> 1280: 3.9 us (an empty launch 1.7); of 4096 -> 16384, Q4_1,
-// 11.2 us, 3.7 TB/s of weights; 2 rows of 1280 -> 20160 9.0; 33 rows of 2080 ->
+// 10.8 us, 3.9 TB/s of weights; 2 rows of 1280 -> 20160 8.3; 33 rows of 2080 ->
 // 1111 8.8; 154 of 768 -> 1280 7.1.
 constexpr int kFewWaves = 8;
 static_assert(kFewThreads == 64 * kFewWaves);
@@ -605,7 +605,8 @@ constexpr int kOperandRows = 8;  // of x a workgroup
 // A wave takes 2 blocks of the 8 rows at a time, 8 lanes a row, so that what it
 // reads of a row lies together and what it writes of them does too; the first
 // kKept such times are kept in registers while the rows' greatest are found
-// (1976 rows of 5120: 30 us with a row a wave, written 16 bytes here and there).
+// (1976 rows of 5120: 30 us with a row a wave, written 16 bytes here and there, now
+// 18.5, 5.9 TB/s).
 template <bool LEAST, bool GATED>
 __global__ __launch_bounds__(kOperandThreads) void q4_operands_kernel(TileArgs t) {
     const Q4Args &a = t.a;
@@ -1129,7 +1130,9 @@ hipError_t launch_tiles(TileArgs t, hipStream_t stream) {
 // 32 MT rows of x; a wave's weights come into LDS of its own by units of 8
 // blocks, two of them in flight, as few rows' do, and x from L2 as the MFMA's
 // lanes want it, a block ahead.  Q4_1's offsets go by bfloat16 parts as the
-// tiles' do, a unit's 8 blocks one step of v_mfma_f32_32x32x8_bf16.
+// tiles' do, a unit's 8 blocks one step of v_mfma_f32_32x32x8_bf16.  Bound by x's
+// loads from L2, 4 KB a wave, block and 32 rows (256 rows of 4096 -> 4096 39.3 us,
+// by tiles 46.0, each workgroup's rows split in it 65.5; 1976 by tiles 148).
 constexpr int kMidCopies = 6;
 constexpr int kMidUnitBytes = kMidCopies * 1024;
 
