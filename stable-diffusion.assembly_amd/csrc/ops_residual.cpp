@@ -159,6 +159,7 @@ sdhip_status sdhip_norm_residual(const sdhip_tensor *y, const sdhip_row_norm *po
     strides_of(sum, a.snb);
     strides_of(out, a.onb);
     a.ne0 = residual->ne[0];
+    a.inverse = 1.0 / static_cast<double>(a.ne0);
     a.ne1 = residual->ne[1];
     a.ne2 = residual->ne[2];
     a.rows = residual->ne[1] * residual->ne[2] * residual->ne[3];

@@ -30,6 +30,7 @@ struct ResidualArgs {
     int64_t ynb[4], rnb[4], snb[4], onb[4];
     int64_t ne0, ne1, ne2, rows;
     int64_t first;  // the launch's first row
+    double inverse;  // 1 / ne0
     float branch_scale, residual_scale;
     RowNorm post, pre;
     RowOperand gate;

@@ -8,7 +8,7 @@
 // and out written once, the row in registers between its sums, T threads a
 // row, up to 4 Q numbers each (norm_residual_rows_kernel); longer rows are
 // read again for every sum (norm_residual_long_kernel).  2 x 4096 rows of 5120
-// 121 us, 5.5 TB/s of their 671 MB; one row of 4096 4.6 us, of which a launch is 1.7
+// 120 us, 5.6 TB/s of their 671 MB; one row of 4096 4.45 us, of which a launch is 1.7
 // and the rest two sums one after the other.
 
 #include "host.h"
@@ -34,13 +34,25 @@ struct Moments {
     float hi, lo, scale;
 };
 
-__device__ __forceinline__ Moments moments(int32_t kind, double mean, double squares, double n, float eps) {
+// 1 / sqrt(v) within 2^-45 of itself: the hardware's, within 2^-24 or so, by one
+// step of Newton's, a fifth of the operations of a root and a division (2 x 988
+// rows of 2048 14.0 us, so 13.4; one of 4096 4.61 and 4.45).
+__device__ __forceinline__ double inverse_root(double v) {
+    const double r = __builtin_amdgcn_rsq(v);
+    const double next = __builtin_fma(0.5 * r, __builtin_fma(-v * r, r, 1.0), r);
+    return v > 0.0 && v < __builtin_inf() ? next : r;
+}
+
+// `squares` over n numbers, of which `inverse` is 1 / n.
+__device__ __forceinline__ Moments moments(int32_t kind, double mean, double squares, double inverse, float eps) {
     Moments m{0.0f, 0.0f, 1.0f};
     if (kind == SDHIP_ROW_NORM_LAYER) {
         m.hi = static_cast<float>(mean);
         m.lo = static_cast<float>(mean - static_cast<double>(m.hi));
     }
-    if (kind != SDHIP_ROW_NORM_NONE) m.scale = static_cast<float>(1.0 / sqrt(squares / n + static_cast<double>(eps)));
+    if (kind != SDHIP_ROW_NORM_NONE) {
+        m.scale = static_cast<float>(inverse_root(__builtin_fma(squares, inverse, static_cast<double>(eps))));
+    }
     return m;
 }
 
@@ -57,6 +69,35 @@ __device__ __forceinline__ double block_sum(double v, double *lds) {
     return s;
 }
 
+// The sum of the wave's lanes, on all of them, the same bits: within rows of 16
+// lanes by DPP, across them by swaps, which wait for no LDS as shuffles do
+// (one row of 4096: 4.96 us by shuffles, so 4.59).
+template <int CTRL>
+__device__ __forceinline__ double moved(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t low = __builtin_amdgcn_update_dpp(0, static_cast<uint32_t>(u), CTRL, 0xf, 0xf, true);
+    const uint32_t high = __builtin_amdgcn_update_dpp(0, static_cast<uint32_t>(u >> 32), CTRL, 0xf, 0xf, true);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(high) << 32 | low);
+}
+
+__device__ __forceinline__ double wave_sum(double v) {
+    v += moved<0xb1>(v);   // lanes i ^ 1
+    v += moved<0x4e>(v);   // i ^ 2
+    v += moved<0x141>(v);  // 8 lanes mirrored
+    v += moved<0x140>(v);  // 16 lanes mirrored
+    const auto joined = [](const auto &low, const auto &high) {
+        return __builtin_bit_cast(double, static_cast<uint64_t>(high[0]) << 32 | low[0]) +
+               __builtin_bit_cast(double, static_cast<uint64_t>(high[1]) << 32 | low[1]);
+    };
+    uint64_t u = __builtin_bit_cast(uint64_t, v);
+    uint32_t low = static_cast<uint32_t>(u), high = static_cast<uint32_t>(u >> 32);
+    v = joined(__builtin_amdgcn_permlane16_swap(low, low, false, false), __builtin_amdgcn_permlane16_swap(high, high, false, false));
+    u = __builtin_bit_cast(uint64_t, v);
+    low = static_cast<uint32_t>(u);
+    high = static_cast<uint32_t>(u >> 32);
+    return joined(__builtin_amdgcn_permlane32_swap(low, low, false, false), __builtin_amdgcn_permlane32_swap(high, high, false, false));
+}
+
 // A row a workgroup, read again for each of its sums: rows of any length.
 __global__ __launch_bounds__(kThreads) void norm_residual_long_kernel(ResidualArgs a) {
     __shared__ double lds[kThreads / 64];
@@ -67,13 +108,12 @@ __global__ __launch_bounds__(kThreads) void norm_residual_long_kernel(ResidualAr
     const float *r = a.residual + row_at(a.rnb, p);
     float *sum = a.sum != nullptr ? a.sum + row_at(a.snb, p) : nullptr;
     float *out = a.out != nullptr ? a.out + row_at(a.onb, p) : nullptr;
-    const double n = static_cast<double>(a.ne0);
     const auto stats = [&](int32_t kind, float eps, auto value) {
         double mean = 0.0, squares = 0.0;
         if (kind == SDHIP_ROW_NORM_LAYER) {
             double s = 0.0;
             for (int64_t i = threadIdx.x; i < a.ne0; i += kThreads) s += static_cast<double>(value(i));
-            mean = block_sum(s, lds) / n;
+            mean = block_sum(s, lds) * a.inverse;
         }
         if (kind != SDHIP_ROW_NORM_NONE) {
             double s = 0.0;
@@ -83,7 +123,7 @@ __global__ __launch_bounds__(kThreads) void norm_residual_long_kernel(ResidualAr
             }
             squares = block_sum(s, lds);
         }
-        return moments(kind, mean, squares, n, eps);
+        return moments(kind, mean, squares, a.inverse, eps);
     };
     const auto affine = [&](const RowNorm &w, float v, int64_t i) {
         if (w.weight.data != nullptr) {
@@ -170,8 +210,7 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void norm_residual_rows_kernel(R
     };
     int sums = 0;
     const auto total = [&](double v) {
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+        v = wave_sum(v);
         if constexpr (T > 64) {
             if ((tid & 63) == 0) lds[sums][tid >> 6] = v;
             __syncthreads();
@@ -190,7 +229,7 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void norm_residual_rows_kernel(R
             for (int u = 0; u < Q; ++u)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) s += static_cast<double>(v[u][k]);
-            mean = total(s) / static_cast<double>(n);
+            mean = total(s) * a.inverse;
         }
 #pragma unroll
         for (int u = 0; u < Q; ++u)
@@ -199,7 +238,7 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void norm_residual_rows_kernel(R
                 const double d = at(u, k) < n ? static_cast<double>(v[u][k]) - mean : 0.0;
                 squares = __builtin_fma(d, d, squares);
             }
-        return moments(kind, mean, total(squares), static_cast<double>(n), eps);
+        return moments(kind, mean, total(squares), a.inverse, eps);
     };
     const auto affine = [&](const RowNorm &w, float (&v)[Q][4]) {
         if (w.weight.data != nullptr) {
@@ -298,11 +337,14 @@ hipError_t launch_norm_residual(const ResidualArgs &a, hipStream_t stream) {
     const bool q = a.ne0 % 4 == 0 && quads(a.y, a.ynb) && quads(a.residual, a.rnb) && quads(a.sum, a.snb) && quads(a.out, a.onb);
     // As few threads a row as hold it in 16 or 20 numbers each, and of up to
     // 1280 numbers a wave alone where there are rows for every wave (2 x 988
-    // rows of 1280: 11.0 us, by four waves 13.5; 400 rows 5.8 and 5.5; one row of
-    // 4096 by four waves 5.1 us, by sixteen 6.2; 2 x 4096 rows of 5120 122 and 210).
+    // rows of 1280: 10.6 us, by four waves 12.6; 512 rows 5.9 and 5.5; one row of
+    // 4096 by four waves 5.0 us, by sixteen 5.6; 2 x 4096 rows of 5120 122 and 182),
+    // in as few registers as hold it (2 x 4096 rows of 640 in 12 numbers a lane
+    // 17.4 us, in 20 20.2).
     const bool many = a.rows >= 4 * static_cast<int64_t>(compute_units());
     if (a.ne0 <= 256) return launch_rows<64, 1>(a, q, stream);
     if (a.ne0 <= 512) return launch_rows<64, 2>(a, q, stream);
+    if (many && a.ne0 <= 768) return launch_rows<64, 3>(a, q, stream);
     if (many && a.ne0 <= 1280) return launch_rows<64, 5>(a, q, stream);
     if (a.ne0 <= 1024) return launch_rows<256, 1>(a, q, stream);
     if (a.ne0 <= 2048) return launch_rows<256, 2>(a, q, stream);
