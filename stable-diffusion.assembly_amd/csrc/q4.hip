@@ -117,26 +117,26 @@ __device__ __forceinline__ uint32_t magnitude(const float4v &v) {
 
 constexpr int kFewThreads = 512;
 
-// The outputs of a workgroup of kFewThreads from its splits' sums in LDS, `step`
+// The outputs of a workgroup of `threads` from its splits' sums in LDS, `step`
 // apart, `count` outputs, with GATED the second half's behind them: their sums
 // in the splits' order, times what `place` gives with an output's row (M or
 // more: none) and column; the redirect's number first, the chain, the gated
 // GELU.  E of a thread's at a time, so that their loads go out together.
 template <bool GATED, int E, class Place>
 __device__ __forceinline__ void write_outputs(const Q4Args &a, const float *sums, int splits, int step, int count, int tid,
-                                              int columns, Place place) {
+                                              int columns, Place place, int threads) {
     constexpr int kHalves = GATED ? 2 : 1;
 #pragma unroll 1
-    for (int first = tid; first < count; first += E * kFewThreads) {
+    for (int first = tid; first < count; first += E * threads) {
         int64_t m[E];
         int n[E];
         bool real[E];
         float v[kHalves * E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int at = first + kFewThreads * e < count ? first + kFewThreads * e : first;
+            const int at = first + threads * e < count ? first + threads * e : first;
             const float back = place(at, m[e], n[e]);
-            real[e] = first + kFewThreads * e < count && m[e] < a.M && n[e] < columns;
+            real[e] = first + threads * e < count && m[e] < a.M && n[e] < columns;
             m[e] = m[e] < a.M ? m[e] : a.M - 1;
             n[e] = n[e] < columns ? n[e] : columns - 1;
 #pragma unroll
@@ -208,7 +208,7 @@ __device__ __forceinline__ void fetched() {
 // ------------------------------------------------------------------ few rows
 
 // Up to 16 rows of x a workgroup.  It takes P tiles of 16 rows of the weights
-// (with GATED, P / 2 of each half) by S splits of K, a wave each, P S = 8; a
+// (with GATED, P / 2 of each half) by S splits of K, a wave each, 8 at most; a
 // split is every S-th unit of 8 blocks, and the splits' sums are added at the
 // end in their order.
 //
@@ -270,7 +270,7 @@ __global__ __launch_bounds__(kFewThreads, 4) void q4_few_kernel(FewArgs f) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, group = lane >> 4;
     const int S = f.splits, P = f.tiles;
-    const int split = wave & (S - 1), tile = wave / S;
+    const int split = wave & (S - 1), tile = wave / S, waves = S * P;
     const int64_t m0 = static_cast<int64_t>(blockIdx.y) * ROWS;
     const int rows = static_cast<int>(a.M - m0 < ROWS ? a.M - m0 : ROWS);
     const int blocks = static_cast<int>(a.K / kBlock);
@@ -283,7 +283,7 @@ __global__ __launch_bounds__(kFewThreads, 4) void q4_few_kernel(FewArgs f) {
     // chunk on; those past the last block repeat it, those past M its last row.
     const auto fetch_parts = [&](int b0, int count, int share) {
 #pragma unroll 1
-        for (int u = wave; u < share; u += kFewWaves) {
+        for (int u = wave; u < share; u += waves) {
             const int row = u % ROWS;
             const float *x = a.x + (m0 + (row < rows ? row : rows - 1)) * a.ldx + static_cast<int64_t>(b0) * kBlock;
             const int first = u / ROWS * (kPart * kBlock), last = count * kBlock;
@@ -303,7 +303,7 @@ __global__ __launch_bounds__(kFewThreads, 4) void q4_few_kernel(FewArgs f) {
     };
     const auto split_parts = [&](int share) {
 #pragma unroll 1
-        for (int u = wave; u < share; u += kFewWaves) {
+        for (int u = wave; u < share; u += waves) {
             // A lane's 8 numbers, 4 group .. and 16 + 4 group .. of a block,
             // make way for their hi and their lo.
             char *place = lds + kPartBytes * u + 128 * (lane >> 2) + 16 * (lane & 3);
@@ -473,10 +473,10 @@ __global__ __launch_bounds__(kFewThreads, 4) void q4_few_kernel(FewArgs f) {
         out = n0 + 16 * (at / (64 * R)) + (at & 15);
         return 1.0f;
     };
-    if (outs * R * 64 <= kFewThreads) {
-        write_outputs<GATED, 1>(a, sums, S, P * R * 64, outs * R * 64, tid, columns, place);
+    if (outs * R * 64 <= 64 * waves) {
+        write_outputs<GATED, 1>(a, sums, S, P * R * 64, outs * R * 64, tid, columns, place, 64 * waves);
     } else {
-        write_outputs<GATED, R>(a, sums, S, P * R * 64, outs * R * 64, tid, columns, place);
+        write_outputs<GATED, R>(a, sums, S, P * R * 64, outs * R * 64, tid, columns, place, 64 * waves);
     }
 }
 
@@ -488,8 +488,11 @@ __global__ __launch_bounds__(kFewThreads, 4) void q4_few_kernel(FewArgs f) {
 // by it 0.2 % slower than the fastest of all).  With 16 rows throughout, 33 rows
 // of 2080 -> 1111 took 12.8 us, now 8.8; 16 of 1280 -> 10240 16.6, now 9.9; 24 of
 // 768 -> 1280 6.8, now 5.0.  With 8 at most, 256 of 1280 -> 1280 18.7, now 14.6.
+// Where the workgroups leave CUs without one, they take as few tiles as fit the
+// device, if a wave splits no more than one and a half parts of x then (320 -> 320
+// 4.4 us, so 3.9; 2 rows of 1280 -> 20160 8.7 and 8.4).
 struct FewShape {
-    int rows, splits;
+    int rows, splits, tiles;
     float time;
 };
 
@@ -497,7 +500,7 @@ FewShape few_shape(int64_t M, int64_t N, int64_t K, bool gated) {
     constexpr int64_t kLdsBytes = 160 * 1024;
     const auto shifted = [](int64_t v, int by) { return (v + (int64_t{1} << by) - 1) >> by; };  // v / 2^by, rounded up
     const int64_t cus = compute_units(), tiles = ceil_div(N, 16), units = ceil_div(K / kBlock, kUnit);
-    FewShape best{0, 0, 0.0f};
+    FewShape best{0, 0, 0, 0.0f};
     int64_t least = 0;
     for (int r = 0; r <= 4; ++r) {
         const int64_t groups = shifted(M, r), parts = ceil_div(K / kBlock, kPart) << r;
@@ -509,33 +512,39 @@ FewShape few_shape(int64_t M, int64_t N, int64_t K, bool gated) {
             // In 0.08 us.
             const int64_t cost = each * (shifted(units, s) * (r < 4 ? 10 : 16) + parts) + (two ? shifted(each, 1) : each) * 13;
             if (best.rows == 0 || cost < least) {
-                best = {1 << r, 1 << s, 2.5f + 0.08f * static_cast<float>(cost)};
+                best = {1 << r, 1 << s, kFewWaves >> s, 2.5f + 0.08f * static_cast<float>(cost)};
                 least = cost;
             }
         }
         if ((1 << r) >= M) break;
     }
+    if (best.rows != 0 && ceil_div(M, best.rows) < cus) {
+        const int64_t groups = ceil_div(M, best.rows), parts = ceil_div(K / kBlock, kPart) * best.rows;
+        const int64_t fit = ceil_div(tiles, cus / groups), least_tiles = gated ? round_up(fit, 2) : fit;
+        if (least_tiles < best.tiles && 2 * parts <= 3 * least_tiles * best.splits) best.tiles = static_cast<int>(least_tiles);
+    }
     return best;
 }
 
 template <bool LEAST, bool GATED, int ROWS>
-hipError_t launch_few(const Q4Args &a, int splits, hipStream_t stream) {
+hipError_t launch_few(const Q4Args &a, const FewShape &shape, hipStream_t stream) {
     static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&q4_few_kernel<LEAST, GATED, ROWS>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize,
                                                        kFewParts * kPartBytes + kFewWaves * kRing);
     if (attr != hipSuccess) return attr;
     FewArgs f{};
     f.a = a;
-    f.splits = splits;
+    f.splits = shape.splits;
     const int64_t columns = GATED ? a.half : a.N;
     const int64_t parts = ceil_div(a.K / kBlock, kPart) * ROWS;
-    f.tiles = kFewWaves / f.splits;
+    f.tiles = shape.tiles;
+    const int waves = f.tiles * f.splits;
     const dim3 grid(static_cast<uint32_t>(ceil_div(columns, 16 * (GATED ? f.tiles / 2 : f.tiles))),
                     static_cast<uint32_t>(ceil_div(a.M, ROWS)));
     f.ring = static_cast<int32_t>(kPartBytes * (parts < kFewParts ? parts : kFewParts));
     f.aligned = reinterpret_cast<uintptr_t>(a.x) % 16 == 0;
-    SDHIP_LAUNCH((q4_few_kernel<LEAST, GATED, ROWS>), grid, dim3(kFewThreads),
-                 static_cast<uint32_t>(f.ring + kFewWaves * kRing), stream, f);
+    SDHIP_LAUNCH((q4_few_kernel<LEAST, GATED, ROWS>), grid, dim3(64 * waves),
+                 static_cast<uint32_t>(f.ring + waves * kRing), stream, f);
     return hipGetLastError();
 }
 
@@ -544,15 +553,15 @@ hipError_t few_rows(const Q4Args &a, hipStream_t stream) {
     const FewShape shape = few_shape(a.M, a.N, a.K, GATED);
     switch (shape.rows) {
     case 1:
-        return launch_few<LEAST, GATED, 1>(a, shape.splits, stream);
+        return launch_few<LEAST, GATED, 1>(a, shape, stream);
     case 2:
-        return launch_few<LEAST, GATED, 2>(a, shape.splits, stream);
+        return launch_few<LEAST, GATED, 2>(a, shape, stream);
     case 4:
-        return launch_few<LEAST, GATED, 4>(a, shape.splits, stream);
+        return launch_few<LEAST, GATED, 4>(a, shape, stream);
     case 8:
-        return launch_few<LEAST, GATED, 8>(a, shape.splits, stream);
+        return launch_few<LEAST, GATED, 8>(a, shape, stream);
     default:
-        return launch_few<LEAST, GATED, 16>(a, shape.splits, stream);
+        return launch_few<LEAST, GATED, 16>(a, shape, stream);
     }
 }
 
@@ -1301,9 +1310,9 @@ __global__ __launch_bounds__(kFewThreads, 2) void q4_mid_kernel(MidArgs f) {
         return t.back[m < a.M ? m : a.M - 1];
     };
     if (outs == 1) {
-        write_outputs<GATED, kTile / kFewThreads>(a, sums, S, P * kTile, kTile, tid, columns, place);
+        write_outputs<GATED, kTile / kFewThreads>(a, sums, S, P * kTile, kTile, tid, columns, place, kFewThreads);
     } else {
-        write_outputs<GATED, 8>(a, sums, S, P * kTile, outs * kTile, tid, columns, place);
+        write_outputs<GATED, 8>(a, sums, S, P * kTile, outs * kTile, tid, columns, place, kFewThreads);
     }
 }
 

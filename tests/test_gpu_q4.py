@@ -585,7 +585,9 @@ def test_more_groups_of_rows_than_a_grid_s_second_dimension(gpu, form):
 SHAPES = [(2, 96, 33), (1, 2080, 40001), (2, 544, 33), (2, 2080, 33), (100, 96, 257), (5, 544, 5001), (5, 2080, 5001),
           (31, 544, 257), (16, 2080, 257), (15, 96, 5001), (33, 2080, 1000), (64, 544, 257), (31, 8224, 257),
           (7, 96, 20000), (15, 544, 5001), (33, 544, 1000), (15, 8224, 1000), (257, 544, 1000), (16, 4128, 5000),
-          (16, 96, 20000), (256, 1280, 1280)]
+          (16, 96, 20000), (256, 1280, 1280),
+          # workgroups of fewer than 8 waves: 1, 3, 5 and 6 tiles by 1 or 2 splits, and of 8
+          (1, 320, 320), (3, 64, 640), (1, 64, 8200), (1, 512, 12301), (2, 1280, 20160), (1, 256, 24001)]
 
 
 @pytest.mark.gpu
@@ -606,6 +608,6 @@ def test_shapes_of_few_rows(gpu, kind, rows, k, n):
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("rows,k,n", [(2, 96, 1000), (2, 544, 1000), (33, 96, 1000), (9, 544, 1000), (31, 96, 2500),
                                       (33, 2080, 1000), (7, 544, 2500), (7, 96, 20000), (31, 544, 2500), (33, 544, 1000),
-                                      (257, 544, 1000), (256, 1280, 1280)])
+                                      (257, 544, 1000), (256, 1280, 1280), (1, 320, 320), (1, 64, 8200), (1, 512, 24002)])
 def test_shapes_of_few_rows_gated(gpu, kind, rows, k, n):
     test_forms_gated(gpu, kind, 1, rows, k, n)
