@@ -184,10 +184,12 @@ int sdhip_profile_entry(int i, const char **name, double *total_ms, int64_t *lau
  * bytes that holds a row, at an even address; from one row of x up, where the
  * others begin at 16.  The products are those of the exact weights with x in
  * 22 bits or more of each row's greatest number, whatever bits asks for; the
- * output shares no byte with w or x.  The work buffer: for more rows than a
- * workgroup's, x in FP16 parts, and for many rows the weights' words and scales
- * in the order the products read them.  An infinity in x reaches its own row only,
- * with Q4_1, whose products are two sums, as infinities or NaN.
+ * output shares no byte with w or x.  Up to 2^25 rows of x and 2^25 of w, 2^36
+ * weights and 2^35 outputs are taken.  The work buffer, none up to 16 rows: where
+ * the size makes them faster laid out first, x in FP16 parts, and for many rows
+ * the weights' words and scales too, in the order the products read them; calls
+ * that may run at once take a buffer each.  An infinity in x reaches its own row
+ * only, with Q4_1, whose products are two sums, as infinities or NaN.
  * Replaces mul_mat_supported / mul_mat_work_size / mul_mat_compute
  * (sources/ops.h:40-44; mul_mat.cc:181-194, 205-215, 1175-1196). */
 int sdhip_mul_mat_supported(const sdhip_tensor *w, const sdhip_tensor *x, const sdhip_tensor *y);

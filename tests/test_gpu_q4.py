@@ -611,3 +611,45 @@ def test_shapes_of_few_rows(gpu, kind, rows, k, n):
                                       (257, 544, 1000), (256, 1280, 1280), (1, 320, 320), (1, 64, 8200), (1, 512, 24002)])
 def test_shapes_of_few_rows_gated(gpu, kind, rows, k, n):
     test_forms_gated(gpu, kind, 1, rows, k, n)
+
+
+@pytest.mark.gpu
+def test_calls_at_once(gpu):
+    """Products and norms on four streams at once, each with its own buffers: the
+    bits of calls one by one."""
+    sizes = [(1, 640, 3000), (40, 640, 1000), (300, 1280, 1300), (700, 640, 1300)]
+    r = rng(9)
+    held = []
+    for rows, k, n in sizes:
+        w, x = dev(q4_lib.random_blocks(r, "q4_1", n, k), gpu), dev(uniform(r, (rows, k), 1.0), gpu)
+        scale = dev(uniform(r, (n,), 1.0), gpu)
+        outs = [unwritten((rows, n), gpu) for _ in range(4)]
+        dw, dx, dy = sdhip.desc(w), sdhip.desc(x), sdhip.desc(outs[0])
+        size = sdhip.load().sdhip_mul_mat_work_size(dw, dx, dy)
+        work = torch.empty(max(size, 16), dtype=torch.uint8, device=gpu)
+        held.append((w, x, scale, outs, work, size, torch.cuda.Stream()))
+
+    def call(w, x, scale, outs, work, size, stream, first):
+        handle = ctypes.c_void_p(stream.cuda_stream)
+        y, n = outs[first:first + 2]
+        sdhip.check(sdhip.load().sdhip_mul_mat(sdhip.desc(w), sdhip.desc(x), sdhip.desc(y), None,
+                                               ctypes.c_void_p(work.data_ptr()), size, handle), "mul_mat")
+        pre = sdhip.row_norm("rms", 1e-6, weight=scale)
+        sdhip.check(sdhip.load().sdhip_norm_residual(None, None, None, 1.0, sdhip.desc(y), 1.0, None, pre,
+                                                     sdhip.desc(n), handle), "norm_residual")
+
+    torch.cuda.synchronize()
+    for h in held:
+        call(*h, 0)
+        torch.cuda.synchronize()
+    for _ in range(5):
+        for h in held:
+            for o in h[3][2:]:
+                o.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for h in held:
+                call(*h, 2)
+        torch.cuda.synchronize()
+        for h in held:
+            assert torch.equal(h[3][0], h[3][2]) and torch.equal(h[3][1], h[3][3])
