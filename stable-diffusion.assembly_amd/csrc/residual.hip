@@ -8,7 +8,7 @@
 // and out written once, the row in registers between its sums, T threads a
 // row, up to 4 Q numbers each (norm_residual_rows_kernel); longer rows are
 // read again for every sum (norm_residual_long_kernel).  2 x 4096 rows of 5120
-// 120 us, 5.6 TB/s of their 671 MB; one row of 4096 4.45 us, of which a launch is 1.7
+// 120 us, 5.6 TB/s of their 671 MB; one row of 4096 4.55 us, of which a launch is 1.7
 // and the rest two sums one after the other.
 
 #include "host.h"
@@ -29,9 +29,11 @@ __device__ __forceinline__ int64_t row_at(const int64_t (&nb)[4], const Place &p
     return p.i1 * nb[1] + p.i2 * nb[2] + p.i3 * nb[3];
 }
 
-// What a norm does to the numbers of a row: (v - hi - lo) scale.
+// What a norm does to the numbers of a row: (v - hi - lo) scale power, `power` a
+// power of two that keeps `scale` a normal number for rows of the greatest and
+// of the least numbers, else 1 (2 % of a row's time in L2).
 struct Moments {
-    float hi, lo, scale;
+    float hi, lo, scale, power;
 };
 
 // 1 / sqrt(v) within 2^-45 of itself: the hardware's, within 2^-24 or so, by one
@@ -45,18 +47,20 @@ __device__ __forceinline__ double inverse_root(double v) {
 
 // `squares` over n numbers, of which `inverse` is 1 / n.
 __device__ __forceinline__ Moments moments(int32_t kind, double mean, double squares, double inverse, float eps) {
-    Moments m{0.0f, 0.0f, 1.0f};
+    Moments m{0.0f, 0.0f, 1.0f, 1.0f};
     if (kind == SDHIP_ROW_NORM_LAYER) {
         m.hi = static_cast<float>(mean);
         m.lo = static_cast<float>(mean - static_cast<double>(m.hi));
     }
     if (kind != SDHIP_ROW_NORM_NONE) {
-        m.scale = static_cast<float>(inverse_root(__builtin_fma(squares, inverse, static_cast<double>(eps))));
+        const double r = inverse_root(__builtin_fma(squares, inverse, static_cast<double>(eps)));
+        m.power = r > 0x1p100 ? 0x1p64f : r < 0x1p-100 ? 0x1p-64f : 1.0f;
+        m.scale = static_cast<float>(r > 0x1p100 ? r * 0x1p-64 : r < 0x1p-100 ? r * 0x1p64 : r);
     }
     return m;
 }
 
-__device__ __forceinline__ float normed(float v, const Moments &m) { return __fmul_rn(v - m.hi - m.lo, m.scale); }
+__device__ __forceinline__ float normed(float v, const Moments &m) { return __fmul_rn(__fmul_rn(v - m.hi - m.lo, m.scale), m.power); }
 
 __device__ __forceinline__ double block_sum(double v, double *lds) {
 #pragma unroll
@@ -132,7 +136,7 @@ __global__ __launch_bounds__(kThreads) void norm_residual_long_kernel(ResidualAr
         if (w.bias.data != nullptr) v = __fadd_rn(v, w.bias.data[row_at(w.bias.nb, p) + i * w.bias.nb[0]]);
         return v;
     };
-    Moments post{0.0f, 0.0f, 1.0f};
+    Moments post{0.0f, 0.0f, 1.0f, 1.0f};
     if (y != nullptr) post = stats(a.post.kind, a.post.eps, [&](int64_t i) { return y[i]; });
     const auto joined = [&](int64_t i) {
         float s = __fmul_rn(a.residual_scale, r[i]);

@@ -276,3 +276,17 @@ def test_more_rows_than_a_launch_takes(gpu):
         z = v * (v.square().mean(-1, keepdim=True) + 1e-6).rsqrt()
         assert ((out[part].double() - (r + z)).abs() <= 10 * U * (z.abs() + r.abs())).all()
     assert not out.isnan().any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [96, 1280, 17000])
+@pytest.mark.parametrize("power", [-140, -130, 126])
+def test_greatest_and_least_numbers(gpu, dim, power):
+    """Rows whose reciprocal root is no normal number of single precision: numbers
+    of 2^power, whole multiples of 2^-149, whose RMS norm is of order 1."""
+    r = rng(dim)
+    shape = (3, dim)
+    y = np.clip(normal(r, shape), -3.5, 3.5).astype(np.float64)
+    y = (y * 2.0 ** power).astype(np.float32)
+    assert np.isfinite(y).all() and (y != 0).mean() > 0.9
+    check(run(gpu, shape, "rms", "layer", eps=0.0, y_np=y), f"2^{power} {dim}")
