@@ -669,8 +669,9 @@ __global__ __launch_bounds__(kOperandThreads) void q4_operands_kernel(TileArgs t
                 *reinterpret_cast<half8 *>(to) = hi;
                 *reinterpret_cast<half8 *>(to + 1024) = lo;
                 if constexpr (LEAST) {
-                    sum = ((l[0] + l[1]) + (l[2] + l[3])) + ((h[0] + h[1]) + (h[2] + h[3]));
-                    sum *= scale;
+                    // Scaled before they are added: sums of x itself may pass single precision.
+                    const float4v p = l * scale, q = h * scale;
+                    sum = ((p[0] + p[1]) + (p[2] + p[3])) + ((q[0] + q[1]) + (q[2] + q[3]));
                 }
             }
             if constexpr (LEAST) {
