@@ -29,9 +29,11 @@ __device__ __forceinline__ int64_t row_at(const int64_t (&nb)[4], const Place &p
     return p.i1 * nb[1] + p.i2 * nb[2] + p.i3 * nb[3];
 }
 
-// What a norm does to the numbers of a row: (v - hi - lo) scale power, `power` a
-// power of two that keeps `scale` a normal number for rows of the greatest and
-// of the least numbers, else 1 (2 % of a row's time in L2).
+// What a norm does to the numbers of a row: (v power - hi - lo) scale, hi and lo
+// of the mean times `power`: a power of two that keeps the differences within
+// single precision, the mean's second part and `scale` normal numbers for rows of
+// the greatest and of the least numbers (3e38 among -3e38 lies 4.5e38 from the
+// mean; of numbers of 2^-140 a second part would be below 2^-149), else 1.
 struct Moments {
     float hi, lo, scale, power;
 };
@@ -48,19 +50,23 @@ __device__ __forceinline__ double inverse_root(double v) {
 // `squares` over n numbers, of which `inverse` is 1 / n.
 __device__ __forceinline__ Moments moments(int32_t kind, double mean, double squares, double inverse, float eps) {
     Moments m{0.0f, 0.0f, 1.0f, 1.0f};
+    if (kind == SDHIP_ROW_NORM_NONE) return m;
+    const float hi = static_cast<float>(mean);
+    const double rest = mean - static_cast<double>(hi);
+    const double r = inverse_root(__builtin_fma(squares, inverse, static_cast<double>(eps)));
+    const double power = r > 0x1p100 ? 0x1p64 : r < 0x1p-100 ? 0x1p-64 : 1.0;
+    m.power = static_cast<float>(power);
+    m.scale = static_cast<float>(r > 0x1p100 ? r * 0x1p-64 : r < 0x1p-100 ? r * 0x1p64 : r);
     if (kind == SDHIP_ROW_NORM_LAYER) {
-        m.hi = static_cast<float>(mean);
-        m.lo = static_cast<float>(mean - static_cast<double>(m.hi));
-    }
-    if (kind != SDHIP_ROW_NORM_NONE) {
-        const double r = inverse_root(__builtin_fma(squares, inverse, static_cast<double>(eps)));
-        m.power = r > 0x1p100 ? 0x1p64f : r < 0x1p-100 ? 0x1p-64f : 1.0f;
-        m.scale = static_cast<float>(r > 0x1p100 ? r * 0x1p-64 : r < 0x1p-100 ? r * 0x1p64 : r);
+        m.hi = hi * m.power;
+        m.lo = static_cast<float>(rest * power);
     }
     return m;
 }
 
-__device__ __forceinline__ float normed(float v, const Moments &m) { return __fmul_rn(__fmul_rn(v - m.hi - m.lo, m.scale), m.power); }
+__device__ __forceinline__ float normed(float v, const Moments &m) {
+    return __fmul_rn(__builtin_fmaf(v, m.power, -m.hi) - m.lo, m.scale);
+}
 
 __device__ __forceinline__ double block_sum(double v, double *lds) {
 #pragma unroll
