@@ -175,22 +175,18 @@ __device__ __forceinline__ void write_outputs(const Q4Args &a, const float *sums
 // A copy of 16 bytes a lane (1 KB) or 4 into LDS at `to` and on, lane after
 // lane.  The compiler does not see these loads, and so does not wait for them
 // where it waits for others or reads LDS: what reads them waits (wait_loads).
-// Nothing else here uses m0.
+// They take the place in LDS from m0, which the compiler sets as their operand
+// (and so knows what it holds); its own copies go a cycle before their use.
 __device__ __forceinline__ void fetch16(const void *from, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(to)),
-                 "v"(from)
-                 : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"{m0}"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory");
 }
 __device__ __forceinline__ void fetch4(const void *from, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(to)),
-                 "v"(from)
-                 : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, off" ::"{m0}"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory");
 }
 
 // fetch16 from an address the wave's lanes share and an offset of each.
 __device__ __forceinline__ void fetch16(const char *from, uint32_t offset, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(from)
-                 : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(to), "v"(offset), "s"(from) : "memory");
 }
 
 __device__ __forceinline__ uint32_t lds_address(const char *p) {
