@@ -182,9 +182,12 @@ int sdhip_profile_entry(int i, const char **name, double *total_ms, int64_t *lau
  * Weights of 4 bits (Q4_0, Q4_1; no counterpart in the reference, which leaves
  * them to ggml): ne[0] a multiple of 32, rows nb[1] apart, any even number of
  * bytes that holds a row, at an even address; from one row of x up, where the
- * others begin at 16.  The products are those of the exact weights with x in
- * 22 bits or more of each row's greatest number, whatever bits asks for; the
- * output shares no byte with w or x.  Up to 2^25 rows of x and 2^25 of w, 2^36
+ * others begin at 16.  No weight is rounded, and of x each number is held to 2^-22
+ * of itself or, below 2^-17 of its row's greatest, to 2^-39 of that, whatever
+ * bits asks for.  Sums are in single precision: with Q4_0 of w x, with Q4_1 of
+ * two terms, d (q - 8) x and (m + 8 d) x, together below 2.1 |x| times the
+ * greatest number that the block can hold, also where they cancel to a weight
+ * of 0.  The output shares no byte with w or x.  Up to 2^25 rows of x and 2^25 of w, 2^36
  * weights and 2^35 outputs are taken.  The work buffer, none up to 16 rows: where
  * the size makes them faster laid out first, x in FP16 parts, and for many rows
  * the weights' words and scales too, in the order the products read them; calls
