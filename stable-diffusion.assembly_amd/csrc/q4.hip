@@ -232,9 +232,9 @@ __device__ __forceinline__ void fetched() {
 // first register and its lo in the second, up to 8 two a group, so that one
 // MFMA takes both parts; from 9 on two do.
 //
-// 1 row of 1280 -> 1280: 3.9 us (an empty launch 1.7); of 4096 -> 16384, Q4_1,
-// 10.8 us, 3.9 TB/s of weights; 2 rows of 1280 -> 20160 8.3; 33 rows of 2080 ->
-// 1111 8.8; 154 of 768 -> 1280 7.1.
+// Without a chain, in a captured graph: 1 row of 1280 -> 1280 3.9 us (an empty
+// launch 1.7); of 4096 -> 16384, Q4_1, 11.1 us, 3.8 TB/s of weights; 2 rows of 1280
+// -> 20160 7.4; 33 rows of 2080 -> 1111 8.5; 154 of 768 -> 1280 7.4.
 constexpr int kFewWaves = 8;
 static_assert(kFewThreads == 64 * kFewWaves);
 constexpr int kUnit = 8;        // blocks
@@ -492,7 +492,7 @@ __global__ __launch_bounds__(kFewThreads, 4) void q4_few_kernel(FewArgs f) {
 // 768 -> 1280 6.8, now 5.0.  With 8 at most, 256 of 1280 -> 1280 18.7, now 14.6.
 // Where the workgroups leave CUs without one, they take as few tiles as fit the
 // device, if a wave splits no more than one and a half parts of x then (320 -> 320
-// 4.4 us, so 3.9; 2 rows of 1280 -> 20160 8.7 and 8.4).
+// with a bias 4.4 us, so 3.9; 2 rows of 1280 -> 20160 8.2 and 7.9).
 struct FewShape {
     int rows, splits, tiles;
     float time;
@@ -776,10 +776,10 @@ __global__ __launch_bounds__(kOperandThreads) void q4_operands_kernel(TileArgs t
 // WK blocks come into LDS in runs, three stages of them in turn, asked for two
 // stages ahead.  With TN 2 a block's sums of products are scaled by d, 64
 // operations beside the 36 that widen the words, 400 of the vector units' cycles
-// a block to 512 of the MFMA's.  Large products run at the clock that their power
-// leaves (1976 rows of 1280 -> 2 x 5120 gated 126 us; without any one of the
-// copies, the scaling, the widening or the barriers 116 .. 127, without the reads
-// of LDS 98).
+// a block to 512 of the MFMA's.  No one unit bounds it: 1976 rows of 1280 -> 2 x
+// 5120 gated take 126 us, the MFMA busy 44 % of the cycles at the 1.9 GHz that
+// this product runs at; without any one of the copies, the scaling, the widening
+// or the barriers 116 .. 127, without the reads of LDS 98.
 template <int WM, int WN, int WK, int TN>
 struct Tiles {
     static constexpr int kWaves = WM * WN * WK;

@@ -8,7 +8,7 @@
 // and out written once, the row in registers between its sums, T threads a
 // row, up to 4 Q numbers each (norm_residual_rows_kernel); longer rows are
 // read again for every sum (norm_residual_long_kernel).  2 x 4096 rows of 5120
-// 120 us, 5.6 TB/s of their 671 MB; one row of 4096 4.55 us, of which a launch is 1.7
+// 119 us, 5.6 TB/s of their 671 MB; one row of 4096 4.65 us, of which a launch is 1.7
 // and the rest two sums one after the other.
 
 #include "host.h"
