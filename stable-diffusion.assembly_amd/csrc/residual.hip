@@ -47,6 +47,14 @@ __device__ __forceinline__ double inverse_root(double v) {
     return v > 0.0 && v < __builtin_inf() ? next : r;
 }
 
+// The mean of n numbers, of which `inverse` is 1 / n: exact where it is a double,
+// by what the rounded quotient leaves of the sum, so that nothing is left of a row
+// of one number (1 / n's rounding alone made 1 or -1 of 123 times 1e20).
+__device__ __forceinline__ double mean_of(double sum, int64_t n, double inverse) {
+    const double mean = sum * inverse;
+    return __builtin_fma(__builtin_fma(-mean, static_cast<double>(n), sum), inverse, mean);
+}
+
 // `squares` over n numbers, of which `inverse` is 1 / n.
 __device__ __forceinline__ Moments moments(int32_t kind, double mean, double squares, double inverse, float eps) {
     Moments m{0.0f, 0.0f, 1.0f, 1.0f};
@@ -54,7 +62,8 @@ __device__ __forceinline__ Moments moments(int32_t kind, double mean, double squ
     const float hi = static_cast<float>(mean);
     const double rest = mean - static_cast<double>(hi);
     const double r = inverse_root(__builtin_fma(squares, inverse, static_cast<double>(eps)));
-    const double power = r > 0x1p100 ? 0x1p64 : r < 0x1p-100 ? 0x1p-64 : 1.0;
+    // A row without a spread, of whatever magnitude, stays: 0 times an infinity.
+    const double power = r > 0x1p100 && r < __builtin_inf() ? 0x1p64 : r < 0x1p-100 ? 0x1p-64 : 1.0;
     m.power = static_cast<float>(power);
     m.scale = static_cast<float>(r > 0x1p100 ? r * 0x1p-64 : r < 0x1p-100 ? r * 0x1p64 : r);
     if (kind == SDHIP_ROW_NORM_LAYER) {
@@ -123,7 +132,7 @@ __global__ __launch_bounds__(kThreads) void norm_residual_long_kernel(ResidualAr
         if (kind == SDHIP_ROW_NORM_LAYER) {
             double s = 0.0;
             for (int64_t i = threadIdx.x; i < a.ne0; i += kThreads) s += static_cast<double>(value(i));
-            mean = block_sum(s, lds) * a.inverse;
+            mean = mean_of(block_sum(s, lds), a.ne0, a.inverse);
         }
         if (kind != SDHIP_ROW_NORM_NONE) {
             double s = 0.0;
@@ -239,7 +248,7 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void norm_residual_rows_kernel(R
             for (int u = 0; u < Q; ++u)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) s += static_cast<double>(v[u][k]);
-            mean = total(s) * a.inverse;
+            mean = mean_of(total(s), n, a.inverse);
         }
 #pragma unroll
         for (int u = 0; u < Q; ++u)

@@ -58,3 +58,24 @@ def test_numbers_further_from_their_mean_than_single_precision_holds(gpu, dim, p
         sdhip.norm_residual(None, dev(v, gpu), None, out, pre=sdhip.row_norm("layer", 0.0))
     # The difference (2 roundings), the scale and their product.
     assert (np.abs(out.cpu().numpy() - z) <= 5 * U * np.abs(z)).all()
+
+
+# Lengths of each width, most of them with 1 / n times the sum of n 1.1's, both rounded, not 1.1.
+LENGTHS = [4, 123, 246, 492, 503, 984, 955, 1280, 1910, 1989, 3781, 4096, 4024, 5013, 7562, 15124, 16365, 16384, 19999, 32768]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", LENGTHS)
+@pytest.mark.parametrize("power", [-140, -60, 0, 30, 60, 80, 127])
+def test_rows_of_one_number(gpu, dim, power):
+    """Nothing is left of them about their mean: 0 with an epsilon, however far
+    below their magnitude, and 0 / 0 without one."""
+    number = np.float32(1.1 * 2.0 ** power)
+    v = torch.full((1100 if power == 80 else 2, dim), float(number), device=gpu)
+    for eps in (1e-6, 0.0):
+        out = torch.full_like(v, 7.0)
+        sdhip.norm_residual(None, v, None, out, pre=sdhip.row_norm("layer", eps))
+        assert (out == 0).all() if eps else out.isnan().all()
+        out = torch.full_like(v, 7.0)
+        sdhip.norm_residual(v, torch.zeros_like(v), out, None, sdhip.row_norm("layer", eps))
+        assert (out == 0).all() if eps else out.isnan().all()
