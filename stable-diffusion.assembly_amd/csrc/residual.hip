@@ -240,6 +240,7 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void norm_residual_rows_kernel(R
         }
         return v;
     };
+    // Of numbers that are 0 past the row's.
     const auto stats = [&](int32_t kind, float eps, const float (&v)[Q][4]) {
         double mean = 0.0, squares = 0.0;
         if (kind == SDHIP_ROW_NORM_LAYER) {
@@ -288,6 +289,15 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void norm_residual_rows_kernel(R
             for (int u = 0; u < Q; ++u)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) z[u][k] = normed(z[u][k], m);
+            // Past the row's numbers the mean was taken from 0: they count in no
+            // later mean (each number tested in the sums instead: 2 x 988 rows of 1280
+            // 10.6 us, so 10.2).
+            if (a.post.kind == SDHIP_ROW_NORM_LAYER && n < 4 * Q * T) {
+#pragma unroll
+                for (int u = 0; u < Q; ++u)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) z[u][k] = at(u, k) < n ? z[u][k] : 0.0f;
+            }
         }
         affine(a.post, z);
         if (a.gate.data != nullptr) {
