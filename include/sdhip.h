@@ -41,8 +41,17 @@ extern "C" {
  * d and 16 bytes, w = d (q - 8); Q4_1, 20 bytes, d, a half-precision least
  * value m and 16 bytes, w = d q + m; byte j holds q of the block's number j in
  * its low four bits and of number 16 + j in its high ones.  A tensor of them
- * has nb[0] the bytes of a block, as ggml_tensor has. */
-enum { SDHIP_TYPE_F32 = 0, SDHIP_TYPE_F16 = 1, SDHIP_TYPE_Q4_0 = 2, SDHIP_TYPE_Q4_1 = 3 };
+ * has nb[0] the bytes of a block, as ggml_tensor has.  F8_E4M3, which ggml has
+ * no number for, are the weights of sdhip_mul_mat_f8: a sign, four bits of
+ * exponent biased by 7 and three of mantissa, 448 the greatest, 0x7f and 0xff
+ * NaN and no infinity. */
+enum {
+    SDHIP_TYPE_F32 = 0,
+    SDHIP_TYPE_F16 = 1,
+    SDHIP_TYPE_Q4_0 = 2,
+    SDHIP_TYPE_Q4_1 = 3,
+    SDHIP_TYPE_F8_E4M3 = 256
+};
 
 typedef enum { SDHIP_OK = 0, SDHIP_UNSUPPORTED = 1, SDHIP_ERROR = 2 } sdhip_status;
 
@@ -211,6 +220,43 @@ sdhip_status sdhip_mul_mat_gated(const sdhip_tensor *w, const sdhip_tensor *x, c
                                  const sdhip_epilogue *chain, const sdhip_tensor *out, void *work, size_t work_size,
                                  void *stream);
 
+/* MUL_MAT of weights in 8-bit floating point with a scale for each block of
+ * 128 x 128 (no counterpart in the reference): w F8_E4M3, ne = [K, N, 1, 1],
+ * nb[0] = 1, rows nb[1] >= K apart, at any address; scales F32, ne =
+ * [ceil(K / 128), ceil(N / 128), 1, 1], nb[0] = 4, nb[1] a multiple of 4 that
+ * holds a row; x, y and the chain as sdhip_mul_mat's, from one row of x up and
+ * any K and N:
+ *
+ *   y[n, m] = sum over b of scales[b, n / 128] sum over k in b of w[k, n] x'[k, m]
+ *
+ * with b the blocks of 128 along K, the last perhaps shorter, and x' what x's
+ * numbers are held to: the numbers of row m and block b as q 2^e, e the least
+ * whole number, -101 at least, that brings the greatest magnitude of them to 448
+ * or less, and q E4M3, to nearest with ties to even.  The products are exact, the
+ * sums in single precision; a scale times 2^e is to be below 2^128.  An infinity or
+ * NaN in x makes its row's outputs NaN, a NaN in w its column's.
+ * What bits asks for is left aside.  The output shares no byte with w, scales or
+ * x.  Up to 2^25 rows of x and 2^25 of w, 2^36 weights, 2^35 outputs and 2^37
+ * numbers of x are taken.  The work buffer, none up to 16 rows: x as its q and e
+ * and, where many rows read them and they do not lie at multiples of 16 bytes in
+ * rows of whole blocks, the weights; calls that may run at once take a buffer
+ * each. */
+int sdhip_mul_mat_f8_supported(const sdhip_tensor *w, const sdhip_tensor *scales, const sdhip_tensor *x,
+                               const sdhip_tensor *y);
+size_t sdhip_mul_mat_f8_work_size(const sdhip_tensor *w, const sdhip_tensor *scales, const sdhip_tensor *x,
+                                  const sdhip_tensor *y);
+sdhip_status sdhip_mul_mat_f8(const sdhip_tensor *w, const sdhip_tensor *scales, const sdhip_tensor *x,
+                              const sdhip_tensor *y, const sdhip_epilogue *chain, void *work, size_t work_size,
+                              void *stream);
+
+/* The same with the GEGLU after it, as sdhip_mul_mat_gated; the work buffer is
+ * sdhip_mul_mat_f8_work_size's. */
+int sdhip_mul_mat_f8_gated_supported(const sdhip_tensor *w, const sdhip_tensor *scales, const sdhip_tensor *x,
+                                     const sdhip_tensor *y, const sdhip_tensor *out);
+sdhip_status sdhip_mul_mat_f8_gated(const sdhip_tensor *w, const sdhip_tensor *scales, const sdhip_tensor *x,
+                                    const sdhip_tensor *y, const sdhip_epilogue *chain, const sdhip_tensor *out,
+                                    void *work, size_t work_size, void *stream);
+
 /* ---------------------------------------------------------------- CONV_2D */
 
 /* GGML_OP_CONV_2D (ggml_conv_2d_direct): kernel ne = [KW, KH, IC, OC]
@@ -303,6 +349,22 @@ sdhip_status sdhip_group_norm(const sdhip_tensor *x, const sdhip_tensor *y, int 
 sdhip_status sdhip_group_norm_static(const sdhip_tensor *x, const sdhip_tensor *y, int groups, float eps,
                                      const sdhip_epilogue *chain, void *stream);
 
+/* GROUP_NORM of channels-last tensors, images as rows of channels and so tokens
+ * too, then the chain (no counterpart in the reference, whose GROUP_NORM takes
+ * ne[2] as the channels): x, y F32 of one shape, ne = [C, W, H, N], nb[0] = 4,
+ * pixels any multiple of 4 bytes apart, nb[2] = W nb[1], images any multiple of
+ * 4 (so channels of a wider tensor); `groups` groups of ceil(C / groups)
+ * channels over ne[0], per image ne[3].  Up to 2^24 channels, 2^31 - 1 pixels of
+ * an image and as many images, 2^40 numbers in all are taken.  Statistics and differences are taken in double, each number rounded once
+ * before the chain.  y may be x's own memory in the same layout; else
+ * it shares no byte range with x, nor do two of its pixels: SDHIP_UNSUPPORTED.
+ * No redirect.  The work buffer holds the partial sums of stretches of an
+ * image's pixels, 0 where a group is small enough for one launch. */
+int sdhip_group_norm_last_supported(const sdhip_tensor *x, const sdhip_tensor *y, int groups);
+size_t sdhip_group_norm_last_work_size(const sdhip_tensor *x, const sdhip_tensor *y, int groups);
+sdhip_status sdhip_group_norm_last(const sdhip_tensor *x, const sdhip_tensor *y, int groups, float eps,
+                                   const sdhip_epilogue *chain, void *work, size_t work_size, void *stream);
+
 /* GGML_OP_NORM over ne[0] (norm.cc:148-175), then the chain.  Replaces
  * norm_supported / norm_compute (ops.h:62-63). */
 int sdhip_norm_supported(const sdhip_tensor *x, const sdhip_tensor *y);
@@ -351,6 +413,46 @@ sdhip_status sdhip_norm_residual(const sdhip_tensor *y, const sdhip_row_norm *po
                                  float branch_scale, const sdhip_tensor *residual, float residual_scale,
                                  const sdhip_tensor *sum, const sdhip_row_norm *pre, const sdhip_tensor *out,
                                  void *stream);
+
+/* ---------------------------------------------------------------- rotary positions */
+
+/* Rotary positions of several axes (time, height, width) of queries or keys,
+ * after the norm of each head's numbers where there is one, in one pass: the
+ * reference has no such node; its graphs hold NORM, MUL and ADD nodes and views
+ * one by one.
+ *
+ *   z = norm(x)                             each row ne[0], a head's numbers; NULL: x
+ *   y[i] = z[i] cos t - z[j] sin t          for each pair p of numbers (i, j) of the
+ *   y[j] = z[i] sin t + z[j] cos t          first n = dims[0] + ... + dims[count - 1]
+ *   y    = z                                for the others
+ *
+ * x F32 and y F32 or F16, ne = [d, tokens, heads, batch] as attention's
+ * queries, d <= 512, nb[0] the element size and the other strides any multiple
+ * of it (queries and keys side by side in a projection's output are one x, their
+ * norms' weights one tensor of ne[2] = heads).  positions F32, ne = [count,
+ * tokens or 1, 1, batch or 1], nb[0] = 4.  The pairs of axis a are the
+ * dims[a] / 2 after those of the axes before, dims even; t is the position
+ * along a times base[a]^(-2 j / dims[a]) for the axis's pair j or, with
+ * `shared`, base[a]^(-2 p / n) for the head's pair p.  Pair p is numbers 2 p and
+ * 2 p + 1 (ADJACENT) or p and n / 2 + p (HALVES).  Angles are taken in double; a
+ * norm is sdhip_row_norm's (sdhip_norm_residual), its sums in double.  y may be
+ * x's own memory in the same layout; else what is written shares no byte range
+ * with what is read, nor do two rows of y: SDHIP_UNSUPPORTED.  No work buffer. */
+enum { SDHIP_ROPE_ADJACENT = 0, SDHIP_ROPE_HALVES = 1 };
+#define SDHIP_MAX_AXES 4
+
+typedef struct sdhip_rope_axes {
+    int32_t count;                 /* 1 to SDHIP_MAX_AXES */
+    int32_t order;                 /* SDHIP_ROPE_ADJACENT or SDHIP_ROPE_HALVES */
+    int32_t shared;                /* 0, or not: the frequencies run on over the axes */
+    int32_t dims[SDHIP_MAX_AXES];  /* a head's numbers of each axis: even, 2 or more */
+    float base[SDHIP_MAX_AXES];    /* above 0, finite */
+} sdhip_rope_axes;
+
+int sdhip_rope_supported(const sdhip_tensor *x, const sdhip_row_norm *norm, const sdhip_tensor *positions,
+                         const sdhip_rope_axes *axes, const sdhip_tensor *y);
+sdhip_status sdhip_rope(const sdhip_tensor *x, const sdhip_row_norm *norm, const sdhip_tensor *positions,
+                        const sdhip_rope_axes *axes, const sdhip_tensor *y, void *stream);
 
 /* ---------------------------------------------------------------- the graph */
 

@@ -212,7 +212,7 @@ int64_t nelements(const sdhip_tensor *t) { return t->ne[0] * t->ne[1] * t->ne[2]
 
 size_t tensor_span(const sdhip_tensor *t) {
     const bool q4 = q4_type(t->type);
-    size_t n = q4 ? static_cast<size_t>(q4_block_bytes(t->type)) : t->type == SDHIP_TYPE_F16 ? 2 : 4;
+    size_t n = q4 ? static_cast<size_t>(q4_block_bytes(t->type)) : t->type == SDHIP_TYPE_F16 ? 2 : t->type == SDHIP_TYPE_F8_E4M3 ? 1 : 4;
     for (int k = 0; k < 4; ++k) {
         if (t->ne[k] <= 0) return 0;
         if (t->nb[k] < 0) return SIZE_MAX;
@@ -231,6 +231,41 @@ bool spans_overlap(const void *a, size_t an, const void *b, size_t bn) {
     const uintptr_t ea = an > UINTPTR_MAX - pa ? UINTPTR_MAX : pa + an;
     const uintptr_t eb = bn > UINTPTR_MAX - pb ? UINTPTR_MAX : pb + bn;
     return pa < eb && pb < ea;
+}
+
+bool broadcasts(const sdhip_tensor *t, const sdhip_tensor *shape) {
+    if (!holds_f32(t) || reinterpret_cast<uintptr_t>(t->data) % 4 != 0) return false;
+    for (int k = 0; k < 4; ++k) {
+        if ((t->ne[k] != shape->ne[k] && t->ne[k] != 1) || t->nb[k] % 4 != 0) return false;
+    }
+    return true;
+}
+
+bool row_norm_taken(const sdhip_row_norm *n, const sdhip_tensor *shape) {
+    if (n == nullptr) return true;
+    return n->kind >= SDHIP_ROW_NORM_NONE && n->kind <= SDHIP_ROW_NORM_RMS &&
+           (n->weight == nullptr || broadcasts(n->weight, shape)) && (n->bias == nullptr || broadcasts(n->bias, shape));
+}
+
+bool elements_apart(const sdhip_tensor *t) {
+    int64_t reach = t->nb[0];
+    bool done[4] = {};
+    for (int pass = 0; pass < 4; ++pass) {
+        int next = -1;
+        for (int k = 0; k < 4; ++k) {
+            if (!done[k] && (next < 0 || t->nb[k] < t->nb[next])) next = k;
+        }
+        done[next] = true;
+        if (t->ne[next] == 1) continue;
+        if (t->nb[next] < reach) return false;
+        if (t->nb[next] > INT64_MAX / t->ne[next]) return false;
+        reach = t->nb[next] * t->ne[next];
+    }
+    return true;
+}
+
+bool tensors_share(const sdhip_tensor *a, const sdhip_tensor *b) {
+    return a != nullptr && b != nullptr && spans_overlap(a->data, tensor_span(a), b->data, tensor_span(b));
 }
 
 int compute_units() {

@@ -250,6 +250,58 @@ __device__ __forceinline__ void copy_lds_buffer(__amdgpu_buffer_rsrc_t rsrc, uin
                                              soffset, 0, 0);
 }
 
+// A copy of 16 bytes a lane (1 KB) or 4 into LDS at `to` and on, lane after
+// lane.  The compiler does not see these loads, and so does not wait for them
+// where it waits for others or reads LDS: what reads them waits (wait_loads).
+// They take the place in LDS from m0, which the compiler sets as their operand
+// (and so knows what it holds); its own copies go a cycle before their use.
+__device__ __forceinline__ void fetch16(const void *from, uint32_t to) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"{m0}"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory");
+}
+__device__ __forceinline__ void fetch4(const void *from, uint32_t to) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, off" ::"{m0}"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory");
+}
+
+// fetch16 from an address the wave's lanes share and an offset of each.
+__device__ __forceinline__ void fetch16(const char *from, uint32_t offset, uint32_t to) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(to), "v"(offset), "s"(from) : "memory");
+}
+
+__device__ __forceinline__ uint32_t lds_address(const char *p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char *)p));
+}
+
+// wait_loads, and no read of LDS before it.
+template <int N>
+__device__ __forceinline__ void fetched() {
+    wait_loads<N>();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// ------------------------------------------------------------------ lanes
+
+// Rows of 16 lanes exchanged: b's even ones with a's odd ones, or b's first 32
+// lanes with a's last.
+__device__ __forceinline__ void swap32(uint32_t &a, uint32_t &b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = r[0];
+    b = r[1];
+}
+
+__device__ __forceinline__ void swap16(uint32_t &a, uint32_t &b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    a = r[0];
+    b = r[1];
+}
+
+// Four numbers at any multiple of 4 bytes.
+__device__ __forceinline__ float4v load4(const float *p) {
+    float4v v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+
 // ------------------------------------------------------------------ grid
 
 // The 8 XCDs of an MI355X each take every 8th workgroup of a launch, and each

@@ -131,6 +131,16 @@ size_t tensor_span(const sdhip_tensor *t);
 // Whether the bytes [a, a + an) and [b, b + bn) share any: the addresses
 // compared as integers, the ends saturating, nothing read.
 bool spans_overlap(const void *a, size_t an, const void *b, size_t bn);
+// Whether t is single precision that broadcasts over `shape`: of its extent or
+// 1 along each dimension, at a multiple of 4 bytes everywhere.
+bool broadcasts(const sdhip_tensor *t, const sdhip_tensor *shape);
+// Whether n is a norm of rows of `shape` (sdhip_row_norm), or none.
+bool row_norm_taken(const sdhip_row_norm *n, const sdhip_tensor *shape);
+// Whether no two numbers of t (nb[0] its element size) lie in one place: along the dimensions in the
+// order of their strides each step passes all that the ones before it reach.
+bool elements_apart(const sdhip_tensor *t);
+// Whether the bytes that two tensors (or none) reach share any.
+bool tensors_share(const sdhip_tensor *a, const sdhip_tensor *b);
 // The compute units of the current device (looked up once a device; 256,
 // MI355X's, where the runtime cannot say).
 int compute_units();

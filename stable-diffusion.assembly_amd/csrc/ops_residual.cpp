@@ -17,75 +17,19 @@ bool rows_of(const sdhip_tensor *t, const sdhip_tensor *shape) {
            reinterpret_cast<uintptr_t>(t->data) % 4 == 0;
 }
 
-bool broadcast(const sdhip_tensor *t, const sdhip_tensor *shape) {
-    if (!holds_f32(t) || reinterpret_cast<uintptr_t>(t->data) % 4 != 0) return false;
-    for (int k = 0; k < 4; ++k) {
-        if ((t->ne[k] != shape->ne[k] && t->ne[k] != 1) || t->nb[k] % 4 != 0) return false;
-    }
-    return true;
-}
-
-bool norm_taken(const sdhip_row_norm *n, const sdhip_tensor *shape) {
-    if (n == nullptr) return true;
-    return n->kind >= SDHIP_ROW_NORM_NONE && n->kind <= SDHIP_ROW_NORM_RMS &&
-           (n->weight == nullptr || broadcast(n->weight, shape)) && (n->bias == nullptr || broadcast(n->bias, shape));
-}
-
-// Whether no two numbers of t lie in one place: along the dimensions in the
-// order of their strides each step passes all that the ones before it reach.
-bool apart(const sdhip_tensor *t) {
-    int64_t reach = 4;
-    bool done[4] = {};
-    for (int pass = 0; pass < 4; ++pass) {
-        int next = -1;
-        for (int k = 0; k < 4; ++k) {
-            if (!done[k] && (next < 0 || t->nb[k] < t->nb[next])) next = k;
-        }
-        done[next] = true;
-        if (t->ne[next] == 1) continue;
-        if (t->nb[next] < reach) return false;
-        if (t->nb[next] > INT64_MAX / t->ne[next]) return false;
-        reach = t->nb[next] * t->ne[next];
-    }
-    return true;
-}
-
-bool share(const sdhip_tensor *a, const sdhip_tensor *b) {
-    return a != nullptr && b != nullptr && spans_overlap(a->data, tensor_span(a), b->data, tensor_span(b));
-}
-
 // A written tensor: apart in itself, and in no byte range that is read, but
 // for y's or residual's own memory in the same layout.
 bool written(const sdhip_tensor *t, const sdhip_tensor *const *rows, const sdhip_tensor *const *operands, int count) {
-    if (!apart(t)) return false;
+    if (!elements_apart(t)) return false;
     for (int i = 0; i < 2; ++i) {
-        if (rows[i] != nullptr && !(t->data == rows[i]->data && same_layout(t, rows[i])) && share(t, rows[i])) {
+        if (rows[i] != nullptr && !(t->data == rows[i]->data && same_layout(t, rows[i])) && tensors_share(t, rows[i])) {
             return false;
         }
     }
     for (int i = 0; i < count; ++i) {
-        if (share(t, operands[i])) return false;
+        if (tensors_share(t, operands[i])) return false;
     }
     return true;
-}
-
-RowOperand operand_of(const sdhip_tensor *t) {
-    RowOperand o{};
-    if (t == nullptr) return o;
-    o.data = static_cast<const float *>(t->data);
-    for (int k = 0; k < 4; ++k) o.nb[k] = t->ne[k] == 1 ? 0 : t->nb[k] / 4;
-    return o;
-}
-
-RowNorm norm_of(const sdhip_row_norm *n) {
-    RowNorm r{};
-    if (n == nullptr) return r;
-    r.kind = n->kind;
-    r.eps = n->eps;
-    r.offset = n->weight_offset;
-    r.weight = operand_of(n->weight);
-    r.bias = operand_of(n->bias);
-    return r;
 }
 
 void strides_of(const sdhip_tensor *t, int64_t (&nb)[4]) {
@@ -93,6 +37,25 @@ void strides_of(const sdhip_tensor *t, int64_t (&nb)[4]) {
 }
 
 }  // namespace
+
+RowOperand row_operand(const sdhip_tensor *t) {
+    RowOperand o{};
+    if (t == nullptr) return o;
+    o.data = static_cast<const float *>(t->data);
+    for (int k = 0; k < 4; ++k) o.nb[k] = t->ne[k] == 1 ? 0 : t->nb[k] / 4;
+    return o;
+}
+
+RowNorm row_norm(const sdhip_row_norm *n) {
+    RowNorm r{};
+    if (n == nullptr) return r;
+    r.kind = n->kind;
+    r.eps = n->eps;
+    r.offset = n->weight_offset;
+    r.weight = row_operand(n->weight);
+    r.bias = row_operand(n->bias);
+    return r;
+}
 
 }  // namespace sdhip
 
@@ -117,7 +80,7 @@ int sdhip_norm_residual_supported(const sdhip_tensor *y, const sdhip_row_norm *p
     for (const sdhip_tensor *t : others) {
         if (t != nullptr && !rows_of(t, residual)) return 0;
     }
-    if (!norm_taken(post, residual) || !norm_taken(pre, residual) || (gate != nullptr && !broadcast(gate, residual))) {
+    if (!row_norm_taken(post, residual) || !row_norm_taken(pre, residual) || (gate != nullptr && !broadcasts(gate, residual))) {
         return 0;
     }
     const sdhip_tensor *const inputs[] = {y, residual};
@@ -127,7 +90,7 @@ int sdhip_norm_residual_supported(const sdhip_tensor *y, const sdhip_row_norm *p
                                             pre != nullptr ? pre->bias : nullptr};
     if (sum != nullptr && !written(sum, inputs, operands, 5)) return 0;
     if (out != nullptr && !written(out, inputs, operands, 5)) return 0;
-    return !share(sum, out);
+    return !tensors_share(sum, out);
 }
 
 sdhip_status sdhip_norm_residual(const sdhip_tensor *y, const sdhip_row_norm *post, const sdhip_tensor *gate,
@@ -165,9 +128,9 @@ sdhip_status sdhip_norm_residual(const sdhip_tensor *y, const sdhip_row_norm *po
     a.rows = residual->ne[1] * residual->ne[2] * residual->ne[3];
     a.branch_scale = branch_scale;
     a.residual_scale = residual_scale;
-    a.post = norm_of(post);
-    a.pre = norm_of(pre);
-    a.gate = operand_of(gate);
+    a.post = row_norm(post);
+    a.pre = row_norm(pre);
+    a.gate = row_operand(gate);
     return launched(launch_norm_residual(a, static_cast<hipStream_t>(stream)), "norm_residual");
 }
 

@@ -23,6 +23,7 @@
 #include <cmath>
 
 #include "host.h"
+#include "outputs.h"
 #include "profile.h"
 #include "q4.h"
 
@@ -47,18 +48,6 @@ __device__ __forceinline__ half8 widen(uint32_t word, uint32_t magic) {
     const half2 c = __builtin_bit_cast(half2, (odd & 0x000f000fu) | magic) + low;
     const half2 e = __builtin_bit_cast(half2, (odd & 0x00f000f0u) | magic) * down + high;
     return half8{a[0], a[1], b[0], b[1], c[0], c[1], e[0], e[1]};
-}
-
-__device__ __forceinline__ void swap32(uint32_t &a, uint32_t &b) {
-    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
-    a = r[0];
-    b = r[1];
-}
-
-__device__ __forceinline__ void swap16(uint32_t &a, uint32_t &b) {
-    const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
-    a = r[0];
-    b = r[1];
 }
 
 // ------------------------------------------------------------------ x
@@ -104,12 +93,6 @@ __device__ __forceinline__ void split8(const float4v &low, const float4v &high, 
     }
 }
 
-__device__ __forceinline__ float4v load4(const float *p) {
-    float4v v;
-    __builtin_memcpy(&v, p, 16);
-    return v;
-}
-
 // The greatest magnitude of four numbers, as bits.
 __device__ __forceinline__ uint32_t magnitude(const float4v &v) {
     uint32_t m = 0;
@@ -122,90 +105,6 @@ __device__ __forceinline__ uint32_t magnitude(const float4v &v) {
 }
 
 constexpr int kFewThreads = 512;
-
-// The outputs of a workgroup of `threads` from its splits' sums in LDS, `step`
-// apart, `count` outputs, with GATED the second half's behind them: their sums
-// in the splits' order, times what `place` gives with an output's row (M or
-// more: none) and column; the redirect's number first, the chain, the gated
-// GELU.  E of a thread's at a time, so that their loads go out together.
-template <bool GATED, int E, class Place>
-__device__ __forceinline__ void write_outputs(const Q4Args &a, const float *sums, int splits, int step, int count, int tid,
-                                              int columns, Place place, int threads) {
-    constexpr int kHalves = GATED ? 2 : 1;
-#pragma unroll 1
-    for (int first = tid; first < count; first += E * threads) {
-        int64_t m[E];
-        int n[E];
-        bool real[E];
-        float v[kHalves * E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int at = first + threads * e < count ? first + threads * e : first;
-            const float back = place(at, m[e], n[e]);
-            real[e] = first + threads * e < count && m[e] < a.M && n[e] < columns;
-            m[e] = m[e] < a.M ? m[e] : a.M - 1;
-            n[e] = n[e] < columns ? n[e] : columns - 1;
-#pragma unroll
-            for (int p = 0; p < kHalves; ++p) {
-                float s[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) s[k] = sums[(k < splits ? k : 0) * step + p * count + at];
-                float total = s[0];
-#pragma unroll
-                for (int k = 1; k < 8; ++k) total = k < splits ? total + s[k] : total;
-                v[kHalves * e + p] = total * back;
-            }
-        }
-        if (!GATED && a.from_redirect) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[kHalves * e] = a.y[m[e] * a.ldy + n[e]] + v[kHalves * e];
-        }
-        apply_chain_block(a.chain, v, [&](int s, int i) {
-            const DevStep &st = a.chain.steps[s];
-            const int64_t at = (n[i / kHalves] + (i % kHalves) * static_cast<int64_t>(columns)) * st.nb[0];
-            const int64_t row = m[i / kHalves];
-            if (st.flat123) return at + row * st.nb[1];
-            uint32_t i1, i2, i3;
-            split_index(static_cast<uint32_t>(row), static_cast<uint32_t>(a.ne1), static_cast<uint32_t>(a.ne2), i1, i2, i3);
-            return at + i1 * st.nb[1] + i2 * st.nb[2] + i3 * st.nb[3];
-        });
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            if (real[e]) a.y[m[e] * a.ldy + n[e]] = GATED ? v[kHalves * e] * gelu(v[kHalves * e + kHalves - 1]) : v[kHalves * e];
-        }
-    }
-}
-
-// ------------------------------------------------------------------ copies
-
-// A copy of 16 bytes a lane (1 KB) or 4 into LDS at `to` and on, lane after
-// lane.  The compiler does not see these loads, and so does not wait for them
-// where it waits for others or reads LDS: what reads them waits (wait_loads).
-// They take the place in LDS from m0, which the compiler sets as their operand
-// (and so knows what it holds); its own copies go a cycle before their use.
-__device__ __forceinline__ void fetch16(const void *from, uint32_t to) {
-    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"{m0}"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory");
-}
-__device__ __forceinline__ void fetch4(const void *from, uint32_t to) {
-    asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, off" ::"{m0}"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory");
-}
-
-// fetch16 from an address the wave's lanes share and an offset of each.
-__device__ __forceinline__ void fetch16(const char *from, uint32_t offset, uint32_t to) {
-    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(to), "v"(offset), "s"(from) : "memory");
-}
-
-__device__ __forceinline__ uint32_t lds_address(const char *p) {
-    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char *)p));
-}
-
-// wait_loads, and no read of LDS before it.
-template <int N>
-__device__ __forceinline__ void fetched() {
-    wait_loads<N>();
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-}
 
 // ------------------------------------------------------------------ few rows
 

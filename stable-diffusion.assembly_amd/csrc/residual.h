@@ -6,21 +6,9 @@
 #include <stdint.h>
 
 #include "device.h"
+#include "row_norm.h"
 
 namespace sdhip {
-
-// A tensor broadcast over the rows: strides 0 along what it is broadcast
-// over; null where there is none.
-struct RowOperand {
-    const float *data;
-    int64_t nb[4];
-};
-
-struct RowNorm {
-    int32_t kind;  // SDHIP_ROW_NORM_*
-    float eps, offset;
-    RowOperand weight, bias;
-};
 
 struct ResidualArgs {
     const float *y;  // or null

@@ -1,0 +1,282 @@
+// Rotary positions of several axes after the norm of each head's numbers: the
+// pair (u, v) of numbers that an axis turns by an angle t becomes
+//     (u cos t - v sin t, u sin t + v cos t),   t = position base^(-2 j / dims).
+// An angle is taken in double and brought to a quarter of a turn before its sine
+// and cosine in single precision, so that one of 10^7 turns keeps its 2^-24.
+//
+// Bound by memory, each number read and written once.  A wave takes a token and a
+// part of its heads: the token's sines and cosines are computed once, a pair a
+// lane, and shared through LDS by the heads, a row of which takes 8, 16 or 64 lanes,
+// each with 8 numbers of it (or 16): those of four pairs.
+
+#include <type_traits>
+
+#include "host.h"
+#include "profile.h"
+#include "rope.h"
+
+namespace sdhip {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kMostPairs = kRopeMost / 2;
+
+// cos and sin of `turns` half turns.
+__device__ __forceinline__ float2 turn(double turns) {
+    const double q = __builtin_rint(2.0 * turns);
+    const float r = static_cast<float>(__builtin_fma(-0.5, q, turns));
+    float s, c;
+    sincospif(r, &s, &c);
+    const int k = static_cast<int>(__builtin_fma(-4.0, __builtin_floor(0.25 * q), q));
+    const float2 t = k & 1 ? make_float2(-s, c) : make_float2(c, s);
+    return k & 2 ? make_float2(-t.x, -t.y) : t;
+}
+
+// The sum of a row's LPR lanes, on all of them.
+template <int LPR>
+__device__ __forceinline__ double row_sum(double v) {
+    if constexpr (LPR == 64) return wave_sum(v);
+    v += moved<0xb1>(v);   // lanes i ^ 1
+    v += moved<0x4e>(v);   // i ^ 2
+    v += moved<0x141>(v);  // 8 lanes mirrored
+    if constexpr (LPR == 16) v += moved<0x140>(v);  // 16 lanes mirrored
+    return v;
+}
+
+// LPR lanes a row, SLOTS groups of four pairs each; QUADS where every four
+// numbers that a lane reads or writes at once lie at a multiple of their size.
+template <int LPR, int SLOTS, bool ADJACENT, bool QUADS>
+__global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
+    __shared__ float2 shared[kWaves][kMostPairs];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int pairs = a.turned / 2;
+    float2 *turns = shared[wave];
+    // The frequencies, in half turns, of the pairs that this lane computes.
+    constexpr int kMine = kMostPairs / 64;
+    double rate[kMine];
+    int axis[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        const int p = lane + 64 * i;
+        axis[i] = 0;
+#pragma unroll
+        for (int j = 1; j < SDHIP_MAX_AXES; ++j)
+            if (j < a.count && p >= a.first[j]) axis[i] = j;
+        rate[i] = 64 * i < pairs ? exp2(a.rate[axis[i]] * (p - a.from[axis[i]])) * 0.31830988618379067154 : 0.0;
+    }
+    // This lane's pairs: the place of each one's numbers, d or more where there is none.
+    const int sub = lane % LPR;
+    const int front = ADJACENT ? 0 : (pairs + 3) / 4;  // groups of halves' pairs, before those that are not turned
+    int at[SLOTS][4][2];
+    bool turned[SLOTS][4];
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int group = sub + LPR * s;
+            if (ADJACENT) {
+                const int p = 4 * group + c;
+                at[s][c][0] = 2 * p;
+                at[s][c][1] = 2 * p + 1;
+                turned[s][c] = p < pairs;
+            } else if (group < front) {
+                const int p = 4 * group + c;
+                at[s][c][0] = p < pairs ? p : a.d;
+                at[s][c][1] = p < pairs ? p + pairs : a.d;
+                turned[s][c] = p < pairs;
+            } else {
+                const int i = a.turned + 8 * (group - front) + c;
+                at[s][c][0] = i;
+                at[s][c][1] = i + 4;
+                turned[s][c] = false;
+            }
+        }
+    // With QUADS the numbers of a group are two runs of four: an ADJACENT one's
+    // pairs are within them, a HALVES one's across.
+    const auto load = [&](const float *row, bool quads, int64_t step, float (&v)[SLOTS][4][2]) {
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s) {
+            if (QUADS && quads) {
+                float4v q[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int i = ADJACENT ? at[s][2 * h][0] : at[s][0][h];
+                    q[h] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+                    if (i < a.d) q[h] = *reinterpret_cast<const float4v *>(row + i);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) v[s][c][h] = ADJACENT ? q[c / 2][2 * (c % 2) + h] : q[h][c];
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) v[s][c][h] = at[s][c][h] < a.d ? row[at[s][c][h] * step] : 0.0f;
+            }
+        }
+    };
+    const auto store = [&](auto *row, const float (&v)[SLOTS][4][2]) {
+        typedef std::conditional_t<sizeof(*row) == 2, half4, float4v> Four;
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s) {
+            if constexpr (QUADS) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int i = ADJACENT ? at[s][2 * h][0] : at[s][0][h];
+                    Four q;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) q[c] = ADJACENT ? v[s][2 * h + c / 2][c % 2] : v[s][c][h];
+                    if (i < a.d) *reinterpret_cast<Four *>(row + i) = q;
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        if (at[s][c][h] < a.d) row[at[s][c][h]] = static_cast<std::remove_reference_t<decltype(*row)>>(v[s][c][h]);
+            }
+        }
+    };
+    const auto quads_of = [&](const RowOperand &o) {
+        return QUADS && o.nb[0] == 1 && reinterpret_cast<uintptr_t>(o.data) % 16 == 0 && o.nb[1] % 4 == 0 && o.nb[2] % 4 == 0 &&
+               o.nb[3] % 4 == 0;
+    };
+    const bool weight_quads = quads_of(a.norm.weight), bias_quads = quads_of(a.norm.bias);
+    constexpr int kRows = 64 / LPR;  // heads of a wave at a time
+    const int share = (a.heads + a.parts - 1) / a.parts;
+    const int64_t items = a.tokens * a.batch * a.parts;
+    for (int64_t item = static_cast<int64_t>(blockIdx.x) * kWaves + wave; item < items;
+         item += static_cast<int64_t>(gridDim.x) * kWaves) {
+        const int64_t token = item / a.parts;
+        const int part = static_cast<int>(item - token * a.parts);
+        const int64_t i3 = token / a.tokens, i1 = token - i3 * a.tokens;
+        const float *positions = a.positions + i1 * a.pnb1 + i3 * a.pnb3;
+        // The turns of the token before are read.
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+            if (64 * i < pairs && lane + 64 * i < pairs) turns[lane + 64 * i] = turn(static_cast<double>(positions[axis[i]]) * rate[i]);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        float2 by[SLOTS][4];
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) by[s][c] = turned[s][c] ? turns[4 * (sub + LPR * s) + c] : make_float2(1.0f, 0.0f);
+        const int h0 = part * share, h1 = h0 + share < a.heads ? h0 + share : a.heads;
+        for (int h = h0 + lane / LPR; h - lane / LPR < h1; h += kRows) {
+            if (h >= h1) continue;  // a row's lanes together
+            float v[SLOTS][4][2];
+            load(a.x + i1 * a.xnb[1] + h * a.xnb[2] + i3 * a.xnb[3], true, 1, v);
+            if (a.norm.kind != SDHIP_ROW_NORM_NONE) {
+                double mean = 0.0, squares = 0.0;
+                if (a.norm.kind == SDHIP_ROW_NORM_LAYER) {
+#pragma unroll
+                    for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) mean += static_cast<double>(v[s][c][0]) + static_cast<double>(v[s][c][1]);
+                    mean = mean_of(row_sum<LPR>(mean), a.d, a.inverse);
+                }
+#pragma unroll
+                for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const double x = at[s][c][k] < a.d ? static_cast<double>(v[s][c][k]) - mean : 0.0;
+                            squares = __builtin_fma(x, x, squares);
+                        }
+                const Moments m = moments(a.norm.kind, mean, row_sum<LPR>(squares), a.inverse, a.norm.eps);
+#pragma unroll
+                for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) v[s][c][k] = normed(v[s][c][k], m);
+            }
+            const auto operand = [&](const RowOperand &o, bool quads, float (&w)[SLOTS][4][2]) {
+                load(o.data + i1 * o.nb[1] + h * o.nb[2] + i3 * o.nb[3], quads, o.nb[0], w);
+            };
+            if (a.norm.weight.data != nullptr) {
+                float w[SLOTS][4][2];
+                operand(a.norm.weight, weight_quads, w);
+#pragma unroll
+                for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) v[s][c][k] = __fmul_rn(v[s][c][k], __fadd_rn(w[s][c][k], a.norm.offset));
+            }
+            if (a.norm.bias.data != nullptr) {
+                float w[SLOTS][4][2];
+                operand(a.norm.bias, bias_quads, w);
+#pragma unroll
+                for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) v[s][c][k] = __fadd_rn(v[s][c][k], w[s][c][k]);
+            }
+#pragma unroll
+            for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if (!turned[s][c]) continue;
+                    const float one = v[s][c][0], two = v[s][c][1], cosine = by[s][c].x, sine = by[s][c].y;
+                    v[s][c][0] = __builtin_fmaf(-two, sine, one * cosine);
+                    v[s][c][1] = __builtin_fmaf(one, sine, two * cosine);
+                }
+            const int64_t to = i1 * a.ynb[1] + h * a.ynb[2] + i3 * a.ynb[3];
+            if (a.half) {
+                store(static_cast<_Float16 *>(a.y) + to, v);
+            } else {
+                store(static_cast<float *>(a.y) + to, v);
+            }
+        }
+    }
+}
+
+template <int LPR, int SLOTS>
+hipError_t launch(RopeArgs a, bool quads, hipStream_t stream) {
+    // Parts of a token's heads until every wave of the device has one, 16 a CU.
+    const int64_t waves = 16 * static_cast<int64_t>(compute_units()), tokens = a.tokens * a.batch;
+    const int64_t most = ceil_div(a.heads, 64 / LPR);
+    a.parts = static_cast<int32_t>(tokens * most <= waves ? most : tokens >= waves ? 1 : ceil_div(waves, tokens));
+    const int64_t items = tokens * a.parts;
+    const dim3 grid(static_cast<uint32_t>(ceil_div(items < 2 * waves ? items : 2 * waves, kWaves))), block(kThreads);
+    if (a.order == SDHIP_ROPE_ADJACENT) {
+        if (quads) {
+            SDHIP_LAUNCH((rope_kernel<LPR, SLOTS, true, true>), grid, block, 0, stream, a);
+        } else {
+            SDHIP_LAUNCH((rope_kernel<LPR, SLOTS, true, false>), grid, block, 0, stream, a);
+        }
+    } else if (quads) {
+        SDHIP_LAUNCH((rope_kernel<LPR, SLOTS, false, true>), grid, block, 0, stream, a);
+    } else {
+        SDHIP_LAUNCH((rope_kernel<LPR, SLOTS, false, false>), grid, block, 0, stream, a);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_rope(RopeArgs a, hipStream_t stream) {
+    KernelScope scope("rope", stream);
+    const auto strides = [](const int64_t (&nb)[4]) { return nb[1] % 4 == 0 && nb[2] % 4 == 0 && nb[3] % 4 == 0; };
+    const bool quads = a.d % 4 == 0 && (a.order == SDHIP_ROPE_ADJACENT || a.turned % 8 == 0) && strides(a.xnb) && strides(a.ynb) &&
+                       reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && reinterpret_cast<uintptr_t>(a.y) % (a.half ? 8 : 16) == 0;
+    // Groups of four pairs of a row; a HALVES row's numbers that are not turned
+    // are groups of their own.
+    const int groups = static_cast<int>(a.order == SDHIP_ROPE_ADJACENT ? ceil_div(a.d, 8)
+                                                                       : ceil_div(a.turned, 8) + ceil_div(a.d - a.turned, 8));
+    if (groups <= 8) return launch<8, 1>(a, quads, stream);
+    if (groups <= 16) return launch<16, 1>(a, quads, stream);
+    if (groups <= 32) return launch<16, 2>(a, quads, stream);
+    return launch<64, 2>(a, quads, stream);
+}
+
+}  // namespace sdhip

@@ -18,12 +18,16 @@ TYPE_F32 = 0
 TYPE_F16 = 1
 TYPE_Q4_0 = 2
 TYPE_Q4_1 = 3
+TYPE_F8_E4M3 = 256
 BLOCK = 32  # weights of a block of Q4_0 or Q4_1 ...
 BLOCK_BYTES = {TYPE_Q4_0: 18, TYPE_Q4_1: 20}  # ... and its bytes
 OK, UNSUPPORTED, ERROR = 0, 1, 2
 STEP_ADD, STEP_MUL, STEP_SILU = 0, 1, 2
 MAX_STEPS = 6
 ROW_NORM_NONE, ROW_NORM_LAYER, ROW_NORM_RMS = 0, 1, 2
+ROPE_ADJACENT, ROPE_HALVES = 0, 1
+MAX_AXES = 4
+F8_BLOCK = 128  # weights of F8_E4M3 share a scale in blocks of this by this
 
 
 class Tensor(ctypes.Structure):
@@ -60,6 +64,18 @@ class RowNorm(ctypes.Structure):
     ]
 
 
+class RopeAxes(ctypes.Structure):
+    """sdhip_rope_axes: the axes of rotary positions."""
+
+    _fields_ = [
+        ("count", ctypes.c_int32),
+        ("order", ctypes.c_int32),
+        ("shared", ctypes.c_int32),
+        ("dims", ctypes.c_int32 * MAX_AXES),
+        ("base", ctypes.c_float * MAX_AXES),
+    ]
+
+
 MAX_SRC = 10
 MAX_OP_PARAMS = 16
 
@@ -91,6 +107,7 @@ class NodePlan(ctypes.Structure):
 _T = ctypes.POINTER(Tensor)
 _E = ctypes.POINTER(Epilogue)
 _R = ctypes.POINTER(RowNorm)
+_X = ctypes.POINTER(RopeAxes)
 _P = ctypes.c_void_p
 _SZ = ctypes.c_size_t
 _I6 = ctypes.c_int32 * 6
@@ -114,6 +131,11 @@ SIGNATURES = [
     ("sdhip_mul_mat", ctypes.c_int, [_T, _T, _T, _E, _P, _SZ, _P]),
     ("sdhip_mul_mat_gated_supported", ctypes.c_int, [_T, _T, _T, _T]),
     ("sdhip_mul_mat_gated", ctypes.c_int, [_T, _T, _T, _E, _T, _P, _SZ, _P]),
+    ("sdhip_mul_mat_f8_supported", ctypes.c_int, [_T, _T, _T, _T]),
+    ("sdhip_mul_mat_f8_work_size", _SZ, [_T, _T, _T, _T]),
+    ("sdhip_mul_mat_f8", ctypes.c_int, [_T, _T, _T, _T, _E, _P, _SZ, _P]),
+    ("sdhip_mul_mat_f8_gated_supported", ctypes.c_int, [_T, _T, _T, _T, _T]),
+    ("sdhip_mul_mat_f8_gated", ctypes.c_int, [_T, _T, _T, _T, _E, _T, _P, _SZ, _P]),
     ("sdhip_conv2d_supported", ctypes.c_int, [_T, _T, _T, _I6]),
     ("sdhip_conv2d_path", ctypes.c_int, [_T, _T, _T, _I6]),
     ("sdhip_conv2d_work_size", _SZ, [_T, _T, _T, _I6]),
@@ -122,10 +144,15 @@ SIGNATURES = [
     ("sdhip_attention_work_size", _SZ, [_T, _T, _T, _T]),
     ("sdhip_attention", ctypes.c_int,
      [_T, _T, _T, _T, ctypes.c_float, ctypes.c_float, ctypes.c_float, _P, _SZ, _P]),
+    ("sdhip_rope_supported", ctypes.c_int, [_T, _R, _T, _X, _T]),
+    ("sdhip_rope", ctypes.c_int, [_T, _R, _T, _X, _T, _P]),
     ("sdhip_group_norm_supported", ctypes.c_int, [_T, _T, ctypes.c_int]),
     ("sdhip_group_norm_work_size", _SZ, [_T, _T, ctypes.c_int]),
     ("sdhip_group_norm", ctypes.c_int, [_T, _T, ctypes.c_int, ctypes.c_float, _E, _P, _SZ, _P]),
     ("sdhip_group_norm_static", ctypes.c_int, [_T, _T, ctypes.c_int, ctypes.c_float, _E, _P]),
+    ("sdhip_group_norm_last_supported", ctypes.c_int, [_T, _T, ctypes.c_int]),
+    ("sdhip_group_norm_last_work_size", _SZ, [_T, _T, ctypes.c_int]),
+    ("sdhip_group_norm_last", ctypes.c_int, [_T, _T, ctypes.c_int, ctypes.c_float, _E, _P, _SZ, _P]),
     ("sdhip_norm_supported", ctypes.c_int, [_T, _T]),
     ("sdhip_norm", ctypes.c_int, [_T, _T, ctypes.c_float, _E, _P]),
     ("sdhip_norm_residual_supported", ctypes.c_int, [_T, _R, _T, _T, _T, _R, _T]),
@@ -194,6 +221,8 @@ def desc(t):
         d.type, size = TYPE_F32, 4
     elif t.dtype == torch.float16:
         d.type, size = TYPE_F16, 2
+    elif t.dtype == torch.float8_e4m3fn:
+        d.type, size = TYPE_F8_E4M3, 1
     else:
         raise ValueError(f"type {t.dtype}")
     shape = list(t.shape)[::-1]
@@ -207,6 +236,12 @@ def desc(t):
             d.nb[k] = d.nb[k - 1] * d.ne[k - 1] if k > 0 else size
     d.data = t.data_ptr()
     return d
+
+
+def _images(t):
+    """The descriptor of channels-last images: [C, W, H, N] of [N, H, W, C], of
+    [N, L, C] with H = 1, of [L, C] with H = N = 1."""
+    return desc(t[:, None] if t.dim() == 3 else t)
 
 
 def view_desc(data_ptr, dtype_code, ne, nb):
@@ -286,6 +321,34 @@ def mul_mat_gated(w, x, y, out, chain=None, work=None):
     return buf
 
 
+def mul_mat_f8(w, scales, x, y, chain=None, work=None):
+    """y = x W^T with the chain; w: [N, K] float8_e4m3fn, scales: [N / 128, K / 128]
+    f32 (rounded up), x: [..., K] f32."""
+    lib = load()
+    dw, ds, dx, dy = desc(w), desc(scales), desc(x), desc(y)
+    size = lib.sdhip_mul_mat_f8_work_size(dw, ds, dx, dy)
+    buf = work
+    if buf is None:
+        buf, _ = _work(size, x.device)
+    ptr = buf.data_ptr() if buf is not None else None
+    check(lib.sdhip_mul_mat_f8(dw, ds, dx, dy, ctypes.byref(chain) if chain else None, ptr, size, stream_handle()),
+          "mul_mat_f8")
+    return buf
+
+
+def mul_mat_f8_gated(w, scales, x, y, out, chain=None, work=None):
+    lib = load()
+    dw, ds, dx, dy, do = desc(w), desc(scales), desc(x), desc(y), desc(out)
+    size = lib.sdhip_mul_mat_f8_work_size(dw, ds, dx, dy)
+    buf = work
+    if buf is None:
+        buf, _ = _work(size, x.device)
+    ptr = buf.data_ptr() if buf is not None else None
+    check(lib.sdhip_mul_mat_f8_gated(dw, ds, dx, dy, ctypes.byref(chain) if chain else None, do, ptr, size,
+                                     stream_handle()), "mul_mat_f8_gated")
+    return buf
+
+
 def conv_params(s0=1, s1=1, p0=0, p1=0, d0=1, d1=1):
     return _I6(s0, s1, p0, p1, d0, d1)
 
@@ -332,6 +395,20 @@ def group_norm(x, y, groups, eps, chain=None, work=None):
     return buf
 
 
+def group_norm_last(x, y, groups, eps, chain=None, work=None):
+    """GROUP_NORM of x [N, H, W, C] (or [N, L, C], [L, C]) over its last dimension's groups."""
+    lib = load()
+    dx, dy = (_images(t) for t in (x, y))
+    size = lib.sdhip_group_norm_last_work_size(dx, dy, groups)
+    buf = work
+    if buf is None:
+        buf, _ = _work(size, x.device)
+    ptr = buf.data_ptr() if buf is not None else None
+    check(lib.sdhip_group_norm_last(dx, dy, groups, eps, ctypes.byref(chain) if chain else None, ptr, size,
+                                    stream_handle()), "group_norm_last")
+    return buf
+
+
 def group_norm_static(x, y, groups, eps, chain=None):
     """sdhip_group_norm_static: no work buffer, the library's static scratch."""
     check(load().sdhip_group_norm_static(desc(x), desc(y), groups, eps, ctypes.byref(chain) if chain else None,
@@ -365,6 +442,29 @@ def norm_residual(y, residual, sum=None, out=None, post=None, pre=None, gate=Non
     dy, ds, do, dg = (desc(t) if t is not None else None for t in (y, sum, out, gate))
     check(load().sdhip_norm_residual(dy, post, dg, branch_scale, desc(residual), residual_scale, ds, pre, do,
                                      stream_handle()), "norm_residual")
+
+
+def rope_axes(dims, base=10000.0, order="adjacent", shared=False):
+    """The axes of rotary positions: `dims` a head's numbers of each, `base` one
+    for all or one each, order 'adjacent' or 'halves'."""
+    dims = list(dims)
+    bases = [base] * len(dims) if isinstance(base, (int, float)) else list(base)
+    if len(bases) != len(dims) or len(dims) > MAX_AXES:
+        raise ValueError(f"{len(dims)} axes and {len(bases)} bases, at most {MAX_AXES}")
+    a = RopeAxes()
+    a.count = len(dims)
+    a.order = {"adjacent": ROPE_ADJACENT, "halves": ROPE_HALVES}[order]
+    a.shared = 1 if shared else 0
+    for i, (d, b) in enumerate(zip(dims, bases)):
+        a.dims[i], a.base[i] = d, b
+    return a
+
+
+def rope(x, positions, axes, y, norm=None):
+    """y = x [batch, heads, tokens, d] turned by the positions [tokens, axes] or [batch, tokens, axes]
+    (extents of 1 are broadcast), after a norm of each head's numbers (row_norm) if there is one."""
+    at = positions if positions.dim() != 3 else positions[:, None]
+    check(load().sdhip_rope(desc(x), norm, desc(at), axes, desc(y), stream_handle()), "rope")
 
 
 def profile_enable(on=True):
