@@ -133,7 +133,10 @@ const char *sdhip_last_error(void);
  * nine taps would be taken directly), q4_form (1 .. 6: the products of 4-bit
  * weights by one of their forms -- each workgroup's rows of x split in it, x laid
  * out first, or both operands, tiles of 128 x 128 by four waves, by eight, of
- * 64 x 128, or, not the gated ones, of 64 x 192 -- whatever the size),
+ * 64 x 128, or, not the gated ones, of 64 x 192 -- whatever the size), f8_form (1
+ * .. 6: those of 8-bit floating-point weights, each workgroup's rows of x brought to
+ * E4M3 in it, x laid out first, or tiles of 128 x 128 by four waves, by eight, of 64
+ * x 128, of 64 x 64),
  * attention_generic, attention_fp32 (forms to compare, same results within
  * the bounds -- qgemm_core's bit for bit), each taking only its documented
  * values.  Returns SDHIP_ERROR

@@ -129,6 +129,7 @@ const Field kFields[] = {
     {"conv_panels", &Tuning::conv_panels, kFlag},
     {"conv3x3_direct", &Tuning::conv3x3_direct, kFlag},
     {"q4_form", &Tuning::q4_form, kForm},
+    {"f8_form", &Tuning::f8_form, kForm},
     {"qgemm_core", &Tuning::qgemm_core, kFlag2},
     {"attention_generic", &Tuning::attention_generic, kFlag},
     {"attention_fp32", &Tuning::attention_fp32, kFlag},

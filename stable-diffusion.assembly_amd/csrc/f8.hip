@@ -20,7 +20,7 @@
 // output, and a block's sums go to the outputs' by one multiplication a lane and an
 // addition each.
 
-#include <algorithm>
+#include <type_traits>
 
 #include "f8.h"
 #include "host.h"
@@ -55,6 +55,14 @@ __device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_ca
 
 __device__ __forceinline__ uint32_t greater(uint32_t a, uint32_t b) { return a > b ? a : b; }
 
+// The greatest of a row of 16 lanes, on all of them.
+__device__ __forceinline__ uint32_t greatest16(uint32_t v) {
+    v = greater(v, __builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, true));   // lanes i ^ 1
+    v = greater(v, __builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, true));   // i ^ 2
+    v = greater(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true));  // 8 lanes mirrored
+    return greater(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true));  // 16 lanes mirrored
+}
+
 // Eight numbers of E4M3 as FP16.
 __device__ __forceinline__ half8 widen(int low, int high) {
     const half2v a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(low, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(low, 1.0f, true);
@@ -70,9 +78,10 @@ __device__ __forceinline__ int four(const float4v &v, float scale, bool finite) 
     return finite ? r : static_cast<int>(kNans);
 }
 
-// Four of a row's K numbers from k on, 0 past its end.
-__device__ __forceinline__ float4v load_x(const float *row, int64_t k, int64_t K) {
-    if (k + 4 <= K) return load4(row + k);
+// Four of a row's K numbers from k on, of the last four there are where those end
+// before; rows of fewer than four number by number, 0 past their end.
+__device__ __forceinline__ float4v load_x(const float *row, int k, int K) {
+    if (K >= 4) return load4(row + (k + 4 <= K ? k : K - 4));
     float4v v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < 3; ++i)
@@ -80,17 +89,52 @@ __device__ __forceinline__ float4v load_x(const float *row, int64_t k, int64_t K
     return v;
 }
 
-// 16 of a row's K weights from k on, 0 past its end: of what follows a row
-// nothing is read, since it may be no memory or hold NaN.
-__device__ __forceinline__ int4v load_w(const uint8_t *row, int64_t k, int64_t K) {
+// What load_x gave at k as the numbers from there on, 0 past the row's end.
+__device__ __forceinline__ float4v ended_x(const float4v &v, int k, int K) {
+    const int past = k + 4 - K;  // numbers that lie before k, and are wanted of none past K
+    if (K < 4 || past <= 0) return v;
+    return past == 1 ? float4v{v[1], v[2], v[3], 0.0f} : past == 2 ? float4v{v[2], v[3], 0.0f, 0.0f}
+                                                    : past == 3 ? float4v{v[3], 0.0f, 0.0f, 0.0f} : float4v{0.0f, 0.0f, 0.0f, 0.0f};
+}
+
+// 16 of a row's K weights from k on, of the last 16 there are where those end
+// before: of what follows a row nothing is read, since it may be no memory.  Rows of
+// fewer than 16 are read byte by byte, 0 past their end.
+__device__ __forceinline__ int4v load_w(const uint8_t *row, int k, int K) {
     int4v v = {0, 0, 0, 0};
-    if (k + 16 <= K) {
-        __builtin_memcpy(&v, row + k, 16);
+    if (K >= 16) {
+        __builtin_memcpy(&v, row + (k + 16 <= K ? k : K - 16), 16);
     } else {
-#pragma unroll
-        for (int i = 0; i < 15; ++i)
-            if (k + i < K) v[i / 4] |= static_cast<int>(row[k + i]) << (8 * (i % 4));
+        uint64_t low = 0, high = 0;
+#pragma unroll 1
+        for (int i = k; i < K; ++i) {
+            const uint64_t byte = static_cast<uint64_t>(row[i]) << (8 * (i & 7));
+            low |= i < 8 ? byte : 0;
+            high |= i < 8 ? 0 : byte;
+        }
+        const uint64_t q[2] = {low, high};
+        __builtin_memcpy(&v, q, 16);
     }
+    return v;
+}
+
+// What load_w gave at k as the weights from there on, 0 past the row's end.
+__device__ __forceinline__ int4v ended_w(int4v v, int k, int K) {
+    const int past = k + 16 - K;  // bytes that lie before k, and are wanted of none past K
+    if (K < 16 || past <= 0) return v;
+    if (past >= 16) return int4v{0, 0, 0, 0};
+    uint64_t q[2];
+    __builtin_memcpy(q, &v, 16);
+    const int bits = 8 * (past & 7);
+    if (past >= 8) {
+        q[0] = q[1];
+        q[1] = 0;
+    }
+    if (bits) {
+        q[0] = q[0] >> bits | q[1] << (64 - bits);
+        q[1] >>= bits;
+    }
+    __builtin_memcpy(&v, q, 16);
     return v;
 }
 
@@ -139,34 +183,34 @@ struct OperandsArgs {
 __global__ __launch_bounds__(kOperandThreads) void f8_operands_kernel(OperandsArgs o) {
     const F8Args &a = o.a;
     if (blockIdx.x >= o.x_grid) {
-        const int64_t pieces = o.w.ld / 16;
-        const int64_t i = static_cast<int64_t>(blockIdx.x - o.x_grid) * kOperandThreads + threadIdx.x;
-        const int64_t n = i / pieces, k = (i - n * pieces) * 16;
-        if (n < a.N) *reinterpret_cast<int4v *>(o.w.w + n * o.w.ld + k) = load_w(a.w + n * a.row_bytes, k, a.K);
+        const int64_t pieces = o.w.ld / 16, all = pieces * a.N, step = static_cast<int64_t>(gridDim.x - o.x_grid) * kOperandThreads;
+        for (int64_t i = static_cast<int64_t>(blockIdx.x - o.x_grid) * kOperandThreads + threadIdx.x; i < all; i += step) {
+            const int64_t n = i / pieces;
+            const int k = static_cast<int>(i - n * pieces) * 16, K = static_cast<int>(a.K);
+            *reinterpret_cast<int4v *>(o.w.w + n * o.w.ld + k) = ended_w(load_w(a.w + n * a.row_bytes, k, K), k, K);
+        }
         return;
     }
-    const uint32_t g = blockIdx.x * (kOperandThreads / 16) + threadIdx.x / 16;
-    if (g >= o.groups) return;  // the 16 lanes of a group together
-    const uint32_t m = g / o.blocks, b = g - m * o.blocks;
-    const int64_t k = static_cast<int64_t>(b) * kBlock + 8 * (threadIdx.x & 15);
-    const float *row = a.x + m * a.ldx;
-    float4v v[2];
-    uint32_t top = 0;
+    // The 16 lanes of a group together.
+    for (uint32_t g = blockIdx.x * (kOperandThreads / 16) + threadIdx.x / 16; g < o.groups; g += o.x_grid * (kOperandThreads / 16)) {
+        const uint32_t m = g / o.blocks, b = g - m * o.blocks;
+        const int k = static_cast<int>(b) * kBlock + 8 * (threadIdx.x & 15), K = static_cast<int>(a.K);
+        const float *row = a.x + m * a.ldx;
+        float4v v[2];
+        uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        v[i] = load_x(row, k + 4 * i, a.K);
+        for (int i = 0; i < 2; ++i) {
+            v[i] = ended_x(load_x(row, k + 4 * i, K), k + 4 * i, K);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) top = greater(top, magnitude(v[i][j]));
+            for (int j = 0; j < 4; ++j) top = greater(top, magnitude(v[i][j]));
+        }
+        top = greatest16(top);
+        const uint32_t e = power_of(top);
+        const float scale = down(e);
+        const bool finite = top < kInfinity;
+        *reinterpret_cast<half8 *>(o.w.q + m * o.w.ld + k) = widen(four(v[0], scale, finite), four(v[1], scale, finite));
+        if ((threadIdx.x & 15) == 0) o.w.powers[b * o.w.rows + m] = finite ? up(e) : 1.0f;
     }
-    top = greater(top, __builtin_amdgcn_update_dpp(0, top, 0xb1, 0xf, 0xf, true));   // lanes i ^ 1
-    top = greater(top, __builtin_amdgcn_update_dpp(0, top, 0x4e, 0xf, 0xf, true));   // i ^ 2
-    top = greater(top, __builtin_amdgcn_update_dpp(0, top, 0x141, 0xf, 0xf, true));  // 8 lanes mirrored
-    top = greater(top, __builtin_amdgcn_update_dpp(0, top, 0x140, 0xf, 0xf, true));  // 16 lanes mirrored
-    const uint32_t e = power_of(top);
-    const float scale = down(e);
-    const bool finite = top < kInfinity;
-    *reinterpret_cast<half8 *>(o.w.q + m * o.w.ld + k) = widen(four(v[0], scale, finite), four(v[1], scale, finite));
-    if ((threadIdx.x & 15) == 0) o.w.powers[b * o.w.rows + m] = finite ? up(e) : 1.0f;
 }
 
 // ------------------------------------------------------------------ few rows
@@ -174,160 +218,600 @@ __global__ __launch_bounds__(kOperandThreads) void f8_operands_kernel(OperandsAr
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 
-struct RowsArgs {
+struct FewArgs {
     F8Args a;
-    F8Work w;
     int32_t splits;  // of K, a wave each; the other waves take further columns
+    int32_t chunk;   // blocks of K whose x is in LDS at a time
+    int32_t row;     // bytes of a row of it
     uint32_t column_blocks;
 };
 
-// A workgroup takes 16 RM rows of x and kWaves / splits tiles of 16 columns, a
-// wave a tile (with GATED its columns of both halves) and every splits-th block of
-// K; its operands come straight from memory into registers, and the splits' sums
-// are joined in LDS.  x comes from the work buffer (LAID) or, for up to 16 rows, as
-// it is: a lane holds the 32 numbers of a row's group that the MFMA wants of it, and
-// four lanes have the group's greatest between them.
-template <bool GATED, bool LAID, int RM>
-__global__ __launch_bounds__(kThreads) void f8_rows_kernel(RowsArgs f) {
+// A workgroup takes 16 RM rows of x and kWaves / splits tiles of 16 rows of the
+// weights (with GATED half of them of each half), a wave a tile and every splits-th
+// block of K.  x is brought to E4M3 in it, a group by 16 lanes, and kept in LDS in FP16 with
+// the groups' powers, by chunks of K where it is long; the weights come straight from
+// memory into registers, kAhead blocks of a wave's under way, 64 bytes of a row side
+// by side in a load.  The splits' sums are joined in LDS.
+// A wave's blocks under way, as many as 128 registers hold: two workgroups a CU.
+constexpr int few_ahead(int rm) { return rm > 1 ? 2 : 3; }
+
+template <bool GATED, int RM>
+__global__ __launch_bounds__(kThreads, 4) void f8_few_kernel(FewArgs f) {
     const F8Args &a = f.a;
-    constexpr int RN = GATED ? 2 : 1;
-    extern __shared__ __attribute__((aligned(16))) float sums[];
+    constexpr int kRows = 16 * RM, kAhead = few_ahead(RM);
+    extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, group = lane >> 4;
     const int S = f.splits, P = kWaves / S;
-    const int split = wave % S, tile = wave / S;
+    const int outs = GATED ? P / 2 : P;  // tiles of the output
+    const int split = wave & (S - 1), second = GATED && wave / S >= outs, tile = wave / S - (second ? outs : 0);
     const uint32_t row_block = blockIdx.x / f.column_blocks;
-    const int64_t m0 = static_cast<int64_t>(row_block) * (16 * RM);
+    const int64_t m0 = static_cast<int64_t>(row_block) * kRows;
+    const int rows = static_cast<int>(a.M - m0 < kRows ? a.M - m0 : kRows);
     const int columns = static_cast<int>(GATED ? a.half : a.N);
-    const int n0 = static_cast<int>(blockIdx.x - row_block * f.column_blocks) * (16 * P);
-    const int blocks = static_cast<int>((a.K + kBlock - 1) / kBlock);
+    const int n0 = static_cast<int>(blockIdx.x - row_block * f.column_blocks) * (16 * outs);
+    const int K = static_cast<int>(a.K), blocks = (K + kBlock - 1) / kBlock;
     const int n = n0 + 16 * tile;
-    const uint8_t *w[RN];
-    const float *scales[RN][2];  // of the lane's first output and of its last, which lie in two blocks at most
-    int across[RN];              // the outputs of the lane in the first one's block
+
+    // Groups of x, 32 at a time by the workgroup, kLoads such passes' loads together.
+    constexpr int kLoads = 2;
+    const int team = tid >> 4, part = tid & 15;
+    float *powers = reinterpret_cast<float *>(lds + rows * f.row);  // [row][block of the chunk]
+    struct Numbers {
+        float4v v[kLoads][2];
+    };
+    const auto load_groups = [&](int b0, int count, int first, Numbers &x) {
 #pragma unroll
-    for (int j = 0; j < RN; ++j) {
-        const int64_t from = j ? columns : 0;
-        w[j] = a.w + (from + (n + col < columns ? n + col : columns - 1)) * a.row_bytes;
-        const int64_t low = from + (n + 4 * group < columns ? n + 4 * group : columns - 1);
-        const int64_t high = low + 3 < a.N ? low + 3 : a.N - 1;
-        scales[j][0] = a.scales + low / kBlock * a.ld_scales;
-        scales[j][1] = a.scales + high / kBlock * a.ld_scales;
-        across[j] = kBlock - static_cast<int>(low % kBlock);
-    }
-    const _Float16 *q[RM];
-    const float *powers[RM], *rows[RM];
+        for (int u = 0; u < kLoads; ++u) {
+            const int g = first + 32 * u + team, r = g / count, k = (b0 + g - r * count) * kBlock + 8 * part;
+            if (r < rows) {
+                const float *from = a.x + (m0 + r) * a.ldx;
+                x.v[u][0] = load_x(from, k, K);
+                x.v[u][1] = load_x(from, k + 4, K);
+            }
+        }
+    };
+    const auto store_groups = [&](int b0, int count, int first, const Numbers &x) {
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) {
+            const int g = first + 32 * u + team, r = g / count, b = g - r * count, k = (b0 + b) * kBlock + 8 * part;
+            float4v v[2];
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                v[i] = ended_x(x.v[u][i], k + 4 * i, K);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) top = greater(top, magnitude(v[i][j]));
+            }
+            top = greatest16(top);
+            const uint32_t e = power_of(top);
+            const float scale = down(e);
+            const bool finite = top < kInfinity;
+            if (r < rows) {
+                *reinterpret_cast<half8 *>(lds + r * f.row + b * (2 * kBlock) + 16 * part) =
+                    widen(four(v[0], scale, finite), four(v[1], scale, finite));
+                if (part == 0) powers[r * f.chunk + b] = finite ? up(e) : 1.0f;
+            }
+        }
+    };
+    Numbers begun;
+    load_groups(0, f.chunk < blocks ? f.chunk : blocks, 0, begun);
+
+    // The lane's row of the weights; the scales of its first output and of its last,
+    // which with GATED lie in two blocks at most, `across` of them in the first.
+    const int64_t from = second ? columns : 0;
+    const uint8_t *w = a.w + (from + (n + col < columns ? n + col : columns - 1)) * a.row_bytes;
+    const int64_t low = from + (n + 4 * group < columns ? n + 4 * group : columns - 1), high = low + 3 < a.N ? low + 3 : a.N - 1;
+    const float *scales[2] = {a.scales + low / kBlock * a.ld_scales, a.scales + high / kBlock * a.ld_scales};
+    const int across = kBlock - static_cast<int>(low % kBlock);
+    struct Weights {
+        int4v q[2];  // numbers 16 group .. of a block and 64 + 16 group ..
+        float s[2];
+    };
+    const auto load_weights = [&](int b, Weights &o) {
+        if (b >= blocks) return;
+        const int k = b * kBlock + 16 * group;
+        o.q[0] = load_w(w, k, K);
+        o.q[1] = load_w(w, k + 64, K);
+        o.s[0] = scales[0][b];
+        o.s[1] = GATED ? scales[1][b] : o.s[0];
+    };
+    Weights weights[kAhead];
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d) load_weights(split + d * S, weights[d]);
+
+    // A lane's rows of x, or the last there is.
+    const char *x_row[RM];
+    const float *x_power[RM];
 #pragma unroll
     for (int i = 0; i < RM; ++i) {
-        const int64_t r = m0 + 16 * i + col < a.M ? m0 + 16 * i + col : a.M - 1;
-        if constexpr (LAID) {
-            q[i] = f.w.q + r * f.w.ld;
-            powers[i] = f.w.powers + r;
-        } else {
-            rows[i] = a.x + r * a.ldx;
-        }
+        const int r = 16 * i + col < rows ? 16 * i + col : rows - 1;
+        x_row[i] = lds + r * f.row + 32 * group;
+        x_power[i] = powers + r * f.chunk;
     }
-    float4v acc[RM][RN];
+    float4v acc[RM];
 #pragma unroll
-    for (int i = 0; i < RM; ++i)
-#pragma unroll
-        for (int j = 0; j < RN; ++j) acc[i][j] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-    // Numbers 16 group .. of a block and 64 + 16 group .., eight an MFMA.
-    for (int b = split; b < blocks; b += S) {
-        const int64_t k = static_cast<int64_t>(b) * kBlock + 16 * group;
-        half8 v[RN][4], x[RM][4];
-        float power[RM], s[RN][2];
-#pragma unroll
-        for (int j = 0; j < RN; ++j) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int4v p = load_w(w[j], k + 64 * h, a.K);
-                v[j][2 * h] = widen(p[0], p[1]);
-                v[j][2 * h + 1] = widen(p[2], p[3]);
-            }
-            s[j][0] = scales[j][0][b];
-            s[j][1] = GATED ? scales[j][1][b] : s[j][0];
+    for (int i = 0; i < RM; ++i) acc[i] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+    store_groups(0, f.chunk < blocks ? f.chunk : blocks, 0, begun);
+    for (int b0 = 0;;) {
+        const int count = blocks - b0 < f.chunk ? blocks - b0 : f.chunk;
+#pragma unroll 1
+        for (int first = b0 == 0 ? 32 * kLoads : 0; first < rows * count; first += 32 * kLoads) {
+            Numbers x;
+            load_groups(b0, count, first, x);
+            store_groups(b0, count, first, x);
         }
+        lds_barrier();
+#pragma unroll 1
+        for (int b1 = split; b1 < count; b1 += kAhead * S) {
 #pragma unroll
-        for (int i = 0; i < RM; ++i) {
-            if constexpr (LAID) {
-#pragma unroll
-                for (int h = 0; h < 4; ++h) x[i][h] = *reinterpret_cast<const half8 *>(q[i] + k + 64 * (h / 2) + 8 * (h % 2));
-                power[i] = powers[i][b * f.w.rows];
-            } else {
-                float4v u[8];
-                uint32_t top = 0;
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    u[c] = load_x(rows[i], k + 64 * (c / 4) + 4 * (c % 4), a.K);
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) top = greater(top, magnitude(u[c][d]));
+            for (int d = 0; d < kAhead; ++d) {
+                const int b = b1 + d * S;
+                if (b >= count) continue;
+                if ((b0 + b + 1) * kBlock > K) {  // a shorter block, the last
+                    const int k = (b0 + b) * kBlock + 16 * group;
+                    weights[d].q[0] = ended_w(weights[d].q[0], k, K);
+                    weights[d].q[1] = ended_w(weights[d].q[1], k + 64, K);
                 }
-                uint32_t other = top;
-                swap16(top, other);
-                top = greater(top, other);
-                other = top;
-                swap32(top, other);
-                top = greater(top, other);
-                const uint32_t e = power_of(top);
-                const float scale = down(e);
-                const bool finite = top < kInfinity;
+                half8 v[4];
 #pragma unroll
-                for (int h = 0; h < 4; ++h) x[i][h] = widen(four(u[2 * h], scale, finite), four(u[2 * h + 1], scale, finite));
-                power[i] = finite ? up(e) : 1.0f;
+                for (int h = 0; h < 4; ++h) v[h] = widen(weights[d].q[h / 2][2 * (h % 2)], weights[d].q[h / 2][2 * (h % 2) + 1]);
+                const float s[2] = {weights[d].s[0], weights[d].s[1]};
+                load_weights(b0 + b + kAhead * S, weights[d]);
+#pragma unroll
+                for (int i = 0; i < RM; ++i) {
+                    half8 x[4];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h)
+                        x[h] = *reinterpret_cast<const half8 *>(x_row[i] + b * (2 * kBlock) + 128 * (h / 2) + 16 * (h % 2));
+                    float4v p = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) p = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[h], x[h], p, 0, 0, 0);
+                    const float power = x_power[i][b], f0 = s[0] * power, f1 = s[1] * power;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) acc[i][c] = __builtin_fmaf(GATED && c >= across ? f1 : f0, p[c], acc[i][c]);
+                }
             }
         }
-#pragma unroll
-        for (int i = 0; i < RM; ++i)
-#pragma unroll
-            for (int j = 0; j < RN; ++j) {
-                float4v p = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int h = 0; h < 4; ++h) p = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[j][h], x[i][h], p, 0, 0, 0);
-                const float f0 = s[j][0] * power[i], f1 = s[j][1] * power[i];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) acc[i][j][c] = __builtin_fmaf(GATED && c >= across[j] ? f1 : f0, p[c], acc[i][j][c]);
-            }
+        lds_barrier();  // the chunk is read
+        b0 += f.chunk;
+        if (b0 >= blocks) break;
     }
-    const int count = P * RM * 256;  // outputs of a workgroup, [tile][16 rows][row][column]
+    float *sums = reinterpret_cast<float *>(lds);
+    const int count = outs * RM * 256;  // outputs of a workgroup, [tile][16 rows][row][column]
 #pragma unroll
     for (int i = 0; i < RM; ++i)
-#pragma unroll
-        for (int j = 0; j < RN; ++j)
-            *reinterpret_cast<float4v *>(sums + (split * RN + j) * count + (tile * RM + i) * 256 + col * 16 + 4 * group) = acc[i][j];
+        *reinterpret_cast<float4v *>(sums + (GATED ? 2 * split + second : split) * count + (tile * RM + i) * 256 + col * 16 + 4 * group) = acc[i];
     lds_barrier();
     const auto place = [&](int at, int64_t &m, int &out) {
         m = m0 + 16 * ((at >> 8) % RM) + ((at >> 4) & 15);
         out = n0 + 16 * ((at >> 8) / RM) + (at & 15);
         return 1.0f;
     };
-    write_outputs<GATED, 2>(a, sums, S, RN * count, count, tid, columns, place, kThreads);
+    write_outputs<GATED, 2>(a, sums, S, (GATED ? 2 : 1) * count, count, tid, columns, place, kThreads);
 }
 
-template <bool GATED, bool LAID, int RM>
-hipError_t launch_rows(RowsArgs f, hipStream_t stream) {
-    constexpr int kLds = kWaves * RM * (GATED ? 2 : 1) * 1024;
-    const int64_t columns = GATED ? f.a.half : f.a.N;
-    const int64_t waves = static_cast<int64_t>(compute_units()) * kWaves, blocks = ceil_div(f.a.K, kF8Block);
-    const int64_t rows = ceil_div(f.a.M, 16 * RM);
+// Splits of K until every wave of the device has one; `halves`, 2 of the gated.
+int few_splits(int64_t M, int64_t columns, int64_t K, int64_t rows, int halves) {
+    const int64_t waves = static_cast<int64_t>(compute_units()) * kWaves, blocks = ceil_div(K, kF8Block);
+    const int64_t tiles = halves * ceil_div(columns, 16) * ceil_div(M, rows);
     int splits = 1;
-    while (splits < kWaves && 2 * splits <= blocks && ceil_div(columns, 16) * rows * splits < waves) splits *= 2;
-    f.splits = splits;
-    f.column_blocks = static_cast<uint32_t>(ceil_div(columns, 16 * (kWaves / splits)));
-    SDHIP_LAUNCH((f8_rows_kernel<GATED, LAID, RM>), dim3(static_cast<uint32_t>(f.column_blocks * rows)), dim3(kThreads), kLds, stream, f);
+    while (splits < kWaves / halves && 2 * splits <= blocks && tiles * splits < waves) splits *= 2;
+    return splits;
+}
+
+template <bool GATED, int RM>
+hipError_t launch_few(const F8Args &a, hipStream_t stream) {
+    constexpr int kAhead = few_ahead(RM), kSums = kWaves * RM * 1024, kMost = 160 * 1024;
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&f8_few_kernel<GATED, RM>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    if (attr != hipSuccess) return attr;
+    const int64_t columns = GATED ? a.half : a.N, blocks = ceil_div(a.K, kF8Block);
+    const int64_t rows = a.M < 16 * RM ? a.M : 16 * RM;
+    const int splits = few_splits(a.M, columns, a.K, 16 * RM, GATED ? 2 : 1), outs = kWaves / splits / (GATED ? 2 : 1);
+    // Whole rounds of the waves' blocks: all of K where that is 64 KB at most, else as
+    // many as 64 KB hold, or one (128 KB of 16 rows, 132 of 32).
+    const int64_t round = kAhead * splits, bytes = 2 * kBlock + 4;
+    const int64_t fit = (64 * 1024 / rows - 16) / bytes / round * round;
+    const int64_t chunk = blocks < fit ? blocks : fit > round ? fit : round < blocks ? round : blocks;
+    // Rows 16 bytes further apart than they are long, so that 16 read at once lie on
+    // different banks.
+    const int64_t row = chunk * (2 * kBlock) + 16, x = rows * (row + 4 * chunk);
+    const FewArgs f{a, splits, static_cast<int32_t>(chunk), static_cast<int32_t>(row),
+                    static_cast<uint32_t>(ceil_div(columns, 16 * outs))};
+    SDHIP_LAUNCH((f8_few_kernel<GATED, RM>), dim3(static_cast<uint32_t>(f.column_blocks * ceil_div(a.M, 16 * RM))), dim3(kThreads),
+                 static_cast<uint32_t>(x > kSums ? x : kSums), stream, f);
+    return hipGetLastError();
+}
+
+// ------------------------------------------------------------------ many rows
+
+// Both operands by tiles through LDS: a workgroup takes 64 WM rows of x by 64 WN
+// of the weights (with GATED 32 WN of each half), waves 64 x 64 of them each, and WK
+// blocks of K at a time, WK waves' sums joined at the end.  A stage is half a block
+// of each: 64 numbers of a row, and the block's powers and scales.  A lane's 16
+// bytes are at a place of their row that spreads 16 rows read at once over LDS's
+// banks; three stages are in LDS, one read and two under way.
+template <int WM, int WN, int WK>
+struct Tiles {
+    static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves * WK;
+    static constexpr int kX = 64 * WM, kW = 64 * WN;  // rows of the tiles
+    static constexpr int kXBytes = 128 * kX, kWBytes = 64 * kW, kPowers = 4 * kX, kScales = 256;
+    static constexpr int kPart = kXBytes + kWBytes + kPowers + kScales;  // of a block
+    static constexpr int kStage = WK * kPart;
+    static constexpr int kXCopies = 8 * WM / kWaves, kWCopies = 4 * WN / kWaves;  // a wave's, of 1 KB
+    static constexpr int kSmallCopies = (WM + 1 + kWaves - 1) / kWaves;          // and of 256 bytes
+    static constexpr int kCopies = kXCopies + kWCopies + kSmallCopies;
+    static_assert(8 * WM % kWaves == 0 && 4 * WN % kWaves == 0);
+    // WK waves' sums are joined in LDS.
+    static constexpr int kSums = WK == 1 ? 0 : 16384 * kWaves * WK;
+    static constexpr int kLds = 3 * kStage > kSums ? 3 * kStage : kSums;
+};
+
+struct TilesArgs {
+    F8Args a;
+    F8Work work;
+    const uint8_t *w;  // rows of whole blocks at multiples of 16 bytes ...
+    int64_t ldw;       // ... this far apart
+    uint32_t row_blocks, column_blocks;
+};
+
+template <bool GATED, int WM, int WN, int WK>
+__global__ __launch_bounds__(64 * WM * WN * WK, 2) void f8_tiles_kernel(TilesArgs t) {
+    using L = Tiles<WM, WN, WK>;
+    const F8Args &a = t.a;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wk = wave / L::kWaves, place = wave % L::kWaves, wm = place % WM, wn = place / WM;
+    const int col = lane & 31, hf = lane >> 5;
+    // Groups of 8 row blocks by all columns: those at work at once in an XCD share
+    // their operands' panels in its L2 both ways.
+    const uint32_t at = xcd_swizzle(blockIdx.x, t.row_blocks * t.column_blocks);
+    const uint32_t group = at / (8 * t.column_blocks), in = at - group * (8 * t.column_blocks);
+    const uint32_t high = t.row_blocks - 8 * group < 8 ? t.row_blocks - 8 * group : 8;
+    const int64_t m0 = static_cast<int64_t>(8 * group + in % high) * L::kX;
+    const int columns = static_cast<int>(GATED ? a.half : a.N);
+    const int n0 = static_cast<int>(in / high) * (GATED ? L::kW / 2 : L::kW);
+    const int blocks = static_cast<int>(t.work.ld / kBlock);
+    const int stages = 2 * ((blocks + WK - 1) / WK);
+
+    // Row r of the weights' tile: its column of the output, in which half.
+    const auto column_of = [&](int r, int &second) {
+        second = GATED ? (r >> 5) & 1 : 0;
+        const int n = GATED ? n0 + 32 * (r >> 6) + (r & 31) : n0 + r;
+        return n < columns ? n : columns - 1;
+    };
+    uint32_t x_offset[L::kXCopies], w_offset[L::kWCopies];
+    const char *w_base[L::kWCopies];
+    const char *x_base = reinterpret_cast<const char *>(t.work.q + m0 * t.work.ld);
+#pragma unroll
+    for (int c = 0; c < L::kXCopies; ++c) {
+        const int r = 8 * (place + L::kWaves * c) + (lane >> 3);
+        const int64_t row = m0 + r < a.M ? r : a.M - 1 - m0;
+        x_offset[c] = static_cast<uint32_t>(2 * row * t.work.ld + 16 * ((lane & 7) ^ ((r >> 1) & 7)));
+    }
+#pragma unroll
+    for (int c = 0; c < L::kWCopies; ++c) {
+        const int r = 16 * (place + L::kWaves * c) + (lane >> 2);
+        int second;
+        const int n = column_of(r, second);
+        w_offset[c] = static_cast<uint32_t>((n - n0) * t.ldw + 16 * ((lane & 3) ^ ((r >> 2) & 3)));
+        const int half = GATED ? ((16 * (place + L::kWaves * c)) >> 5) & 1 : 0;
+        w_base[c] = reinterpret_cast<const char *>(t.w + (static_cast<int64_t>(n0) + (half ? columns : 0)) * t.ldw);
+    }
+    // A lane's number of the small copies: of 64 of the rows' powers, or the scales of
+    // each 32 rows of the weights' tile, the first's block's and the last's by lanes 2 i
+    // and 2 i + 1; and how far apart those of the next block are.
+    const float *small[L::kSmallCopies];
+    int64_t small_step[L::kSmallCopies];
+    uint32_t small_to[L::kSmallCopies];
+#pragma unroll
+    for (int c = 0; c < L::kSmallCopies; ++c) {
+        const int r = place + L::kWaves * c;
+        int second;
+        const int i = (lane >> 1) % (L::kW / 32), n = column_of(32 * i, second);
+        const int64_t first = n + (second ? columns : 0), last = first + 31 < a.N ? first + 31 : a.N - 1;
+        small[c] = r < WM ? t.work.powers + m0 + 64 * r + lane : a.scales + (lane & 1 ? last : first) / kBlock * a.ld_scales;
+        small_step[c] = r < WM ? t.work.rows : 1;
+        small_to[c] = L::kXBytes + L::kWBytes + (r < WM ? 256 * r : L::kPowers);
+    }
+    char *part = lds + wk * L::kPart;
+    const auto copy = [&](int s, int buffer) {
+        // Past the last block it once more, and past the last stage.
+        const int pair = (s < stages ? s : stages - 1) >> 1;
+        const int b = pair * WK + wk < blocks ? pair * WK + wk : blocks - 1;
+        const int64_t k = static_cast<int64_t>(b) * kBlock + 64 * (s & 1);
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(part) + buffer * L::kStage);
+#pragma unroll
+        for (int c = 0; c < L::kXCopies; ++c) fetch16(x_base + 2 * k, x_offset[c], to + 1024 * (place + L::kWaves * c));
+#pragma unroll
+        for (int c = 0; c < L::kWCopies; ++c) fetch16(w_base[c] + k, w_offset[c], to + L::kXBytes + 1024 * (place + L::kWaves * c));
+#pragma unroll
+        for (int c = 0; c < L::kSmallCopies; ++c) fetch4(small[c] + b * small_step[c], to + small_to[c]);
+    };
+    copy(0, 0);
+    copy(1, 1);
+    copy(2, 2);
+
+    float16v acc[4], p[4];  // tile k: rows of x 32 (k % 2) .., of the weights 32 (k / 2) ..
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] = p[k] = float16v{};
+    struct Operands {
+        half8 v[2][2], x[2][2];  // [32 rows][8 numbers]
+        int4v q[2];              // v before it is widened
+    };
+    // Rows of the tiles as the MFMA's lanes read them: of a quarter of a block.
+    const char *x_row = part + 128 * (64 * wm + col), *w_row = part + L::kXBytes + 64 * (64 * wn + col);
+    const int x_turn = (col >> 1) & 7, w_turn = (col >> 2) & 3;
+    const auto read = [&](Operands &o, int buffer, int u) {
+        const char *xs = x_row + buffer * L::kStage, *ws = w_row + buffer * L::kStage;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) o.q[j] = *reinterpret_cast<const int4v *>(ws + 64 * 32 * j + 16 * ((2 * u + hf) ^ w_turn));
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                o.x[i][h] = *reinterpret_cast<const half8 *>(xs + 128 * 32 * i + 16 * ((4 * u + 2 * hf + h) ^ x_turn));
+    };
+    const auto widen_one = [&](Operands &o, int j) {
+        o.v[j][0] = widen(o.q[j][0], o.q[j][1]);
+        o.v[j][1] = widen(o.q[j][2], o.q[j][3]);
+    };
+    // A block's powers and scales; GATED: the second half's rows may lie in two
+    // blocks of the scales, `across` of them in the first.
+    float power[2], scale_of[2][2];
+    const int across = GATED ? kBlock - static_cast<int>((columns + n0 + 32 * wn) % kBlock) : kBlock;
+    const auto read_scales = [&](int buffer) {
+        const char *small = part + buffer * L::kStage + L::kXBytes + L::kWBytes;
+        const float *scales = reinterpret_cast<const float *>(small + L::kPowers) + 4 * wn;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            power[i] = reinterpret_cast<const float *>(small)[64 * wm + 32 * i + col];
+            scale_of[i][0] = scales[2 * i];
+            scale_of[i][1] = scales[2 * i + 1];
+        }
+    };
+    const auto add = [&](int k) {
+        const float f = scale_of[k >> 1][0] * power[k & 1];
+        if (GATED && k >= 2 && across < 32) {
+            const float g = scale_of[k >> 1][1] * power[k & 1];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[k][e] = __builtin_fmaf(tile_row(e) + 4 * hf < across ? f : g, p[k][e], acc[k][e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[k][e] = __builtin_fmaf(f, p[k][e], acc[k][e]);
+        }
+    };
+    // A quarter of a block: its products from registers while the next one's
+    // operands are read and widened; with `ends` a tile's sums are added while the
+    // next tile's are made, the last one's with the first of the next quarter
+    // (`kept`).
+    const auto quarter = [&](const Operands &now, Operands &next, int buffer, int u, auto begins_, auto kept_, auto ends_) {
+        constexpr bool begins = decltype(begins_)::value, kept = decltype(kept_)::value, ends = decltype(ends_)::value;
+        read(next, buffer, u);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = k & 1, j = k >> 1;
+            p[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now.v[j][0], now.x[i][0], begins ? float16v{} : p[k], 0, 0, 0);
+            p[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now.v[j][1], now.x[i][1], p[k], 0, 0, 0);
+            if (k == 0 && kept) add(3);
+            if (k > 0 && ends) add(k - 1);
+            if (k >= 2) {
+                widen_one(next, k - 2);
+                // Here, not where they are used.
+                asm volatile("" : "+v"(next.v[k - 2][0]), "+v"(next.v[k - 2][1]));
+            }
+            // In this order: an MFMA and half of the other operations, twice.
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, ends ? 13 : 9, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    const auto next = [](int b) { return b == 2 ? 0 : b + 1; };
+    int buffer = 0;
+    fetched<2 * L::kCopies>();
+    lds_barrier();
+    Operands even, odd;
+    read(even, 0, 0);
+    widen_one(even, 0);
+    widen_one(even, 1);
+    // Stage s is in registers or being read; the copies of s + 1 and s + 2 are under
+    // way, and once s is read those of s + 3 take its buffer.
+    const auto arrive = [&](int s) {
+        fetched<L::kCopies>();
+        lds_barrier();  // every wave's copies of stage s + 1 are in, and stage s is read
+        copy(s + 3, buffer);
+        buffer = next(buffer);
+    };
+    power[0] = power[1] = scale_of[0][0] = scale_of[0][1] = scale_of[1][0] = scale_of[1][1] = 0.0f;
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
+#pragma unroll 1
+    for (int s = 0; s < stages; s += 2) {
+        quarter(even, odd, buffer, 1, yes, yes, no);  // the block before's last tile, times 0 at first
+        arrive(s);
+        quarter(odd, even, buffer, 0, no, no, no);
+        read_scales(buffer);
+        if constexpr (WK > 1) {
+            // Past the last block nothing is added (an infinite scale would make it NaN).
+            const uint32_t keep = (s >> 1) * WK + wk < blocks ? 0xffffffffu : 0;
+            const auto kept = [&](float v) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & keep); };
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                power[i] = kept(power[i]);
+                scale_of[i][0] = kept(scale_of[i][0]);
+                scale_of[i][1] = kept(scale_of[i][1]);
+            }
+        }
+        quarter(even, odd, buffer, 1, no, no, no);
+        arrive(s + 1);
+        quarter(odd, even, buffer, 0, no, no, yes);
+    }
+    add(3);
+    fetched<0>();
+
+    // The outputs, by rows of x a lane: of E of a tile's 16 registers, which are 4
+    // columns each.
+    constexpr int E = WK == 4 ? 8 : 16;
+    const int64_t last = a.M - 1;
+    const int base = n0 + (GATED ? 32 * wn : 64 * wn) + 4 * hf;
+    const auto write = [&](int i, int e0, float (&v)[2][E]) {
+        const int64_t m = m0 + 64 * wm + 32 * i + col, row = m < last ? m : last;
+        // Column of number e of j's tile, and whether all of the tile's are there.
+        const auto column = [&](int j, int e) { return base + (GATED ? 0 : 32 * j) + tile_row(e0 + e); };
+        const auto full = [&](int j) { return n0 + (GATED ? 32 * wn : 64 * wn + 32 * j) + 32 <= columns; };
+        const auto load = [&](const float *from, int64_t step, int j, float (&o)[E]) {
+            if (step == 1 && full(j)) {
+#pragma unroll
+                for (int e = 0; e < E; e += 4) {
+                    const float4v q = load4(from + column(j, e));
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) o[e + c] = q[c];
+                }
+            } else if (step == 0) {
+                const float one = *from;
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] = one;
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] = from[(column(j, e) < columns ? column(j, e) : columns - 1) * step];
+            }
+        };
+        if (!GATED && a.from_redirect) {
+            float o[2][E];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) load(a.y + row * a.ldy, 1, j, o[j]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[j][e] = o[j][e] + v[j][e];
+        }
+#pragma unroll 1
+        for (int c = 0; c < a.chain.count; ++c) {
+            const DevStep &st = a.chain.steps[c];
+            if (st.kind == kSilu) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) v[j][e] = silu(v[j][e]);
+                continue;
+            }
+            const float *from = st.operand;
+            if (st.flat123) {
+                from += row * st.nb[1];
+            } else {
+                uint32_t i1, i2, i3;
+                split_index(static_cast<uint32_t>(row), static_cast<uint32_t>(a.ne1), static_cast<uint32_t>(a.ne2), i1, i2, i3);
+                from += i1 * st.nb[1] + i2 * st.nb[2] + i3 * st.nb[3];
+            }
+            float o[2][E];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) load(from + (GATED && j ? a.half * st.nb[0] : 0), st.nb[0], j, o[j]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[j][e] = st.kind == kAdd ? __fadd_rn(v[j][e], o[j][e]) : __fmul_rn(v[j][e], o[j][e]);
+        }
+        if (m > last) return;
+        float *y = a.y + m * a.ldy;
+#pragma unroll
+        for (int j = 0; j < (GATED ? 1 : 2); ++j)
+#pragma unroll
+            for (int e = 0; e < E; e += 4) {
+                float4v q;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) q[c] = GATED ? v[0][e + c] * gelu(v[1][e + c]) : v[j][e + c];
+                if (full(j)) {
+                    __builtin_memcpy(y + column(j, e), &q, 16);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (column(j, e + c) < columns) y[column(j, e + c)] = q[c];
+                }
+            }
+    };
+    if constexpr (WK == 1) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float v[2][E];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[j][e] = acc[2 * j + i][e];
+            write(i, 0, v);
+        }
+    } else {
+        // [block][wave][tile][4 registers][lane]; a wave adds up a WK-th of them.
+        lds_barrier();  // the last stage is read, and no copy is under way
+        float4v *sums = reinterpret_cast<float4v *>(lds) + lane;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                sums[64 * (((wk * L::kWaves + place) * 4 + k) * 4 + g)] = float4v{acc[k][4 * g], acc[k][4 * g + 1], acc[k][4 * g + 2], acc[k][4 * g + 3]};
+        lds_barrier();
+        const int i = WK == 2 ? wk : wk >> 1, g0 = WK == 2 ? 0 : 2 * (wk & 1);
+        float v[2][E];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int g = 0; g < E / 4; ++g) {
+                float4v q = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int b = 0; b < WK; ++b) q += sums[64 * (((b * L::kWaves + place) * 4 + 2 * j + i) * 4 + g0 + g)];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) v[j][4 * g + c] = q[c];
+            }
+        write(i, 4 * g0, v);
+    }
+}
+
+template <bool GATED, int WM, int WN, int WK>
+hipError_t launch_tiles(TilesArgs t, hipStream_t stream) {
+    using L = Tiles<WM, WN, WK>;
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&f8_tiles_kernel<GATED, WM, WN, WK>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, L::kLds);
+    if (attr != hipSuccess) return attr;
+    t.row_blocks = static_cast<uint32_t>(ceil_div(t.a.M, L::kX));
+    t.column_blocks = static_cast<uint32_t>(GATED ? ceil_div(t.a.half, L::kW / 2) : ceil_div(t.a.N, L::kW));
+    SDHIP_LAUNCH((f8_tiles_kernel<GATED, WM, WN, WK>), dim3(t.row_blocks * t.column_blocks), dim3(L::kThreads), L::kLds, stream, t);
     return hipGetLastError();
 }
 
 // ------------------------------------------------------------------ the choice
 
-// Which kernels a product takes, numbered as the f8_form tuning asks for them.
-enum class Form { few = 1, rows };
+// Which kernels a product takes, numbered as the f8_form tuning asks for them: the
+// rows' kernel with x as it is or laid out, or tiles of 128 x 128 by four waves, by
+// eight, of 64 x 128 by four, of 64 x 64 by four.
+enum class Form { few = 1, rows, tiles4, tiles8, tiles64, tiles64x64 };
 
-Form form_of(int64_t M) { return M <= 16 ? Form::few : Form::rows; }
+// The tiles' copies reach 128 rows of x by 32 bits of offset.
+constexpr int64_t kTilesK = int64_t{1} << 22;
+
+Form form_of(int64_t M, int64_t N, int64_t K) {
+    const int asked = tuning().f8_form;
+    // The rows' kernel takes a wave for 16 x 16 outputs, of the 2^26 a launch counts.
+    const bool fits = (M / 16 + 1) * (N / 16 + 8) < (int64_t{1} << 25);
+    if (asked > 0 && (asked <= 2 ? fits : K <= kTilesK)) return static_cast<Form>(asked);
+    if (M <= 48) return Form::few;
+    if (M <= 160 || K > kTilesK) return Form::rows;
+    const int64_t tiles = ceil_div(M, 128) * ceil_div(N, 128);
+    if (tiles >= 384) return Form::tiles4;
+    if (tiles >= 128) return Form::tiles8;
+    return ceil_div(M, 64) * ceil_div(N, 128) >= 60 ? Form::tiles64 : Form::tiles64x64;
+}
+
+bool tiles(Form form) { return form != Form::few && form != Form::rows; }
 
 hipError_t lay_out(const F8Args &a, const F8Work &w, hipStream_t stream) {
-    const int64_t blocks = w.ld / kF8Block, groups = blocks * a.M, x_grid = ceil_div(groups, kOperandThreads / 16);
-    const int64_t w_grid = w.w != nullptr ? ceil_div(a.N * (w.ld / 16), kOperandThreads) : 0;
+    // 2^20 workgroups of each at most, of the 2^32 threads that a launch counts.
+    const auto most = [](int64_t n) { return n < (1 << 20) ? n : 1 << 20; };
+    const int64_t blocks = w.ld / kF8Block, groups = blocks * a.M, x_grid = most(ceil_div(groups, kOperandThreads / 16));
+    const int64_t w_grid = w.w != nullptr ? most(ceil_div(a.N * (w.ld / 16), kOperandThreads)) : 0;
     const OperandsArgs o{a, w, static_cast<uint32_t>(blocks), static_cast<uint32_t>(groups), static_cast<uint32_t>(x_grid)};
     SDHIP_LAUNCH(f8_operands_kernel, dim3(static_cast<uint32_t>(x_grid + w_grid)), dim3(kOperandThreads), 0, stream, o);
     return hipGetLastError();
@@ -335,18 +819,29 @@ hipError_t lay_out(const F8Args &a, const F8Work &w, hipStream_t stream) {
 
 template <bool GATED>
 hipError_t launch_form(const F8Args &a, bool whole, void *work, hipStream_t stream) {
-    const Form form = form_of(a.M);
-    if (form == Form::few) return launch_rows<GATED, false, 1>(RowsArgs{a, F8Work{}, 1, 0}, stream);
-    const F8Work w = work_of(a.M, a.N, a.K, false, work);
+    const Form form = form_of(a.M, a.N, a.K);
+    if (form == Form::few) return launch_few<GATED, 1>(a, stream);
+    if (form == Form::rows) return launch_few<GATED, 2>(a, stream);
+    const F8Work w = work_of(a.M, a.N, a.K, !whole, work);
     if (const hipError_t e = lay_out(a, w, stream); e != hipSuccess) return e;
-    return launch_rows<GATED, true, 2>(RowsArgs{a, w, 1, 0}, stream);
+    const TilesArgs t{a, w, whole ? a.w : w.w, whole ? a.row_bytes : w.ld, 0, 0};
+    switch (form) {
+    case Form::tiles4:
+        return launch_tiles<GATED, 2, 2, 1>(t, stream);
+    case Form::tiles8:
+        return launch_tiles<GATED, 2, 2, 2>(t, stream);
+    case Form::tiles64:
+        return launch_tiles<GATED, 1, 2, 2>(t, stream);
+    default:
+        return launch_tiles<GATED, 1, 1, 4>(t, stream);
+    }
 }
 
 }  // namespace
 
 size_t f8_work_size(int64_t M, int64_t N, int64_t K, bool whole) {
-    const Form form = form_of(M);
-    return form == Form::few ? 0 : work_of(M, N, K, false, nullptr).bytes;
+    const Form form = form_of(M, N, K);
+    return tiles(form) ? work_of(M, N, K, !whole, nullptr).bytes : 0;
 }
 
 hipError_t launch_f8_mul_mat(const F8Args &a, bool whole, void *work, hipStream_t stream) {

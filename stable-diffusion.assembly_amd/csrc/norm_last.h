@@ -9,6 +9,9 @@
 
 namespace sdhip {
 
+// The steps of a chain that is some of these, in this order, by one number a channel.
+enum : int32_t { kPlainMul = 1, kPlainAdd = 2, kPlainSilu = 4 };
+
 struct GroupNormLastArgs {
     const float *x;
     float *y;
@@ -17,14 +20,15 @@ struct GroupNormLastArgs {
     int64_t groups, per_group;               // groups of an image that have channels; channels of a group
     float eps;
     DevChain chain;
-    // How it is split (group_norm_last_shape).
-    int64_t image0;              // the launch's first image
-    int32_t slab_groups, slabs;  // groups of a workgroup's channels; of those in an image
-    int32_t chunks;              // of an image's pixels, a workgroup each
-    int32_t parts;               // the chunks that sums were taken over
-    int64_t chunk;               // pixels
-    double *partials;            // [image][group][part][2]: sums of x - c and of its squares, c the group's first number
-    double *firsts;              // [image][group]: c
+    int32_t plain;  // its steps, where it is such a chain; else 0
+    // A launch's workgroups: from image0 on, slab_groups groups' channels and `chunk`
+    // pixels each, `chunks` of an image.
+    int64_t image0, chunk;
+    int32_t slab_groups, slabs, chunks;
+    int32_t parts;     // the chunks that sums were taken over
+    double *partials;  // [image][group][part][2]: sums of x - c and of its squares, c the group's first number
+    double *firsts;    // [image][group]: c
+    double *joined;    // [image][group][2]: the mean, and what x less it is multiplied by; or null
 };
 
 // The extents of a call, for its split and its work buffer.

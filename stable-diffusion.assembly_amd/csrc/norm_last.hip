@@ -8,11 +8,13 @@
 //     mean = c + S1 / n,  variance = (S2 - S1^2 / n) / n.
 // (mean - c)^2 is at most n times the variance, c being one of the group's numbers,
 // so that what cancels in the difference costs the variance n 2^-53 of itself at
-// most.  The output is (x - mean) / sqrt(variance + eps) in double, rounded once,
-// and then the chain.
+// most.  The output is (x - mean) / sqrt(variance + eps), the mean in two parts as
+// sdhip_norm_residual's (row_norm.h), and then the chain.
 //
-// Bound by memory: x is read twice, the second time from the Infinity Cache where it
-// fits, and y written once.
+// Bound by memory.  A slab whose pixels' numbers fit a workgroup's registers takes
+// one launch and one read of x; others a launch for the sums and one for the
+// outputs, which reads x again, the last chunks first: those the Infinity Cache
+// still holds.
 
 #include "host.h"
 #include "norm_last.h"
@@ -23,19 +25,16 @@ namespace sdhip {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
-
 // What a workgroup takes: channels [c0, c1) and pixels [p0, p1) of an image.
 struct View {
     int64_t image, p0, p1;
     int c0, c1, g0, groups, chunk;
 };
 
-__device__ __forceinline__ View view_of(const GroupNormLastArgs &a) {
+__device__ __forceinline__ View view_of(const GroupNormLastArgs &a, uint32_t block) {
     View v;
-    const uint32_t item = blockIdx.x / static_cast<uint32_t>(a.chunks);
-    v.chunk = static_cast<int>(blockIdx.x - item * static_cast<uint32_t>(a.chunks));
+    const uint32_t item = block / static_cast<uint32_t>(a.chunks);
+    v.chunk = static_cast<int>(block - item * static_cast<uint32_t>(a.chunks));
     const uint32_t image = item / static_cast<uint32_t>(a.slabs);
     v.image = a.image0 + image;
     const int slab = static_cast<int>(item - image * static_cast<uint32_t>(a.slabs));
@@ -49,22 +48,18 @@ __device__ __forceinline__ View view_of(const GroupNormLastArgs &a) {
     return v;
 }
 
-struct Sums {
-    double first, squares;
-};
-
-// The threads' places in a slab: its channels V at a time, kThreads of them a
-// pass, by columns of threads, and the pixels by rows of them.
+// The T threads' places in a slab: its channels V at a time, T of them a pass, by
+// columns of threads, and the pixels by rows of them.
 struct Place {
     int columns, rows, row, c, count;  // count: channels of the pass
 };
 
-template <int V>
+template <int V, int T>
 __device__ __forceinline__ Place place_of(const View &v, int from) {
     Place p;
-    p.count = v.c1 - from < kThreads * V ? v.c1 - from : kThreads * V;
+    p.count = v.c1 - from < T * V ? v.c1 - from : T * V;
     p.columns = (p.count + V - 1) / V;
-    p.rows = kThreads / p.columns;
+    p.rows = T / p.columns;
     p.row = static_cast<int>(threadIdx.x) / p.columns;
     p.c = from + (static_cast<int>(threadIdx.x) - p.row * p.columns) * V;
     return p;
@@ -81,71 +76,229 @@ __device__ __forceinline__ void load_channels(const float *at, float (&q)[V]) {
     }
 }
 
+struct Sums {
+    double first, squares;
+};
+
+// The first channel of channel c's group, and of that of c + i, i < V: a division
+// for all of them.
+__device__ __forceinline__ int first_of(int c, uint32_t per_group) {
+    return static_cast<int>(static_cast<uint32_t>(c) / per_group * per_group);
+}
+template <int V>
+__device__ __forceinline__ int at_of(int first, int c, int i, uint32_t per_group) {
+    const int n = static_cast<int>(per_group);
+    if (n >= V) return c + i - first < n ? first : first + n;
+    while (first + n <= c + i) first += n;
+    return first;
+}
+
+// The sums of V channels of a thread, of x less the channel's group's first number.
+template <int V>
+struct Channels {
+    double first[V], squares[V], shift[V];
+    __device__ __forceinline__ void begin(const float *x, int c, uint32_t per_group, bool in) {
+        const int of = first_of(c, per_group);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            first[i] = squares[i] = shift[i] = 0.0;
+            if (in) shift[i] = static_cast<double>(x[at_of<V>(of, c, i, per_group)]);
+        }
+    }
+    __device__ __forceinline__ void add(const float (&q)[V]) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const double d = static_cast<double>(q[i]) - shift[i];
+            first[i] += d;
+            squares[i] = __builtin_fma(d, d, squares[i]);
+        }
+    }
+};
+
+// The sum of 8 neighbouring lanes, on all of them.
+__device__ __forceinline__ double eight_sum(double v) {
+    v += moved<0xb1>(v);          // lanes i ^ 1
+    v += moved<0x4e>(v);          // i ^ 2
+    return v + moved<0x141>(v);  // 8 lanes mirrored
+}
+
+// Adds the threads' sums of a pass's channels, from `from` on, to the slab's
+// groups': over the rows by a thread a channel, over a group's channels by 8.
+template <int V, int T>
+__device__ __forceinline__ void add_up(const Channels<V> &mine, const View &v, const Place &at, int from, uint32_t per_group,
+                                       Sums *sums, Sums *totals) {
+    const int tid = threadIdx.x;
+    __syncthreads();  // the pass before is added up
+    if (at.row < at.rows) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) sums[tid * V + i] = Sums{mine.first[i], mine.squares[i]};
+    }
+    __syncthreads();
+    // The rows of a channel in two rounds: each `step`-th by a thread of their own where
+    // there are threads for that, then `step` of them.
+    const int pitch = at.columns * V;
+    const int most = T / at.count;
+    int step = 1;
+    while (step < most && step * step < at.rows) ++step;
+    for (int i = tid; i < at.count * step; i += T) {
+        const int r0 = i / at.count, c = i - r0 * at.count;
+        Sums s = sums[r0 * pitch + c];
+#pragma unroll 4
+        for (int r = r0 + step; r < at.rows; r += step) {
+            const Sums o = sums[r * pitch + c];
+            s.first += o.first;
+            s.squares += o.squares;
+        }
+        sums[r0 * pitch + c] = s;
+    }
+    __syncthreads();
+    for (int c = tid; step > 1 && c < at.count; c += T) {
+        Sums s = sums[c];
+#pragma unroll 4
+        for (int r = 1; r < step; ++r) {
+            const Sums o = sums[r * pitch + c];
+            s.first += o.first;
+            s.squares += o.squares;
+        }
+        sums[c] = s;
+    }
+    __syncthreads();
+    for (int g = tid / 8; g < v.groups; g += T / 8) {
+        const int64_t whole0 = static_cast<int64_t>(v.g0 + g) * per_group, whole1 = whole0 + per_group;
+        const int low = static_cast<int>(whole0 > from ? whole0 - from : 0);
+        const int high = static_cast<int>(whole1 < from + at.count ? whole1 - from : at.count);
+        if (low >= high) continue;  // the 8 lanes of a group together
+        double s = 0.0, t = 0.0;
+        for (int c = low + (tid & 7); c < high; c += 8) {
+            s += sums[c].first;
+            t += sums[c].squares;
+        }
+        s = eight_sum(s);
+        t = eight_sum(t);
+        if ((tid & 7) == 0) {
+            totals[g].first += s;
+            totals[g].squares += t;
+        }
+    }
+}
+
+// Of a group's sums over n numbers.
+__device__ __forceinline__ Moments moments_of(double shift, double first, double squares, double n, float eps) {
+    const double inverse = 1.0 / n, off = first * inverse, variance = (squares - first * off) * inverse;
+    // Below 0 by rounding alone; a NaN stays one.
+    return moments(SDHIP_ROW_NORM_LAYER, shift + off, variance < 0.0 ? 0.0 : variance, 1.0, eps);
+}
+
+// x / (1 + exp(-x)) within 4 roundings of itself by the hardware's power of two and
+// reciprocal, the exponent's rounding made up for: a third of the operations of
+// silu(), which the outputs of a group norm would wait for (2 x 64 x 64 x 320 TIME).
+__device__ __forceinline__ float fast_silu(float x) {
+    const float t = -1.44269504088896341f * x, rest = __builtin_fmaf(-1.44269504088896341f, x, -t);
+    const float e = __builtin_amdgcn_exp2f(t), low = __builtin_fmaf(-1.925963033500e-8f, x, rest);
+    return x * __builtin_amdgcn_rcpf(__builtin_fmaf(e, 0.693147180559945f * low, e) + 1.0f);
+}
+
+// An image's group's numbers.
+__device__ __forceinline__ double numbers_of(const GroupNormLastArgs &a, int64_t g) {
+    const int64_t c = g * a.per_group, width = c + a.per_group < a.channels ? a.per_group : a.channels - c;
+    return static_cast<double>(width) * static_cast<double>(a.pixels);
+}
+
+// The outputs of a thread's V channels: their statistics, and the scale and shift of
+// a chain that is a multiplication, an addition and SiLU, or some of them in that
+// order, by one number a channel (and image): held in registers (`plain`).  Any
+// other chain reads its operands for each pixel.  (Six steps of any kind in registers
+// are 60 KB of instructions, most of them never run and each launch fetched again:
+// 2 x 64 x 64 x 320 15 us for the outputs, so 5.)
+template <int V>
+struct Outputs {
+    Moments stats[V];
+    float scale[V], shift[V];
+    __device__ __forceinline__ void operands(const GroupNormLastArgs &a, const View &v, int c) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            scale[i] = 1.0f;
+            shift[i] = 0.0f;
+        }
+        if (a.plain & kPlainMul) load(a.chain.steps[0], v, c, scale);
+        if (a.plain & kPlainAdd) load(a.chain.steps[a.plain & kPlainMul ? 1 : 0], v, c, shift);
+    }
+    __device__ __forceinline__ void statistics(const GroupNormLastArgs &a, const Moments *of, const View &v, int c) {
+        const uint32_t per_group = static_cast<uint32_t>(a.per_group), g = static_cast<uint32_t>(c) / per_group;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            // The group of c + i: c's or, V being less than its channels, the next; else divided.
+            const uint32_t mine = per_group < V ? static_cast<uint32_t>(c + i) / per_group : c + i < static_cast<int>((g + 1) * per_group) ? g : g + 1;
+            stats[i] = of[mine - v.g0];
+        }
+    }
+    __device__ __forceinline__ void load(const DevStep &st, const View &v, int c, float (&o)[V]) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = st.operand[(c + i) * st.nb[0] + v.image * st.nb[3]];
+    }
+    __device__ __forceinline__ void write(const GroupNormLastArgs &a, const View &v, int c, int64_t p, const float (&q)[V]) const {
+        float r[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) r[i] = normed(q[i], stats[i]);
+        if (a.plain) {
+            // Times 1 and plus 0 where there is no such step: the same number, but for the
+            // sign of a zero.
+#pragma unroll
+            for (int i = 0; i < V; ++i) r[i] = __fadd_rn(__fmul_rn(r[i], scale[i]), shift[i]);
+            if (a.plain & kPlainSilu) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) r[i] = fast_silu(r[i]);
+            }
+        } else if (a.chain.count > 0) {
+            const uint32_t width = static_cast<uint32_t>(a.width);
+            const uint32_t i2 = static_cast<uint32_t>(p) / width, i1 = static_cast<uint32_t>(p) - i2 * width;
+            apply_chain_block(a.chain, r, [&](int s, int i) {
+                const DevStep &st = a.chain.steps[s];
+                return (c + i) * st.nb[0] + i1 * st.nb[1] + i2 * st.nb[2] + v.image * st.nb[3];
+            });
+        }
+        float *to = a.y + v.image * a.yimage + p * a.ypixel + c;
+        if constexpr (V == 4) {
+            *reinterpret_cast<float4v *>(to) = float4v{r[0], r[1], r[2], r[3]};
+        } else {
+            to[0] = r[0];
+        }
+    }
+};
+
+constexpr int kThreads = 256;
 constexpr int kAhead = 4;  // pixels of a thread that are loaded together
 
+// The sums of a slab's groups over a chunk of pixels.
 template <int V>
-__global__ __launch_bounds__(kThreads) void group_sums_kernel(GroupNormLastArgs a) {
+__global__ __launch_bounds__(kThreads) void group_last_sums_kernel(GroupNormLastArgs a) {
     __shared__ Sums sums[kThreads * V];
     extern __shared__ Sums totals[];  // the slab's groups'
-    const View v = view_of(a);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const View v = view_of(a, blockIdx.x);
+    const int tid = threadIdx.x;
     const float *x = a.x + v.image * a.ximage;
     const uint32_t per_group = static_cast<uint32_t>(a.per_group);
     for (int g = tid; g < v.groups; g += kThreads) totals[g] = Sums{0.0, 0.0};
     for (int from = v.c0; from < v.c1; from += kThreads * V) {
-        const Place at = place_of<V>(v, from);
+        const Place at = place_of<V, kThreads>(v, from);
         const bool in = at.row < at.rows;
-        double first[V], squares[V], shift[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            first[i] = squares[i] = shift[i] = 0.0;
-            if (in) shift[i] = static_cast<double>(x[static_cast<uint32_t>(at.c + i) / per_group * per_group]);
-        }
-        const auto add = [&](const float (&q)[V]) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const double d = static_cast<double>(q[i]) - shift[i];
-                first[i] += d;
-                squares[i] = __builtin_fma(d, d, squares[i]);
-            }
-        };
-        int64_t p = in ? v.p0 + at.row : v.p1;
+        Channels<V> mine;
+        mine.begin(x, at.c, per_group, in);
         const float *from_x = x + at.c;
+        int64_t p = in ? v.p0 + at.row : v.p1;
         for (; p + (kAhead - 1) * at.rows < v.p1; p += kAhead * at.rows) {
             float q[kAhead][V];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) load_channels<V>(from_x + (p + u * at.rows) * a.xpixel, q[u]);
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) add(q[u]);
+            for (int u = 0; u < kAhead; ++u) mine.add(q[u]);
         }
         for (; p < v.p1; p += at.rows) {
             float q[V];
             load_channels<V>(from_x + p * a.xpixel, q);
-            add(q);
+            mine.add(q);
         }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < V; ++i) sums[tid * V + i] = Sums{first[i], squares[i]};
-        __syncthreads();
-        // A group's channels of this pass, over all rows, by a wave.
-        for (int g = wave; g < v.groups; g += kWaves) {
-            const int64_t whole0 = static_cast<int64_t>(v.g0 + g) * a.per_group, whole1 = whole0 + a.per_group;
-            const int low = static_cast<int>(whole0 > from ? whole0 - from : 0);
-            const int high = static_cast<int>(whole1 < from + at.count ? whole1 - from : at.count);
-            if (low >= high) continue;
-            double s = 0.0, t = 0.0;
-            for (int r = 0; r < at.rows; ++r)
-                for (int i = low + lane; i < high; i += 64) {
-                    s += sums[r * at.columns * V + i].first;
-                    t += sums[r * at.columns * V + i].squares;
-                }
-            s = wave_sum(s);
-            t = wave_sum(t);
-            if (lane == 0) {
-                totals[g].first += s;
-                totals[g].squares += t;
-            }
-        }
+        add_up<V, kThreads>(mine, v, at, from, per_group, sums, totals);
     }
     __syncthreads();
     for (int g = tid; g < v.groups; g += kThreads) {
@@ -158,136 +311,294 @@ __global__ __launch_bounds__(kThreads) void group_sums_kernel(GroupNormLastArgs 
     }
 }
 
-struct Stats {
-    double mean, scale;
+// The sums over a group's parts from `first` on, each `step`-th.
+__device__ __forceinline__ Sums parts_of(const GroupNormLastArgs &a, int64_t group, int first, int step) {
+    const double2 *from = reinterpret_cast<const double2 *>(a.partials) + group * a.parts;
+    Sums s{0.0, 0.0};
+#pragma unroll 4
+    for (int i = first; i < a.parts; i += step) {
+        const double2 o = from[i];
+        s.first += o.x;
+        s.squares += o.y;
+    }
+    return Sums{wave_sum(s.first), wave_sum(s.squares)};
+}
+
+// A group's statistics from its parts' sums, by a wave; on its first lane.
+__device__ __forceinline__ Moments join(const GroupNormLastArgs &a, int64_t image, int64_t g) {
+    const int64_t group = image * a.groups + g;
+    const double c = a.firsts[group];
+    const Sums s = parts_of(a, group, threadIdx.x & 63, 64);
+    return moments_of(c, s.first, s.squares, numbers_of(a, g), a.eps);
+}
+
+// The statistics of all groups, a workgroup each, where their parts are too many for
+// every workgroup of outputs to add up.
+__global__ __launch_bounds__(256) void group_last_join_kernel(GroupNormLastArgs a) {
+    __shared__ Sums sums[4];
+    const int64_t image = blockIdx.x / a.groups, g = blockIdx.x - image * a.groups, group = (a.image0 + image) * a.groups + g;
+    const double c = a.firsts[group];
+    const Sums mine = parts_of(a, group, threadIdx.x, 256);
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x / 64] = mine;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    const Moments s = moments_of(c, (sums[0].first + sums[1].first) + (sums[2].first + sums[3].first),
+                             (sums[0].squares + sums[1].squares) + (sums[2].squares + sums[3].squares), numbers_of(a, g), a.eps);
+    reinterpret_cast<Moments *>(a.joined)[group] = s;
+}
+
+// The outputs of a slab's channels and a chunk of pixels.
+template <int V>
+__global__ __launch_bounds__(kThreads) void group_last_apply_kernel(GroupNormLastArgs a) {
+    extern __shared__ Moments stats[];  // the slab's groups'
+    // The last chunks that the sums read, first.
+    const View v = view_of(a, gridDim.x - 1 - blockIdx.x);
+    const int tid = threadIdx.x;
+    const float *x = a.x + v.image * a.ximage;
+    Outputs<V> out;
+    float q[kAhead][V];
+    const auto load = [&](const Place &at, int64_t p0) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int64_t p = p0 + u * at.rows;
+            load_channels<V>(x + at.c + (p < v.p1 ? p : v.p0) * a.xpixel, q[u]);
+        }
+    };
+    // The first pixels and the operands are under way while the statistics are joined.
+    {
+        const Place at = place_of<V, kThreads>(v, v.c0);
+        if (at.row < at.rows) {
+            out.operands(a, v, at.c);
+            load(at, v.p0 + at.row);
+        }
+    }
+    if (a.joined != nullptr) {
+        for (int g = tid; g < v.groups; g += kThreads) {
+            stats[g] = reinterpret_cast<const Moments *>(a.joined)[v.image * a.groups + v.g0 + g];
+        }
+    } else {
+        for (int g = tid / 64; g < v.groups; g += kThreads / 64) {
+            const Moments s = join(a, v.image, v.g0 + g);
+            if ((tid & 63) == 0) stats[g] = s;
+        }
+    }
+    __syncthreads();
+    for (int from = v.c0; from < v.c1; from += kThreads * V) {
+        const Place at = place_of<V, kThreads>(v, from);
+        if (at.row >= at.rows) continue;
+        if (from > v.c0) {
+            out.operands(a, v, at.c);
+            load(at, v.p0 + at.row);
+        }
+        out.statistics(a, stats, v, at.c);
+        for (int64_t p0 = v.p0 + at.row; p0 < v.p1; p0 += kAhead * at.rows) {
+            if (p0 > v.p0 + at.row) load(at, p0);
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int64_t p = p0 + u * at.rows;
+                if (p < v.p1) out.write(a, v, at.c, p, q[u]);
+            }
+        }
+    }
+}
+
+// Sums and outputs in one launch: a workgroup holds a slab's numbers of an image,
+// R pixels a thread.
+template <int V, int T, int R>
+__global__ __launch_bounds__(T) void group_last_whole_kernel(GroupNormLastArgs a) {
+    extern __shared__ Sums sums[];
+    Sums *totals = sums + T * V;  // the slab's groups', and then their statistics
+    const View v = view_of(a, blockIdx.x);
+    const int tid = threadIdx.x;
+    const float *x = a.x + v.image * a.ximage;
+    const uint32_t per_group = static_cast<uint32_t>(a.per_group);
+    const Place at = place_of<V, T>(v, v.c0);
+    const bool in = at.row < at.rows;
+    const int pixels = static_cast<int>(v.p1);
+    float q[R][V];
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+        const int p = at.row + u * at.rows;
+        load_channels<V>(x + at.c + (in && p < pixels ? p : 0) * a.xpixel, q[u]);
+    }
+    Channels<V> mine;
+    mine.begin(x, at.c, per_group, in);
+    Outputs<V> out;
+    if (in) out.operands(a, v, at.c);
+    // A slab's groups are fewer than the threads.
+    const float first = tid < v.groups ? x[static_cast<int64_t>(v.g0 + tid) * a.per_group] : 0.0f;
+    if (tid < v.groups) totals[tid] = Sums{0.0, 0.0};
+#pragma unroll
+    for (int u = 0; u < R; ++u)
+        if (in && at.row + u * at.rows < pixels) mine.add(q[u]);
+    add_up<V, T>(mine, v, at, v.c0, per_group, sums, totals);
+    __syncthreads();
+    Moments *stats = reinterpret_cast<Moments *>(totals);
+    if (tid < v.groups) {
+        stats[tid] = moments_of(static_cast<double>(first), totals[tid].first, totals[tid].squares, numbers_of(a, v.g0 + tid), a.eps);
+    }
+    __syncthreads();  // and x is read, which y may be
+    if (!in) return;
+    out.statistics(a, stats, v, at.c);
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+        const int p = at.row + u * at.rows;
+        if (p < pixels) out.write(a, v, at.c, p, q[u]);
+    }
+}
+
+// ------------------------------------------------------------------ the split
+
+constexpr int kMostParts = 256;  // that every workgroup of outputs adds up
+// The threads of the one launch, and the pixels of each: as few threads as hold a
+// slab's numbers (what a wave does once is as much as five pixels).
+struct Whole {
+    int threads, pixels;
+};
+constexpr Whole kWhole[] = {{256, 4}, {512, 4}, {1024, 4}, {1024, 8}};
+
+int64_t gcd(int64_t a, int64_t b) { return b == 0 ? a : gcd(b, a % b); }
+
+// Groups of a slab of `channels` or more of them, a multiple of 4 where the tensor's
+// are (and so the slab begins at one).
+int64_t slab_of(const GroupNormLastShape &s, int64_t channels) {
+    const int64_t unit = s.channels % 4 == 0 ? 4 / gcd(4, s.per_group) : 1;
+    const int64_t groups = round_up(ceil_div(channels, s.per_group), unit);
+    return groups < s.groups ? groups : s.groups;
+}
+
+// Rows of T threads by V channels over a slab of so many groups.
+int64_t rows_of(const GroupNormLastShape &s, int64_t slab, int64_t threads, int v) {
+    const int64_t channels = slab * s.per_group < s.channels ? slab * s.per_group : s.channels, columns = ceil_div(channels, v);
+    return columns < threads ? threads / columns : 1;
+}
+
+struct Split {
+    int whole;                   // which of kWhole one launch is of, or -1: two launches or three
+    int64_t slab, slabs;         // of the sums (or of the one launch)
+    int64_t parts;
+    int64_t apply, apply_slabs;  // of the outputs
+    int64_t chunks;
+    bool joined;                 // three launches
 };
 
-__device__ __forceinline__ Stats stats_of(double shift, double first, double squares, double n, float eps) {
-    const double variance = (squares - first * (first / n)) / n;
-    // Below 0 by rounding alone; a NaN stays one.
-    return Stats{shift + first / n, 1.0 / sqrt((variance < 0.0 ? 0.0 : variance) + static_cast<double>(eps))};
+// By the layout's V channels a thread; the work buffer is of the larger.
+Split split_of(const GroupNormLastShape &s, int v) {
+    Split p{};
+    const int64_t cus = compute_units();
+    p.slab = slab_of(s, 16);
+    p.slabs = ceil_div(s.groups, p.slab);
+    for (p.whole = 0; p.whole < 4; ++p.whole) {
+        const Whole &w = kWhole[p.whole];
+        if (p.slab * s.per_group <= w.threads * v && s.pixels <= w.pixels * rows_of(s, p.slab, w.threads, v)) return p;
+    }
+    p.whole = -1;
+    // Whole lines of up to 1024 channels; chunks until each CU has four workgroups,
+    // of 8 pixels a thread at least.
+    p.slab = slab_of(s, ceil_div(s.channels, ceil_div(s.channels, 1024)));
+    p.slabs = ceil_div(s.groups, p.slab);
+    const auto chunks = [&](int64_t slab, int64_t slabs, int64_t least) {
+        const int64_t wanted = ceil_div(8 * cus, s.images * slabs), most = ceil_div(s.pixels, least * rows_of(s, slab, kThreads, v));
+        return wanted < most ? wanted : most;
+    };
+    p.parts = chunks(p.slab, p.slabs, 8);
+    p.joined = p.parts > kMostParts;
+    // Where the outputs' workgroups add up the parts, of few groups each.
+    p.apply = p.joined ? p.slab : slab_of(s, 64);
+    p.apply_slabs = ceil_div(s.groups, p.apply);
+    p.chunks = chunks(p.apply, p.apply_slabs, 8);
+    return p;
+}
+
+// The chain's steps as a multiplication, an addition and SiLU of one number a
+// channel; 0: it is another, or none.
+int32_t plain_of(const DevChain &c) {
+    int32_t plain = 0;
+    for (int s = 0; s < c.count; ++s) {
+        const DevStep &st = c.steps[s];
+        const int32_t step = st.kind == kMul ? kPlainMul : st.kind == kAdd ? kPlainAdd : kPlainSilu;
+        if (plain >= step || (st.kind != kSilu && (st.nb[1] != 0 || st.nb[2] != 0))) return 0;
+        plain |= step;
+    }
+    return plain;
+}
+
+size_t work_of(const GroupNormLastShape &s, const Split &p) {
+    return p.whole >= 0 ? 0 : static_cast<size_t>(s.images * s.groups * (2 * p.parts + 1 + (p.joined ? 2 : 0))) * sizeof(double);
+}
+
+template <int V, int T, int R, class ByImages>
+hipError_t launch_whole(ByImages by_images, const Split &split, const GroupNormLastArgs &a, hipStream_t stream) {
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&group_last_whole_kernel<V, T, R>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    if (attr != hipSuccess) return attr;
+    return by_images(split.slab, split.slabs, 1, [&](int64_t, dim3 grid, uint32_t lds) {
+        SDHIP_LAUNCH((group_last_whole_kernel<V, T, R>), grid, dim3(T), static_cast<uint32_t>(T * V * sizeof(Sums)) + lds, stream, a);
+    });
 }
 
 template <int V>
-__global__ __launch_bounds__(kThreads) void group_last_apply_kernel(GroupNormLastArgs a) {
-    extern __shared__ Stats stats[];  // the slab's groups'
-    const View v = view_of(a);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const float *x = a.x + v.image * a.ximage;
-    float *y = a.y + v.image * a.yimage;
-    for (int g = wave; g < v.groups; g += kWaves) {
-        const int64_t group = v.image * a.groups + v.g0 + g;
-        const double *from = a.partials + group * a.parts * 2;
-        double s = 0.0, t = 0.0;
-        for (int i = lane; i < a.parts; i += 64) {
-            s += from[2 * i];
-            t += from[2 * i + 1];
+hipError_t launch(GroupNormLastArgs a, const Split &split, void *work, hipStream_t stream) {
+    // A launch holds 2^32 - 1 threads at most: 2^21 workgroups of an image or more (one
+    // has 2^18 slabs or, where it has several chunks, a few thousand of both).
+    const auto by_images = [&](int64_t slab, int64_t slabs, int64_t chunks, auto run) {
+        a.slab_groups = static_cast<int32_t>(slab);
+        a.slabs = static_cast<int32_t>(slabs);
+        a.chunks = static_cast<int32_t>(chunks);
+        a.chunk = ceil_div(a.pixels, chunks);
+        const int64_t most = (int64_t{1} << 21) / (slabs * chunks);
+        for (a.image0 = 0; a.image0 < a.images; a.image0 += most) {
+            const int64_t images = a.images - a.image0 < most ? a.images - a.image0 : most;
+            run(images, dim3(static_cast<uint32_t>(images * slabs * chunks)), static_cast<uint32_t>(slab * sizeof(Sums)));
+            if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
         }
-        s = wave_sum(s);
-        t = wave_sum(t);
-        const int64_t c = static_cast<int64_t>(v.g0 + g) * a.per_group;
-        const int64_t width = c + a.per_group < a.channels ? a.per_group : a.channels - c;
-        if (lane == 0) stats[g] = stats_of(a.firsts[group], s, t, static_cast<double>(width) * static_cast<double>(a.pixels), a.eps);
+        return hipSuccess;
+    };
+    static_assert(sizeof(Sums) == sizeof(Moments));
+    if (split.whole == 0) return launch_whole<V, kWhole[0].threads, kWhole[0].pixels>(by_images, split, a, stream);
+    if (split.whole == 1) return launch_whole<V, kWhole[1].threads, kWhole[1].pixels>(by_images, split, a, stream);
+    if (split.whole == 2) return launch_whole<V, kWhole[2].threads, kWhole[2].pixels>(by_images, split, a, stream);
+    if (split.whole == 3) return launch_whole<V, kWhole[3].threads, kWhole[3].pixels>(by_images, split, a, stream);
+    a.parts = static_cast<int32_t>(split.parts);
+    a.partials = static_cast<double *>(work);
+    double *at = a.partials + 2 * a.images * a.groups * split.parts;
+    if (split.joined) {
+        a.joined = at;
+        at += 2 * a.images * a.groups;
     }
-    __syncthreads();
-    const uint32_t per_group = static_cast<uint32_t>(a.per_group), width = static_cast<uint32_t>(a.width);
-    for (int from = v.c0; from < v.c1; from += kThreads * V) {
-        const Place at = place_of<V>(v, from);
-        if (at.row >= at.rows) continue;
-        Stats mine[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) mine[i] = stats[static_cast<uint32_t>(at.c + i) / per_group - v.g0];
-        const float *from_x = x + at.c;
-        float *to = y + at.c;
-        for (int64_t p0 = v.p0 + at.row; p0 < v.p1; p0 += kAhead * at.rows) {
-            float q[kAhead][V];
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int64_t p = p0 + u * at.rows;
-                load_channels<V>(from_x + (p < v.p1 ? p : p0) * a.xpixel, q[u]);
-            }
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int64_t p = p0 + u * at.rows;
-                if (p >= v.p1) continue;
-                float r[V];
-#pragma unroll
-                for (int i = 0; i < V; ++i) r[i] = static_cast<float>((static_cast<double>(q[u][i]) - mine[i].mean) * mine[i].scale);
-                const uint32_t i2 = static_cast<uint32_t>(p) / width, i1 = static_cast<uint32_t>(p) - i2 * width;
-                apply_chain_block(a.chain, r, [&](int s, int i) {
-                    const DevStep &st = a.chain.steps[s];
-                    return (at.c + i) * st.nb[0] + i1 * st.nb[1] + i2 * st.nb[2] + v.image * st.nb[3];
-                });
-                if constexpr (V == 4) {
-                    *reinterpret_cast<float4v *>(to + p * a.ypixel) = float4v{r[0], r[1], r[2], r[3]};
-                } else {
-                    to[p * a.ypixel] = r[0];
-                }
-            }
-        }
+    a.firsts = at;
+    hipError_t e = by_images(split.slab, split.slabs, split.parts, [&](int64_t, dim3 grid, uint32_t lds) {
+        SDHIP_LAUNCH(group_last_sums_kernel<V>, grid, dim3(kThreads), lds, stream, a);
+    });
+    if (e == hipSuccess && split.joined) {
+        e = by_images(1, a.groups, 1, [&](int64_t images, dim3, uint32_t) {
+            SDHIP_LAUNCH(group_last_join_kernel, dim3(static_cast<uint32_t>(images * a.groups)), dim3(256), 0, stream, a);
+        });
     }
-}
-
-// Slabs of whole groups, of 64 channels or more and a multiple of 4 of them where
-// the channels are; chunks until each CU has four workgroups, of 8 pixels a
-// thread at least.
-struct Split {
-    int64_t slab_groups, slabs, chunks;
-};
-
-Split split_of(const GroupNormLastShape &s) {
-    Split p;
-    int64_t groups = ceil_div(64, s.per_group);
-    while (s.channels % 4 == 0 && groups * s.per_group % 4 != 0) ++groups;
-    p.slab_groups = groups < s.groups ? groups : s.groups;
-    p.slabs = ceil_div(s.groups, p.slab_groups);
-    const int64_t rows = kThreads / (p.slab_groups * s.per_group / 4 < kThreads ? p.slab_groups * s.per_group / 4 + 1 : kThreads);
-    const int64_t wanted = ceil_div(4 * static_cast<int64_t>(compute_units()), s.images * p.slabs);
-    const int64_t most = ceil_div(s.pixels, 8 * rows);
-    p.chunks = wanted < most ? wanted : most;
-    return p;
+    if (e != hipSuccess) return e;
+    return by_images(split.apply, split.apply_slabs, split.chunks, [&](int64_t, dim3 grid, uint32_t lds) {
+        SDHIP_LAUNCH(group_last_apply_kernel<V>, grid, dim3(kThreads), lds, stream, a);
+    });
 }
 
 }  // namespace
 
 size_t group_norm_last_work_size(const GroupNormLastShape &s) {
-    return static_cast<size_t>(s.images * s.groups * (2 * split_of(s).chunks + 1)) * sizeof(double);
+    const size_t four = work_of(s, split_of(s, 4)), one = work_of(s, split_of(s, 1));
+    return four > one ? four : one;
 }
 
 hipError_t launch_group_norm_last(GroupNormLastArgs a, void *work, hipStream_t stream) {
     KernelScope scope("group_norm_last", stream);
-    const Split split = split_of({a.channels, a.pixels, a.images, a.groups, a.per_group});
-    a.slab_groups = static_cast<int32_t>(split.slab_groups);
-    a.slabs = static_cast<int32_t>(split.slabs);
-    a.chunks = a.parts = static_cast<int32_t>(split.chunks);
-    a.chunk = ceil_div(a.pixels, split.chunks);
-    a.partials = static_cast<double *>(work);
-    a.firsts = a.partials + 2 * a.images * a.groups * a.chunks;
+    a.plain = plain_of(a.chain);
     const auto quads = [](const void *p, int64_t pixel, int64_t image) {
         return reinterpret_cast<uintptr_t>(p) % 16 == 0 && pixel % 4 == 0 && image % 4 == 0;
     };
-    const bool four = a.channels % 4 == 0 && quads(a.x, a.xpixel, a.ximage) && quads(a.y, a.ypixel, a.yimage);
-    const size_t sums = split.slab_groups * sizeof(Sums), stats = split.slab_groups * sizeof(Stats);
-    // A launch holds 2^32 - 1 threads at most: 2^23 workgroups of an image or more
-    // (one has 2^18 slabs or, where it has several chunks, a few thousand of both).
-    const int64_t of_image = split.slabs * split.chunks, most = (int64_t{1} << 23) / of_image;
-    for (a.image0 = 0; a.image0 < a.images; a.image0 += most) {
-        const int64_t images = a.images - a.image0 < most ? a.images - a.image0 : most;
-        const dim3 grid(static_cast<uint32_t>(images * of_image)), block(kThreads);
-        if (four) {
-            SDHIP_LAUNCH(group_sums_kernel<4>, grid, block, sums, stream, a);
-        } else {
-            SDHIP_LAUNCH(group_sums_kernel<1>, grid, block, sums, stream, a);
-        }
-        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-        if (four) {
-            SDHIP_LAUNCH(group_last_apply_kernel<4>, grid, block, stats, stream, a);
-        } else {
-            SDHIP_LAUNCH(group_last_apply_kernel<1>, grid, block, stats, stream, a);
-        }
-        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    const GroupNormLastShape s{a.channels, a.pixels, a.images, a.groups, a.per_group};
+    if (a.channels % 4 == 0 && quads(a.x, a.xpixel, a.ximage) && quads(a.y, a.ypixel, a.yimage)) {
+        return launch<4>(a, split_of(s, 4), work, stream);
     }
-    return hipSuccess;
+    return launch<1>(a, split_of(s, 1), work, stream);
 }
 
 }  // namespace sdhip

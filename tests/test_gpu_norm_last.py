@@ -1,6 +1,7 @@
 """GROUP_NORM of channels-last tensors with its chain, on the device against
-float64.  Bounds: a normed number is rounded once from double, the chain's steps
-once each; SiLU's slope is below 1.1 and its own error 8 roundings."""
+float64.  Bounds: a normed number is rounded four times (its differences from the
+mean's two parts, the scale, their product), the chain's steps once each; SiLU's
+slope is below 1.1 and its own error 8 roundings."""
 
 import numpy as np
 import pytest
@@ -25,7 +26,7 @@ def reference(x, groups, eps):
 
 def affine(v, scale, shift, silu):
     y = v * scale.astype(np.float64) + shift.astype(np.float64)
-    err = 2.0 ** -24 * (4 * np.abs(v * scale) + 2 * np.abs(shift))
+    err = 2.0 ** -24 * (6 * np.abs(v * scale) + 2 * np.abs(shift))
     if silu:
         y = y / (1.0 + np.exp(-y))
         err = 1.1 * err + 8 * 2.0 ** -24 * np.abs(y) + 2.0 ** -126
@@ -139,7 +140,7 @@ def test_chains(gpu, shape, groups):
         torch.cuda.synchronize()
         o64, p64 = o.astype(np.float64), p.astype(np.float64)
         want = (v * o64 + p64 + o64) * p64 + o64
-        assert (np.abs(y.cpu().numpy() - want) <= 2.0 ** -24 * 8 * (np.abs(v) + 3)).all()
+        assert (np.abs(y.cpu().numpy() - want) <= 2.0 ** -24 * 10 * (np.abs(v) + 3)).all()
     tokens = torch.empty((n, h * w, c), device=gpu)
     image = torch.empty_like(xd)
     sdhip.group_norm_last(xd.view(n, h * w, c), tokens, groups, 1e-5)
@@ -152,7 +153,8 @@ def test_chains(gpu, shape, groups):
         sdhip.group_norm_last(xd, apart, groups, 1e-5, chain)
         sdhip.set_tuning("")
         sdhip.group_norm_last(xd, fused, groups, 1e-5, chain)
-        assert torch.equal(apart, fused)
+        # Each SiLU is within 8 roundings.
+        assert ((apart - fused).abs() <= 16 * 2.0 ** -24 * fused.abs() + 2.0 ** -126).all()
     finally:
         sdhip.set_tuning("")
 
