@@ -438,7 +438,8 @@ sdhip_status sdhip_norm_residual(const sdhip_tensor *y, const sdhip_row_norm *po
  * along a times base[a]^(-2 j / dims[a]) for the axis's pair j or, with
  * `shared`, base[a]^(-2 p / n) for the head's pair p.  Pair p is numbers 2 p and
  * 2 p + 1 (ADJACENT) or p and n / 2 + p (HALVES).  Angles are taken in double; a
- * norm is sdhip_row_norm's (sdhip_norm_residual), its sums in double.  y may be
+ * norm is sdhip_row_norm's (sdhip_norm_residual), its sums in double or, of squares
+ * far from single precision's limits, in that.  y may be
  * x's own memory in the same layout; else what is written shares no byte range
  * with what is read, nor do two rows of y: SDHIP_UNSUPPORTED.  No work buffer. */
 enum { SDHIP_ROPE_ADJACENT = 0, SDHIP_ROPE_HALVES = 1 };

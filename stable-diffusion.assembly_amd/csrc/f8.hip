@@ -35,32 +35,35 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
 constexpr int kBlock = static_cast<int>(kF8Block);
 constexpr int kLeast = -101 + 127;  // e's least, biased as an exponent's bits
-constexpr uint32_t kNans = 0x7f7f7f7fu;  // four NaN of E4M3
 constexpr uint32_t kInfinity = 0x7f800000u;
 
 // ------------------------------------------------------------------ numbers
 
 // e's bits, biased by 127, for a greatest magnitude of these bits: 448 is 1.75 x
-// 2^8.  Those of an infinity or NaN are not used.
+// 2^8.
 __device__ __forceinline__ uint32_t power_of(uint32_t greatest) {
     const int e = static_cast<int>((greatest + 0x1fffffu) >> 23) - 8;
     return static_cast<uint32_t>(e > kLeast ? e : kLeast);
 }
 
-// 2^e and 2^-e, e at most 120.
+// 2^e and 2^-e.
 __device__ __forceinline__ float up(uint32_t e) { return __builtin_bit_cast(float, e << 23); }
 __device__ __forceinline__ float down(uint32_t e) { return __builtin_bit_cast(float, (254 - e) << 23); }
 
-__device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
-
-__device__ __forceinline__ uint32_t greater(uint32_t a, uint32_t b) { return a > b ? a : b; }
-
-// The greatest of a row of 16 lanes, on all of them.
-__device__ __forceinline__ uint32_t greatest16(uint32_t v) {
-    v = greater(v, __builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, true));   // lanes i ^ 1
-    v = greater(v, __builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, true));   // i ^ 2
-    v = greater(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true));  // 8 lanes mirrored
-    return greater(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true));  // 16 lanes mirrored
+// The greatest magnitude of a group's eight numbers of each of 16 lanes, as bits, on
+// all of them: of NaN among them nothing is seen.
+__device__ __forceinline__ uint32_t greatest(const float4v &u, const float4v &v) {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = __builtin_fmaxf(m, __builtin_fabsf(u[i]));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = __builtin_fmaxf(m, __builtin_fabsf(v[i]));
+    uint32_t top = __builtin_bit_cast(uint32_t, m);
+    const auto greater = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+    top = greater(top, __builtin_amdgcn_update_dpp(0, top, 0xb1, 0xf, 0xf, true));   // lanes i ^ 1
+    top = greater(top, __builtin_amdgcn_update_dpp(0, top, 0x4e, 0xf, 0xf, true));   // i ^ 2
+    top = greater(top, __builtin_amdgcn_update_dpp(0, top, 0x141, 0xf, 0xf, true));  // 8 lanes mirrored
+    return greater(top, __builtin_amdgcn_update_dpp(0, top, 0x140, 0xf, 0xf, true));  // 16 lanes mirrored
 }
 
 // Eight numbers of E4M3 as FP16.
@@ -70,12 +73,19 @@ __device__ __forceinline__ half8 widen(int low, int high) {
     return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// Four numbers times `scale` as E4M3, those of a group with an infinity or NaN as
-// NaN.
-__device__ __forceinline__ int four(const float4v &v, float scale, bool finite) {
-    int r = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * scale, v[1] * scale, 0, false);
-    r = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * scale, v[3] * scale, r, true);
-    return finite ? r : static_cast<int>(kNans);
+// Four numbers times `scale` as E4M3.
+__device__ __forceinline__ int four(const float4v &v, float scale) {
+    const int r = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * scale, v[1] * scale, 0, false);
+    return __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * scale, v[3] * scale, r, true);
+}
+
+// A lane's eight numbers of a group as q in FP16, and the group's 2^e.  An infinity
+// makes them all NaN; a NaN stays one.
+__device__ __forceinline__ half8 held(const float4v &u, const float4v &v, float &power) {
+    const uint32_t top = greatest(u, v), e = power_of(top);
+    const float scale = top < kInfinity ? down(e) : __builtin_nanf("");
+    power = up(e);
+    return widen(four(u, scale), four(v, scale));
 }
 
 // Four of a row's K numbers from k on, of the last four there are where those end
@@ -92,7 +102,7 @@ __device__ __forceinline__ float4v load_x(const float *row, int k, int K) {
 // What load_x gave at k as the numbers from there on, 0 past the row's end.
 __device__ __forceinline__ float4v ended_x(const float4v &v, int k, int K) {
     const int past = k + 4 - K;  // numbers that lie before k, and are wanted of none past K
-    if (K < 4 || past <= 0) return v;
+    if (!__any(past > 0) || K < 4 || past <= 0) return v;
     return past == 1 ? float4v{v[1], v[2], v[3], 0.0f} : past == 2 ? float4v{v[2], v[3], 0.0f, 0.0f}
                                                     : past == 3 ? float4v{v[3], 0.0f, 0.0f, 0.0f} : float4v{0.0f, 0.0f, 0.0f, 0.0f};
 }
@@ -196,20 +206,10 @@ __global__ __launch_bounds__(kOperandThreads) void f8_operands_kernel(OperandsAr
         const uint32_t m = g / o.blocks, b = g - m * o.blocks;
         const int k = static_cast<int>(b) * kBlock + 8 * (threadIdx.x & 15), K = static_cast<int>(a.K);
         const float *row = a.x + m * a.ldx;
-        float4v v[2];
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            v[i] = ended_x(load_x(row, k + 4 * i, K), k + 4 * i, K);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) top = greater(top, magnitude(v[i][j]));
-        }
-        top = greatest16(top);
-        const uint32_t e = power_of(top);
-        const float scale = down(e);
-        const bool finite = top < kInfinity;
-        *reinterpret_cast<half8 *>(o.w.q + m * o.w.ld + k) = widen(four(v[0], scale, finite), four(v[1], scale, finite));
-        if ((threadIdx.x & 15) == 0) o.w.powers[b * o.w.rows + m] = finite ? up(e) : 1.0f;
+        const float4v u = ended_x(load_x(row, k, K), k, K), v = ended_x(load_x(row, k + 4, K), k + 4, K);
+        float power;
+        *reinterpret_cast<half8 *>(o.w.q + m * o.w.ld + k) = held(u, v, power);
+        if ((threadIdx.x & 15) == 0) o.w.powers[b * o.w.rows + m] = power;
     }
 }
 
@@ -232,11 +232,14 @@ struct FewArgs {
 // the groups' powers, by chunks of K where it is long; the weights come straight from
 // memory into registers, kAhead blocks of a wave's under way, 64 bytes of a row side
 // by side in a load.  The splits' sums are joined in LDS.
-// A wave's blocks under way, as many as 128 registers hold: two workgroups a CU.
+// A wave's blocks under way: with few of x's groups loaded together as many as 128
+// registers hold, for two workgroups a CU; with many, for one.
 constexpr int few_ahead(int rm) { return rm > 1 ? 2 : 3; }
 
-template <bool GATED, int RM>
-__global__ __launch_bounds__(kThreads, 4) void f8_few_kernel(FewArgs f) {
+// LOADS groups of x a team of 16 lanes has under way.  TAIL: K ends within a block,
+// which is taken apart from the whole ones.
+template <bool GATED, bool TAIL, int RM, int LOADS>
+__global__ __launch_bounds__(kThreads, LOADS > 2 ? 2 : 4) void f8_few_kernel(FewArgs f) {
     const F8Args &a = f.a;
     constexpr int kRows = 16 * RM, kAhead = few_ahead(RM);
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -253,49 +256,48 @@ __global__ __launch_bounds__(kThreads, 4) void f8_few_kernel(FewArgs f) {
     const int K = static_cast<int>(a.K), blocks = (K + kBlock - 1) / kBlock;
     const int n = n0 + 16 * tile;
 
-    // Groups of x, 32 at a time by the workgroup, kLoads such passes' loads together.
-    constexpr int kLoads = 2;
+    // Groups of x, 32 at a time by the workgroup, LOADS such passes' loads together; the
+    // row of group g by a product that is exact for the few thousands there are.
+    const auto row_of = [](int g, float inverse) { return static_cast<int>((static_cast<float>(g) + 0.5f) * inverse); };
     const int team = tid >> 4, part = tid & 15;
     float *powers = reinterpret_cast<float *>(lds + rows * f.row);  // [row][block of the chunk]
+    const auto x_row_of = [&](int r) {
+        return a.x + m0 * K + static_cast<uint64_t>(static_cast<uint32_t>(r)) * static_cast<uint32_t>(K);
+    };
     struct Numbers {
-        float4v v[kLoads][2];
+        float4v v[LOADS][2];
     };
     const auto load_groups = [&](int b0, int count, int first, Numbers &x) {
+        const float inverse = 1.0f / static_cast<float>(count);
 #pragma unroll
-        for (int u = 0; u < kLoads; ++u) {
-            const int g = first + 32 * u + team, r = g / count, k = (b0 + g - r * count) * kBlock + 8 * part;
-            if (r < rows) {
-                const float *from = a.x + (m0 + r) * a.ldx;
-                x.v[u][0] = load_x(from, k, K);
-                x.v[u][1] = load_x(from, k + 4, K);
-            }
+        for (int u = 0; u < LOADS; ++u) {
+            const int g = first + 32 * u + team, r = row_of(g, inverse), k = (b0 + g - r * count) * kBlock + 8 * part;
+            const float *from = x_row_of(r < rows ? r : rows - 1) + k;
+            x.v[u][0] = load4(from);
+            x.v[u][1] = load4(from + 4);
         }
     };
-    const auto store_groups = [&](int b0, int count, int first, const Numbers &x) {
+    const auto store_group = [&](int r, int b, const half8 &q, float power) {
+        *reinterpret_cast<half8 *>(lds + r * f.row + b * (2 * kBlock) + 16 * part) = q;
+        if (part == 0) powers[r * f.chunk + b] = power;
+    };
+    const auto store_groups = [&](int count, int first, const Numbers &x) {
+        const float inverse = 1.0f / static_cast<float>(count);
 #pragma unroll
-        for (int u = 0; u < kLoads; ++u) {
-            const int g = first + 32 * u + team, r = g / count, b = g - r * count, k = (b0 + b) * kBlock + 8 * part;
-            float4v v[2];
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                v[i] = ended_x(x.v[u][i], k + 4 * i, K);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) top = greater(top, magnitude(v[i][j]));
-            }
-            top = greatest16(top);
-            const uint32_t e = power_of(top);
-            const float scale = down(e);
-            const bool finite = top < kInfinity;
-            if (r < rows) {
-                *reinterpret_cast<half8 *>(lds + r * f.row + b * (2 * kBlock) + 16 * part) =
-                    widen(four(v[0], scale, finite), four(v[1], scale, finite));
-                if (part == 0) powers[r * f.chunk + b] = finite ? up(e) : 1.0f;
-            }
+        for (int u = 0; u < LOADS; ++u) {
+            const int g = first + 32 * u + team, r = row_of(g, inverse);
+            float power;
+            const half8 q = held(x.v[u][0], x.v[u][1], power);
+            if (r < rows) store_group(r, g - r * count, q, power);
         }
+    };
+    // The whole blocks of a chunk from b0 on.
+    const auto whole_of = [&](int b0) {
+        const int whole = K / kBlock - b0;
+        return whole < f.chunk ? whole : f.chunk;
     };
     Numbers begun;
-    load_groups(0, f.chunk < blocks ? f.chunk : blocks, 0, begun);
+    if (!TAIL || whole_of(0) > 0) load_groups(0, whole_of(0), 0, begun);
 
     // The lane's row of the weights; the scales of its first output and of its last,
     // which with GATED lie in two blocks at most, `across` of them in the first.
@@ -311,8 +313,13 @@ __global__ __launch_bounds__(kThreads, 4) void f8_few_kernel(FewArgs f) {
     const auto load_weights = [&](int b, Weights &o) {
         if (b >= blocks) return;
         const int k = b * kBlock + 16 * group;
-        o.q[0] = load_w(w, k, K);
-        o.q[1] = load_w(w, k + 64, K);
+        if (TAIL && (b + 1) * kBlock > K) {
+            o.q[0] = load_w(w, k, K);
+            o.q[1] = load_w(w, k + 64, K);
+        } else {
+            __builtin_memcpy(&o.q[0], w + k, 16);
+            __builtin_memcpy(&o.q[1], w + k + 64, 16);
+        }
         o.s[0] = scales[0][b];
         o.s[1] = GATED ? scales[1][b] : o.s[0];
     };
@@ -332,14 +339,21 @@ __global__ __launch_bounds__(kThreads, 4) void f8_few_kernel(FewArgs f) {
     float4v acc[RM];
 #pragma unroll
     for (int i = 0; i < RM; ++i) acc[i] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-    store_groups(0, f.chunk < blocks ? f.chunk : blocks, 0, begun);
+    if (!TAIL || whole_of(0) > 0) store_groups(whole_of(0), 0, begun);
     for (int b0 = 0;;) {
-        const int count = blocks - b0 < f.chunk ? blocks - b0 : f.chunk;
+        const int count = blocks - b0 < f.chunk ? blocks - b0 : f.chunk, whole = whole_of(b0);
 #pragma unroll 1
-        for (int first = b0 == 0 ? 32 * kLoads : 0; first < rows * count; first += 32 * kLoads) {
+        for (int first = b0 == 0 ? 32 * LOADS : 0; first < rows * whole; first += 32 * LOADS) {
             Numbers x;
-            load_groups(b0, count, first, x);
-            store_groups(b0, count, first, x);
+            load_groups(b0, whole, first, x);
+            store_groups(whole, first, x);
+        }
+        if (TAIL && whole < count && team < rows) {
+            const int k = (blocks - 1) * kBlock + 8 * part;
+            const float *from = x_row_of(team);
+            float power;
+            const half8 q = held(ended_x(load_x(from, k, K), k, K), ended_x(load_x(from, k + 4, K), k + 4, K), power);
+            store_group(team, whole, q, power);
         }
         lds_barrier();
 #pragma unroll 1
@@ -348,7 +362,7 @@ __global__ __launch_bounds__(kThreads, 4) void f8_few_kernel(FewArgs f) {
             for (int d = 0; d < kAhead; ++d) {
                 const int b = b1 + d * S;
                 if (b >= count) continue;
-                if ((b0 + b + 1) * kBlock > K) {  // a shorter block, the last
+                if (TAIL && (b0 + b + 1) * kBlock > K) {  // a shorter block, the last
                     const int k = (b0 + b) * kBlock + 16 * group;
                     weights[d].q[0] = ended_w(weights[d].q[0], k, K);
                     weights[d].q[1] = ended_w(weights[d].q[1], k + 64, K);
@@ -400,28 +414,44 @@ int few_splits(int64_t M, int64_t columns, int64_t K, int64_t rows, int halves) 
     return splits;
 }
 
-template <bool GATED, int RM>
-hipError_t launch_few(const F8Args &a, hipStream_t stream) {
-    constexpr int kAhead = few_ahead(RM), kSums = kWaves * RM * 1024, kMost = 160 * 1024;
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&f8_few_kernel<GATED, RM>),
+template <bool GATED, bool TAIL, int RM, int LOADS>
+hipError_t launch_few(FewArgs f, int64_t rows, int64_t row_blocks, hipStream_t stream) {
+    constexpr int kSums = kWaves * RM * 1024, kMost = 160 * 1024;
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&f8_few_kernel<GATED, TAIL, RM, LOADS>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
     if (attr != hipSuccess) return attr;
+    const int64_t x = rows * (f.row + 4 * static_cast<int64_t>(f.chunk));
+    SDHIP_LAUNCH((f8_few_kernel<GATED, TAIL, RM, LOADS>), dim3(static_cast<uint32_t>(f.column_blocks * row_blocks)), dim3(kThreads),
+                 static_cast<uint32_t>(x > kSums ? x : kSums), stream, f);
+    return hipGetLastError();
+}
+
+template <bool GATED, bool TAIL, int RM>
+hipError_t few_rows(const F8Args &a, hipStream_t stream) {
     const int64_t columns = GATED ? a.half : a.N, blocks = ceil_div(a.K, kF8Block);
-    const int64_t rows = a.M < 16 * RM ? a.M : 16 * RM;
+    const int64_t rows = a.M < 16 * RM ? a.M : 16 * RM, row_blocks = ceil_div(a.M, 16 * RM);
     const int splits = few_splits(a.M, columns, a.K, 16 * RM, GATED ? 2 : 1), outs = kWaves / splits / (GATED ? 2 : 1);
     // Whole rounds of the waves' blocks: all of K where that is 64 KB at most, else as
-    // many as 64 KB hold, or one (128 KB of 16 rows, 132 of 32).
-    const int64_t round = kAhead * splits, bytes = 2 * kBlock + 4;
+    // many as 64 KB hold, or one (100 KB of 16 rows, 133 of 32).
+    const int64_t round = few_ahead(RM) * splits, bytes = 2 * kBlock + 4;
     const int64_t fit = (64 * 1024 / rows - 16) / bytes / round * round;
     const int64_t chunk = blocks < fit ? blocks : fit > round ? fit : round < blocks ? round : blocks;
     // Rows 16 bytes further apart than they are long, so that 16 read at once lie on
     // different banks.
-    const int64_t row = chunk * (2 * kBlock) + 16, x = rows * (row + 4 * chunk);
-    const FewArgs f{a, splits, static_cast<int32_t>(chunk), static_cast<int32_t>(row),
+    const FewArgs f{a, splits, static_cast<int32_t>(chunk), static_cast<int32_t>(chunk * (2 * kBlock) + 16),
                     static_cast<uint32_t>(ceil_div(columns, 16 * outs))};
-    SDHIP_LAUNCH((f8_few_kernel<GATED, RM>), dim3(static_cast<uint32_t>(f.column_blocks * ceil_div(a.M, 16 * RM))), dim3(kThreads),
-                 static_cast<uint32_t>(x > kSums ? x : kSums), stream, f);
-    return hipGetLastError();
+    // All of a chunk's groups loaded together where a workgroup is alone on its CU;
+    // else two passes, in the registers that leave room for another workgroup.
+    const int64_t passes = ceil_div(rows * chunk, kThreads / 16);
+    const bool alone = f.column_blocks * row_blocks <= compute_units();
+    if (passes <= 1) return launch_few<GATED, TAIL, RM, 1>(f, rows, row_blocks, stream);
+    if (passes <= 2 || !alone) return launch_few<GATED, TAIL, RM, 2>(f, rows, row_blocks, stream);
+    return launch_few<GATED, TAIL, RM, 4>(f, rows, row_blocks, stream);
+}
+
+template <bool GATED, int RM>
+hipError_t few_rows(const F8Args &a, hipStream_t stream) {
+    return a.K % kF8Block != 0 ? few_rows<GATED, true, RM>(a, stream) : few_rows<GATED, false, RM>(a, stream);
 }
 
 // ------------------------------------------------------------------ many rows
@@ -820,8 +850,8 @@ hipError_t lay_out(const F8Args &a, const F8Work &w, hipStream_t stream) {
 template <bool GATED>
 hipError_t launch_form(const F8Args &a, bool whole, void *work, hipStream_t stream) {
     const Form form = form_of(a.M, a.N, a.K);
-    if (form == Form::few) return launch_few<GATED, 1>(a, stream);
-    if (form == Form::rows) return launch_few<GATED, 2>(a, stream);
+    if (form == Form::few) return few_rows<GATED, 1>(a, stream);
+    if (form == Form::rows) return few_rows<GATED, 2>(a, stream);
     const F8Work w = work_of(a.M, a.N, a.K, !whole, work);
     if (const hipError_t e = lay_out(a, w, stream); e != hipSuccess) return e;
     const TilesArgs t{a, w, whole ? a.w : w.w, whole ? a.row_bytes : w.ld, 0, 0};

@@ -21,15 +21,24 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kMostPairs = kRopeMost / 2;
 
-// cos and sin of `turns` half turns.
+// cos and sin of `turns` half turns: of what is left of them by the nearest quarter
+// of a turn, 45 degrees at most, by Taylor's series to x^9 and x^10 (off by 2e-9 of
+// themselves), in the quarter's place.  The quarters are counted in the last bits of
+// a sum with 1.5 x 2^52.
 __device__ __forceinline__ float2 turn(double turns) {
-    const double q = __builtin_rint(2.0 * turns);
-    const float r = static_cast<float>(__builtin_fma(-0.5, q, turns));
-    float s, c;
-    sincospif(r, &s, &c);
-    const int k = static_cast<int>(__builtin_fma(-4.0, __builtin_floor(0.25 * q), q));
+    const double magic = 6755399441055744.0, sum = __builtin_fma(2.0, turns, magic), q = sum - magic;
+    const float x = static_cast<float>(3.14159265358979323846 * __builtin_fma(-0.5, q, turns)), x2 = x * x;
+    float s = __builtin_fmaf(x2, 2.7557319e-6f, -1.9841270e-4f);
+    s = __builtin_fmaf(s, x2, 8.3333333e-3f);
+    s = __builtin_fmaf(s, x2, -1.6666667e-1f);
+    s = __builtin_fmaf(x * x2, s, x);
+    float c = __builtin_fmaf(x2, -2.7557319e-7f, 2.4801587e-5f);
+    c = __builtin_fmaf(c, x2, -1.3888889e-3f);
+    c = __builtin_fmaf(c, x2, 4.1666667e-2f);
+    c = __builtin_fmaf(c, x2, -0.5f);
+    c = __builtin_fmaf(c, x2, 1.0f);
+    const uint32_t k = static_cast<uint32_t>(__builtin_bit_cast(uint64_t, sum));
     const float2 t = k & 1 ? make_float2(-s, c) : make_float2(c, s);
     return k & 2 ? make_float2(-t.x, -t.y) : t;
 }
@@ -45,16 +54,36 @@ __device__ __forceinline__ double row_sum(double v) {
     return v;
 }
 
+template <int LPR>
+__device__ __forceinline__ float row_sum(float v) {
+    const auto add = [](float v, auto control) {
+        return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(control)::value, 0xf, 0xf, true));
+    };
+    v = add(v, std::integral_constant<int, 0xb1>{});
+    v = add(v, std::integral_constant<int, 0x4e>{});
+    v = add(v, std::integral_constant<int, 0x141>{});
+    if constexpr (LPR >= 16) v = add(v, std::integral_constant<int, 0x140>{});
+    if constexpr (LPR == 64) {
+        uint32_t a = __builtin_bit_cast(uint32_t, v), b = a;
+        swap16(a, b);
+        v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+        a = b = __builtin_bit_cast(uint32_t, v);
+        swap32(a, b);
+        v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+    }
+    return v;
+}
+
 // LPR lanes a row, SLOTS groups of four pairs each; QUADS where every four
 // numbers that a lane reads or writes at once lie at a multiple of their size.
 template <int LPR, int SLOTS, bool ADJACENT, bool QUADS>
-__global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
-    __shared__ float2 shared[kWaves][kMostPairs];
+__global__ __launch_bounds__(kThreads, SLOTS == 1 ? 4 : 1) void rope_kernel(RopeArgs a) {
+    __shared__ float2 shared[kWaves][64 * (LPR * SLOTS <= 16 ? 1 : LPR * SLOTS <= 32 ? 2 : 4)];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int pairs = a.turned / 2;
     float2 *turns = shared[wave];
     // The frequencies, in half turns, of the pairs that this lane computes.
-    constexpr int kMine = kMostPairs / 64;
+    constexpr int kMine = LPR * SLOTS <= 16 ? 1 : LPR * SLOTS <= 32 ? 2 : 4;
     double rate[kMine];
     int axis[kMine];
 #pragma unroll
@@ -147,6 +176,9 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
     const bool weight_quads = quads_of(a.norm.weight), bias_quads = quads_of(a.norm.bias);
     constexpr int kRows = 64 / LPR;  // heads of a wave at a time
     const int share = (a.heads + a.parts - 1) / a.parts;
+    // How far a lane's row lies from the wave's first.
+    const int64_t x_lane = lane / LPR * a.xnb[2], y_lane = lane / LPR * a.ynb[2];
+    const int64_t w_lane = lane / LPR * a.norm.weight.nb[2], b_lane = lane / LPR * a.norm.bias.nb[2];
     const int64_t items = a.tokens * a.batch * a.parts;
     for (int64_t item = static_cast<int64_t>(blockIdx.x) * kWaves + wave; item < items;
          item += static_cast<int64_t>(gridDim.x) * kWaves) {
@@ -167,43 +199,68 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
         for (int s = 0; s < SLOTS; ++s)
 #pragma unroll
             for (int c = 0; c < 4; ++c) by[s][c] = turned[s][c] ? turns[4 * (sub + LPR * s) + c] : make_float2(1.0f, 0.0f);
-        const int h0 = part * share, h1 = h0 + share < a.heads ? h0 + share : a.heads;
-        for (int h = h0 + lane / LPR; h - lane / LPR < h1; h += kRows) {
-            if (h >= h1) continue;  // a row's lanes together
+        const int h0 = part * share, h1 = h0 + share < a.heads ? h0 + share : a.heads, mine = lane / LPR;
+        const float *x = a.x + i1 * a.xnb[1] + i3 * a.xnb[3] + h0 * a.xnb[2] + x_lane;
+        int64_t to = i1 * a.ynb[1] + i3 * a.ynb[3] + h0 * a.ynb[2] + y_lane;
+        const float *weight = a.norm.weight.data, *bias = a.norm.bias.data;
+        if (weight != nullptr) weight += i1 * a.norm.weight.nb[1] + i3 * a.norm.weight.nb[3] + h0 * a.norm.weight.nb[2] + w_lane;
+        if (bias != nullptr) bias += i1 * a.norm.bias.nb[1] + i3 * a.norm.bias.nb[3] + h0 * a.norm.bias.nb[2] + b_lane;
+        for (int h = h0; h < h1; h += kRows) {
+            if (h + mine >= h1) continue;  // a row's lanes together
             float v[SLOTS][4][2];
-            load(a.x + i1 * a.xnb[1] + h * a.xnb[2] + i3 * a.xnb[3], true, 1, v);
+            load(x, true, 1, v);
+            x += kRows * a.xnb[2];
             if (a.norm.kind != SDHIP_ROW_NORM_NONE) {
-                double mean = 0.0, squares = 0.0;
-                if (a.norm.kind == SDHIP_ROW_NORM_LAYER) {
+                float sum = 0.0f;
+                if (a.norm.kind == SDHIP_ROW_NORM_RMS) {
 #pragma unroll
                     for (int s = 0; s < SLOTS; ++s)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) mean += static_cast<double>(v[s][c][0]) + static_cast<double>(v[s][c][1]);
-                    mean = mean_of(row_sum<LPR>(mean), a.d, a.inverse);
+                        for (int c = 0; c < 4; ++c)
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) sum = __builtin_fmaf(v[s][c][k], v[s][c][k], sum);
+                    sum = row_sum<LPR>(sum);
                 }
+                if (a.norm.kind == SDHIP_ROW_NORM_RMS && sum > 0x1p-60f && sum < 0x1p100f) {
+                    const float scale = __builtin_amdgcn_rsqf(__builtin_fmaf(sum, static_cast<float>(a.inverse), a.norm.eps));
 #pragma unroll
-                for (int s = 0; s < SLOTS; ++s)
+                    for (int s = 0; s < SLOTS; ++s)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                        for (int c = 0; c < 4; ++c)
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const double x = at[s][c][k] < a.d ? static_cast<double>(v[s][c][k]) - mean : 0.0;
-                            squares = __builtin_fma(x, x, squares);
-                        }
-                const Moments m = moments(a.norm.kind, mean, row_sum<LPR>(squares), a.inverse, a.norm.eps);
+                            for (int k = 0; k < 2; ++k) v[s][c][k] *= scale;
+                } else {
+                    // In double: means, and squares near single precision's limits.
+                    double mean = 0.0, squares = 0.0;
+                    if (a.norm.kind == SDHIP_ROW_NORM_LAYER) {
 #pragma unroll
-                for (int s = 0; s < SLOTS; ++s)
+                        for (int s = 0; s < SLOTS; ++s)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                            for (int c = 0; c < 4; ++c) mean += static_cast<double>(v[s][c][0]) + static_cast<double>(v[s][c][1]);
+                        mean = mean_of(row_sum<LPR>(mean), a.d, a.inverse);
+                    }
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) v[s][c][k] = normed(v[s][c][k], m);
+                    for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                const double d = at[s][c][k] < a.d ? static_cast<double>(v[s][c][k]) - mean : 0.0;
+                                squares = __builtin_fma(d, d, squares);
+                            }
+                    const Moments m = moments(a.norm.kind, mean, row_sum<LPR>(squares), a.inverse, a.norm.eps);
+#pragma unroll
+                    for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) v[s][c][k] = normed(v[s][c][k], m);
+                }
             }
-            const auto operand = [&](const RowOperand &o, bool quads, float (&w)[SLOTS][4][2]) {
-                load(o.data + i1 * o.nb[1] + h * o.nb[2] + i3 * o.nb[3], quads, o.nb[0], w);
-            };
-            if (a.norm.weight.data != nullptr) {
+            if (weight != nullptr) {
                 float w[SLOTS][4][2];
-                operand(a.norm.weight, weight_quads, w);
+                load(weight, weight_quads, a.norm.weight.nb[0], w);
+                weight += kRows * a.norm.weight.nb[2];
 #pragma unroll
                 for (int s = 0; s < SLOTS; ++s)
 #pragma unroll
@@ -211,9 +268,10 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
 #pragma unroll
                         for (int k = 0; k < 2; ++k) v[s][c][k] = __fmul_rn(v[s][c][k], __fadd_rn(w[s][c][k], a.norm.offset));
             }
-            if (a.norm.bias.data != nullptr) {
+            if (bias != nullptr) {
                 float w[SLOTS][4][2];
-                operand(a.norm.bias, bias_quads, w);
+                load(bias, bias_quads, a.norm.bias.nb[0], w);
+                bias += kRows * a.norm.bias.nb[2];
 #pragma unroll
                 for (int s = 0; s < SLOTS; ++s)
 #pragma unroll
@@ -225,17 +283,18 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
             for (int s = 0; s < SLOTS; ++s)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    if (!turned[s][c]) continue;
                     const float one = v[s][c][0], two = v[s][c][1], cosine = by[s][c].x, sine = by[s][c].y;
-                    v[s][c][0] = __builtin_fmaf(-two, sine, one * cosine);
-                    v[s][c][1] = __builtin_fmaf(one, sine, two * cosine);
+                    const float u = __builtin_fmaf(-two, sine, one * cosine), w = __builtin_fmaf(one, sine, two * cosine);
+                    // Not turned: as they are, whatever the other of the two is.
+                    v[s][c][0] = turned[s][c] ? u : one;
+                    v[s][c][1] = turned[s][c] ? w : two;
                 }
-            const int64_t to = i1 * a.ynb[1] + h * a.ynb[2] + i3 * a.ynb[3];
             if (a.half) {
                 store(static_cast<_Float16 *>(a.y) + to, v);
             } else {
                 store(static_cast<float *>(a.y) + to, v);
             }
+            to += kRows * a.ynb[2];
         }
     }
 }
