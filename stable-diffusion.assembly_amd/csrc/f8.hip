@@ -79,13 +79,13 @@ __device__ __forceinline__ int four(const float4v &v, float scale) {
     return __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * scale, v[3] * scale, r, true);
 }
 
-// A lane's eight numbers of a group as q in FP16, and the group's 2^e.  An infinity
-// makes them all NaN; a NaN stays one.
-__device__ __forceinline__ half8 held(const float4v &u, const float4v &v, float &power) {
+// A lane's eight numbers of a group as q, and the group's 2^e.  An infinity makes them
+// all NaN; a NaN stays one.
+__device__ __forceinline__ int2 held(const float4v &u, const float4v &v, float &power) {
     const uint32_t top = greatest(u, v), e = power_of(top);
     const float scale = top < kInfinity ? down(e) : __builtin_nanf("");
     power = up(e);
-    return widen(four(u, scale), four(v, scale));
+    return make_int2(four(u, scale), four(v, scale));
 }
 
 // Four of a row's K numbers from k on, of the last four there are where those end
@@ -150,14 +150,14 @@ __device__ __forceinline__ int4v ended_w(int4v v, int k, int K) {
 
 // ------------------------------------------------------------------ the work buffer
 
-// x's q in FP16 as rows of whole blocks, zeros past K, and its 2^e, [block][row];
-// the weights as rows of whole blocks, zeros past K, where the tiles need them so.
+// x's q by halves of a block, zeros past K: [half][row][64]; its 2^e, [block][row]; the
+// weights as rows of whole blocks, zeros past K, where the tiles need them so.
 struct F8Work {
-    _Float16 *q;
+    uint8_t *q;
     float *powers;
     uint8_t *w;
     int64_t ld;    // K rounded up to whole blocks
-    int64_t rows;  // of `powers`: M rounded up
+    int64_t rows;  // M rounded up to whole tiles
     size_t bytes;
 };
 
@@ -172,7 +172,7 @@ F8Work work_of(int64_t M, int64_t N, int64_t K, bool weights, void *work) {
         at += static_cast<size_t>(round_up(bytes, 256));
         return p != nullptr ? p + from : nullptr;
     };
-    w.q = reinterpret_cast<_Float16 *>(take(2 * M * w.ld));
+    w.q = reinterpret_cast<uint8_t *>(take(w.rows * w.ld));
     w.powers = reinterpret_cast<float *>(take(4 * w.rows * (w.ld / kF8Block)));
     if (weights) w.w = reinterpret_cast<uint8_t *>(take(N * w.ld));
     w.bytes = at;
@@ -184,8 +184,8 @@ constexpr int kOperandThreads = 256;
 struct OperandsArgs {
     F8Args a;
     F8Work w;
-    uint32_t blocks, groups;  // of K; of all of x
-    uint32_t x_grid;          // the workgroups that lay out x
+    uint32_t groups;  // of x
+    uint32_t x_grid;  // the workgroups that lay out x
 };
 
 // A group of x by 16 lanes, 8 numbers each; behind them the weights' rows, 16
@@ -203,13 +203,14 @@ __global__ __launch_bounds__(kOperandThreads) void f8_operands_kernel(OperandsAr
     }
     // The 16 lanes of a group together.
     for (uint32_t g = blockIdx.x * (kOperandThreads / 16) + threadIdx.x / 16; g < o.groups; g += o.x_grid * (kOperandThreads / 16)) {
-        const uint32_t m = g / o.blocks, b = g - m * o.blocks;
-        const int k = static_cast<int>(b) * kBlock + 8 * (threadIdx.x & 15), K = static_cast<int>(a.K);
+        const uint32_t rows = static_cast<uint32_t>(a.M), b = g / rows, m = g - b * rows, part = threadIdx.x & 15;
+        const int k = static_cast<int>(b) * kBlock + 8 * static_cast<int>(part), K = static_cast<int>(a.K);
         const float *row = a.x + m * a.ldx;
         const float4v u = ended_x(load_x(row, k, K), k, K), v = ended_x(load_x(row, k + 4, K), k + 4, K);
         float power;
-        *reinterpret_cast<half8 *>(o.w.q + m * o.w.ld + k) = held(u, v, power);
-        if ((threadIdx.x & 15) == 0) o.w.powers[b * o.w.rows + m] = power;
+        const int2 q = held(u, v, power);
+        *reinterpret_cast<int2 *>(o.w.q + ((2 * b + part / 8) * o.w.rows + m) * 64 + 8 * (part & 7)) = q;
+        if (part == 0) o.w.powers[b * o.w.rows + m] = power;
     }
 }
 
@@ -277,8 +278,8 @@ __global__ __launch_bounds__(kThreads, LOADS > 2 ? 2 : 4) void f8_few_kernel(Few
             x.v[u][1] = load4(from + 4);
         }
     };
-    const auto store_group = [&](int r, int b, const half8 &q, float power) {
-        *reinterpret_cast<half8 *>(lds + r * f.row + b * (2 * kBlock) + 16 * part) = q;
+    const auto store_group = [&](int r, int b, int2 q, float power) {
+        *reinterpret_cast<half8 *>(lds + r * f.row + b * (2 * kBlock) + 16 * part) = widen(q.x, q.y);
         if (part == 0) powers[r * f.chunk + b] = power;
     };
     const auto store_groups = [&](int count, int first, const Numbers &x) {
@@ -287,7 +288,7 @@ __global__ __launch_bounds__(kThreads, LOADS > 2 ? 2 : 4) void f8_few_kernel(Few
         for (int u = 0; u < LOADS; ++u) {
             const int g = first + 32 * u + team, r = row_of(g, inverse);
             float power;
-            const half8 q = held(x.v[u][0], x.v[u][1], power);
+            const int2 q = held(x.v[u][0], x.v[u][1], power);
             if (r < rows) store_group(r, g - r * count, q, power);
         }
     };
@@ -352,7 +353,7 @@ __global__ __launch_bounds__(kThreads, LOADS > 2 ? 2 : 4) void f8_few_kernel(Few
             const int k = (blocks - 1) * kBlock + 8 * part;
             const float *from = x_row_of(team);
             float power;
-            const half8 q = held(ended_x(load_x(from, k, K), k, K), ended_x(load_x(from, k + 4, K), k + 4, K), power);
+            const int2 q = held(ended_x(load_x(from, k, K), k, K), ended_x(load_x(from, k + 4, K), k + 4, K), power);
             store_group(team, whole, q, power);
         }
         lds_barrier();
@@ -459,23 +460,28 @@ hipError_t few_rows(const F8Args &a, hipStream_t stream) {
 // Both operands by tiles through LDS: a workgroup takes 64 WM rows of x by 64 WN
 // of the weights (with GATED 32 WN of each half), waves 64 x 64 of them each, and WK
 // blocks of K at a time, WK waves' sums joined at the end.  A stage is half a block
-// of each: 64 numbers of a row, and the block's powers and scales.  A lane's 16
-// bytes are at a place of their row that spreads 16 rows read at once over LDS's
-// banks; three stages are in LDS, one read and two under way.
+// of each, 64 numbers of a row, and the block's powers and scales.  Both are in LDS as
+// E4M3, widened by each wave that reads them: of x in FP16 there the copies and the
+// reads would be half as much again, and they weigh more than the vector operations
+// saved (4096 x 4096 -> 16384: 588 us against 554).  A lane's 16 bytes are at a place of their row
+// that spreads 16 rows read at once over LDS's banks.  kRing stages are in LDS, one
+// read and the others under way (four: 1976 x 1280 -> 10240 71.6 us against 69.0).
+constexpr int kRing = 3;
+
 template <int WM, int WN, int WK>
 struct Tiles {
     static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves * WK;
     static constexpr int kX = 64 * WM, kW = 64 * WN;  // rows of the tiles
-    static constexpr int kXBytes = 128 * kX, kWBytes = 64 * kW, kPowers = 4 * kX, kScales = 256;
+    static constexpr int kXBytes = 64 * kX, kWBytes = 64 * kW, kPowers = 4 * kX, kScales = 256;
     static constexpr int kPart = kXBytes + kWBytes + kPowers + kScales;  // of a block
     static constexpr int kStage = WK * kPart;
-    static constexpr int kXCopies = 8 * WM / kWaves, kWCopies = 4 * WN / kWaves;  // a wave's, of 1 KB
+    static constexpr int kXCopies = 4 * WM / kWaves, kWCopies = 4 * WN / kWaves;  // a wave's, of 1 KB
     static constexpr int kSmallCopies = (WM + 1 + kWaves - 1) / kWaves;          // and of 256 bytes
     static constexpr int kCopies = kXCopies + kWCopies + kSmallCopies;
-    static_assert(8 * WM % kWaves == 0 && 4 * WN % kWaves == 0);
+    static_assert(4 * WM % kWaves == 0 && 4 * WN % kWaves == 0);
     // WK waves' sums are joined in LDS.
     static constexpr int kSums = WK == 1 ? 0 : 16384 * kWaves * WK;
-    static constexpr int kLds = 3 * kStage > kSums ? 3 * kStage : kSums;
+    static constexpr int kLds = kRing * kStage > kSums ? kRing * kStage : kSums;
 };
 
 struct TilesArgs {
@@ -511,14 +517,15 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void f8_tiles_kernel(TilesArg
         const int n = GATED ? n0 + 32 * (r >> 6) + (r & 31) : n0 + r;
         return n < columns ? n : columns - 1;
     };
+    // 16 rows a copy, a row by 4 lanes, its 16 bytes in the order of their places in LDS.
     uint32_t x_offset[L::kXCopies], w_offset[L::kWCopies];
     const char *w_base[L::kWCopies];
-    const char *x_base = reinterpret_cast<const char *>(t.work.q + m0 * t.work.ld);
+    const char *x_base = reinterpret_cast<const char *>(t.work.q + m0 * 64);
+    const int64_t x_step = t.work.rows * 64;
 #pragma unroll
     for (int c = 0; c < L::kXCopies; ++c) {
-        const int r = 8 * (place + L::kWaves * c) + (lane >> 3);
-        const int64_t row = m0 + r < a.M ? r : a.M - 1 - m0;
-        x_offset[c] = static_cast<uint32_t>(2 * row * t.work.ld + 16 * ((lane & 7) ^ ((r >> 1) & 7)));
+        const int r = 16 * (place + L::kWaves * c) + (lane >> 2);
+        x_offset[c] = 64 * r + 16 * ((lane & 3) ^ ((r >> 2) & 3));
     }
 #pragma unroll
     for (int c = 0; c < L::kWCopies; ++c) {
@@ -553,39 +560,40 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void f8_tiles_kernel(TilesArg
         const int64_t k = static_cast<int64_t>(b) * kBlock + 64 * (s & 1);
         const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(part) + buffer * L::kStage);
 #pragma unroll
-        for (int c = 0; c < L::kXCopies; ++c) fetch16(x_base + 2 * k, x_offset[c], to + 1024 * (place + L::kWaves * c));
+        for (int c = 0; c < L::kXCopies; ++c) fetch16(x_base + (2 * b + (s & 1)) * x_step, x_offset[c], to + 1024 * (place + L::kWaves * c));
 #pragma unroll
         for (int c = 0; c < L::kWCopies; ++c) fetch16(w_base[c] + k, w_offset[c], to + L::kXBytes + 1024 * (place + L::kWaves * c));
 #pragma unroll
         for (int c = 0; c < L::kSmallCopies; ++c) fetch4(small[c] + b * small_step[c], to + small_to[c]);
     };
-    copy(0, 0);
-    copy(1, 1);
-    copy(2, 2);
+#pragma unroll
+    for (int s = 0; s < kRing; ++s) copy(s, s);
 
     float16v acc[4], p[4];  // tile k: rows of x 32 (k % 2) .., of the weights 32 (k / 2) ..
 #pragma unroll
     for (int k = 0; k < 4; ++k) acc[k] = p[k] = float16v{};
+    // Operand o is 32 rows of x (0, 1) or of the weights (2, 3): as they are in LDS, and
+    // as FP16 for two MFMAs.
     struct Operands {
-        half8 v[2][2], x[2][2];  // [32 rows][8 numbers]
-        int4v q[2];              // v before it is widened
+        int4v q[4];
+        half8 v[4][2];
     };
     // Rows of the tiles as the MFMA's lanes read them: of a quarter of a block.
-    const char *x_row = part + 128 * (64 * wm + col), *w_row = part + L::kXBytes + 64 * (64 * wn + col);
-    const int x_turn = (col >> 1) & 7, w_turn = (col >> 2) & 3;
+    const char *x_row = part + 64 * (64 * wm + col), *w_row = part + L::kXBytes + 64 * (64 * wn + col);
+    const int turn = (col >> 2) & 3;
     const auto read = [&](Operands &o, int buffer, int u) {
-        const char *xs = x_row + buffer * L::kStage, *ws = w_row + buffer * L::kStage;
+        const int at = buffer * L::kStage + 16 * ((2 * u + hf) ^ turn);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) o.q[j] = *reinterpret_cast<const int4v *>(ws + 64 * 32 * j + 16 * ((2 * u + hf) ^ w_turn));
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                o.x[i][h] = *reinterpret_cast<const half8 *>(xs + 128 * 32 * i + 16 * ((4 * u + 2 * hf + h) ^ x_turn));
+        for (int i = 0; i < 2; ++i) {
+            o.q[i] = *reinterpret_cast<const int4v *>(x_row + at + 64 * 32 * i);
+            o.q[2 + i] = *reinterpret_cast<const int4v *>(w_row + at + 64 * 32 * i);
+        }
     };
-    const auto widen_one = [&](Operands &o, int j) {
-        o.v[j][0] = widen(o.q[j][0], o.q[j][1]);
-        o.v[j][1] = widen(o.q[j][2], o.q[j][3]);
+    const auto widen_one = [&](Operands &o, int i) {
+        o.v[i][0] = widen(o.q[i][0], o.q[i][1]);
+        o.v[i][1] = widen(o.q[i][2], o.q[i][3]);
+        // Here, not where they are used.
+        asm volatile("" : "+v"(o.v[i][0]), "+v"(o.v[i][1]));
     };
     // A block's powers and scales; GATED: the second half's rows may lie in two
     // blocks of the scales, `across` of them in the first.
@@ -616,46 +624,48 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void f8_tiles_kernel(TilesArg
     // operands are read and widened; with `ends` a tile's sums are added while the
     // next tile's are made, the last one's with the first of the next quarter
     // (`kept`).
-    const auto quarter = [&](const Operands &now, Operands &next, int buffer, int u, auto begins_, auto kept_, auto ends_) {
-        constexpr bool begins = decltype(begins_)::value, kept = decltype(kept_)::value, ends = decltype(ends_)::value;
+    const auto quarter = [&](const Operands &now, Operands &next, int buffer, int u, auto begins, auto kept, auto ends) {
         read(next, buffer, u);
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int i = k & 1, j = k >> 1;
-            p[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now.v[j][0], now.x[i][0], begins ? float16v{} : p[k], 0, 0, 0);
-            p[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now.v[j][1], now.x[i][1], p[k], 0, 0, 0);
+        const auto tile = [&](auto tile_) {
+            constexpr int k = decltype(tile_)::value;
+            p[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now.v[2 + k / 2][0], now.v[k % 2][0], begins ? float16v{} : p[k], 0, 0, 0);
+            p[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now.v[2 + k / 2][1], now.v[k % 2][1], p[k], 0, 0, 0);
             if (k == 0 && kept) add(3);
             if (k > 0 && ends) add(k - 1);
-            if (k >= 2) {
-                widen_one(next, k - 2);
-                // Here, not where they are used.
-                asm volatile("" : "+v"(next.v[k - 2][0]), "+v"(next.v[k - 2][1]));
+            if (k == 1) widen_one(next, 0);
+            if (k == 2) {
+                widen_one(next, 2);
+                widen_one(next, 1);
             }
+            if (k == 3) widen_one(next, 3);
             // In this order: an MFMA and half of the other operations, twice.
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x002, ends ? 13 : 9, 0);
-            }
+            constexpr int others = (k == 0 ? decltype(kept)::value : decltype(ends)::value ? 1 : 0) * 17 + (k == 0 ? 0 : k == 2 ? 16 : 8);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, (others + 1) / 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, (others + 1) / 2, 0);
             __builtin_amdgcn_sched_barrier(0);
-        }
+        };
+        tile(std::integral_constant<int, 0>{});
+        tile(std::integral_constant<int, 1>{});
+        tile(std::integral_constant<int, 2>{});
+        tile(std::integral_constant<int, 3>{});
     };
-    const auto next = [](int b) { return b == 2 ? 0 : b + 1; };
     int buffer = 0;
-    fetched<2 * L::kCopies>();
+    fetched<(kRing - 1) * L::kCopies>();
     lds_barrier();
     Operands even, odd;
     read(even, 0, 0);
-    widen_one(even, 0);
-    widen_one(even, 1);
-    // Stage s is in registers or being read; the copies of s + 1 and s + 2 are under
-    // way, and once s is read those of s + 3 take its buffer.
+#pragma unroll
+    for (int i = 0; i < 4; ++i) widen_one(even, i);
+    // Stage s is in registers or being read; the copies of the kRing - 2 after it are
+    // under way, and once s is read those of the next take its buffer.
     const auto arrive = [&](int s) {
-        fetched<L::kCopies>();
+        fetched<(kRing - 2) * L::kCopies>();
         lds_barrier();  // every wave's copies of stage s + 1 are in, and stage s is read
-        copy(s + 3, buffer);
-        buffer = next(buffer);
+        copy(s + kRing, buffer);
+        buffer = buffer == kRing - 1 ? 0 : buffer + 1;
     };
     power[0] = power[1] = scale_of[0][0] = scale_of[0][1] = scale_of[1][0] = scale_of[1][1] = 0.0f;
     constexpr std::true_type yes{};
@@ -842,7 +852,7 @@ hipError_t lay_out(const F8Args &a, const F8Work &w, hipStream_t stream) {
     const auto most = [](int64_t n) { return n < (1 << 20) ? n : 1 << 20; };
     const int64_t blocks = w.ld / kF8Block, groups = blocks * a.M, x_grid = most(ceil_div(groups, kOperandThreads / 16));
     const int64_t w_grid = w.w != nullptr ? most(ceil_div(a.N * (w.ld / 16), kOperandThreads)) : 0;
-    const OperandsArgs o{a, w, static_cast<uint32_t>(blocks), static_cast<uint32_t>(groups), static_cast<uint32_t>(x_grid)};
+    const OperandsArgs o{a, w, static_cast<uint32_t>(groups), static_cast<uint32_t>(x_grid)};
     SDHIP_LAUNCH(f8_operands_kernel, dim3(static_cast<uint32_t>(x_grid + w_grid)), dim3(kOperandThreads), 0, stream, o);
     return hipGetLastError();
 }
