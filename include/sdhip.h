@@ -134,10 +134,9 @@ const char *sdhip_last_error(void);
  * weights by one of their forms -- each workgroup's rows of x split in it, x laid
  * out first, or both operands, tiles of 128 x 128 by four waves, by eight, of
  * 64 x 128, or, not the gated ones, of 64 x 192 -- whatever the size), f8_form (1
- * .. 6: those of 8-bit floating-point weights, each workgroup's rows of x brought to
- * E4M3 in it, x laid out first, or tiles of 128 x 128 by four waves, by eight, of 64
- * x 128, of 64 x 64),
- * attention_generic, attention_fp32 (forms to compare, same results within
+ * .. 5: those of 8-bit floating-point weights, each workgroup's 16 or 32 rows of x
+ * brought to E4M3 in it, or x laid out first, tiles of 128 x 128, of 64 x 128, of 64
+ * x 64), attention_generic, attention_fp32 (forms to compare, same results within
  * the bounds -- qgemm_core's bit for bit), each taking only its documented
  * values.  Returns SDHIP_ERROR
  * naming the first unknown name or refused value.  "" resets the defaults. */
@@ -240,10 +239,11 @@ sdhip_status sdhip_mul_mat_gated(const sdhip_tensor *w, const sdhip_tensor *x, c
  * NaN in x makes its row's outputs NaN, a NaN in w its column's.
  * What bits asks for is left aside.  The output shares no byte with w, scales or
  * x.  Up to 2^25 rows of x and 2^25 of w, 2^36 weights, 2^35 outputs and 2^37
- * numbers of x are taken.  The work buffer, none up to 16 rows: x as its q and e
- * and, where many rows read them and they do not lie at multiples of 16 bytes in
- * rows of whole blocks, the weights; calls that may run at once take a buffer
- * each. */
+ * numbers of x are taken.  The work buffer, none where few rows read the
+ * weights: x as its q and e and, where they do not lie at multiples of 16 bytes in
+ * rows of whole blocks, the weights; calls that may run at once take a buffer each.
+ * Its size follows the f8_form tuning, which is to be the same when the size is
+ * asked for and when the product is made. */
 int sdhip_mul_mat_f8_supported(const sdhip_tensor *w, const sdhip_tensor *scales, const sdhip_tensor *x,
                                const sdhip_tensor *y);
 size_t sdhip_mul_mat_f8_work_size(const sdhip_tensor *w, const sdhip_tensor *scales, const sdhip_tensor *x,
@@ -358,8 +358,8 @@ sdhip_status sdhip_group_norm_static(const sdhip_tensor *x, const sdhip_tensor *
  * pixels any multiple of 4 bytes apart, nb[2] = W nb[1], images any multiple of
  * 4 (so channels of a wider tensor); `groups` groups of ceil(C / groups)
  * channels over ne[0], per image ne[3].  Up to 2^24 channels, 2^31 - 1 pixels of
- * an image and as many images, 2^40 numbers in all are taken.  Statistics and differences are taken in double, each number rounded once
- * before the chain.  y may be x's own memory in the same layout; else
+ * an image and as many images, 2^40 numbers in all are taken.  The statistics are
+ * taken in double.  y may be x's own memory in the same layout; else
  * it shares no byte range with x, nor do two of its pixels: SDHIP_UNSUPPORTED.
  * No redirect.  The work buffer holds the partial sums of stretches of an
  * image's pixels, 0 where a group is small enough for one launch. */

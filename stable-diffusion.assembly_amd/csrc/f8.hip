@@ -825,27 +825,56 @@ hipError_t launch_tiles(TilesArgs t, hipStream_t stream) {
 // ------------------------------------------------------------------ the choice
 
 // Which kernels a product takes, numbered as the f8_form tuning asks for them: the
-// rows' kernel with x as it is or laid out, or tiles of 128 x 128 by four waves, by
-// eight, of 64 x 128 by four, of 64 x 64 by four.
-enum class Form { few = 1, rows, tiles4, tiles8, tiles64, tiles64x64 };
+// few rows' kernel by 16 rows or by 32, or tiles of 128 x 128, of 64 x 128 by two
+// waves' halves of K, of 64 x 64 by four's quarters.
+enum class Form { few = 1, rows, tiles, tiles64, tiles64x64 };
 
-// The tiles' copies reach 128 rows of x by 32 bits of offset.
+// Tiles' copies reach 128 rows of the weights by 32 bits of offset.
 constexpr int64_t kTilesK = int64_t{1} << 22;
 
-Form form_of(int64_t M, int64_t N, int64_t K) {
-    const int asked = tuning().f8_form;
-    // The rows' kernel takes a wave for 16 x 16 outputs, of the 2^26 a launch counts.
-    const bool fits = (M / 16 + 1) * (N / 16 + 8) < (int64_t{1} << 25);
-    if (asked > 0 && (asked <= 2 ? fits : K <= kTilesK)) return static_cast<Form>(asked);
-    if (M <= 48) return Form::few;
-    if (M <= 160 || K > kTilesK) return Form::rows;
-    const int64_t tiles = ceil_div(M, 128) * ceil_div(N, 128);
-    if (tiles >= 384) return Form::tiles4;
-    if (tiles >= 128) return Form::tiles8;
-    return ceil_div(M, 64) * ceil_div(N, 128) >= 60 ? Form::tiles64 : Form::tiles64x64;
+// Microseconds of the few rows' kernel by 16 RM rows: a launch and, for each round of
+// workgroups over the CUs, its blocks of the weights and all of its rows' x.
+double few_time(int64_t M, int64_t columns, int64_t K, int rm, int halves) {
+    const int splits = few_splits(M, columns, K, 16 * rm, halves);
+    const int64_t blocks = ceil_div(K, kF8Block), groups = ceil_div(columns, 16 * (kWaves / splits / halves)) * ceil_div(M, 16 * rm);
+    const double rounds = static_cast<double>(ceil_div(groups, compute_units()));
+    const double own = static_cast<double>(ceil_div(blocks, splits)), all = static_cast<double>(blocks);
+    return rm == 1 ? 4.0 + rounds * (0.4 + 0.55 * own + 0.08 * all) : 4.4 + rounds * (0.8 + 0.6 * own + 0.2 * all);
 }
 
-bool tiles(Form form) { return form != Form::few && form != Form::rows; }
+// Tiles, the smallest of which there are no more than CUs, else the largest: of 1280
+// columns and K 1280, us by 64 x 64 | 64 x 128 | 128 x 128: 768 rows 13.8 | 14.8 | 18.9,
+// 1024 20.9 | 15.3 | 19.6, 8192 94 | 56 | 50.  Or a kernel of few rows, where that takes
+// less by the times of a launch fitted to 28 such shapes, of 1 to 8192 rows (the rule
+// is 1% slower than the best choice in the mean, 36% at most): of K 640 to 640 columns
+// by 16 rows | 32 | tiles: 160 rows 5.3 | 6.4 | 10.3, 384 7.3 | 6.7 | 10.5, 1536 - | 13.0 |
+// 11.9; of K 4096 to 4096 columns 32 rows 14.0 | 15.8 | -, 64 17.7 | 19.4 | 17.6.
+Form form_of(int64_t M, int64_t N, int64_t K, bool gated) {
+    const int halves = gated ? 2 : 1, asked = tuning().f8_form;
+    const int64_t columns = N / halves;
+    // The few rows' kernel takes a wave for 16 x 16 outputs, of the 2^26 a launch counts.
+    const bool fits = (M / 16 + 1) * (N / 16 + 8) < (int64_t{1} << 25);
+    if (asked > 0 && (asked <= 2 ? fits : K <= kTilesK)) return static_cast<Form>(asked);
+    const double blocks = static_cast<double>(ceil_div(K, kF8Block));
+    const auto tiles = [&](int64_t x, int64_t w) { return ceil_div(M, x) * ceil_div(columns, w / halves); };
+    Form form = Form::tiles;
+    double least = 8.2 + 1e-6 * static_cast<double>(M) * static_cast<double>(K);  // x is laid out
+    if (tiles(64, 64) <= compute_units()) {
+        form = Form::tiles64x64;
+        least += 0.3 * blocks;
+    } else if (tiles(64, 128) <= compute_units()) {
+        form = Form::tiles64;
+        least += 0.5 * blocks;
+    } else {
+        least += 0.9 * blocks * static_cast<double>(ceil_div(tiles(128, 128), 2 * compute_units()));
+    }
+    if (!fits) return form;
+    const double few = few_time(M, columns, K, 1, halves), rows = few_time(M, columns, K, 2, halves);
+    if (K <= kTilesK && least <= few && least <= rows) return form;
+    return few <= rows ? Form::few : Form::rows;
+}
+
+bool by_tiles(Form form) { return form != Form::few && form != Form::rows; }
 
 hipError_t lay_out(const F8Args &a, const F8Work &w, hipStream_t stream) {
     // 2^20 workgroups of each at most, of the 2^32 threads that a launch counts.
@@ -859,29 +888,28 @@ hipError_t lay_out(const F8Args &a, const F8Work &w, hipStream_t stream) {
 
 template <bool GATED>
 hipError_t launch_form(const F8Args &a, bool whole, void *work, hipStream_t stream) {
-    const Form form = form_of(a.M, a.N, a.K);
+    const Form form = form_of(a.M, a.N, a.K, GATED);
     if (form == Form::few) return few_rows<GATED, 1>(a, stream);
     if (form == Form::rows) return few_rows<GATED, 2>(a, stream);
     const F8Work w = work_of(a.M, a.N, a.K, !whole, work);
     if (const hipError_t e = lay_out(a, w, stream); e != hipSuccess) return e;
     const TilesArgs t{a, w, whole ? a.w : w.w, whole ? a.row_bytes : w.ld, 0, 0};
     switch (form) {
-    case Form::tiles4:
-        return launch_tiles<GATED, 2, 2, 1>(t, stream);
-    case Form::tiles8:
-        return launch_tiles<GATED, 2, 2, 2>(t, stream);
     case Form::tiles64:
         return launch_tiles<GATED, 1, 2, 2>(t, stream);
-    default:
+    case Form::tiles64x64:
         return launch_tiles<GATED, 1, 1, 4>(t, stream);
+    default:
+        return launch_tiles<GATED, 2, 2, 1>(t, stream);
     }
 }
 
 }  // namespace
 
 size_t f8_work_size(int64_t M, int64_t N, int64_t K, bool whole) {
-    const Form form = form_of(M, N, K);
-    return tiles(form) ? work_of(M, N, K, !whole, nullptr).bytes : 0;
+    // Enough for the product and for the gated one.
+    const bool tiles = by_tiles(form_of(M, N, K, false)) || (N % 2 == 0 && by_tiles(form_of(M, N, K, true)));
+    return tiles ? work_of(M, N, K, !whole, nullptr).bytes : 0;
 }
 
 hipError_t launch_f8_mul_mat(const F8Args &a, bool whole, void *work, hipStream_t stream) {

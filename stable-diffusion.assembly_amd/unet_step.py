@@ -5,7 +5,8 @@ SD1.5's UNet at 512x512 (latent 64x64, batch 2 for classifier-free guidance,
 a 77-token context of 768), random-initialised weights of that architecture
 (FP16 conv and linear weights ~N(0, 0.02), as the reference's tests fill
 them; the linear layers' in ggml's 4-bit blocks where the model is made with
-weights="q4_0" or "q4_1"), with every node the reference takes over from ggml -- CONV_2D,
+weights="q4_0" or "q4_1", or in E4M3 with block scales where it is made with
+"f8"), with every node the reference takes over from ggml -- CONV_2D,
 MUL_MAT, the gated GEGLU product, FLASH_ATTN_EXT, GROUP_NORM, NORM and the
 chains after them -- run by libsdhip.  The nodes the reference does not take
 (ggml computes them: nearest upsampling, concatenation, the permutes between
@@ -62,13 +63,63 @@ def quantize(w, kind):
     return torch.cat([h.half().contiguous().view(torch.uint8) for h in heads] + [nibbles], dim=-1).contiguous()
 
 
+class BlockScaled:
+    """Weights [n, k] in E4M3 (`values`) with a scale (`scales`) for each 128 x 128 of
+    them."""
+
+    def __init__(self, values, scales):
+        self.values, self.scales = values, scales
+
+    shape = property(lambda self: self.values.shape)
+    dtype = property(lambda self: self.values.dtype)
+    device = property(lambda self: self.values.device)
+
+    def to(self, device):
+        return BlockScaled(self.values.to(device), self.scales.to(device))
+
+
+def _tiles(w):
+    """[n, k], zeros past its ends, as [n / 128, 128, k / 128, 128]."""
+    n, k = w.shape
+    b = sdhip.F8_BLOCK
+    return F.pad(w, (0, -k % b, 0, -n % b)).reshape(-(-n // b), b, -(-k // b), b)
+
+
+def scaled(w):
+    """Weights [n, k] as BlockScaled: a block's furthest number is E4M3's, 448."""
+    n, k = w.shape
+    if w.device.type == "meta":
+        return BlockScaled(w.to(torch.float8_e4m3fn), torch.empty((-(-n // 128), -(-k // 128)), device="meta"))
+    t = _tiles(w.float())
+    top = t.abs().amax(dim=(1, 3), keepdim=True) / 448.0
+    scales = torch.where(top > 0, top, torch.ones_like(top))
+    q = (t / scales).clamp(-448.0, 448.0).reshape(t.shape[0] * t.shape[1], -1)[:n, :k]
+    return BlockScaled(q.contiguous().to(torch.float8_e4m3fn), scales[:, 0, :, 0].contiguous())
+
+
+def held(x):
+    """Rows of x as the products of E4M3 weights take them: each 128 of a row as q 2^e,
+    q in E4M3 and e the least integer, -101 at least, that holds the greatest."""
+    k = x.shape[-1]
+    g = F.pad(x, (0, -k % 128)).unflatten(-1, (-1, 128))
+    m, e = torch.frexp(g.abs().amax(dim=-1, keepdim=True))  # top = m 2^e, 1/2 <= m < 1; 448 = 7/8 2^9
+    step = torch.exp2((e - 9 + (m > 0.875).to(e.dtype)).clamp(min=-101).to(x.dtype))
+    # E4M3's step at a number: 2^-3 of its power of two, which is 2^-6 at least.
+    fine = step * torch.exp2((torch.frexp(g / step)[1] - 1).clamp(min=-6).to(x.dtype) - 3)
+    q = (g / fine).round() * fine
+    return q.flatten(-2)[..., :k].contiguous()
+
+
 def extents(w):
-    """(n, k) of a linear layer's weights, FP16 [n, k] or 4-bit blocks."""
+    """(n, k) of a linear layer's weights: FP16 [n, k], 4-bit blocks or BlockScaled."""
     return (w.shape[0], w.shape[1] * sdhip.BLOCK) if w.dtype == torch.uint8 else tuple(w.shape)
 
 
 def widen(w, dtype):
     """A linear layer's weights [n, k] as numbers of `dtype`."""
+    if isinstance(w, BlockScaled):
+        n, k = w.shape
+        return (_tiles(w.values.to(dtype)) * w.scales.to(dtype)[:, None, :, None]).flatten(0, 1).flatten(1)[:n, :k]
     if w.dtype != torch.uint8:
         return w.to(dtype)
     n, k = extents(w)
@@ -199,7 +250,7 @@ class HipOps(Ops):
         n, k = extents(w)
         m = x.numel() // k
         self.count_linear(x, w)
-        if m < 16 and w.dtype != torch.uint8:
+        if m < 16 and w.dtype == torch.float16:
             # Not taken by the reference (mul_mat.cc:181-194): ggml's node,
             # with the weights widened once and kept, as ggml's CPU backend
             # reads them without converting the tensor each time.
@@ -215,12 +266,26 @@ class HipOps(Ops):
         y = torch.empty((*x.shape[:-1], n), device=x.device)
         steps = ([("add", bias)] if bias is not None else []) + [("add", a) for a in add]
         chain = self._chain(steps)
+        if isinstance(w, BlockScaled):
+            return self._product_f8(w, x, y, chain if steps else None)
         dw, dx, dy = sdhip.desc(w), sdhip.desc(x), sdhip.desc(y)
         size = self.lib.sdhip_mul_mat_work_size(dw, dx, dy)
         ptr, sz = self._work(size)
         sdhip.check(self.lib.sdhip_mul_mat(dw, dx, dy, ctypes.byref(chain) if steps else None, ptr, sz,
                                            sdhip.stream_handle()), f"mul_mat {m}x{n}x{k}")
         return y
+
+    def _product_f8(self, w, x, y, chain, out=None):
+        """`y`, or with `out` the gated product's output."""
+        operands = [sdhip.desc(t) for t in (w.values, w.scales, x, y)]
+        ptr, sz = self._work(self.lib.sdhip_mul_mat_f8_work_size(*operands))
+        chain = ctypes.byref(chain) if chain is not None else None
+        what = f"mul_mat_f8 {tuple(x.shape)} -> {w.shape[0]}"
+        if out is None:
+            sdhip.check(self.lib.sdhip_mul_mat_f8(*operands, chain, ptr, sz, sdhip.stream_handle()), what)
+            return y
+        sdhip.check(self.lib.sdhip_mul_mat_f8_gated(*operands, chain, sdhip.desc(out), ptr, sz, sdhip.stream_handle()), what)
+        return out
 
     def geglu(self, x, w, bias):
         n, k = extents(w)
@@ -229,6 +294,8 @@ class HipOps(Ops):
         y = torch.empty((*x.shape[:-1], n), device=x.device)  # described, never written
         out = torch.empty((*x.shape[:-1], n // 2), device=x.device)
         chain = self._chain([("add", bias)])
+        if isinstance(w, BlockScaled):
+            return self._product_f8(w, x, y, chain, out)
         dw, dx, dy, do = sdhip.desc(w), sdhip.desc(x), sdhip.desc(y), sdhip.desc(out)
         size = self.lib.sdhip_mul_mat_work_size(dw, dx, dy)
         ptr, sz = self._work(size)
@@ -281,7 +348,7 @@ class TorchOps(Ops):
 
     def linear(self, x, w, bias=None, add=()):
         self.count_linear(x, w)
-        y = x @ widen(w, self.dtype).t()
+        y = (held(x) if isinstance(w, BlockScaled) else x) @ widen(w, self.dtype).t()
         if bias is not None:
             y = y + bias.to(self.dtype)
         for a in add:
@@ -319,7 +386,8 @@ class Model:
     """SD1.5's UNet with random weights: FP16 weight tensors ~N(0, 0.02),
     biases ~N(0, 0.01), norm scales ~N(1, 0.1) and shifts ~N(0, 0.1).  With
     weights "q4_0" or "q4_1" the linear layers' are those numbers in 4-bit
-    blocks, where a row is of whole blocks."""
+    blocks, where a row is of whole blocks, with "f8" in E4M3 with a scale for
+    each 128 x 128."""
 
     def __init__(self, cfg, device, seed=0, weights="f16"):
         self.cfg = cfg
@@ -375,6 +443,8 @@ class Model:
 
     def _linear_w(self, n, k):
         w = self._w(n, k)
+        if self.weights == "f8":
+            return scaled(w)
         return w if self.weights == "f16" or k % sdhip.BLOCK else quantize(w, self.weights)
 
     def _lin(self, n, k, bias=True):
@@ -387,7 +457,10 @@ class Model:
         return (self._randn(c, std=0.1, mean=1.0), self._randn(c, std=0.1))
 
     def _res(self, ic, oc):
-        return {"norm1": self._norm(ic), "conv1": self._conv(oc, ic, 3), "emb": self._lin(oc, self.cfg.time_dim),
+        # Weights of 8 bits are made of all blocks' projections at once: a scale may span two blocks' rows.
+        td = self.cfg.time_dim
+        emb = (self._w(oc, td), self._randn(oc, std=0.01)) if self.weights == "f8" else self._lin(oc, td)
+        return {"norm1": self._norm(ic), "conv1": self._conv(oc, ic, 3), "emb": emb,
                 "norm2": self._norm(oc), "conv2": self._conv(oc, oc, 3),
                 "skip": self._conv(oc, ic, 1) if ic != oc else None}
 
@@ -420,7 +493,8 @@ class Model:
             at += w.shape[0]
             ws.append(w)
             bs.append(b)
-        self.emb_all = (torch.cat(ws), torch.cat(bs))
+        w = torch.cat(ws)
+        self.emb_all = (scaled(w) if self.weights == "f8" else w, torch.cat(bs))
 
     # -- blocks
 
@@ -507,7 +581,7 @@ class Model:
         ref.device = device
 
         def move(o):
-            if isinstance(o, torch.Tensor):
+            if isinstance(o, (torch.Tensor, BlockScaled)):
                 return o.to(device)
             if isinstance(o, dict):
                 return {k: move(v) for k, v in o.items()}
@@ -565,7 +639,7 @@ class SdxlBlock:
     projection with its bias and the residual, LayerNorm, the GEGLU FF
     (C -> 2 x 4C with bias, gated) and its projection back with bias and the
     residual; FP16 weights ~N(0, 0.02), or those in 4-bit blocks (weights "q4_0"
-    or "q4_1"), biases ~N(0, 0.01), norms ~N(1, 0.1) / ~N(0, 0.1).
+    or "q4_1") or in E4M3 with block scales ("f8"), biases ~N(0, 0.01), norms ~N(1, 0.1) / ~N(0, 0.1).
     `forward(ops, x)` for tokens x [b, L, C]."""
 
     def __init__(self, device, channels=1280, heads=20, seed=0, weights="f16"):

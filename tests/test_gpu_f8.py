@@ -66,7 +66,7 @@ def run(gpu, rows, k, n, seed, steps=(), layout=(None, 0), x=None, apart=0, w=No
     return y.check(), *f8_lib.exact(bytes_, scales, x)
 
 
-FORMS = [0, 1, 2, 3, 4, 5, 6]
+FORMS = [0, 1, 2, 3, 4, 5]
 
 
 @pytest.fixture(params=FORMS)
@@ -364,15 +364,19 @@ def test_several_streams_at_once(gpu):
 
 @pytest.mark.gpu
 def test_work_buffer_checked(gpu):
-    lib = sdhip.load()
-    w, s = weights(np.zeros((64, 256), np.uint8), gpu), torch.ones((1, 2), device=gpu)
-    x, y = torch.zeros((100, 256), device=gpu), unwritten((100, 64), gpu)
-    d = [sdhip.desc(t) for t in (w, s, x, y)]
-    size = lib.sdhip_mul_mat_f8_work_size(*d)
-    assert size > 0
-    buf = torch.zeros(size + 16, dtype=torch.uint8, device=gpu)
-    for ptr, n in ((None, size), (buf.data_ptr(), size - 1), (buf.data_ptr() + 8, size)):
-        assert lib.sdhip_mul_mat_f8(*d, None, ptr, n, sdhip.stream_handle()) == sdhip.ERROR
-    sdhip.check(lib.sdhip_mul_mat_f8(*d, None, ctypes.c_void_p(buf.data_ptr()), size, sdhip.stream_handle()), "mul_mat_f8")
-    torch.cuda.synchronize()
-    assert (y == 0).all()
+    sdhip.set_tuning("f8_form=3")  # whose x is laid out
+    try:
+        lib = sdhip.load()
+        w, s = weights(np.zeros((64, 256), np.uint8), gpu), torch.ones((1, 2), device=gpu)
+        x, y = torch.zeros((100, 256), device=gpu), unwritten((100, 64), gpu)
+        d = [sdhip.desc(t) for t in (w, s, x, y)]
+        size = lib.sdhip_mul_mat_f8_work_size(*d)
+        assert size > 0
+        buf = torch.zeros(size + 16, dtype=torch.uint8, device=gpu)
+        for ptr, n in ((None, size), (buf.data_ptr(), size - 1), (buf.data_ptr() + 8, size)):
+            assert lib.sdhip_mul_mat_f8(*d, None, ptr, n, sdhip.stream_handle()) == sdhip.ERROR
+        sdhip.check(lib.sdhip_mul_mat_f8(*d, None, ctypes.c_void_p(buf.data_ptr()), size, sdhip.stream_handle()), "mul_mat_f8")
+        torch.cuda.synchronize()
+        assert (y == 0).all()
+    finally:
+        sdhip.set_tuning("")

@@ -61,6 +61,24 @@ def test_products_taken(m, k, n):
                                                     rows(m, n // 2, data=1 << 42))
 
 
+def test_forms_of_the_products():
+    """f8_form takes the forms there are, and the work buffer follows it."""
+    lib = sdhip.load()
+    d = weights(320, 512), rows(3, 4, data=2 * FAKE), rows(40, 512, data=4 * FAKE), rows(40, 320, data=16 * FAKE)
+    try:
+        sizes = []
+        for form in range(6):
+            sdhip.set_tuning(f"f8_form={form}")
+            sizes.append(lib.sdhip_mul_mat_f8_work_size(*d))
+        # None for the forms of few rows, x's numbers and powers of whole tiles for the others.
+        assert sizes[1] == sizes[2] == 0 and sizes[3] == sizes[4] == sizes[5] >= 128 * (512 + 4 * 4)
+        for wrong in ("-1", "6", "x"):
+            with pytest.raises(Exception):
+                sdhip.set_tuning(f"f8_form={wrong}")
+    finally:
+        sdhip.set_tuning("")
+
+
 def test_products_of_matrices_taken():
     assert taken(weights(70, 320), scales(70, 320), rows(2, 3, 4, 320), rows(2, 3, 4, 70))
 
@@ -109,12 +127,16 @@ def test_products_that_are_errors():
         d = {"w": w, "s": s, "x": x}[name]
         assert call(**{name: changed(d, "data", 0, None)}) == sdhip.ERROR
     assert call(y=rows(4, 320, data=None)) == sdhip.ERROR
-    many = rows(4000, 320), rows(4000, 320, data=1 << 40)
-    assert lib.sdhip_mul_mat_f8(w, s, *many, None, None, 0, None) == sdhip.ERROR
-    assert b"work" in lib.sdhip_last_error()
-    size = lib.sdhip_mul_mat_f8_work_size(w, s, *many)
-    for ptr, n in ((1 << 44, size - 1), ((1 << 44) + 8, size)):
-        assert lib.sdhip_mul_mat_f8(w, s, *many, None, ptr, n, None) == sdhip.ERROR
+    sdhip.set_tuning("f8_form=3")  # whose x is laid out
+    try:
+        many = rows(4000, 320), rows(4000, 320, data=1 << 40)
+        assert lib.sdhip_mul_mat_f8(w, s, *many, None, None, 0, None) == sdhip.ERROR
+        assert b"work" in lib.sdhip_last_error()
+        size = lib.sdhip_mul_mat_f8_work_size(w, s, *many)
+        for ptr, n in ((1 << 44, size - 1), ((1 << 44) + 8, size)):
+            assert lib.sdhip_mul_mat_f8(w, s, *many, None, ptr, n, None) == sdhip.ERROR
+    finally:
+        sdhip.set_tuning("")
 
 
 def test_extents_that_a_launch_counts():
