@@ -184,12 +184,14 @@ constexpr int kOperandThreads = 256;
 struct OperandsArgs {
     F8Args a;
     F8Work w;
-    uint32_t groups;  // of x
-    uint32_t x_grid;  // the workgroups that lay out x
+    uint32_t across, tiles;  // tiles of x: along K, and all
+    uint32_t x_grid;         // the workgroups that lay out x
 };
 
-// A group of x by 16 lanes, 8 numbers each; behind them the weights' rows, 16
-// numbers a lane.
+// Tiles of 4 rows of x by 4 blocks of K, a group by 16 lanes, 8 numbers each: pieces of
+// 2 KB read and 256 bytes written (16 rows by a block: 4096 x 4096 28 us, so
+// 19; 1976 x 5120 10.5 both ways).
+// Behind them the weights' rows, 16 numbers a lane.
 __global__ __launch_bounds__(kOperandThreads) void f8_operands_kernel(OperandsArgs o) {
     const F8Args &a = o.a;
     if (blockIdx.x >= o.x_grid) {
@@ -201,9 +203,11 @@ __global__ __launch_bounds__(kOperandThreads) void f8_operands_kernel(OperandsAr
         }
         return;
     }
-    // The 16 lanes of a group together.
-    for (uint32_t g = blockIdx.x * (kOperandThreads / 16) + threadIdx.x / 16; g < o.groups; g += o.x_grid * (kOperandThreads / 16)) {
-        const uint32_t rows = static_cast<uint32_t>(a.M), b = g / rows, m = g - b * rows, part = threadIdx.x & 15;
+    const uint32_t team = threadIdx.x / 16, part = threadIdx.x & 15, blocks = static_cast<uint32_t>(o.w.ld / kBlock);
+    for (uint32_t g = blockIdx.x; g < o.tiles; g += o.x_grid) {
+        const uint32_t down = g / o.across;
+        const int64_t m = 4 * static_cast<int64_t>(down) + team / 4, b = 4 * (g - down * o.across) + team % 4;
+        if (m >= a.M || b >= blocks) continue;  // the 16 lanes of a group together
         const int k = static_cast<int>(b) * kBlock + 8 * static_cast<int>(part), K = static_cast<int>(a.K);
         const float *row = a.x + m * a.ldx;
         const float4v u = ended_x(load_x(row, k, K), k, K), v = ended_x(load_x(row, k + 4, K), k + 4, K);
@@ -227,18 +231,20 @@ struct FewArgs {
     uint32_t column_blocks;
 };
 
-// A workgroup takes 16 RM rows of x and kWaves / splits tiles of 16 rows of the
-// weights (with GATED half of them of each half), a wave a tile and every splits-th
-// block of K.  x is brought to E4M3 in it, a group by 16 lanes, and kept in LDS in FP16 with
-// the groups' powers, by chunks of K where it is long; the weights come straight from
-// memory into registers, kAhead blocks of a wave's under way, 64 bytes of a row side
-// by side in a load.  The splits' sums are joined in LDS.
-// A wave's blocks under way: with few of x's groups loaded together as many as 128
-// registers hold, for two workgroups a CU; with many, for one.
+// A wave's blocks of the weights under way: as many as 128 registers hold, for two
+// workgroups a CU.
 constexpr int few_ahead(int rm) { return rm > 1 ? 2 : 3; }
 
-// LOADS groups of x a team of 16 lanes has under way.  TAIL: K ends within a block,
-// which is taken apart from the whole ones.
+// A workgroup takes 16 RM rows of x and kWaves / splits tiles of 16 rows of the
+// weights (with GATED half of them of each half), a wave a tile and every splits-th
+// block of K.  x is brought to E4M3 in it, a group by 16 lanes, LOADS of them under
+// way, and kept in LDS in FP16 with the groups' powers, by chunks of K where it is
+// long; the weights come straight from memory into registers, few_ahead blocks of a
+// wave's under way, 64 bytes of a row side by side in a load.  The splits' sums are
+// joined in LDS.  TAIL: K ends within a block, which is taken apart from the whole ones.
+// Of 1 x 4096 -> 16384 the weights' bytes are the bound (14.5 us, 4.6 TB/s); at 1280 ->
+// 1280 (4.4 us) the launch and what waits for one another: x, its greatest, a barrier,
+// the products and the splits' sums.
 template <bool GATED, bool TAIL, int RM, int LOADS>
 __global__ __launch_bounds__(kThreads, LOADS > 2 ? 2 : 4) void f8_few_kernel(FewArgs f) {
     const F8Args &a = f.a;
@@ -463,9 +469,15 @@ hipError_t few_rows(const F8Args &a, hipStream_t stream) {
 // of each, 64 numbers of a row, and the block's powers and scales.  Both are in LDS as
 // E4M3, widened by each wave that reads them: of x in FP16 there the copies and the
 // reads would be half as much again, and they weigh more than the vector operations
-// saved (4096 x 4096 -> 16384: 588 us against 554).  A lane's 16 bytes are at a place of their row
-// that spreads 16 rows read at once over LDS's banks.  kRing stages are in LDS, one
+// saved (4096 x 4096 -> 16384: 588 us against 554).  A lane's 16 bytes are at a place
+// of their row that spreads 16 rows read at once over LDS's banks.  kRing stages are in LDS, one
 // read and the others under way (four: 1976 x 1280 -> 10240 71.6 us against 69.0).
+//
+// 4096 x 4096 -> 16384 takes 550 us, 1.0 PFLOP/s, where a library's product of FP16
+// takes 460: its MFMAs are busy 82% of the cycles at the 1.55 GHz that the card then
+// runs, these 55% at 1.76, with 7.4 other vector operations a MFMA (4 that widen, 2 that
+// add a block's sums) on the same ports, LDS read or written 75% of the MFMAs' time.
+// Whole rounds of tiles are the rest: 1976 x 5120 -> 1280 has 160 for 256 CUs.
 constexpr int kRing = 3;
 
 template <int WM, int WN, int WK>
@@ -879,9 +891,9 @@ bool by_tiles(Form form) { return form != Form::few && form != Form::rows; }
 hipError_t lay_out(const F8Args &a, const F8Work &w, hipStream_t stream) {
     // 2^20 workgroups of each at most, of the 2^32 threads that a launch counts.
     const auto most = [](int64_t n) { return n < (1 << 20) ? n : 1 << 20; };
-    const int64_t blocks = w.ld / kF8Block, groups = blocks * a.M, x_grid = most(ceil_div(groups, kOperandThreads / 16));
+    const int64_t across = ceil_div(w.ld / kF8Block, 4), tiles = across * ceil_div(a.M, 4), x_grid = most(tiles);
     const int64_t w_grid = w.w != nullptr ? most(ceil_div(a.N * (w.ld / 16), kOperandThreads)) : 0;
-    const OperandsArgs o{a, w, static_cast<uint32_t>(groups), static_cast<uint32_t>(x_grid)};
+    const OperandsArgs o{a, w, static_cast<uint32_t>(across), static_cast<uint32_t>(tiles), static_cast<uint32_t>(x_grid)};
     SDHIP_LAUNCH(f8_operands_kernel, dim3(static_cast<uint32_t>(x_grid + w_grid)), dim3(kOperandThreads), 0, stream, o);
     return hipGetLastError();
 }
