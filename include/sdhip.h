@@ -134,9 +134,9 @@ const char *sdhip_last_error(void);
  * weights by one of their forms -- each workgroup's rows of x split in it, x laid
  * out first, or both operands, tiles of 128 x 128 by four waves, by eight, of
  * 64 x 128, or, not the gated ones, of 64 x 192 -- whatever the size), f8_form (1
- * .. 5: those of 8-bit floating-point weights, each workgroup's 16 or 32 rows of x
- * brought to E4M3 in it, or x laid out first, tiles of 128 x 128, of 64 x 128, of 64
- * x 64), attention_generic, attention_fp32 (forms to compare, same results within
+ * .. 6: those of 8-bit floating-point weights, each workgroup's 16 or 32 rows of x
+ * brought to E4M3 in it, or x laid out first, tiles of 128 x 128 by four waves, by
+ * eight, of 64 x 128, of 64 x 64), attention_generic, attention_fp32 (forms to compare, same results within
  * the bounds -- qgemm_core's bit for bit), each taking only its documented
  * values.  Returns SDHIP_ERROR
  * naming the first unknown name or refused value.  "" resets the defaults. */

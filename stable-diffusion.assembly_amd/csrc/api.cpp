@@ -67,7 +67,7 @@ namespace {
 // names take any integer, as its parser does (cpu.cc:180-212), and clamp or
 // read them as it does (quant.cc:53-67, winograd.cc:1204-1206): kAny.  This
 // library's own names take only the values they are documented with.
-enum Range { kAny, kFlag, kStages, kTiles, kNonNegative, kBits, kCore, kFlag2, kPanels, kForm, kForm5 };
+enum Range { kAny, kFlag, kStages, kTiles, kNonNegative, kBits, kCore, kFlag2, kPanels, kForm };
 
 struct Field {
     const char *name;
@@ -129,7 +129,7 @@ const Field kFields[] = {
     {"conv_panels", &Tuning::conv_panels, kFlag},
     {"conv3x3_direct", &Tuning::conv3x3_direct, kFlag},
     {"q4_form", &Tuning::q4_form, kForm},
-    {"f8_form", &Tuning::f8_form, kForm5},
+    {"f8_form", &Tuning::f8_form, kForm},
     {"qgemm_core", &Tuning::qgemm_core, kFlag2},
     {"attention_generic", &Tuning::attention_generic, kFlag},
     {"attention_fp32", &Tuning::attention_fp32, kFlag},
@@ -162,9 +162,6 @@ bool in_range(Range r, long v, const char *&takes) {
     case kForm:
         takes = "0 to 6";
         return v >= 0 && v <= 6;
-    case kForm5:
-        takes = "0 to 5";
-        return v >= 0 && v <= 5;
     case kNonNegative:
         takes = "0 or more";
         return v >= 0 && v <= INT32_MAX;

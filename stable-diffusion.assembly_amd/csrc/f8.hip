@@ -837,9 +837,9 @@ hipError_t launch_tiles(TilesArgs t, hipStream_t stream) {
 // ------------------------------------------------------------------ the choice
 
 // Which kernels a product takes, numbered as the f8_form tuning asks for them: the
-// few rows' kernel by 16 rows or by 32, or tiles of 128 x 128, of 64 x 128 by two
-// waves' halves of K, of 64 x 64 by four's quarters.
-enum class Form { few = 1, rows, tiles, tiles64, tiles64x64 };
+// few rows' kernel by 16 rows or by 32, or tiles of 128 x 128 by four waves, of as many
+// by eight's halves of K, of 64 x 128 by four's, of 64 x 64 by four's quarters.
+enum class Form { few = 1, rows, tiles, tiles8, tiles64, tiles64x64 };
 
 // Tiles' copies reach 128 rows of the weights by 32 bits of offset.
 constexpr int64_t kTilesK = int64_t{1} << 22;
@@ -856,7 +856,9 @@ double few_time(int64_t M, int64_t columns, int64_t K, int rm, int halves) {
 
 // Tiles, the smallest of which there are no more than CUs, else the largest: of 1280
 // columns and K 1280, us by 64 x 64 | 64 x 128 | 128 x 128: 768 rows 13.8 | 14.8 | 18.9,
-// 1024 20.9 | 15.3 | 19.6, 8192 94 | 56 | 50.  Or a kernel of few rows, where that takes
+// 1024 20.9 | 15.3 | 19.6, 8192 94 | 56 | 50.  Of the largest no more than CUs too, so
+// one on each, and of a long K by eight waves: 2048 rows of 5120 to 1280 columns 51.7 by
+// eight, 54.5 by four, 1024 of 320 to 2560 15.4 and 13.4.  Or a kernel of few rows, where that takes
 // less by the times of a launch fitted to 28 such shapes, of 1 to 8192 rows (the rule
 // is 1% slower than the best choice in the mean, 36% at most): of K 640 to 640 columns
 // by 16 rows | 32 | tiles: 160 rows 5.3 | 6.4 | 10.3, 384 7.3 | 6.7 | 10.5, 1536 - | 13.0 |
@@ -878,6 +880,7 @@ Form form_of(int64_t M, int64_t N, int64_t K, bool gated) {
         form = Form::tiles64;
         least += 0.5 * blocks;
     } else {
+        if (tiles(128, 128) <= compute_units() && K >= 2048) form = Form::tiles8;
         least += 0.9 * blocks * static_cast<double>(ceil_div(tiles(128, 128), 2 * compute_units()));
     }
     if (!fits) return form;
@@ -907,6 +910,8 @@ hipError_t launch_form(const F8Args &a, bool whole, void *work, hipStream_t stre
     if (const hipError_t e = lay_out(a, w, stream); e != hipSuccess) return e;
     const TilesArgs t{a, w, whole ? a.w : w.w, whole ? a.row_bytes : w.ld, 0, 0};
     switch (form) {
+    case Form::tiles8:
+        return launch_tiles<GATED, 2, 2, 2>(t, stream);
     case Form::tiles64:
         return launch_tiles<GATED, 1, 2, 2>(t, stream);
     case Form::tiles64x64:

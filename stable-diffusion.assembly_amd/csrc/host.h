@@ -77,8 +77,8 @@ struct Tuning {
     int q4_form = 0;
     // This library's own: the products of 8-bit floating-point weights by one form,
     // or 0 to choose by the size, for comparison; results agree within the same
-    // bound.  1, 2 each workgroup's 16 or 32 rows of x brought to E4M3 in it; 3 .. 5 x
-    // laid out first, tiles of 128 x 128, of 64 x 128, of 64 x 64.
+    // bound.  1, 2 each workgroup's 16 or 32 rows of x brought to E4M3 in it; 3 .. 6 x
+    // laid out first, tiles of 128 x 128 by four waves, by eight, of 64 x 128, of 64 x 64.
     int f8_form = 0;
     // This library's own: attention by its generic form (1) even where the
     // fast one takes the operands (0), for comparison; results agree within

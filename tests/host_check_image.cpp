@@ -143,7 +143,7 @@ int main(int argc, char **argv) {
     const int cases = argc > 1 ? std::atoi(argv[1]) : 20000;
     if (argc > 2) rng.seed(std::strtoull(argv[2], nullptr, 10));
     for (int i = 0; i < cases; ++i) {
-        if (i % 100 == 0) sdhip_set_tuning(("f8_form=" + std::to_string(rng() % 6)).c_str());
+        if (i % 100 == 0) sdhip_set_tuning(("f8_form=" + std::to_string(rng() % 7)).c_str());
         products();
         turns();
         norms();

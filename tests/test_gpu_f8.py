@@ -66,7 +66,7 @@ def run(gpu, rows, k, n, seed, steps=(), layout=(None, 0), x=None, apart=0, w=No
     return y.check(), *f8_lib.exact(bytes_, scales, x)
 
 
-FORMS = [0, 1, 2, 3, 4, 5]
+FORMS = [0, 1, 2, 3, 4, 5, 6]
 
 
 @pytest.fixture(params=FORMS)
