@@ -15,8 +15,8 @@
 // one launch and one read of x; others a launch for the sums and one for the
 // outputs, which reads x again, the last chunks first: those the Infinity Cache
 // still holds.  1024 x 1024 pixels of 128 channels take 316 us (the sums 119 at 4.5
-// TB/s, the outputs 192 at 5.6); 2 x 8 x 8 of 1280 5.9, a launch and four waits one
-// after another: x, its sums through LDS, the statistics, the writes.
+// TB/s, the outputs 192 at 5.6); 2 x 8 x 8 of 1280 4.6, a launch and three waits one
+// after another: x, its sums through LDS, the writes.
 
 #include "host.h"
 #include "norm_last.h"
@@ -437,15 +437,40 @@ __global__ __launch_bounds__(T) void group_last_whole_kernel(GroupNormLastArgs a
 #pragma unroll
     for (int u = 0; u < R; ++u)
         if (in && at.row + u * at.rows < pixels) mine.add(q[u]);
-    add_up<V, U, T>(mine, v, at, v.c0, per_group, sums, totals);
-    __syncthreads();
-    Moments *stats = reinterpret_cast<Moments *>(totals);
-    if (tid < v.groups) {
-        stats[tid] = moments_of(static_cast<double>(first), totals[tid].first, totals[tid].squares, numbers_of(a, v.g0 + tid), a.eps);
+    if (v.groups == 1) {
+        // Of one group the sums of all threads, by waves (2 x 8 x 8 x 1280 5.9 us by its
+        // channels, so 4.6).
+        double one = 0.0, two = 0.0;
+#pragma unroll
+        for (int i = 0; i < V / U; ++i) {
+            one += mine.first[i];
+            two += mine.squares[i];
+        }
+        one = wave_sum(one);
+        two = wave_sum(two);
+        if ((tid & 63) == 0) sums[tid / 64] = Sums{one, two};
+        __syncthreads();  // and x is read, which y may be
+        one = two = 0.0;
+#pragma unroll
+        for (int w = 0; w < T / 64; ++w) {
+            one += sums[w].first;
+            two += sums[w].squares;
+        }
+        if (!in) return;
+        const Moments m = moments_of(mine.shift[0], one, two, numbers_of(a, v.g0), a.eps);
+#pragma unroll
+        for (int i = 0; i < V; ++i) out.stats[i] = m;
+    } else {
+        add_up<V, U, T>(mine, v, at, v.c0, per_group, sums, totals);
+        __syncthreads();
+        Moments *stats = reinterpret_cast<Moments *>(totals);
+        if (tid < v.groups) {
+            stats[tid] = moments_of(static_cast<double>(first), totals[tid].first, totals[tid].squares, numbers_of(a, v.g0 + tid), a.eps);
+        }
+        __syncthreads();  // and x is read, which y may be
+        if (!in) return;
+        out.statistics(a, stats, v, at.c);
     }
-    __syncthreads();  // and x is read, which y may be
-    if (!in) return;
-    out.statistics(a, stats, v, at.c);
 #pragma unroll
     for (int u = 0; u < R; ++u) {
         const int p = at.row + u * at.rows;
