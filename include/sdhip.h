@@ -238,8 +238,9 @@ sdhip_status sdhip_mul_mat_gated(const sdhip_tensor *w, const sdhip_tensor *x, c
  * sums in single precision; a scale times 2^e is to be below 2^128.  An infinity or
  * NaN in x makes its row's outputs NaN, a NaN in w its column's.
  * What bits asks for is left aside.  The output shares no byte with w, scales or
- * x.  Up to 2^25 rows of x and 2^25 of w, 2^36 weights, 2^35 outputs and 2^37
- * numbers of x are taken.  The work buffer, none where few rows read the
+ * x, nor with an operand of the chain but one that is its own memory in its layout
+ * (with fuse = 0 not that): SDHIP_UNSUPPORTED.  Up to 2^25 rows of x and 2^25 of w,
+ * 2^36 weights, 2^35 outputs and 2^37 numbers of x are taken.  The work buffer, none where few rows read the
  * weights: x as its q and e and, where they do not lie at multiples of 16 bytes in
  * rows of whole blocks, the weights; calls that may run at once take a buffer each.
  * Its size follows the f8_form tuning, which is to be the same when the size is
@@ -355,12 +356,14 @@ sdhip_status sdhip_group_norm_static(const sdhip_tensor *x, const sdhip_tensor *
 /* GROUP_NORM of channels-last tensors, images as rows of channels and so tokens
  * too, then the chain (no counterpart in the reference, whose GROUP_NORM takes
  * ne[2] as the channels): x, y F32 of one shape, ne = [C, W, H, N], nb[0] = 4,
- * pixels any multiple of 4 bytes apart, nb[2] = W nb[1], images any multiple of
- * 4 (so channels of a wider tensor); `groups` groups of ceil(C / groups)
+ * pixels any multiple of 4 bytes apart, 0 or more, nb[2] = W nb[1], images any
+ * multiple of 4 (so channels of a wider tensor); `groups` groups of ceil(C / groups)
  * channels over ne[0], per image ne[3].  Up to 2^24 channels, 2^31 - 1 pixels of
  * an image and as many images, 2^40 numbers in all are taken.  The statistics are
  * taken in double.  y may be x's own memory in the same layout; else
- * it shares no byte range with x, nor do two of its pixels: SDHIP_UNSUPPORTED.
+ * it shares no byte range with x, nor do two of its pixels, nor an operand of the
+ * chain with y but y's own memory in its layout (fuse = 0: nor that):
+ * SDHIP_UNSUPPORTED.
  * No redirect.  The work buffer holds the partial sums of stretches of an
  * image's pixels, 0 where a group is small enough for one launch. */
 int sdhip_group_norm_last_supported(const sdhip_tensor *x, const sdhip_tensor *y, int groups);
@@ -430,8 +433,8 @@ sdhip_status sdhip_norm_residual(const sdhip_tensor *y, const sdhip_row_norm *po
  *   y    = z                                for the others
  *
  * x F32 and y F32 or F16, ne = [d, tokens, heads, batch] as attention's
- * queries, d <= 512, nb[0] the element size and the other strides any multiple
- * of it (queries and keys side by side in a projection's output are one x, their
+ * queries, d <= 512, up to 2^24 heads and 2^40 tokens of all batches, nb[0] the
+ * element size and the other strides any multiple of it from 0 up (queries and keys side by side in a projection's output are one x, their
  * norms' weights one tensor of ne[2] = heads).  positions F32, ne = [count,
  * tokens or 1, 1, batch or 1], nb[0] = 4.  The pairs of axis a are the
  * dims[a] / 2 after those of the axes before, dims even; t is the position

@@ -269,6 +269,21 @@ bool tensors_share(const sdhip_tensor *a, const sdhip_tensor *b) {
     return a != nullptr && b != nullptr && spans_overlap(a->data, tensor_span(a), b->data, tensor_span(b));
 }
 
+bool chain_apart(const sdhip_tensor *y, const sdhip_epilogue *e) {
+    if (e == nullptr) return true;
+    const sdhip_tensor *to = e->redirect != nullptr ? e->redirect : y;
+    const bool first = tuning().fuse == 0 || (e->redirect != nullptr && tuning().fuse_residual == 0);
+    for (int i = 0; i < e->count && i < SDHIP_MAX_STEPS; ++i) {
+        if (e->steps[i].kind == SDHIP_STEP_SILU) continue;
+        const sdhip_tensor *t = &e->steps[i].operand;
+        if (first && tensors_share(y, t)) return false;
+        bool own = t->data == to->data;
+        for (int k = 0; k < 4; ++k) own = own && t->ne[k] == to->ne[k] && (t->ne[k] == 1 || t->nb[k] == to->nb[k]);
+        if (!own && tensors_share(to, t)) return false;
+    }
+    return true;
+}
+
 int compute_units() {
     constexpr int kDevices = 64;
     static std::atomic<int> known[kDevices] = {};

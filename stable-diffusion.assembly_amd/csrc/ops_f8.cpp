@@ -102,6 +102,10 @@ sdhip_status sdhip_mul_mat_f8(const sdhip_tensor *w, const sdhip_tensor *scales,
     ChainRun run;
     sdhip_status s = chain_plan(y, chain, run);
     if (s != SDHIP_OK) return s;
+    if (!chain_apart(y, chain)) return fail(SDHIP_UNSUPPORTED, "mul_mat_f8: the output overlaps a chain operand");
+    for (const sdhip_tensor *t : {w, scales, x}) {
+        if (chain != nullptr && tensors_share(chain->redirect, t)) return fail(SDHIP_ERROR, "mul_mat_f8: the output lies over an operand");
+    }
     const hipStream_t st = static_cast<hipStream_t>(stream);
     F8Args a = args_of(w, scales, x, y);
     a.chain = run.fused;

@@ -12,7 +12,8 @@ namespace {
 // Images of evenly spaced pixels, their channels side by side.
 bool pixels_of(const sdhip_tensor *t) {
     int64_t row;
-    return holds_f32(t) && t->nb[1] % 4 == 0 && t->nb[2] % 4 == 0 && t->nb[3] % 4 == 0 &&
+    return holds_f32(t) && t->nb[1] % 4 == 0 && t->nb[2] % 4 == 0 && t->nb[3] % 4 == 0 && t->nb[1] >= 0 && t->nb[2] >= 0 &&
+           t->nb[3] >= 0 &&
            reinterpret_cast<uintptr_t>(t->data) % 4 == 0 &&
            (t->ne[1] == 1 || t->ne[2] == 1 || (!__builtin_mul_overflow(t->nb[1], t->ne[1], &row) && t->nb[2] == row));
 }
@@ -62,6 +63,7 @@ sdhip_status sdhip_group_norm_last(const sdhip_tensor *x, const sdhip_tensor *y,
     ChainRun run;
     sdhip_status s = chain_plan(y, chain, run);
     if (s != SDHIP_OK) return s;
+    if (!chain_apart(y, chain)) return fail(SDHIP_UNSUPPORTED, "group_norm_last: the output overlaps a chain operand");
     const GroupNormLastShape shape = shape_of(x, groups);
     const size_t need = group_norm_last_work_size(shape);
     if (const sdhip_status ws = check_work("group_norm_last", work, work_size, need); ws != SDHIP_OK) return ws;

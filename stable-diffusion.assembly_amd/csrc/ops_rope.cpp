@@ -12,10 +12,15 @@ namespace sdhip {
 
 namespace {
 
+// Strides of 0 or more: what a tensor reaches lies behind its data.
+bool forward(const sdhip_tensor *t) {
+    return t == nullptr || (t->nb[0] >= 0 && t->nb[1] >= 0 && t->nb[2] >= 0 && t->nb[3] >= 0);
+}
+
 // Rows of `size` bytes a number: nb[0] that, the others any multiple of it, at
 // such an address.
 bool rows_of(const sdhip_tensor *t, int64_t size) {
-    return t->nb[0] == size && t->nb[1] % size == 0 && t->nb[2] % size == 0 && t->nb[3] % size == 0 &&
+    return t->nb[0] == size && t->nb[1] % size == 0 && t->nb[2] % size == 0 && t->nb[3] % size == 0 && forward(t) &&
            reinterpret_cast<uintptr_t>(t->data) % static_cast<uintptr_t>(size) == 0;
 }
 
@@ -46,11 +51,12 @@ int sdhip_rope_supported(const sdhip_tensor *x, const sdhip_row_norm *norm, cons
     for (int k = 0; k < 4; ++k) {
         if (x->ne[k] < 1 || x->ne[k] > INT32_MAX) return 0;
     }
-    // Tokens, and parts of their heads, are counted in 64 bits.
-    if (x->ne[1] > (int64_t{1} << 40) / x->ne[3]) return 0;
+    // Heads are counted in 32 bits, tokens, and parts of their heads, in 64.
+    if (x->ne[2] > (int64_t{1} << 24) || x->ne[1] > (int64_t{1} << 40) / x->ne[3]) return 0;
     if (!holds_f32(x) || !rows_of(x, 4)) return 0;
     if (!(holds_f32(y) && rows_of(y, 4)) && !(holds_f16(y) && rows_of(y, 2))) return 0;
     if (turned_of(axes, x->ne[0]) < 0 || !row_norm_taken(norm, x)) return 0;
+    if (norm != nullptr && (!forward(norm->weight) || !forward(norm->bias))) return 0;
     if (!holds_f32(positions) || !rows_of(positions, 4) || positions->ne[0] != axes->count ||
         (positions->ne[1] != x->ne[1] && positions->ne[1] != 1) || positions->ne[2] != 1 ||
         (positions->ne[3] != x->ne[3] && positions->ne[3] != 1)) {

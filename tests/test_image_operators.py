@@ -139,6 +139,39 @@ def test_products_that_are_errors():
         sdhip.set_tuning("")
 
 
+def test_chain_operands_over_the_output():
+    """Refused but where an element is read at its own place: the output's memory in its
+    layout; with the chain apart that is overwritten before it is read."""
+    lib = sdhip.load()
+    w, s, x, at = weights(320, 320), scales(320, 320), rows(400, 320), 1 << 40
+    y, other = rows(400, 320, data=at), rows(400, 320, data=1 << 41)
+
+    def call(operand, redirect=None, from_redirect=0):
+        e = sdhip.Epilogue()
+        e.count = 1
+        e.steps[0].kind, e.steps[0].operand = 0, operand
+        e.from_redirect = from_redirect
+        if redirect is not None:
+            e.redirect = ctypes.pointer(redirect)
+        norm = lib.sdhip_group_norm_last(rows(1, 1, 400, 320), rows(1, 1, 400, 320, data=at), 8, 1e-5, e, None, 0, None)
+        return lib.sdhip_mul_mat_f8(w, s, x, y, e, None, 0, None), norm
+
+    try:
+        for fuse in (1, 0):
+            sdhip.set_tuning(f"f8_form=3,fuse={fuse}")
+            for operand in (rows(320, data=at), rows(320, data=at + 4 * 320 * 399), rows(400, 320, data=at + 16), rows(400, 320, data=at - 16)):
+                assert call(operand) == (sdhip.UNSUPPORTED, sdhip.UNSUPPORTED)
+            # What is taken lacks its work buffer.
+            assert call(y)[0] == (sdhip.ERROR if fuse else sdhip.UNSUPPORTED)
+            assert call(rows(320, data=1 << 42))[0] == sdhip.ERROR and b"work" in lib.sdhip_last_error()
+            assert call(other, redirect=other)[0] == sdhip.ERROR
+            assert call(rows(400, 320, data=(1 << 41) + 16), redirect=other)[0] == sdhip.UNSUPPORTED
+            assert call(y, redirect=other)[0] == (sdhip.ERROR if fuse else sdhip.UNSUPPORTED)
+            assert call(rows(320, data=1 << 42), redirect=rows(400, 320))[0] == sdhip.ERROR and b"lies over" in lib.sdhip_last_error()
+    finally:
+        sdhip.set_tuning("")
+
+
 def test_extents_that_a_launch_counts():
     """Up to 2^25 rows of x and of the weights, 2^36 weights, 2^35 outputs, 2^37 numbers of x."""
     most = 1 << 25
@@ -231,6 +264,12 @@ def test_rope_refused():
     for n in (norm(3), norm(-1), norm(weight=rows(63, data=9 * FAKE)), norm(bias=rows(3, 3, 7, 64, data=9 * FAKE)),
               norm(weight=rows(64, data=9 * FAKE, type=F16)), norm(weight=rows(64, data=9 * FAKE + 1))):
         bad.append((X, n, AT, axes(), Y))
+    # Strides below 0, which reach before the data; more heads than are counted.
+    for k in (1, 2, 3):
+        bad += [(changed(X, "nb", k, -256), None, AT, axes(), Y), (X, None, changed(AT, "nb", k, -8), axes(), Y)]
+        bad += [(X, f(changed(rows(2, 3, 7, 64, data=9 * FAKE), "nb", k, -256)), AT, axes(), Y) for f in (lambda w: norm(weight=w), lambda b: norm(bias=b))]
+    many = (1 << 24) + 1
+    bad.append((rows(many, 1, 2), None, rows(1, 1, data=1 << 41), axes((2,)), rows(many, 1, 2, data=1 << 40)))
     # What is written over what is read, or over itself.
     bad += [(X, None, AT, axes(), rows(2, 3, 7, 64, data=FAKE + 4)), (X, None, AT, axes(), rows(2, 3, 7, 64, data=3 * FAKE - 256)),
             (X, None, AT, axes(), changed(Y, "nb", 1, 4 * 63)), (X, None, AT, axes(), changed(Y, "nb", 3, 0)),
@@ -287,7 +326,7 @@ def test_group_norm_refused():
     lib = sdhip.load()
     bad = [(None, J, 8), (I, None, 8), (I, J, 0), (I, J, -1)]
     for f, k, v in (("type", 0, F16), ("type", 0, F8), ("ne", 0, 63), ("ne", 1, 0), ("ne", 2, 6), ("ne", 3, 3), ("nb", 0, 8),
-                    ("nb", 1, 258), ("nb", 2, 7 * 256 + 4), ("nb", 3, 2), ("data", 0, 8 * FAKE + 2)):
+                    ("nb", 1, 258), ("nb", 2, 7 * 256 + 4), ("nb", 3, 2), ("nb", 3, -64), ("data", 0, 8 * FAKE + 2)):
         bad += [(changed(I, f, k, v), J, 8), (I, changed(J, f, k, v), 8)]
     bad += [(I, rows(2, 5, 7, 64, data=FAKE + 256), 8), (wide(FAKE), I, 8),
             (I, sdhip.view_desc(2 * FAKE, F32, [64, 7, 5, 2], [4, 252, 252 * 7, 252 * 35]), 8), (I, changed(J, "nb", 3, 0), 8)]
