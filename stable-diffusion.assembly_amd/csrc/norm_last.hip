@@ -525,12 +525,13 @@ Split split_of(const GroupNormLastShape &s, int v) {
     }
     p.whole = -1;
     // Whole lines of up to 1024 channels; chunks until each CU has four workgroups,
-    // of 8 pixels a thread at least.
+    // of 8 pixels a thread at least.  None is empty: as many as chunks of the pixels of
+    // one of them are (the outputs' kernel reads its chunk's first pixel).
     p.slab = slab_of(s, ceil_div(s.channels, ceil_div(s.channels, 1024)));
     p.slabs = ceil_div(s.groups, p.slab);
     const auto chunks = [&](int64_t slab, int64_t slabs, int64_t least) {
         const int64_t wanted = ceil_div(8 * cus, s.images * slabs), most = ceil_div(s.pixels, least * rows_of(s, slab, kThreads, v));
-        return wanted < most ? wanted : most;
+        return ceil_div(s.pixels, ceil_div(s.pixels, wanted < most ? wanted : most));
     };
     p.parts = chunks(p.slab, p.slabs, 8);
     p.joined = p.parts > kMostParts;

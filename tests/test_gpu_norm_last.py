@@ -197,3 +197,10 @@ def test_many_images(gpu):
     for i in (0, 1, 29999):
         sdhip.group_norm_last(x[i:i + 1], one, 2, 1e-5)
         assert torch.allclose(one, y[i:i + 1], rtol=0, atol=2.0 ** -22)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,groups", [((3, 1, 100003, 64), 32), ((3, 69, 565, 96), 32), ((1, 1, 263001, 12), 3), ((2, 1, 70001, 30), 3)])
+def test_pixels_that_no_even_chunks_hold(gpu, shape, groups):
+    """Chunks of as many pixels as the most wanted would leave the last of them none."""
+    check(gpu, shape, groups)

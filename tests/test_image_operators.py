@@ -346,3 +346,14 @@ def test_group_norm_refused():
     big = rows(1, 1024, 1024, 128, data=1 << 33)
     assert lib.sdhip_group_norm_last(big, big, 32, 1e-5, None, None, 0, None) == sdhip.ERROR
     assert b"work" in lib.sdhip_last_error()
+
+
+@pytest.mark.parametrize("shape,groups", [((3, 69, 565, 960), 32), ((3, 1, 100003, 64), 32), ((1, 1, 263001, 12), 3), ((2, 300, 701, 320), 32),
+                                          ((1, 1024, 1024, 128), 32), ((5, 333, 77, 512), 32)])
+def test_no_part_of_an_image_is_empty(shape, groups):
+    """As many chunks of its pixels as the work buffer holds sums of: the last begins before their end."""
+    n, h, w, c = shape
+    x = rows(*shape, data=1 << 40)
+    sums = sdhip.load().sdhip_group_norm_last_work_size(x, x, groups) // (8 * n * groups)
+    parts = (sums - 1) // 2 if (sums - 1) // 2 <= 256 else (sums - 3) // 2
+    assert parts > 1 and (parts - 1) * -(-h * w // parts) < h * w
