@@ -481,19 +481,18 @@ __global__ __launch_bounds__(T) void group_last_whole_kernel(GroupNormLastArgs a
 // ------------------------------------------------------------------ the split
 
 constexpr int kMostParts = 256;  // that every workgroup of outputs adds up
-// The threads of the one launch, and the pixels of each: as few threads as hold a
-// slab's numbers (what a wave does once is as much as five pixels).
+// The threads of the one launch, and the numbers of each: as few threads as hold a
+// slab's (what a wave does once is as much as five pixels).
 struct Whole {
-    int threads, pixels;
+    int threads, numbers;
 };
-constexpr Whole kWhole[] = {{256, 4}, {512, 4}, {1024, 4}, {1024, 8}};
+constexpr Whole kWhole[] = {{256, 16}, {512, 16}, {1024, 16}, {1024, 32}};
 
 int64_t gcd(int64_t a, int64_t b) { return b == 0 ? a : gcd(b, a % b); }
 
-// Groups of a slab of `channels` or more of them, a multiple of 4 where the tensor's
-// are (and so the slab begins at one).
-int64_t slab_of(const GroupNormLastShape &s, int64_t channels) {
-    const int64_t unit = s.channels % 4 == 0 ? 4 / gcd(4, s.per_group) : 1;
+// Groups of a slab of `channels` or more of them, beginning at a multiple of V.
+int64_t slab_of(const GroupNormLastShape &s, int64_t channels, int v) {
+    const int64_t unit = v / gcd(v, s.per_group);
     const int64_t groups = round_up(ceil_div(channels, s.per_group), unit);
     return groups < s.groups ? groups : s.groups;
 }
@@ -505,6 +504,7 @@ int64_t rows_of(const GroupNormLastShape &s, int64_t slab, int64_t threads, int 
 }
 
 struct Split {
+    int v;                       // channels a thread
     int whole;                   // which of kWhole one launch is of, or -1: two launches or three
     int64_t slab, slabs;         // of the sums (or of the one launch)
     int64_t parts;
@@ -513,21 +513,22 @@ struct Split {
     bool joined;                 // three launches
 };
 
-// By the layout's V channels a thread; the work buffer is of the larger.
-Split split_of(const GroupNormLastShape &s, int v) {
+// By V channels a thread, in one launch slabs of `least` channels or more.
+Split split_of(const GroupNormLastShape &s, int v, int64_t least) {
     Split p{};
+    p.v = v;
     const int64_t cus = compute_units();
-    p.slab = slab_of(s, 16);
+    p.slab = slab_of(s, least, v);
     p.slabs = ceil_div(s.groups, p.slab);
     for (p.whole = 0; p.whole < 4; ++p.whole) {
         const Whole &w = kWhole[p.whole];
-        if (p.slab * s.per_group <= w.threads * v && s.pixels <= w.pixels * rows_of(s, p.slab, w.threads, v)) return p;
+        if (p.slab * s.per_group <= w.threads * v && s.pixels <= w.numbers / v * rows_of(s, p.slab, w.threads, v)) return p;
     }
     p.whole = -1;
     // Whole lines of up to 1024 channels; chunks until each CU has four workgroups,
     // of 8 pixels a thread at least.  None is empty: as many as chunks of the pixels of
     // one of them are (the outputs' kernel reads its chunk's first pixel).
-    p.slab = slab_of(s, ceil_div(s.channels, ceil_div(s.channels, 1024)));
+    p.slab = slab_of(s, ceil_div(s.channels, ceil_div(s.channels, 1024)), v);
     p.slabs = ceil_div(s.groups, p.slab);
     const auto chunks = [&](int64_t slab, int64_t slabs, int64_t least) {
         const int64_t wanted = ceil_div(8 * cus, s.images * slabs), most = ceil_div(s.pixels, least * rows_of(s, slab, kThreads, v));
@@ -536,10 +537,25 @@ Split split_of(const GroupNormLastShape &s, int v) {
     p.parts = chunks(p.slab, p.slabs, 8);
     p.joined = p.parts > kMostParts;
     // Where the outputs' workgroups add up the parts, of few groups each.
-    p.apply = p.joined ? p.slab : slab_of(s, 64);
+    p.apply = p.joined ? p.slab : slab_of(s, 64, v);
     p.apply_slabs = ceil_div(s.groups, p.apply);
     p.chunks = chunks(p.apply, p.apply_slabs, 8);
     return p;
+}
+
+// Slabs of 64 bytes or more, by four channels a thread where they lie so.  Where that
+// leaves half of the CUs without one, slabs of 32 bytes by one launch, by single
+// channels where a group is of no multiple of four: a CU's operations, not memory,
+// bound the slabs of many numbers (more than 6000; 33 x 24 of 352 11.2 us by 44 channels,
+// 8.7 by 11, 3 x 53 x 7 of 288 10.4 and 7.7; 3 x 5 x 40 of 48, by 4800 numbers, 6.4 and
+// 7.3), single channels cost more a number, and of 10000 and more as much as two launches
+// (2 x 109 x 17 of 288, by 16700, 16.0 us, so 12.2).
+Split choose(const GroupNormLastShape &s, bool quads) {
+    const Split wide = split_of(s, quads ? 4 : 1, 16);
+    const auto numbers = [&](const Split &p) { return p.slab * s.per_group * s.pixels; };
+    if (wide.whole >= 0 && (2 * s.images * wide.slabs >= compute_units() || numbers(wide) <= 6000)) return wide;
+    const Split narrow = split_of(s, quads && s.per_group % 4 == 0 ? 4 : 1, 8);
+    return narrow.whole >= 0 && narrow.slabs > wide.slabs && numbers(narrow) <= 10000 ? narrow : wide;
 }
 
 // The chain's steps as a multiplication, an addition and SiLU of one number a
@@ -587,10 +603,10 @@ hipError_t launch(GroupNormLastArgs a, const Split &split, void *work, hipStream
         return hipSuccess;
     };
     static_assert(sizeof(Sums) == sizeof(Moments));
-    if (split.whole == 0) return launch_whole<V, U, kWhole[0].threads, kWhole[0].pixels>(by_images, split, a, stream);
-    if (split.whole == 1) return launch_whole<V, U, kWhole[1].threads, kWhole[1].pixels>(by_images, split, a, stream);
-    if (split.whole == 2) return launch_whole<V, U, kWhole[2].threads, kWhole[2].pixels>(by_images, split, a, stream);
-    if (split.whole == 3) return launch_whole<V, U, kWhole[3].threads, kWhole[3].pixels>(by_images, split, a, stream);
+    if (split.whole == 0) return launch_whole<V, U, kWhole[0].threads, kWhole[0].numbers / V>(by_images, split, a, stream);
+    if (split.whole == 1) return launch_whole<V, U, kWhole[1].threads, kWhole[1].numbers / V>(by_images, split, a, stream);
+    if (split.whole == 2) return launch_whole<V, U, kWhole[2].threads, kWhole[2].numbers / V>(by_images, split, a, stream);
+    if (split.whole == 3) return launch_whole<V, U, kWhole[3].threads, kWhole[3].numbers / V>(by_images, split, a, stream);
     a.parts = static_cast<int32_t>(split.parts);
     a.partials = static_cast<double *>(work);
     double *at = a.partials + 2 * a.images * a.groups * split.parts;
@@ -616,7 +632,8 @@ hipError_t launch(GroupNormLastArgs a, const Split &split, void *work, hipStream
 }  // namespace
 
 size_t group_norm_last_work_size(const GroupNormLastShape &s) {
-    const size_t four = work_of(s, split_of(s, 4)), one = work_of(s, split_of(s, 1));
+    // Of either, as the tensors may lie.
+    const size_t four = s.channels % 4 == 0 ? work_of(s, choose(s, true)) : 0, one = work_of(s, choose(s, false));
     return four > one ? four : one;
 }
 
@@ -627,12 +644,10 @@ hipError_t launch_group_norm_last(GroupNormLastArgs a, void *work, hipStream_t s
         return reinterpret_cast<uintptr_t>(p) % 16 == 0 && pixel % 4 == 0 && image % 4 == 0;
     };
     const GroupNormLastShape s{a.channels, a.pixels, a.images, a.groups, a.per_group};
-    if (a.channels % 4 == 0 && quads(a.x, a.xpixel, a.ximage) && quads(a.y, a.ypixel, a.yimage)) {
-        const Split split = split_of(s, 4);
-        if (a.per_group % 4 == 0) return launch<4, 4>(a, split, work, stream);
-        return a.per_group % 2 == 0 ? launch<4, 2>(a, split, work, stream) : launch<4, 1>(a, split, work, stream);
-    }
-    return launch<1, 1>(a, split_of(s, 1), work, stream);
+    const Split split = choose(s, a.channels % 4 == 0 && quads(a.x, a.xpixel, a.ximage) && quads(a.y, a.ypixel, a.yimage));
+    if (split.v == 1) return launch<1, 1>(a, split, work, stream);
+    if (a.per_group % 4 == 0) return launch<4, 4>(a, split, work, stream);
+    return a.per_group % 2 == 0 ? launch<4, 2>(a, split, work, stream) : launch<4, 1>(a, split, work, stream);
 }
 
 }  // namespace sdhip
