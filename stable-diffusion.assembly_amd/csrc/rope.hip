@@ -77,28 +77,34 @@ __device__ __forceinline__ float row_sum(float v) {
 }
 
 // LPR lanes a row, SLOTS groups of four pairs each; QUADS where every four
-// numbers that a lane reads or writes at once lie at a multiple of their size.
-template <int LPR, int SLOTS, bool ADJACENT, bool QUADS>
+// numbers that a lane reads or writes at once lie at a multiple of their size; FEW
+// where a token's heads are half of a wave's rows or fewer: it takes rows of as many
+// tokens as there is room for, and each lane computes its own pairs' sines and cosines
+// (50688 tokens of one head of 40 32 us by a token a wave, so 10.6; 4096 of two of 128 6.5
+// and 5.7, but 2048 5.1 and 5.3: where waves are as many as tokens four turns a lane take
+// longer than one).
+template <int LPR, int SLOTS, bool ADJACENT, bool QUADS, bool FEW>
 __global__ __launch_bounds__(kThreads, SLOTS == 1 ? 4 : 1) void rope_kernel(RopeArgs a) {
-    __shared__ float2 shared[kWaves][64 * (LPR * SLOTS <= 16 ? 1 : LPR * SLOTS <= 32 ? 2 : 4)];
+    __shared__ float2 shared[FEW ? 1 : kWaves][FEW ? 1 : 64 * (LPR * SLOTS <= 16 ? 1 : LPR * SLOTS <= 32 ? 2 : 4)];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int pairs = a.turned / 2;
-    float2 *turns = shared[wave];
-    // The frequencies, in half turns, of the pairs that this lane computes.
-    constexpr int kMine = LPR * SLOTS <= 16 ? 1 : LPR * SLOTS <= 32 ? 2 : 4;
+    float2 *turns = shared[FEW ? 0 : wave];
+    const int sub = lane % LPR;
+    // The frequencies, in half turns, of the pairs that this lane computes: each 64th of
+    // a token's, or its own.
+    constexpr int kMine = FEW ? 4 * SLOTS : LPR * SLOTS <= 16 ? 1 : LPR * SLOTS <= 32 ? 2 : 4;
     double rate[kMine];
     int axis[kMine];
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
-        const int p = lane + 64 * i;
+        const int p = FEW ? 4 * (sub + LPR * (i / 4)) + i % 4 : lane + 64 * i;
         axis[i] = 0;
 #pragma unroll
         for (int j = 1; j < SDHIP_MAX_AXES; ++j)
             if (j < a.count && p >= a.first[j]) axis[i] = j;
-        rate[i] = 64 * i < pairs ? exp2(a.rate[axis[i]] * (p - a.from[axis[i]])) * 0.31830988618379067154 : 0.0;
+        rate[i] = FEW || 64 * i < pairs ? exp2(a.rate[axis[i]] * (p - a.from[axis[i]])) * 0.31830988618379067154 : 0.0;
     }
     // This lane's pairs: the place of each one's numbers, d or more where there is none.
-    const int sub = lane % LPR;
     const int front = ADJACENT ? 0 : (pairs + 3) / 4;  // groups of halves' pairs, before those that are not turned
     int at[SLOTS][4][2];
     bool turned[SLOTS][4];
@@ -177,13 +183,125 @@ __global__ __launch_bounds__(kThreads, SLOTS == 1 ? 4 : 1) void rope_kernel(Rope
     };
     const bool weight_quads = quads_of(a.norm.weight), bias_quads = quads_of(a.norm.bias);
     constexpr int kRows = 64 / LPR;  // heads of a wave at a time
+    // A row's norm and turns; a row's lanes together.
+    const auto row = [&](const float *x, const float *weight, const float *bias, int64_t to, const float2 (&by)[SLOTS][4]) {
+        float v[SLOTS][4][2];
+        load(x, true, 1, v);
+        if (a.norm.kind != SDHIP_ROW_NORM_NONE) {
+            float sum = 0.0f;
+            if (a.norm.kind == SDHIP_ROW_NORM_RMS) {
+#pragma unroll
+                for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) sum = __builtin_fmaf(v[s][c][k], v[s][c][k], sum);
+                sum = row_sum<LPR>(sum);
+            }
+            if (a.norm.kind == SDHIP_ROW_NORM_RMS && sum > 0x1p-60f && sum < 0x1p100f) {
+                const float scale = __builtin_amdgcn_rsqf(__builtin_fmaf(sum, static_cast<float>(a.inverse), a.norm.eps));
+#pragma unroll
+                for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) v[s][c][k] *= scale;
+            } else {
+                // In double: means, and squares near single precision's limits.
+                double mean = 0.0, squares = 0.0;
+                if (a.norm.kind == SDHIP_ROW_NORM_LAYER) {
+#pragma unroll
+                    for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) mean += static_cast<double>(v[s][c][0]) + static_cast<double>(v[s][c][1]);
+                    mean = mean_of(row_sum<LPR>(mean), a.d, a.inverse);
+                }
+#pragma unroll
+                for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const double d = at[s][c][k] < a.d ? static_cast<double>(v[s][c][k]) - mean : 0.0;
+                            squares = __builtin_fma(d, d, squares);
+                        }
+                const Moments m = moments(a.norm.kind, mean, row_sum<LPR>(squares), a.inverse, a.norm.eps);
+#pragma unroll
+                for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) v[s][c][k] = normed(v[s][c][k], m);
+            }
+        }
+        if (weight != nullptr) {
+            float w[SLOTS][4][2];
+            load(weight, weight_quads, a.norm.weight.nb[0], w);
+#pragma unroll
+            for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) v[s][c][k] = __fmul_rn(v[s][c][k], __fadd_rn(w[s][c][k], a.norm.offset));
+        }
+        if (bias != nullptr) {
+            float w[SLOTS][4][2];
+            load(bias, bias_quads, a.norm.bias.nb[0], w);
+#pragma unroll
+            for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) v[s][c][k] = __fadd_rn(v[s][c][k], w[s][c][k]);
+        }
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float one = v[s][c][0], two = v[s][c][1], cosine = by[s][c].x, sine = by[s][c].y;
+                const float u = __builtin_fmaf(-two, sine, one * cosine), w = __builtin_fmaf(one, sine, two * cosine);
+                // Not turned: as they are, whatever the other of the two is.
+                v[s][c][0] = turned[s][c] ? u : one;
+                v[s][c][1] = turned[s][c] ? w : two;
+            }
+        if (a.half) {
+            store(static_cast<_Float16 *>(a.y) + to, v);
+        } else {
+            store(static_cast<float *>(a.y) + to, v);
+        }
+    };
+    const int mine = lane / LPR;
+    const int64_t tokens = a.tokens * a.batch, step = static_cast<int64_t>(gridDim.x) * kWaves;
+    if constexpr (FEW) {
+        const int64_t items = (tokens * a.heads + kRows - 1) / kRows;
+        for (int64_t item = static_cast<int64_t>(blockIdx.x) * kWaves + wave; item < items; item += step) {
+            const int64_t first = item * kRows / a.heads;  // the token of the wave's first row
+            const int ahead = static_cast<int>(item * kRows - first * a.heads) + mine, skip = ahead / a.heads, h = ahead - skip * a.heads;
+            if (first + skip >= tokens) continue;
+            int64_t i3 = first / a.tokens, i1 = first - i3 * a.tokens + skip;
+            while (i1 >= a.tokens) {
+                i1 -= a.tokens;
+                ++i3;
+            }
+            const float *positions = a.positions + i1 * a.pnb1 + i3 * a.pnb3;
+            float2 by[SLOTS][4];
+#pragma unroll
+            for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    by[s][c] = turned[s][c] ? turn(static_cast<double>(positions[axis[4 * s + c]]) * rate[4 * s + c]) : make_float2(1.0f, 0.0f);
+            const auto of = [&](const RowOperand &o) { return o.data != nullptr ? o.data + i1 * o.nb[1] + i3 * o.nb[3] + h * o.nb[2] : nullptr; };
+            row(a.x + i1 * a.xnb[1] + i3 * a.xnb[3] + h * a.xnb[2], of(a.norm.weight), of(a.norm.bias),
+                i1 * a.ynb[1] + i3 * a.ynb[3] + h * a.ynb[2], by);
+        }
+        return;
+    }
     const int share = (a.heads + a.parts - 1) / a.parts;
     // How far a lane's row lies from the wave's first.
     const int64_t x_lane = lane / LPR * a.xnb[2], y_lane = lane / LPR * a.ynb[2];
     const int64_t w_lane = lane / LPR * a.norm.weight.nb[2], b_lane = lane / LPR * a.norm.bias.nb[2];
-    const int64_t items = a.tokens * a.batch * a.parts;
-    for (int64_t item = static_cast<int64_t>(blockIdx.x) * kWaves + wave; item < items;
-         item += static_cast<int64_t>(gridDim.x) * kWaves) {
+    const int64_t items = tokens * a.parts;
+    for (int64_t item = static_cast<int64_t>(blockIdx.x) * kWaves + wave; item < items; item += step) {
         const int64_t token = item / a.parts;
         const int part = static_cast<int>(item - token * a.parts);
         const int64_t i3 = token / a.tokens, i1 = token - i3 * a.tokens;
@@ -201,7 +319,7 @@ __global__ __launch_bounds__(kThreads, SLOTS == 1 ? 4 : 1) void rope_kernel(Rope
         for (int s = 0; s < SLOTS; ++s)
 #pragma unroll
             for (int c = 0; c < 4; ++c) by[s][c] = turned[s][c] ? turns[4 * (sub + LPR * s) + c] : make_float2(1.0f, 0.0f);
-        const int h0 = part * share, h1 = h0 + share < a.heads ? h0 + share : a.heads, mine = lane / LPR;
+        const int h0 = part * share, h1 = h0 + share < a.heads ? h0 + share : a.heads;
         const float *x = a.x + i1 * a.xnb[1] + i3 * a.xnb[3] + h0 * a.xnb[2] + x_lane;
         int64_t to = i1 * a.ynb[1] + i3 * a.ynb[3] + h0 * a.ynb[2] + y_lane;
         const float *weight = a.norm.weight.data, *bias = a.norm.bias.data;
@@ -209,118 +327,44 @@ __global__ __launch_bounds__(kThreads, SLOTS == 1 ? 4 : 1) void rope_kernel(Rope
         if (bias != nullptr) bias += i1 * a.norm.bias.nb[1] + i3 * a.norm.bias.nb[3] + h0 * a.norm.bias.nb[2] + b_lane;
         for (int h = h0; h < h1; h += kRows) {
             if (h + mine >= h1) continue;  // a row's lanes together
-            float v[SLOTS][4][2];
-            load(x, true, 1, v);
+            row(x, weight, bias, to, by);
             x += kRows * a.xnb[2];
-            if (a.norm.kind != SDHIP_ROW_NORM_NONE) {
-                float sum = 0.0f;
-                if (a.norm.kind == SDHIP_ROW_NORM_RMS) {
-#pragma unroll
-                    for (int s = 0; s < SLOTS; ++s)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-#pragma unroll
-                            for (int k = 0; k < 2; ++k) sum = __builtin_fmaf(v[s][c][k], v[s][c][k], sum);
-                    sum = row_sum<LPR>(sum);
-                }
-                if (a.norm.kind == SDHIP_ROW_NORM_RMS && sum > 0x1p-60f && sum < 0x1p100f) {
-                    const float scale = __builtin_amdgcn_rsqf(__builtin_fmaf(sum, static_cast<float>(a.inverse), a.norm.eps));
-#pragma unroll
-                    for (int s = 0; s < SLOTS; ++s)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-#pragma unroll
-                            for (int k = 0; k < 2; ++k) v[s][c][k] *= scale;
-                } else {
-                    // In double: means, and squares near single precision's limits.
-                    double mean = 0.0, squares = 0.0;
-                    if (a.norm.kind == SDHIP_ROW_NORM_LAYER) {
-#pragma unroll
-                        for (int s = 0; s < SLOTS; ++s)
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) mean += static_cast<double>(v[s][c][0]) + static_cast<double>(v[s][c][1]);
-                        mean = mean_of(row_sum<LPR>(mean), a.d, a.inverse);
-                    }
-#pragma unroll
-                    for (int s = 0; s < SLOTS; ++s)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-#pragma unroll
-                            for (int k = 0; k < 2; ++k) {
-                                const double d = at[s][c][k] < a.d ? static_cast<double>(v[s][c][k]) - mean : 0.0;
-                                squares = __builtin_fma(d, d, squares);
-                            }
-                    const Moments m = moments(a.norm.kind, mean, row_sum<LPR>(squares), a.inverse, a.norm.eps);
-#pragma unroll
-                    for (int s = 0; s < SLOTS; ++s)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-#pragma unroll
-                            for (int k = 0; k < 2; ++k) v[s][c][k] = normed(v[s][c][k], m);
-                }
-            }
-            if (weight != nullptr) {
-                float w[SLOTS][4][2];
-                load(weight, weight_quads, a.norm.weight.nb[0], w);
-                weight += kRows * a.norm.weight.nb[2];
-#pragma unroll
-                for (int s = 0; s < SLOTS; ++s)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) v[s][c][k] = __fmul_rn(v[s][c][k], __fadd_rn(w[s][c][k], a.norm.offset));
-            }
-            if (bias != nullptr) {
-                float w[SLOTS][4][2];
-                load(bias, bias_quads, a.norm.bias.nb[0], w);
-                bias += kRows * a.norm.bias.nb[2];
-#pragma unroll
-                for (int s = 0; s < SLOTS; ++s)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) v[s][c][k] = __fadd_rn(v[s][c][k], w[s][c][k]);
-            }
-#pragma unroll
-            for (int s = 0; s < SLOTS; ++s)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const float one = v[s][c][0], two = v[s][c][1], cosine = by[s][c].x, sine = by[s][c].y;
-                    const float u = __builtin_fmaf(-two, sine, one * cosine), w = __builtin_fmaf(one, sine, two * cosine);
-                    // Not turned: as they are, whatever the other of the two is.
-                    v[s][c][0] = turned[s][c] ? u : one;
-                    v[s][c][1] = turned[s][c] ? w : two;
-                }
-            if (a.half) {
-                store(static_cast<_Float16 *>(a.y) + to, v);
-            } else {
-                store(static_cast<float *>(a.y) + to, v);
-            }
+            if (weight != nullptr) weight += kRows * a.norm.weight.nb[2];
+            if (bias != nullptr) bias += kRows * a.norm.bias.nb[2];
             to += kRows * a.ynb[2];
         }
     }
 }
 
-template <int LPR, int SLOTS>
-hipError_t launch(RopeArgs a, bool quads, hipStream_t stream) {
-    // Parts of a token's heads until every wave of the device has one, 16 a CU.
-    const int64_t waves = 16 * static_cast<int64_t>(compute_units()), tokens = a.tokens * a.batch;
-    const int64_t most = ceil_div(a.heads, 64 / LPR);
-    a.parts = static_cast<int32_t>(tokens * most <= waves ? most : tokens >= waves ? 1 : ceil_div(waves, tokens));
-    const int64_t items = tokens * a.parts;
-    const dim3 grid(static_cast<uint32_t>(ceil_div(items < 2 * waves ? items : 2 * waves, kWaves))), block(kThreads);
+template <int LPR, int SLOTS, bool FEW>
+hipError_t launch(const RopeArgs &a, bool quads, dim3 grid, hipStream_t stream) {
+    const dim3 block(kThreads);
     if (a.order == SDHIP_ROPE_ADJACENT) {
         if (quads) {
-            SDHIP_LAUNCH((rope_kernel<LPR, SLOTS, true, true>), grid, block, 0, stream, a);
+            SDHIP_LAUNCH((rope_kernel<LPR, SLOTS, true, true, FEW>), grid, block, 0, stream, a);
         } else {
-            SDHIP_LAUNCH((rope_kernel<LPR, SLOTS, true, false>), grid, block, 0, stream, a);
+            SDHIP_LAUNCH((rope_kernel<LPR, SLOTS, true, false, FEW>), grid, block, 0, stream, a);
         }
     } else if (quads) {
-        SDHIP_LAUNCH((rope_kernel<LPR, SLOTS, false, true>), grid, block, 0, stream, a);
+        SDHIP_LAUNCH((rope_kernel<LPR, SLOTS, false, true, FEW>), grid, block, 0, stream, a);
     } else {
-        SDHIP_LAUNCH((rope_kernel<LPR, SLOTS, false, false>), grid, block, 0, stream, a);
+        SDHIP_LAUNCH((rope_kernel<LPR, SLOTS, false, false, FEW>), grid, block, 0, stream, a);
     }
     return hipGetLastError();
+}
+
+template <int LPR, int SLOTS>
+hipError_t launch(RopeArgs a, bool quads, hipStream_t stream) {
+    constexpr int64_t kRows = 64 / LPR;
+    const int64_t waves = 16 * static_cast<int64_t>(compute_units()), tokens = a.tokens * a.batch;
+    const auto grid = [&](int64_t items) { return dim3(static_cast<uint32_t>(ceil_div(items < 2 * waves ? items : 2 * waves, kWaves))); };
+    if constexpr (LPR < 64 && SLOTS == 1) {
+        if (2 * a.heads <= kRows && tokens >= waves) return launch<LPR, SLOTS, true>(a, quads, grid(ceil_div(tokens * a.heads, kRows)), stream);
+    }
+    // Parts of a token's heads until every wave of the device has one, 16 a CU.
+    const int64_t most = ceil_div(a.heads, kRows);
+    a.parts = static_cast<int32_t>(tokens * most <= waves ? most : tokens >= waves ? 1 : ceil_div(waves, tokens));
+    return launch<LPR, SLOTS, false>(a, quads, grid(tokens * a.parts), stream);
 }
 
 }  // namespace

@@ -223,3 +223,18 @@ def test_many_tokens(gpu):
     for l in (0, 1, 4097, 39999):
         sdhip.rope(x[:, :, l:l + 1], at[l:l + 1], sdhip.rope_axes([32]), one)
         assert torch.equal(one, y[:, :, l:l + 1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ORDERS)
+@pytest.mark.parametrize("norm", [None, "rms", "layer"])
+@pytest.mark.parametrize("shape,dims", [((1, 1, 5000, 64), [64]), ((2500, 1, 2, 40), [16, 8]), ((3, 2, 1501, 128), [40, 42, 46]), ((2, 4, 2100, 64), [2, 62]),
+                                        ((7, 3, 601, 33), [30]), ((4999, 1, 1, 72), [72])])
+def test_many_tokens_of_few_heads(gpu, order, norm, shape, dims):
+    """Rows of several tokens, and batches, by a wave; weights and offsets a head, strides of any kind."""
+    b, h, l, d = shape
+    r = rng(l)
+    weight, bias = uniform(r, (1, h, 1, d), 2.0), uniform(r, (b, 1, 1, d), 1.0)
+    for layout in (("tokens", "tokens"), ("projection", "odd")):
+        check(gpu, shape, dims, order=order, norm=norm, weight=weight, bias=bias, layout=layout, half=layout[1] == "tokens",
+              at=np.floor(r.uniform(0, 100, (b, l, len(dims)))).astype(np.float32))
