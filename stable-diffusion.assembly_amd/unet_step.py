@@ -27,6 +27,7 @@ tests as the checker of a whole step at reduced sizes.
 """
 
 import ctypes
+import gc
 import math
 
 import torch
@@ -609,9 +610,18 @@ class Graph:
         ops.frozen = True
         stream = torch.cuda.Stream()
         stream.wait_stream(torch.cuda.current_stream())
-        with torch.cuda.stream(stream):
-            with torch.cuda.graph(self.graph, stream=stream):
-                self.out = fn()
+        # A graph that the collector frees during a capture ends the process: what is to be
+        # collected is collected before.
+        collecting = gc.isenabled()
+        gc.collect()
+        gc.disable()
+        try:
+            with torch.cuda.stream(stream):
+                with torch.cuda.graph(self.graph, stream=stream):
+                    self.out = fn()
+        finally:
+            if collecting:
+                gc.enable()
         torch.cuda.current_stream().wait_stream(stream)
         torch.cuda.synchronize()
         ops.frozen = False
@@ -629,8 +639,8 @@ class Step(Graph):
 
     def __init__(self, model, ops, inputs):
         self.model = model
-        self.x, self.t, self.ctx = inputs
-        super().__init__(lambda: model.forward(ops, self.x, self.t, self.ctx), ops)
+        self.x, self.t, self.ctx = x, t, ctx = inputs
+        super().__init__(lambda: model.forward(ops, x, t, ctx), ops)  # not of self: a cycle outlives its last use
 
 
 class SdxlBlock:

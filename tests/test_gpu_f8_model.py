@@ -6,7 +6,9 @@ their numbers lie on two sides of a rounding's midpoint.  Each operator is there
 held against 64 bits of what it was given, and the whole against the block of numbers
 not rounded to the roundings' own noise."""
 
+import gc
 import math
+import weakref
 
 import pytest
 import torch
@@ -206,3 +208,34 @@ def test_sdxl_block(gpu, tokens):
     for _ in range(2):
         assert torch.equal(graph.run(), first)
         torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_graphs_that_are_no_longer_used(gpu):
+    """A step's graph goes with its last use, and one in a cycle before another is captured."""
+    block = u.SdxlBlock(gpu, channels=128, heads=2, seed=2, weights="f8")
+    x = torch.randn((1, 20, 128), device=gpu)
+
+    def graph():
+        ops = u.HipOps(gpu)
+        return u.Graph(lambda: block.forward(ops, x), ops)
+
+    class Forward:
+        def forward(self, ops, x, t, ctx):
+            return block.forward(ops, x)
+
+    gone = weakref.ref(u.Step(Forward(), u.HipOps(gpu), (x, None, None)))
+    assert gone() is None
+    first = graph()
+    first.itself, gone = first, weakref.ref(first)
+    want = first.run().clone()
+    torch.cuda.synchronize()
+    del first
+    threshold = gc.get_threshold()
+    gc.set_threshold(1, 1, 1)
+    try:
+        again = graph()
+    finally:
+        gc.set_threshold(*threshold)
+    assert gone() is None and gc.isenabled()
+    assert torch.equal(again.run(), want)
