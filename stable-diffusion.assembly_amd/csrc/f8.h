@@ -32,7 +32,7 @@ struct F8Args {
 };
 
 // The work buffer of a product (gated or not) of M rows; `whole`, whether the
-// weights' rows are of whole blocks of 128 at multiples of 16 bytes.
+// weights' rows are of whole 16 bytes at multiples of them.
 size_t f8_work_size(int64_t M, int64_t N, int64_t K, bool whole);
 hipError_t launch_f8_mul_mat(const F8Args &a, bool whole, void *work, hipStream_t stream);
 

@@ -151,7 +151,8 @@ __device__ __forceinline__ int4v ended_w(int4v v, int k, int K) {
 // ------------------------------------------------------------------ the work buffer
 
 // x's q by halves of a block, zeros past K: [half][row][64]; its 2^e, [block][row]; the
-// weights as rows of whole blocks, zeros past K, where the tiles need them so.
+// weights as rows of whole blocks, zeros past K, where theirs are at other places than
+// multiples of 16 bytes.
 struct F8Work {
     uint8_t *q;
     float *powers;
@@ -499,12 +500,14 @@ struct Tiles {
 struct TilesArgs {
     F8Args a;
     F8Work work;
-    const uint8_t *w;  // rows of whole blocks at multiples of 16 bytes ...
+    const uint8_t *w;  // rows at multiples of 16 bytes, of a multiple of 16 ...
     int64_t ldw;       // ... this far apart
+    int32_t end;       // ... and this long
     uint32_t row_blocks, column_blocks;
 };
 
-template <bool GATED, int WM, int WN, int WK>
+// ENDS: the weights' rows end within a block.
+template <bool GATED, bool ENDS, int WM, int WN, int WK>
 __global__ __launch_bounds__(64 * WM * WN * WK, 2) void f8_tiles_kernel(TilesArgs t) {
     using L = Tiles<WM, WN, WK>;
     const F8Args &a = t.a;
@@ -530,6 +533,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void f8_tiles_kernel(TilesArg
         return n < columns ? n : columns - 1;
     };
     // 16 rows a copy, a row by 4 lanes, its 16 bytes in the order of their places in LDS.
+    const int piece = 16 * ((lane & 3) ^ (lane >> 4));
     uint32_t x_offset[L::kXCopies], w_offset[L::kWCopies];
     const char *w_base[L::kWCopies];
     const char *x_base = reinterpret_cast<const char *>(t.work.q + m0 * 64);
@@ -537,14 +541,14 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void f8_tiles_kernel(TilesArg
 #pragma unroll
     for (int c = 0; c < L::kXCopies; ++c) {
         const int r = 16 * (place + L::kWaves * c) + (lane >> 2);
-        x_offset[c] = 64 * r + 16 * ((lane & 3) ^ ((r >> 2) & 3));
+        x_offset[c] = 64 * r + piece;
     }
 #pragma unroll
     for (int c = 0; c < L::kWCopies; ++c) {
         const int r = 16 * (place + L::kWaves * c) + (lane >> 2);
         int second;
         const int n = column_of(r, second);
-        w_offset[c] = static_cast<uint32_t>((n - n0) * t.ldw + 16 * ((lane & 3) ^ ((r >> 2) & 3)));
+        w_offset[c] = static_cast<uint32_t>((n - n0) * t.ldw + piece);
         const int half = GATED ? ((16 * (place + L::kWaves * c)) >> 5) & 1 : 0;
         w_base[c] = reinterpret_cast<const char *>(t.w + (static_cast<int64_t>(n0) + (half ? columns : 0)) * t.ldw);
     }
@@ -574,7 +578,14 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void f8_tiles_kernel(TilesArg
 #pragma unroll
         for (int c = 0; c < L::kXCopies; ++c) fetch16(x_base + (2 * b + (s & 1)) * x_step, x_offset[c], to + 1024 * (place + L::kWaves * c));
 #pragma unroll
-        for (int c = 0; c < L::kWCopies; ++c) fetch16(w_base[c] + k, w_offset[c], to + L::kXBytes + 1024 * (place + L::kWaves * c));
+        for (int c = 0; c < L::kWCopies; ++c) {
+            const uint32_t at = to + L::kXBytes + 1024 * (place + L::kWaves * c);
+            // Past a row's end its beginning, by x's zeros: a NaN there is its column's
+            // anyway.  (By a branch the copies are apart: 76 x 1344 -> 14027 17.7 us, so 15.8.)
+            const bool last = ENDS && k + 64 > t.end;
+            const int back = last && k + piece >= t.end ? static_cast<int>(k) + piece : 0;
+            fetch16(w_base[c] + (last ? 0 : k), last ? w_offset[c] + static_cast<int>(k) - back : w_offset[c], at);
+        }
 #pragma unroll
         for (int c = 0; c < L::kSmallCopies; ++c) fetch4(small[c] + b * small_step[c], to + small_to[c]);
     };
@@ -822,15 +833,15 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void f8_tiles_kernel(TilesArg
     }
 }
 
-template <bool GATED, int WM, int WN, int WK>
+template <bool GATED, bool ENDS, int WM, int WN, int WK>
 hipError_t launch_tiles(TilesArgs t, hipStream_t stream) {
     using L = Tiles<WM, WN, WK>;
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&f8_tiles_kernel<GATED, WM, WN, WK>),
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&f8_tiles_kernel<GATED, ENDS, WM, WN, WK>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, L::kLds);
     if (attr != hipSuccess) return attr;
     t.row_blocks = static_cast<uint32_t>(ceil_div(t.a.M, L::kX));
     t.column_blocks = static_cast<uint32_t>(GATED ? ceil_div(t.a.half, L::kW / 2) : ceil_div(t.a.N, L::kW));
-    SDHIP_LAUNCH((f8_tiles_kernel<GATED, WM, WN, WK>), dim3(t.row_blocks * t.column_blocks), dim3(L::kThreads), L::kLds, stream, t);
+    SDHIP_LAUNCH((f8_tiles_kernel<GATED, ENDS, WM, WN, WK>), dim3(t.row_blocks * t.column_blocks), dim3(L::kThreads), L::kLds, stream, t);
     return hipGetLastError();
 }
 
@@ -901,6 +912,23 @@ hipError_t lay_out(const F8Args &a, const F8Work &w, hipStream_t stream) {
     return hipGetLastError();
 }
 
+// Tiles whose weights' rows end within a block have kernels of their own: what their
+// last copies take on costs the others 3 to 6% (4096 x 4096 -> 16384 582 us, so 600),
+// and weights laid out first as much as the product (76 x 1344 -> 14027 25 us, so 15.8).
+template <bool GATED, bool ENDS>
+hipError_t launch_tiles(Form form, const TilesArgs &t, hipStream_t stream) {
+    switch (form) {
+    case Form::tiles8:
+        return launch_tiles<GATED, ENDS, 2, 2, 2>(t, stream);
+    case Form::tiles64:
+        return launch_tiles<GATED, ENDS, 1, 2, 2>(t, stream);
+    case Form::tiles64x64:
+        return launch_tiles<GATED, ENDS, 1, 1, 4>(t, stream);
+    default:
+        return launch_tiles<GATED, ENDS, 2, 2, 1>(t, stream);
+    }
+}
+
 template <bool GATED>
 hipError_t launch_form(const F8Args &a, bool whole, void *work, hipStream_t stream) {
     const Form form = form_of(a.M, a.N, a.K, GATED);
@@ -908,17 +936,8 @@ hipError_t launch_form(const F8Args &a, bool whole, void *work, hipStream_t stre
     if (form == Form::rows) return few_rows<GATED, 2>(a, stream);
     const F8Work w = work_of(a.M, a.N, a.K, !whole, work);
     if (const hipError_t e = lay_out(a, w, stream); e != hipSuccess) return e;
-    const TilesArgs t{a, w, whole ? a.w : w.w, whole ? a.row_bytes : w.ld, 0, 0};
-    switch (form) {
-    case Form::tiles8:
-        return launch_tiles<GATED, 2, 2, 2>(t, stream);
-    case Form::tiles64:
-        return launch_tiles<GATED, 1, 2, 2>(t, stream);
-    case Form::tiles64x64:
-        return launch_tiles<GATED, 1, 1, 4>(t, stream);
-    default:
-        return launch_tiles<GATED, 2, 2, 1>(t, stream);
-    }
+    const TilesArgs t{a, w, whole ? a.w : w.w, whole ? a.row_bytes : w.ld, static_cast<int32_t>(whole ? a.K : w.ld), 0, 0};
+    return t.end % kBlock != 0 ? launch_tiles<GATED, true>(form, t, stream) : launch_tiles<GATED, false>(form, t, stream);
 }
 
 }  // namespace

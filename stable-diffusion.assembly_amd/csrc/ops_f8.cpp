@@ -29,10 +29,10 @@ F8Args args_of(const sdhip_tensor *w, const sdhip_tensor *scales, const sdhip_te
     return a;
 }
 
-// Whether rows of the weights are of whole blocks at multiples of 16 bytes, 128 of
-// them within 32 bits.
+// Whether rows of the weights are of whole 16 bytes at multiples of them, 128 rows
+// within 32 bits.
 bool whole(const sdhip_tensor *w) {
-    return w->ne[0] % kF8Block == 0 && w->nb[1] % 16 == 0 && w->nb[1] <= (int64_t{1} << 24) &&
+    return w->ne[0] % 16 == 0 && w->nb[1] % 16 == 0 && w->nb[1] <= (int64_t{1} << 24) &&
            reinterpret_cast<uintptr_t>(w->data) % 16 == 0;
 }
 

@@ -380,3 +380,33 @@ def test_work_buffer_checked(gpu):
         assert (y == 0).all()
     finally:
         sdhip.set_tuning("")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("k", [16, 32, 48, 80, 112, 144, 176, 208, 240, 272, 528])
+def test_rows_that_end_within_a_block(gpu, form, k, gated):
+    """Rows of whole 16 bytes, read as they lie: what follows each, NaN in the gap between
+    them or in the next row, is no part of it."""
+    m, n, odd = 70, 134, 5
+    r = rng(k)
+    bytes_, scales = f8_lib.random_weights(r, n, k)
+    bytes_[odd] = 127
+    x = uniform(r, (m, k), 1.0)
+    for row in (k, k + 16):
+        y, out = Guarded((m, n), gpu), Guarded((m, n // 2), gpu)
+        if gated:
+            sdhip.mul_mat_f8_gated(weights(bytes_, gpu, row), dev(scales, gpu), dev(x, gpu), y.t, out.t)
+        else:
+            sdhip.mul_mat_f8(weights(bytes_, gpu, row), dev(scales, gpu), dev(x, gpu), y.t)
+        torch.cuda.synchronize()
+        exact, mag = f8_lib.exact(bytes_, scales, x)
+        got = (out if gated else y).check()
+        err = f8_lib.bound(k) * mag
+        if gated:
+            a, g = exact[:, :n // 2], exact[:, n // 2:]
+            err = err[:, :n // 2] * np.abs(g) + 1.13 * (np.abs(a) + err[:, :n // 2]) * err[:, n // 2:] + 16 * 2.0 ** -24 * np.abs(a * g)
+            exact = a * gelu64(g)
+        others = np.arange(got.shape[1]) != odd
+        assert np.isnan(got[:, odd]).all()
+        assert (np.abs(got - exact) <= err)[:, others].all()
