@@ -14,8 +14,8 @@
 // Bound by memory.  A slab whose pixels' numbers fit a workgroup's registers takes
 // one launch and one read of x; others a launch for the sums and one for the
 // outputs, which reads x again, the last chunks first: those the Infinity Cache
-// still holds.  1024 x 1024 pixels of 128 channels take 316 us (the sums 119 at 4.5
-// TB/s, the outputs 192 at 5.6); 2 x 8 x 8 of 1280 4.6, a launch and three waits one
+// still holds.  1024 x 1024 pixels of 128 channels take 308 us, 5.2 TB/s of the three
+// times that they are read or written; 2 x 8 x 8 of 1280 4.6, a launch and three waits one
 // after another: x, its sums through LDS, the writes.
 
 #include "host.h"
@@ -557,13 +557,14 @@ Split split_of(const GroupNormLastShape &s, int v, int64_t least) {
         if (p.slab * s.per_group <= w.threads * v && s.pixels <= w.numbers / v * rows_of(s, p.slab, w.threads, v)) return p;
     }
     p.whole = -1;
-    // Whole lines of up to 1024 channels; chunks until each CU has four workgroups,
-    // of 8 pixels a thread at least.  None is empty: as many as chunks of the pixels of
+    // Whole lines of up to 1024 channels; chunks until each CU has 16 workgroups, three
+    // rounds of them, whose last leaves less to wait for than that of 8 (4 x 108 x 183 x
+    // 1376 296 us, so 264, 1024 x 1024 x 128 315 and 308), of 8 pixels a thread at least.  None is empty: as many as chunks of the pixels of
     // one of them are (the outputs' kernel reads its chunk's first pixel).
     p.slab = slab_of(s, ceil_div(s.channels, ceil_div(s.channels, 1024)), v);
     p.slabs = ceil_div(s.groups, p.slab);
     const auto chunks = [&](int64_t slab, int64_t slabs, int64_t least) {
-        const int64_t wanted = ceil_div(8 * cus, s.images * slabs), most = ceil_div(s.pixels, least * rows_of(s, slab, kThreads, v));
+        const int64_t wanted = ceil_div(16 * cus, s.images * slabs), most = ceil_div(s.pixels, least * rows_of(s, slab, kThreads, v));
         return ceil_div(s.pixels, ceil_div(s.pixels, wanted < most ? wanted : most));
     };
     p.parts = chunks(p.slab, p.slabs, 8);
