@@ -856,13 +856,14 @@ enum class Form { few = 1, rows, tiles, tiles8, tiles64, tiles64x64 };
 constexpr int64_t kTilesK = int64_t{1} << 22;
 
 // Microseconds of the few rows' kernel by 16 RM rows: a launch and, for each round of
-// workgroups over the CUs, its blocks of the weights and all of its rows' x.
+// workgroups over the CUs, a wave's blocks of the weights and all of its rows' x.
 double few_time(int64_t M, int64_t columns, int64_t K, int rm, int halves) {
     const int splits = few_splits(M, columns, K, 16 * rm, halves);
     const int64_t blocks = ceil_div(K, kF8Block), groups = ceil_div(columns, 16 * (kWaves / splits / halves)) * ceil_div(M, 16 * rm);
     const double rounds = static_cast<double>(ceil_div(groups, compute_units()));
-    const double own = static_cast<double>(ceil_div(blocks, splits)), all = static_cast<double>(blocks);
-    return rm == 1 ? 4.0 + rounds * (0.4 + 0.55 * own + 0.08 * all) : 4.4 + rounds * (0.8 + 0.6 * own + 0.2 * all);
+    const double rows = static_cast<double>(M < 16 * rm ? M : 16 * rm) / (16 * rm);
+    const double own = static_cast<double>(ceil_div(blocks, splits)), x = rows * static_cast<double>(blocks);
+    return rm == 1 ? 4.0 + rounds * (0.4 + 0.5 * own + 0.12 * x) : 4.4 + rounds * (0.8 + 0.6 * own + 0.27 * x);
 }
 
 // Tiles, the smallest of which there are no more than CUs, else the largest: of 1280
@@ -871,7 +872,7 @@ double few_time(int64_t M, int64_t columns, int64_t K, int rm, int halves) {
 // one on each, and of a long K by eight waves: 2048 rows of 5120 to 1280 columns 51.7 by
 // eight, 54.5 by four, 1024 of 320 to 2560 15.4 and 13.4.  Or a kernel of few rows, where that takes
 // less by the times of a launch fitted to 28 such shapes, of 1 to 8192 rows (the rule
-// is 1% slower than the best choice in the mean, 36% at most): of K 640 to 640 columns
+// is 1% slower than the best choice in the mean, 20% at most): of K 640 to 640 columns
 // by 16 rows | 32 | tiles: 160 rows 5.3 | 6.4 | 10.3, 384 7.3 | 6.7 | 10.5, 1536 - | 13.0 |
 // 11.9; of K 4096 to 4096 columns 32 rows 14.0 | 15.8 | -, 64 17.7 | 19.4 | 17.6.
 Form form_of(int64_t M, int64_t N, int64_t K, bool gated) {
@@ -883,7 +884,7 @@ Form form_of(int64_t M, int64_t N, int64_t K, bool gated) {
     const double blocks = static_cast<double>(ceil_div(K, kF8Block));
     const auto tiles = [&](int64_t x, int64_t w) { return ceil_div(M, x) * ceil_div(columns, w / halves); };
     Form form = Form::tiles;
-    double least = 8.2 + 1e-6 * static_cast<double>(M) * static_cast<double>(K);  // x is laid out
+    double least = 8.2 + 0.5e-6 * static_cast<double>(M) * static_cast<double>(K);  // x is laid out
     if (tiles(64, 64) <= compute_units()) {
         form = Form::tiles64x64;
         least += 0.3 * blocks;
