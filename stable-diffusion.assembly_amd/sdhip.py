@@ -293,17 +293,26 @@ def _work(nbytes, device):
     return buf, nbytes
 
 
+def _buffer(work, nbytes, device):
+    """The work buffer of a call that needs `nbytes`: the caller's, or one made here
+    (None where none is needed), its address, and the bytes that it holds, by which the
+    library refuses one that is too small."""
+    buf = work if work is not None else _work(nbytes, device)[0]
+    if buf is None:
+        return None, None, 0
+    if not buf.is_contiguous():
+        raise ValueError("a work buffer is a contiguous tensor")
+    return buf, buf.data_ptr(), buf.nbytes
+
+
 def mul_mat(w, x, y, chain=None, work=None):
     """y (ne = [N, M...]) = x W^T with the chain; w: [N, K] f16 or f32, or 4-bit
     weights as bytes (desc); x: [..., K] f32."""
     lib = load()
     dw, dx, dy = desc(w), desc(x), desc(y)
     size = lib.sdhip_mul_mat_work_size(dw, dx, dy)
-    buf = work
-    if buf is None:
-        buf, _ = _work(size, x.device)
-    ptr = buf.data_ptr() if buf is not None else None
-    check(lib.sdhip_mul_mat(dw, dx, dy, ctypes.byref(chain) if chain else None, ptr, size, stream_handle()),
+    buf, ptr, held = _buffer(work, size, x.device)
+    check(lib.sdhip_mul_mat(dw, dx, dy, ctypes.byref(chain) if chain else None, ptr, held, stream_handle()),
           "mul_mat")
     return buf
 
@@ -312,11 +321,8 @@ def mul_mat_gated(w, x, y, out, chain=None, work=None):
     lib = load()
     dw, dx, dy, do = desc(w), desc(x), desc(y), desc(out)
     size = lib.sdhip_mul_mat_work_size(dw, dx, dy)
-    buf = work
-    if buf is None:
-        buf, _ = _work(size, x.device)
-    ptr = buf.data_ptr() if buf is not None else None
-    check(lib.sdhip_mul_mat_gated(dw, dx, dy, ctypes.byref(chain) if chain else None, do, ptr, size,
+    buf, ptr, held = _buffer(work, size, x.device)
+    check(lib.sdhip_mul_mat_gated(dw, dx, dy, ctypes.byref(chain) if chain else None, do, ptr, held,
                                   stream_handle()), "mul_mat_gated")
     return buf
 
@@ -327,11 +333,8 @@ def mul_mat_f8(w, scales, x, y, chain=None, work=None):
     lib = load()
     dw, ds, dx, dy = desc(w), desc(scales), desc(x), desc(y)
     size = lib.sdhip_mul_mat_f8_work_size(dw, ds, dx, dy)
-    buf = work
-    if buf is None:
-        buf, _ = _work(size, x.device)
-    ptr = buf.data_ptr() if buf is not None else None
-    check(lib.sdhip_mul_mat_f8(dw, ds, dx, dy, ctypes.byref(chain) if chain else None, ptr, size, stream_handle()),
+    buf, ptr, held = _buffer(work, size, x.device)
+    check(lib.sdhip_mul_mat_f8(dw, ds, dx, dy, ctypes.byref(chain) if chain else None, ptr, held, stream_handle()),
           "mul_mat_f8")
     return buf
 
@@ -340,11 +343,8 @@ def mul_mat_f8_gated(w, scales, x, y, out, chain=None, work=None):
     lib = load()
     dw, ds, dx, dy, do = desc(w), desc(scales), desc(x), desc(y), desc(out)
     size = lib.sdhip_mul_mat_f8_work_size(dw, ds, dx, dy)
-    buf = work
-    if buf is None:
-        buf, _ = _work(size, x.device)
-    ptr = buf.data_ptr() if buf is not None else None
-    check(lib.sdhip_mul_mat_f8_gated(dw, ds, dx, dy, ctypes.byref(chain) if chain else None, do, ptr, size,
+    buf, ptr, held = _buffer(work, size, x.device)
+    check(lib.sdhip_mul_mat_f8_gated(dw, ds, dx, dy, ctypes.byref(chain) if chain else None, do, ptr, held,
                                      stream_handle()), "mul_mat_f8_gated")
     return buf
 
@@ -361,11 +361,8 @@ def conv2d(kernel, x, y, params, chain=None, work=None):
     lib = load()
     dk, dx, dy = desc(kernel), desc(x), desc(y)
     size = lib.sdhip_conv2d_work_size(dk, dx, dy, params)
-    buf = work
-    if buf is None:
-        buf, _ = _work(size, x.device)
-    ptr = buf.data_ptr() if buf is not None else None
-    check(lib.sdhip_conv2d(dk, dx, dy, params, ctypes.byref(chain) if chain else None, ptr, size,
+    buf, ptr, held = _buffer(work, size, x.device)
+    check(lib.sdhip_conv2d(dk, dx, dy, params, ctypes.byref(chain) if chain else None, ptr, held,
                            stream_handle()), "conv2d")
     return buf
 
@@ -374,11 +371,8 @@ def attention(q, k, v, y, scale, work=None):
     lib = load()
     dq, dk, dv, dy = desc(q), desc(k), desc(v), desc(y)
     size = lib.sdhip_attention_work_size(dq, dk, dv, dy)
-    buf = work
-    if buf is None:
-        buf, _ = _work(size, q.device)
-    ptr = buf.data_ptr() if buf is not None else None
-    check(lib.sdhip_attention(dq, dk, dv, dy, scale, 0.0, 0.0, ptr, size, stream_handle()), "attention")
+    buf, ptr, held = _buffer(work, size, q.device)
+    check(lib.sdhip_attention(dq, dk, dv, dy, scale, 0.0, 0.0, ptr, held, stream_handle()), "attention")
     return buf
 
 
@@ -386,11 +380,8 @@ def group_norm(x, y, groups, eps, chain=None, work=None):
     lib = load()
     dx, dy = desc(x), desc(y)
     size = lib.sdhip_group_norm_work_size(dx, dy, groups)
-    buf = work
-    if buf is None:
-        buf, _ = _work(size, x.device)
-    ptr = buf.data_ptr() if buf is not None else None
-    check(lib.sdhip_group_norm(dx, dy, groups, eps, ctypes.byref(chain) if chain else None, ptr, size,
+    buf, ptr, held = _buffer(work, size, x.device)
+    check(lib.sdhip_group_norm(dx, dy, groups, eps, ctypes.byref(chain) if chain else None, ptr, held,
                                stream_handle()), "group_norm")
     return buf
 
@@ -400,11 +391,8 @@ def group_norm_last(x, y, groups, eps, chain=None, work=None):
     lib = load()
     dx, dy = (_images(t) for t in (x, y))
     size = lib.sdhip_group_norm_last_work_size(dx, dy, groups)
-    buf = work
-    if buf is None:
-        buf, _ = _work(size, x.device)
-    ptr = buf.data_ptr() if buf is not None else None
-    check(lib.sdhip_group_norm_last(dx, dy, groups, eps, ctypes.byref(chain) if chain else None, ptr, size,
+    buf, ptr, held = _buffer(work, size, x.device)
+    check(lib.sdhip_group_norm_last(dx, dy, groups, eps, ctypes.byref(chain) if chain else None, ptr, held,
                                     stream_handle()), "group_norm_last")
     return buf
 
