@@ -237,11 +237,12 @@ sdhip_status sdhip_mul_mat_gated(const sdhip_tensor *w, const sdhip_tensor *x, c
  * or less, and q E4M3, to nearest with ties to even.  The products are exact, the
  * sums in single precision; a scale times 2^e is to be below 2^128.  An infinity or
  * NaN in x makes its row's outputs NaN, a NaN in w its column's.
- * What bits asks for is left aside.  The output shares no byte with w, scales or
- * x, nor with an operand of the chain but one that is its own memory in its layout
- * (with fuse = 0 not that): SDHIP_UNSUPPORTED.  Up to 2^25 rows of x and 2^25 of w,
- * 2^36 weights, 2^35 outputs and 2^37 numbers of x are taken.  The work buffer, none where few rows read the
- * weights: x as its q and e and, where their rows are not of whole 16 bytes at
+ * What bits asks for is left aside.  The output (or the redirect) shares no byte
+ * with w, scales or x: SDHIP_ERROR, as sdhip_mul_mat's, which _supported does not
+ * look at.  Nor with an operand of the chain but one that is its own memory in its
+ * layout (with fuse = 0 not that): SDHIP_UNSUPPORTED.  Up to 2^25 rows of x and 2^25
+ * of w, 2^36 weights, 2^35 outputs and 2^37 numbers of x are taken.  The work buffer,
+ * none where few rows read the weights: x as its q and e and, where their rows are not of whole 16 bytes at
  * multiples of 16, the weights; calls that may run at once take a buffer each.
  * Its size follows the f8_form tuning, which is to be the same when the size is
  * asked for and when the product is made. */
@@ -254,7 +255,8 @@ sdhip_status sdhip_mul_mat_f8(const sdhip_tensor *w, const sdhip_tensor *scales,
                               void *stream);
 
 /* The same with the GEGLU after it, as sdhip_mul_mat_gated; the work buffer is
- * sdhip_mul_mat_f8_work_size's. */
+ * sdhip_mul_mat_f8_work_size's.  out shares no byte with w, scales, x or y, nor with
+ * an operand of the chain: SDHIP_UNSUPPORTED, the former by _supported too. */
 int sdhip_mul_mat_f8_gated_supported(const sdhip_tensor *w, const sdhip_tensor *scales, const sdhip_tensor *x,
                                      const sdhip_tensor *y, const sdhip_tensor *out);
 sdhip_status sdhip_mul_mat_f8_gated(const sdhip_tensor *w, const sdhip_tensor *scales, const sdhip_tensor *x,
