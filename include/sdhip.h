@@ -242,8 +242,9 @@ sdhip_status sdhip_mul_mat_gated(const sdhip_tensor *w, const sdhip_tensor *x, c
  * look at.  Nor with an operand of the chain but one that is its own memory in its
  * layout (with fuse = 0 not that): SDHIP_UNSUPPORTED.  Up to 2^25 rows of x and 2^25
  * of w, 2^36 weights, 2^35 outputs and 2^37 numbers of x are taken.  The work buffer,
- * none where few rows read the weights: x as its q and e and, where their rows are not of whole 16 bytes at
- * multiples of 16, the weights; calls that may run at once take a buffer each.
+ * none where few rows read the weights: x as its q and e and, where their rows are
+ * not of whole 16 bytes at multiples of 16, the weights; calls that may run at once
+ * take a buffer each.
  * Its size follows the f8_form tuning, which is to be the same when the size is
  * asked for and when the product is made. */
 int sdhip_mul_mat_f8_supported(const sdhip_tensor *w, const sdhip_tensor *scales, const sdhip_tensor *x,
