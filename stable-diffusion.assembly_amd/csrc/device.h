@@ -267,11 +267,6 @@ __device__ __forceinline__ void fetch16(const char *from, uint32_t offset, uint3
     asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(to), "v"(offset), "s"(from) : "memory");
 }
 
-// fetch4 from an address the wave's lanes share and an offset of each.
-__device__ __forceinline__ void fetch4(const char *from, uint32_t offset, uint32_t to) {
-    asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, %2" ::"{m0}"(to), "v"(offset), "s"(from) : "memory");
-}
-
 __device__ __forceinline__ uint32_t lds_address(const char *p) {
     return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char *)p));
 }

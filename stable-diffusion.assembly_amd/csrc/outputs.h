@@ -13,12 +13,11 @@ namespace sdhip {
 // apart, `count` outputs, with GATED the second half's behind them: their sums
 // in the splits' order, times what `place` gives with an output's row (M or
 // more: none) and column; the redirect's number first, the chain, the gated
-// GELU.  E of a thread's at a time, so that their loads go out together.  MOST, the
-// most splits there are.
-template <bool GATED, int E, int MOST = 8, class Args, class Place>
+// GELU.  E of a thread's at a time, so that their loads go out together.
+template <bool GATED, int E, class Args, class Place>
 __device__ __forceinline__ void write_outputs(const Args &a, const float *sums, int splits, int step, int count, int tid,
                                               int columns, Place place, int threads) {
-    constexpr int kHalves = GATED ? 2 : 1;
+    constexpr int kHalves = GATED ? 2 : 1, kMost = 8;  // the most splits there are
 #pragma unroll 1
     for (int first = tid; first < count; first += E * threads) {
         int64_t m[E];
@@ -34,12 +33,12 @@ __device__ __forceinline__ void write_outputs(const Args &a, const float *sums, 
             n[e] = n[e] < columns ? n[e] : columns - 1;
 #pragma unroll
             for (int p = 0; p < kHalves; ++p) {
-                float s[MOST];
+                float s[kMost];
 #pragma unroll
-                for (int k = 0; k < MOST; ++k) s[k] = sums[(k < splits ? k : 0) * step + p * count + at];
+                for (int k = 0; k < kMost; ++k) s[k] = sums[(k < splits ? k : 0) * step + p * count + at];
                 float total = s[0];
 #pragma unroll
-                for (int k = 1; k < MOST; ++k) total = k < splits ? total + s[k] : total;
+                for (int k = 1; k < kMost; ++k) total = k < splits ? total + s[k] : total;
                 v[kHalves * e + p] = total * back;
             }
         }
