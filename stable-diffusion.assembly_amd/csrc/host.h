@@ -146,12 +146,12 @@ bool row_norm_taken(const sdhip_row_norm *n, const sdhip_tensor *shape);
 bool elements_apart(const sdhip_tensor *t);
 // Whether the bytes that two tensors (or none) reach share any.
 bool tensors_share(const sdhip_tensor *a, const sdhip_tensor *b);
-// The compute units of the current device (looked up once a device; 256,
-// MI355X's, where the runtime cannot say).
 // Whether no operand of the chain lies where the operation writes, but one that is its
 // output's own memory in its layout, read before it is written; with the chain apart
 // (fuse = 0) y is written first.
 bool chain_apart(const sdhip_tensor *y, const sdhip_epilogue *e);
+// The compute units of the current device (looked up once a device; 256,
+// MI355X's, where the runtime cannot say).
 int compute_units();
 // The address `bytes` past p as an integer (no pointer arithmetic on what
 // may be a null or foreign pointer).
