@@ -251,7 +251,7 @@ class HipOps(Ops):
         n, k = extents(w)
         m = x.numel() // k
         self.count_linear(x, w)
-        if m < 16 and w.dtype == torch.float16:
+        if m < 16 and not isinstance(w, BlockScaled) and w.dtype != torch.uint8:
             # Not taken by the reference (mul_mat.cc:181-194): ggml's node,
             # with the weights widened once and kept, as ggml's CPU backend
             # reads them without converting the tensor each time.
