@@ -15,14 +15,23 @@ namespace sdhip {
 namespace {
 
 // Element i of a contiguous output of extents ne, its steps' operands at
-// sum(ik nb[k]); the values into out (the output itself, or the redirect).
+// sum(ik nb[k]); the values into out (the output itself, or the redirect).  WIDE:
+// of 2^32 rows or more (images of few channels, channels last).
+template <bool WIDE>
 __global__ __launch_bounds__(256) void chain_apart_kernel(const float *in, float *out, int64_t n,
                                                           uint32_t ne0, uint32_t ne1, uint32_t ne2, DevChain c) {
     for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
-        const uint32_t row = static_cast<uint32_t>(i / ne0);
-        const uint32_t i0 = static_cast<uint32_t>(i - static_cast<int64_t>(row) * ne0);
+        const int64_t row = i / ne0;
+        const uint32_t i0 = static_cast<uint32_t>(i - row * ne0);
         uint32_t i1, i2, i3;
-        split_index(row, ne1, ne2, i1, i2, i3);
+        if (WIDE) {
+            const int64_t matrix = row / ne1;
+            i1 = static_cast<uint32_t>(row - matrix * ne1);
+            i3 = static_cast<uint32_t>(matrix / ne2);
+            i2 = static_cast<uint32_t>(matrix - static_cast<int64_t>(i3) * ne2);
+        } else {
+            split_index(static_cast<uint32_t>(row), ne1, ne2, i1, i2, i3);
+        }
         float v[1] = {in[i]};
         apply_chain_block(c, v, [&](int s, int) {
             const DevStep &st = c.steps[s];
@@ -116,9 +125,16 @@ sdhip_status chain_after(const ChainRun &r, hipStream_t stream) {
     const int64_t n = r.ne[0] * r.ne[1] * r.ne[2] * r.ne[3];
     if (n == 0) return SDHIP_OK;
     KernelScope prof("chain.apart", stream);
-    SDHIP_LAUNCH(chain_apart_kernel, dim3(grid_of(n)), dim3(256), 0, stream, r.apart_in, r.apart_out, n,
-                 static_cast<uint32_t>(r.ne[0]), static_cast<uint32_t>(r.ne[1]), static_cast<uint32_t>(r.ne[2]),
-                 r.after);
+    const auto run = [&](auto kernel) {
+        SDHIP_LAUNCH(kernel, dim3(grid_of(n)), dim3(256), 0, stream, r.apart_in, r.apart_out, n,
+                     static_cast<uint32_t>(r.ne[0]), static_cast<uint32_t>(r.ne[1]), static_cast<uint32_t>(r.ne[2]),
+                     r.after);
+    };
+    if (n / r.ne[0] > UINT32_MAX) {
+        run(chain_apart_kernel<true>);
+    } else {
+        run(chain_apart_kernel<false>);
+    }
     return launched(hipGetLastError(), "chain apart");
 }
 
