@@ -36,15 +36,19 @@ bool whole(const sdhip_tensor *w) {
            reinterpret_cast<uintptr_t>(w->data) % 16 == 0;
 }
 
+bool whole_floats(const sdhip_tensor *t) { return reinterpret_cast<uintptr_t>(t->data) % 4 == 0; }
+
+sdhip_status misaligned(const char *what) {
+    return fail(SDHIP_ERROR, "%s: single precision at an address that is no multiple of 4", what);
+}
+
 // The product into a.y, `columns` wide, which what it reads shares no byte with.
 sdhip_status product(const F8Args &a, const sdhip_tensor *w, const sdhip_tensor *scales, const sdhip_tensor *x,
                      int64_t columns, void *work, size_t work_size, hipStream_t stream, const char *what) {
     if (w->data == nullptr || scales->data == nullptr || x->data == nullptr || a.y == nullptr) {
         return fail(SDHIP_ERROR, "%s: a tensor without data", what);
     }
-    const uintptr_t at = reinterpret_cast<uintptr_t>(x->data) | reinterpret_cast<uintptr_t>(a.y) |
-                         reinterpret_cast<uintptr_t>(scales->data);
-    if (at % 4 != 0) return fail(SDHIP_ERROR, "%s: single precision at an address that is no multiple of 4", what);
+    if (!whole_floats(x) || !whole_floats(scales) || reinterpret_cast<uintptr_t>(a.y) % 4 != 0) return misaligned(what);
     const size_t on = static_cast<size_t>((a.M - 1) * a.ldy + columns) * 4;
     for (const sdhip_tensor *t : {w, scales, x}) {
         if (spans_overlap(a.y, on, t->data, tensor_span(t))) {
@@ -103,6 +107,7 @@ sdhip_status sdhip_mul_mat_f8(const sdhip_tensor *w, const sdhip_tensor *scales,
     sdhip_status s = chain_plan(y, chain, run);
     if (s != SDHIP_OK) return s;
     if (!chain_apart(y, chain)) return fail(SDHIP_UNSUPPORTED, "mul_mat_f8: the output overlaps a chain operand");
+    if (chain != nullptr && chain->redirect != nullptr && !whole_floats(chain->redirect)) return misaligned("mul_mat_f8");
     for (const sdhip_tensor *t : {w, scales, x}) {
         if (chain != nullptr && tensors_share(chain->redirect, t)) return fail(SDHIP_ERROR, "mul_mat_f8: the output lies over an operand");
     }
@@ -140,12 +145,13 @@ sdhip_status sdhip_mul_mat_f8_gated(const sdhip_tensor *w, const sdhip_tensor *s
         return fail(SDHIP_UNSUPPORTED, "mul_mat_f8_gated: a chain with a residual redirect is not gated");
     }
     const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (out->data == nullptr) return fail(SDHIP_ERROR, "mul_mat_f8_gated: a tensor without data");
+    if (!whole_floats(out)) return misaligned("mul_mat_f8_gated");
     if (tuning().fuse == 0) {
         // The gated GELU apart: the product and its chain into y, then out from
         // y's halves.
         const sdhip_status s = sdhip_mul_mat_f8(w, scales, x, y, chain, work, work_size, stream);
         if (s != SDHIP_OK) return s;
-        if (out->data == nullptr) return fail(SDHIP_ERROR, "mul_mat_f8_gated: a tensor without data");
         return gated_after(static_cast<const float *>(y->data), static_cast<float *>(out->data),
                            x->ne[1] * x->ne[2] * x->ne[3], y->ne[0] / 2, y->nb[1] / 4, out->nb[1] / 4, st);
     }
