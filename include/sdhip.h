@@ -235,8 +235,9 @@ sdhip_status sdhip_mul_mat_gated(const sdhip_tensor *w, const sdhip_tensor *x, c
  * numbers are held to: the numbers of row m and block b as q 2^e, e the least
  * whole number, -101 at least, that brings the greatest magnitude of them to 448
  * or less, and q E4M3, to nearest with ties to even.  The products are exact, the
- * sums in single precision; a scale times 2^e is to be below 2^128.  An infinity or
- * NaN in x makes its row's outputs NaN, a NaN in w its column's.
+ * sums in single precision; a scale times 2^e is to be below 2^128, and keeps its 24
+ * bits from 2^-126 up.  An infinity or NaN in x makes its row's outputs NaN, a NaN in
+ * w its column's.
  * What bits asks for is left aside.  The output (or the redirect) shares no byte
  * with w, scales or x: SDHIP_ERROR, as sdhip_mul_mat's, which _supported does not
  * look at.  Nor with an operand of the chain but one that is its own memory in its
@@ -368,7 +369,8 @@ sdhip_status sdhip_group_norm_static(const sdhip_tensor *x, const sdhip_tensor *
  * chain with y but y's own memory in its layout (fuse = 0: nor that):
  * SDHIP_UNSUPPORTED.
  * No redirect.  The work buffer holds the partial sums of stretches of an
- * image's pixels, 0 where a group is small enough for one launch. */
+ * image's pixels, 0 where a group is small enough for one launch; calls that may
+ * run at once take a buffer each. */
 int sdhip_group_norm_last_supported(const sdhip_tensor *x, const sdhip_tensor *y, int groups);
 size_t sdhip_group_norm_last_work_size(const sdhip_tensor *x, const sdhip_tensor *y, int groups);
 sdhip_status sdhip_group_norm_last(const sdhip_tensor *x, const sdhip_tensor *y, int groups, float eps,
@@ -437,15 +439,17 @@ sdhip_status sdhip_norm_residual(const sdhip_tensor *y, const sdhip_row_norm *po
  *
  * x F32 and y F32 or F16, ne = [d, tokens, heads, batch] as attention's
  * queries, d <= 512, up to 2^24 heads and 2^40 tokens of all batches, nb[0] the
- * element size and the other strides any multiple of it from 0 up (queries and keys side by side in a projection's output are one x, their
+ * element size and the other strides any multiple of it from 0 up (queries and
+ * keys side by side in a projection's output are one x, their
  * norms' weights one tensor of ne[2] = heads).  positions F32, ne = [count,
  * tokens or 1, 1, batch or 1], nb[0] = 4.  The pairs of axis a are the
  * dims[a] / 2 after those of the axes before, dims even; t is the position
  * along a times base[a]^(-2 j / dims[a]) for the axis's pair j or, with
  * `shared`, base[a]^(-2 p / n) for the head's pair p.  Pair p is numbers 2 p and
- * 2 p + 1 (ADJACENT) or p and n / 2 + p (HALVES).  Angles are taken in double; a
- * norm is sdhip_row_norm's (sdhip_norm_residual), its sums in double or, of squares
- * far from single precision's limits, in that.  y may be
+ * 2 p + 1 (ADJACENT) or p and n / 2 + p (HALVES).  Angles are taken in double and
+ * are to be below 2^50, where that holds a quarter of one still; a norm is
+ * sdhip_row_norm's (sdhip_norm_residual), its sums in double or, of squares far from
+ * single precision's limits, in single precision.  y may be
  * x's own memory in the same layout; else what is written shares no byte range
  * with what is read, nor do two rows of y: SDHIP_UNSUPPORTED.  No work buffer. */
 enum { SDHIP_ROPE_ADJACENT = 0, SDHIP_ROPE_HALVES = 1 };

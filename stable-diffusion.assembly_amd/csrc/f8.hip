@@ -474,9 +474,9 @@ hipError_t few_rows(const F8Args &a, hipStream_t stream) {
 // of their row that spreads 16 rows read at once over LDS's banks.  kRing stages are in LDS, one
 // read and the others under way (four: 1976 x 1280 -> 10240 71.6 us against 69.0).
 //
-// 4096 x 4096 -> 16384 takes 550 us, 1.0 PFLOP/s, where a library's product of FP16
-// takes 460: its MFMAs are busy 82% of the cycles at the 1.55 GHz that the card then
-// runs, these 55% at 1.76, with 7.4 other vector operations a MFMA (4 that widen, 2 that
+// 4096 x 4096 -> 16384 takes 520 to 550 us, 1.0 PFLOP/s, where a library's product of
+// FP16 takes 380 to 460, as the card and the numbers are: its MFMAs are busy 82% of the
+// cycles at the 1.55 GHz that the card then runs, these 55% at 1.76, with 7.4 other vector operations a MFMA (4 that widen, 2 that
 // add a block's sums) on the same ports, LDS read or written 75% of the MFMAs' time.
 // Whole rounds of tiles are the rest: 1976 x 5120 -> 1280 has 160 for 256 CUs.
 constexpr int kRing = 3;

@@ -14,9 +14,10 @@
 // Bound by memory.  A slab whose pixels' numbers fit a workgroup's registers takes
 // one launch and one read of x; others a launch for the sums and one for the
 // outputs, which reads x again, the last chunks first: those the Infinity Cache
-// still holds.  1024 x 1024 pixels of 128 channels take 308 us, 5.2 TB/s of the three
-// times that they are read or written; 2 x 8 x 8 of 1280 4.6, a launch and three waits one
-// after another: x, its sums through LDS, the writes.
+// still holds.  1024 x 1024 pixels of 128 channels take 310 us in the kernels (318 a pass
+// in a captured graph, 322 with other tensors each time), 5.2 TB/s of the three times that
+// they are read or written; 2 x 8 x 8 of 1280 4.7, a launch and three waits one after
+// another: x, its sums through LDS, the writes.
 
 #include "host.h"
 #include "norm_last.h"
@@ -201,8 +202,8 @@ __device__ __forceinline__ Moments moments_of(double shift, double first, double
 // reciprocal the least normal number, within |x| 2^-126.  Where the exponent passes 2^7
 // the power is an infinity or 0 and stays so: what is made up for would be NaN, an
 // infinity times a rounding below 0 or an infinite exponent's own (the comparison is 0.15
-// us of 2 x 64 x 64 x 320's 15.8 in a captured graph).  Half of the operations of
-// silu(), which the outputs of a group norm would wait for: 1.2 us of the same.
+// us of 2 x 64 x 64 x 320's 15.8 in a captured graph).  Fewer than half of the operations
+// of silu(), which the outputs of a group norm would wait for: 1.2 us of the same.
 __device__ __forceinline__ float fast_silu(float x) {
     const float t = -1.44269504088896341f * x, rest = __builtin_fmaf(-1.44269504088896341f, x, -t);
     const float e = __builtin_amdgcn_exp2f(t), low = __builtin_fmaf(-1.925963033500e-8f, x, rest);
@@ -220,8 +221,8 @@ __device__ __forceinline__ double numbers_of(const GroupNormLastArgs &a, int64_t
 // a chain that is a multiplication, an addition and SiLU, or some of them in that
 // order, by one number a channel (and image): held in registers (`plain`).  Any
 // other chain reads its operands for each pixel.  (Six steps of any kind in registers
-// are 60 KB of instructions, most of them never run and each launch fetched again:
-// 2 x 64 x 64 x 320 15 us for the outputs, so 5.)
+// are 60 KB of instructions, most of them never run and each launch fetched again: the
+// outputs of 2 x 64 x 64 x 320, 9.5 us in a trace, took three times as long by them.)
 template <int V>
 struct Outputs {
     Moments stats[V];

@@ -387,7 +387,9 @@ def group_norm(x, y, groups, eps, chain=None, work=None):
 
 
 def group_norm_last(x, y, groups, eps, chain=None, work=None):
-    """GROUP_NORM of x [N, H, W, C] (or [N, L, C], [L, C]) over its last dimension's groups."""
+    """GROUP_NORM of x [N, H, W, C] (or [N, L, C], [L, C]) over its last dimension's groups.
+    The chain's operands are broadcast over [N, H, W, C] whatever x is: one number a channel
+    and image of tokens [N, L, C] is a tensor [N, 1, 1, C]."""
     lib = load()
     dx, dy = (_images(t) for t in (x, y))
     size = lib.sdhip_group_norm_last_work_size(dx, dy, groups)
